@@ -15,6 +15,7 @@ from ._lib import Fe2o3Error, Slice, check, lib
 DROP_ROUTE = 0xFFFFFFFF
 SCHEDULE_EXACT_ORDER, SCHEDULE_TCGEN05, SCHEDULE_AUTO = 0, 1, 2
 DTYPE_F32, DTYPE_BF16 = 0, 1
+KV_BF16, KV_E4M3, KV_I8 = 0, 1, 2
 ERR_NO_DISPATCH = 1000
 
 

@@ -68,6 +68,21 @@ MoeEpFfnArgs = _struct("MoeEpFfnArgs",
                         "epoch_counter", "progress"],
                        [("tokens", u32), ("d_model", u32), ("d_ff", u32), ("experts", u32), ("world", u32), ("rank", u32),
                         ("epoch", u32), ("max_rows", u32), ("spin_limit", u32), ("reserved", u32)])
+KvCacheAppendArgs = _struct("KvCacheAppendArgs",
+                            ["k", "v", "page_table", "lengths", "token_offsets", "k_cache", "v_cache", "k_scales", "v_scales"],
+                            [("tokens", u32), ("batch", u32), ("kv_heads", u32), ("dim", u32), ("page_size", u32), ("table_width", u32),
+                             ("k_token_stride", u32), ("k_head_stride", u32), ("v_token_stride", u32), ("v_head_stride", u32),
+                             ("input_dtype", u32), ("format", u32)])
+KvCacheReadArgs = _struct("KvCacheReadArgs",
+                          ["k_cache", "v_cache", "k_scales", "v_scales", "page_table", "lengths", "token_offsets", "k", "v"],
+                          [("tokens", u32), ("batch", u32), ("kv_heads", u32), ("dim", u32), ("page_size", u32), ("table_width", u32),
+                           ("k_token_stride", u32), ("k_head_stride", u32), ("v_token_stride", u32), ("v_head_stride", u32),
+                           ("output_dtype", u32), ("format", u32)])
+PagedAttentionArgs = _struct("PagedAttentionArgs",
+                             ["q", "k_cache", "v_cache", "k_scales", "v_scales", "page_table", "lengths", "output", "lse"],
+                             [("batch", u32), ("heads", u32), ("kv_heads", u32), ("dim", u32), ("page_size", u32), ("table_width", u32),
+                              ("q_stride", u32), ("q_head_stride", u32), ("scale", f32), ("window", u32), ("q_dtype", u32),
+                              ("output_dtype", u32), ("format", u32), ("reserved", u32)])
 MaskedReduceArgs = _struct("MaskedReduceArgs", ["values", "active", "output"])
 MaskedReducePackedArgs = _struct("MaskedReducePackedArgs", ["values", "mask", "output"])
 DeviceScanArgs = _struct("DeviceScanArgs", ["values", "output"], [("exclusive", u32), ("reserved", u32)])
@@ -124,6 +139,9 @@ OPS = {
     "moe_expert_ffn_combine_v1": (MoeExpertFfnCombineArgs, 144, False),
     "moe_ep_exchange_v1": (MoeEpExchangeArgs, 296, False),
     "moe_ep_ffn_v1": (MoeEpFfnArgs, 216, False),
+    "kv_cache_append_v1": (KvCacheAppendArgs, 192, False),
+    "kv_cache_read_v1": (KvCacheReadArgs, 192, False),
+    "paged_attention_v1": (PagedAttentionArgs, 200, False),
     "masked_reduce_u32": (MaskedReduceArgs, 48, False),
     "masked_reduce_u32_packed": (MaskedReducePackedArgs, 48, False),
     "device_scan_u32": (DeviceScanArgs, 40, False),

@@ -3,6 +3,7 @@
 // fe2o3-core (crates/fe2o3-core/src/{context,stream,memory,event}.rs), the
 // generated host adapters (crates/fe2o3-host/src/generated_*.rs) and the
 // executable lifecycle adapter (crates/fe2o3-host/src/hsa_executable_lifecycle.rs).
+#include <math.h>
 #include <stdarg.h>
 #include <stdio.h>
 #include <string.h>
@@ -34,6 +35,9 @@ int32_t launch_moe_top2(fe2o3_ctx *, cudaStream_t, const void *, fe2o3_geometry 
 int32_t launch_moe_route_weights(fe2o3_ctx *, cudaStream_t, const void *, fe2o3_geometry *, bool);
 int32_t launch_moe_combine(fe2o3_ctx *, cudaStream_t, const void *, fe2o3_geometry *, bool);
 int32_t launch_moe_ep_exchange(fe2o3_ctx *, cudaStream_t, const void *, fe2o3_geometry *, bool);
+int32_t launch_kv_cache_append(fe2o3_ctx *, cudaStream_t, const void *, fe2o3_geometry *, bool);
+int32_t launch_kv_cache_read(fe2o3_ctx *, cudaStream_t, const void *, fe2o3_geometry *, bool);
+int32_t launch_paged_attention(fe2o3_ctx *, cudaStream_t, const void *, fe2o3_geometry *, bool);
 int32_t launch_moe_compact(cudaStream_t, uint64_t x, uint64_t perm, uint64_t compact_x, uint32_t rows,
                            uint32_t d_model, uint32_t tokens);
 int32_t launch_gemm_exact(fe2o3_ctx *, cudaStream_t, uint32_t dtype, bool epilogue, uint64_t a, uint64_t b, uint64_t c, uint32_t M,
@@ -99,7 +103,7 @@ enum OpId : uint32_t {
     OP_MOE_GATE, OP_MOE_ROUTE_WEIGHTS, OP_MOE_EXPERT_FFN, OP_MOE_COMBINE, OP_MASKED_REDUCE, OP_MASKED_REDUCE_PACKED,
     OP_WAVE_LDS, OP_WAVE64_COLLECTIVES, OP_WAVE64_SEGMENTED, OP_LDS_REDUCE_I32, OP_SCOPED_ATOMIC_ADD,
     OP_MOE_COMPACT, OP_MOE_GROUPED_FFN, OP_MOE_EP_EXCHANGE, OP_DEVICE_SCAN_U32, OP_DEVICE_SCAN_F32, OP_MOE_EP_FFN,
-    OP_MOE_FFN_COMBINE, OP_COUNT
+    OP_MOE_FFN_COMBINE, OP_KV_APPEND, OP_KV_READ, OP_PAGED_ATTENTION, OP_COUNT
 };
 
 struct OpInfo {
@@ -133,6 +137,9 @@ static const OpInfo kOps[OP_COUNT] = {
     {"device_scan_sum_f32", sizeof(fe2o3_device_scan_f32_args), launch_device_scan_f32},
     {"moe_ep_ffn_v1", sizeof(fe2o3_moe_ep_ffn_v1_args), nullptr},
     {"moe_expert_ffn_combine_v1", sizeof(fe2o3_moe_expert_ffn_combine_v1_args), nullptr},
+    {"kv_cache_append_v1", sizeof(fe2o3_kv_cache_append_v1_args), launch_kv_cache_append},
+    {"kv_cache_read_v1", sizeof(fe2o3_kv_cache_read_v1_args), launch_kv_cache_read},
+    {"paged_attention_v1", sizeof(fe2o3_paged_attention_v1_args), launch_paged_attention},
 };
 
 struct fe2o3_prepared {
@@ -340,6 +347,61 @@ int32_t check_ctx_device(fe2o3_ctx *ctx, const Region *r, int n) {
 }
 
 #define RGN(role_, slice_, expected_, bytes_, out_) Region{role_, slice_, (uint64_t)(expected_), bytes_, out_}
+
+// The cache's own slices, common to the three operators on it: dims, format, pages, and what a row of the tables holds.
+// Appends to r from n on; returns the new count, or 0 with *status set.
+template <typename Args>
+int kv_cache_regions(const Args *a, Region *r, int n, bool writes, int32_t *status) {
+    if (a->kv_heads == 0 || a->dim == 0 || a->dim % 16 || a->dim > 256 || a->page_size == 0 || a->format > FE2O3_KV_I8) {
+        *status = unsupported("a key-value cache has kv_heads >= 1, dim a multiple of 16 up to 256, page_size >= 1, format bf16, e4m3 or i8");
+        return 0;
+    }
+    uint64_t rows;   // of one page
+    if (mul_overflow(a->kv_heads, a->page_size, &rows) || rows > 0xffffffffu) {
+        *status = unsupported("a page holds fewer than 2^32 rows");
+        return 0;
+    }
+    const uint64_t page = rows * a->dim, pages = a->k_cache.len / page;
+    if (pages > 0xffffffffu) { *status = unsupported("page numbers are u32"); return 0; }
+    if ((a->k_cache.ptr | a->v_cache.ptr) & 15u) {
+        fe2o3_set_error("Alignment{role=%s}: the caches start on 16 bytes", a->k_cache.ptr & 15u ? "KeyCache" : "ValueCache");
+        *status = FE2O3_ERR_ALIGNMENT;
+        return 0;
+    }
+    const uint32_t eb = a->format == FE2O3_KV_BF16 ? 2 : 1;
+    const uint64_t scales = a->format == FE2O3_KV_BF16 ? 0 : pages * rows;
+    r[n++] = RGN("KeyCache", a->k_cache, pages * page, eb, writes);
+    r[n++] = RGN("ValueCache", a->v_cache, pages * page, eb, writes);
+    r[n++] = RGN("KeyScales", a->k_scales, scales, 4, writes);
+    r[n++] = RGN("ValueScales", a->v_scales, scales, 4, writes);
+    r[n++] = RGN("PageTable", a->page_table, (uint64_t)a->batch * a->table_width, 4, false);
+    r[n++] = RGN("Lengths", a->lengths, a->batch, 4, false);
+    return n;
+}
+
+// New tokens' rows (append: inputs, read: outputs) and which sequence they belong to.
+template <typename Args>
+int kv_rows_regions(const Args *a, Region *r, int n, uint32_t dtype, bool writes, int32_t *status) {
+    if (dtype > FE2O3_DTYPE_BF16) { *status = unsupported("rows are f32 or bf16"); return 0; }
+    const bool each = a->token_offsets.ptr == 0 && a->token_offsets.len == 0;
+    if (each && a->tokens != a->batch) { *status = unsupported("without token_offsets every sequence has one token: tokens == batch"); return 0; }
+    if (!each) r[n++] = RGN("TokenOffsets", a->token_offsets, (uint64_t)a->batch + 1, 4, false);
+    const fe2o3_slice rows[2] = {a->k, a->v};
+    const uint64_t ts[2] = {a->k_token_stride, a->v_token_stride}, hs[2] = {a->k_head_stride, a->v_head_stride};
+    for (int i = 0; i < 2; ++i) {
+        uint64_t len = 0;
+        if (a->tokens) {
+            const uint64_t t = (a->tokens - 1) * ts[i], h = (a->kv_heads - 1) * hs[i];
+            if (t + h < t || t + h + a->dim < t) { fe2o3_set_error("ExtentOverflow"); *status = FE2O3_ERR_SIZE_OVERFLOW; return 0; }
+            len = t + h + a->dim;
+            const bool heads_inside = (a->kv_heads == 1 || hs[i] >= a->dim) && (a->tokens == 1 || ts[i] >= h + a->dim);
+            const bool tokens_inside = (a->tokens == 1 || ts[i] >= a->dim) && (a->kv_heads == 1 || hs[i] >= t + a->dim);
+            if (writes && !heads_inside && !tokens_inside) { *status = unsupported("output rows overlap"); return 0; }
+        }
+        r[n++] = Region{i ? "Value" : "Key", rows[i], len, dtype == FE2O3_DTYPE_F32 ? 4u : 2u, writes};
+    }
+    return n;
+}
 
 // Per-op region tables.  Returns the number of regions, fills `r`.
 int regions_for(uint32_t op, const void *args, Region *r, int32_t *status) {
@@ -579,6 +641,38 @@ int regions_for(uint32_t op, const void *args, Region *r, int32_t *status) {
             r[1] = RGN("Mask", a->mask, (a->values.len + 63) / 64, 8, false);
             r[2] = RGN("Output", a->output, 1, 4, true);
             return 3;
+        }
+        case OP_KV_APPEND: {
+            const fe2o3_kv_cache_append_v1_args *a = static_cast<const fe2o3_kv_cache_append_v1_args *>(args);
+            const int n = kv_cache_regions(a, r, 0, true, status);
+            return n ? kv_rows_regions(a, r, n, a->input_dtype, false, status) : 0;
+        }
+        case OP_KV_READ: {
+            const fe2o3_kv_cache_read_v1_args *a = static_cast<const fe2o3_kv_cache_read_v1_args *>(args);
+            const int n = kv_cache_regions(a, r, 0, false, status);
+            return n ? kv_rows_regions(a, r, n, a->output_dtype, true, status) : 0;
+        }
+        case OP_PAGED_ATTENTION: {
+            const fe2o3_paged_attention_v1_args *a = static_cast<const fe2o3_paged_attention_v1_args *>(args);
+            int n = kv_cache_regions(a, r, 0, false, status);
+            if (!n) return 0;
+            if (a->heads == 0 || a->heads % a->kv_heads || a->q_dtype > FE2O3_DTYPE_BF16 || a->output_dtype > FE2O3_DTYPE_BF16 ||
+                !isfinite(a->scale) || (uint64_t)a->batch * a->heads > 0x7fffffffu) {
+                *status = unsupported("paged_attention_v1 needs heads a multiple of kv_heads, batch * heads < 2^31, f32 or bf16 queries "
+                                      "and output, a finite scale");
+                return 0;
+            }
+            uint64_t len = 0;
+            if (a->batch) {
+                const uint64_t b = (uint64_t)(a->batch - 1) * a->q_stride, h = (uint64_t)(a->heads - 1) * a->q_head_stride;
+                if (b + h < b || b + h + a->dim < b) { fe2o3_set_error("ExtentOverflow"); *status = FE2O3_ERR_SIZE_OVERFLOW; return 0; }
+                len = b + h + a->dim;
+            }
+            const uint64_t out = (uint64_t)a->batch * a->heads;
+            r[n++] = RGN("Query", a->q, len, a->q_dtype == FE2O3_DTYPE_F32 ? 4u : 2u, false);
+            r[n++] = RGN("Output", a->output, out * a->dim, a->output_dtype == FE2O3_DTYPE_F32 ? 4u : 2u, true);
+            if (a->lse.ptr || a->lse.len) r[n++] = RGN("LogSumExp", a->lse, out, 4, true);
+            return n;
         }
         case OP_DEVICE_SCAN_U32:
         case OP_DEVICE_SCAN_F32: {   // same block; elements are 4 bytes in both
@@ -1346,6 +1440,9 @@ DEFINE_CHECK(moe_gate_v1, OP_MOE_GATE)
 DEFINE_CHECK(moe_route_weights_v1, OP_MOE_ROUTE_WEIGHTS)
 DEFINE_CHECK(moe_expert_ffn_v1, OP_MOE_EXPERT_FFN)
 DEFINE_CHECK(moe_expert_combine_v1, OP_MOE_COMBINE)
+DEFINE_CHECK(kv_cache_append_v1, OP_KV_APPEND)
+DEFINE_CHECK(kv_cache_read_v1, OP_KV_READ)
+DEFINE_CHECK(paged_attention_v1, OP_PAGED_ATTENTION)
 DEFINE_CHECK(masked_reduce_u32, OP_MASKED_REDUCE)
 DEFINE_CHECK(masked_reduce_u32_packed, OP_MASKED_REDUCE_PACKED)
 DEFINE_CHECK(device_scan_u32, OP_DEVICE_SCAN_U32)
@@ -1369,6 +1466,9 @@ DEFINE_SIMPLE_PREPARE(moe_top2_v1, OP_MOE_TOP2)
 DEFINE_SIMPLE_PREPARE(moe_gate_v1, OP_MOE_GATE)
 DEFINE_SIMPLE_PREPARE(moe_route_weights_v1, OP_MOE_ROUTE_WEIGHTS)
 DEFINE_SIMPLE_PREPARE(moe_expert_combine_v1, OP_MOE_COMBINE)
+DEFINE_SIMPLE_PREPARE(kv_cache_append_v1, OP_KV_APPEND)
+DEFINE_SIMPLE_PREPARE(kv_cache_read_v1, OP_KV_READ)
+DEFINE_SIMPLE_PREPARE(paged_attention_v1, OP_PAGED_ATTENTION)
 DEFINE_SIMPLE_PREPARE(masked_reduce_u32, OP_MASKED_REDUCE)
 DEFINE_SIMPLE_PREPARE(masked_reduce_u32_packed, OP_MASKED_REDUCE_PACKED)
 DEFINE_SIMPLE_PREPARE(device_scan_u32, OP_DEVICE_SCAN_U32)

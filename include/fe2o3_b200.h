@@ -420,6 +420,67 @@ typedef struct fe2o3_moe_ep_ffn_v1_args {
     uint32_t tokens, d_model, d_ff, experts, world, rank, epoch, max_rows, spin_limit, reserved;
 } fe2o3_moe_ep_ffn_v1_args;
 
+/* ---- paged key-value cache (no counterpart in the reference, which has prompt attention only) ----
+ * For serving: the keys and values of every token so far, and the attention of one new token a sequence.
+ *
+ * The cache is two arrays, k_cache and v_cache, [pages][kv_heads][page_size][dim]: the rows of one head in
+ * one page are contiguous.  Position p of sequence b is slot p % page_size of page
+ * page_table[b * table_width + p / page_size]; only the entries that lengths[b] reaches are read.  Pages may
+ * be shared by sequences that only read them.  `format` says what an element is:
+ *   FE2O3_KV_BF16   bfloat16 (u16); k_scales and v_scales are empty
+ *   FE2O3_KV_E4M3   8-bit floating point, four exponent and three mantissa bits (u8)
+ *   FE2O3_KV_I8     8-bit integers, -127 .. 127
+ * 8-bit elements stand for code * scale, one f32 scale a row: k_scales and v_scales are
+ * [pages][kv_heads][page_size].  For a row x and the format's largest code C (448 and 127):
+ *   scale = max |x| / C, code = x / scale rounded to the nearest code, ties to even,
+ * both quotients rounded to f32; a row of zeros has scale 0, a row with an infinity or a NaN has scale NaN and
+ * reads back as NaN.  bf16 elements are rounded to nearest even.
+ * dim is a multiple of 16 up to 256, page_size any number from 1; both caches start on 16 bytes.
+ *
+ * Device-side reports (the host sees neither lengths nor page numbers): a sequence whose length its row of the page table
+ * cannot hold, or that has more new tokens than positions, is FE2O3_KSTATUS_LENGTH and is left out (its
+ * outputs are not written); a page number outside the cache is FE2O3_KSTATUS_SLOT_RANGE: rows there are not
+ * written, and count as zeros where they are read. */
+#define FE2O3_KV_BF16 0u
+#define FE2O3_KV_E4M3 1u
+#define FE2O3_KV_I8 2u
+
+/* Writes new tokens into the cache.  Rows token_offsets[b] .. token_offsets[b + 1] - 1 of k and v belong to
+ * sequence b and go to its last positions before lengths[b] (lengths count the new tokens); without
+ * token_offsets (empty slice) row b is sequence b's one new token, and tokens == batch.  Row (t, h) starts at
+ * element t * token_stride + h * head_stride; k and v hold (tokens - 1) * token_stride +
+ * (kv_heads - 1) * head_stride + dim elements.  No two new tokens may share a slot. */
+typedef struct fe2o3_kv_cache_append_v1_args {
+    fe2o3_slice k, v, page_table, lengths, token_offsets, k_cache, v_cache, k_scales, v_scales;
+    uint32_t tokens, batch, kv_heads, dim, page_size, table_width;
+    uint32_t k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+    uint32_t input_dtype, format;
+} fe2o3_kv_cache_append_v1_args;
+
+/* Reads rows back into contiguous storage: the same rows, positions and strides as the append, in the
+ * other direction.  code * scale is rounded once to f32, and once more for a bf16 output.  Rows of one output may not overlap. */
+typedef struct fe2o3_kv_cache_read_v1_args {
+    fe2o3_slice k_cache, v_cache, k_scales, v_scales, page_table, lengths, token_offsets, k, v;
+    uint32_t tokens, batch, kv_heads, dim, page_size, table_width;
+    uint32_t k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+    uint32_t output_dtype, format;
+} fe2o3_kv_cache_read_v1_args;
+
+/* Attention of one new token a sequence over its cached positions [max(0, n - window), n), n = lengths[b]
+ * (window 0: all of them):
+ *   output[b][h] = sum_j softmax_j(scale * q[b][h] . k_j) v_j,   lse[b][h] = log sum_j exp(scale * q[b][h] . k_j)
+ * with the keys and values of head h / (heads / kv_heads).  heads is a multiple of kv_heads.  q row (b, h) starts at
+ * element b * q_stride + h * q_head_stride; output [batch][heads][dim] is packed, f32 or bf16; lse
+ * [batch][heads] f32 is optional.  A sequence of length 0 gives zeros and -inf.  Sums, maxima and
+ * probabilities are f32 (for a bf16 output the probabilities have 16 significant bits).  The result does not
+ * depend on which blocks finish first.  One launch of a prepared object at a time (it owns a workspace). */
+typedef struct fe2o3_paged_attention_v1_args {
+    fe2o3_slice q, k_cache, v_cache, k_scales, v_scales, page_table, lengths, output, lse;
+    uint32_t batch, heads, kv_heads, dim, page_size, table_width, q_stride, q_head_stride;
+    float scale;
+    uint32_t window, q_dtype, output_dtype, format, reserved;
+} fe2o3_paged_attention_v1_args;
+
 /* examples/moe_expert_v1/src/kernel.rs:104-109
  * moe_expert_combine_f32_t8_k2_o16_v1(compact_output, inverse, route_weights,
  * combined_output) generalised to tokens x width. */
@@ -523,6 +584,9 @@ int32_t fe2o3_moe_grouped_ffn_v1_check(const fe2o3_moe_grouped_ffn_v1_args *args
 int32_t fe2o3_moe_expert_ffn_combine_v1_check(const fe2o3_moe_expert_ffn_combine_v1_args *args);
 int32_t fe2o3_moe_ep_exchange_v1_check(const fe2o3_moe_ep_exchange_v1_args *args);
 int32_t fe2o3_moe_ep_ffn_v1_check(const fe2o3_moe_ep_ffn_v1_args *args);
+int32_t fe2o3_kv_cache_append_v1_check(const fe2o3_kv_cache_append_v1_args *args);
+int32_t fe2o3_kv_cache_read_v1_check(const fe2o3_kv_cache_read_v1_args *args);
+int32_t fe2o3_paged_attention_v1_check(const fe2o3_paged_attention_v1_args *args);
 int32_t fe2o3_masked_reduce_u32_check(const fe2o3_masked_reduce_u32_args *args);
 int32_t fe2o3_masked_reduce_u32_packed_check(const fe2o3_masked_reduce_u32_packed_args *args);
 int32_t fe2o3_device_scan_u32_check(const fe2o3_device_scan_u32_args *args);
@@ -561,6 +625,9 @@ int32_t fe2o3_moe_expert_ffn_combine_v1_prepare(fe2o3_ctx *ctx, const fe2o3_moe_
 int32_t fe2o3_moe_ep_exchange_v1_prepare(fe2o3_ctx *ctx, const fe2o3_moe_ep_exchange_v1_args *args,
                                          fe2o3_prepared **out);
 int32_t fe2o3_moe_ep_ffn_v1_prepare(fe2o3_ctx *ctx, const fe2o3_moe_ep_ffn_v1_args *args, fe2o3_prepared **out);
+int32_t fe2o3_kv_cache_append_v1_prepare(fe2o3_ctx *ctx, const fe2o3_kv_cache_append_v1_args *args, fe2o3_prepared **out);
+int32_t fe2o3_kv_cache_read_v1_prepare(fe2o3_ctx *ctx, const fe2o3_kv_cache_read_v1_args *args, fe2o3_prepared **out);
+int32_t fe2o3_paged_attention_v1_prepare(fe2o3_ctx *ctx, const fe2o3_paged_attention_v1_args *args, fe2o3_prepared **out);
 int32_t fe2o3_masked_reduce_u32_prepare(fe2o3_ctx *ctx, const fe2o3_masked_reduce_u32_args *args,
                                         fe2o3_prepared **out);
 int32_t fe2o3_masked_reduce_u32_packed_prepare(fe2o3_ctx *ctx, const fe2o3_masked_reduce_u32_packed_args *args,

@@ -1,0 +1,113 @@
+"""Admission of the paged key-value cache's operators: pure host checks, no GPU."""
+import math
+
+import pytest
+
+import fe2o3_b200 as fe
+
+BASE = 0x7F0000000000
+
+
+def sl(megabyte, n, off=0):
+    return (BASE + (megabyte << 20) + off, n)
+
+
+def err(op, **kw):
+    with pytest.raises(fe.Fe2o3Error) as e:
+        fe.check_args(op, fe.make_args(op, **kw))
+    return e.value.name
+
+
+def cache(form=fe.KV_BF16, pages=10, kv_heads=2, dim=64, page=16, batch=3, width=4):
+    rows = pages * kv_heads * page
+    scales = (0, 0) if form == fe.KV_BF16 else None
+    return dict(k_cache=sl(0, rows * dim), v_cache=sl(8, rows * dim), k_scales=scales or sl(16, rows), v_scales=scales or sl(17, rows),
+                page_table=sl(18, batch * width), lengths=sl(19, batch), batch=batch, kv_heads=kv_heads, dim=dim, page_size=page,
+                table_width=width, format=form)
+
+
+def rows(tokens=3, kv_heads=2, dim=64):
+    n = tokens * kv_heads * dim
+    return dict(k=sl(24, n), v=sl(32, n), tokens=tokens, k_token_stride=kv_heads * dim, k_head_stride=dim, v_token_stride=kv_heads * dim,
+                v_head_stride=dim)
+
+
+def queries(batch=3, heads=4, dim=64):
+    n = batch * heads * dim
+    return dict(q=sl(40, n), output=sl(48, n), lse=sl(56, batch * heads), heads=heads, q_stride=heads * dim, q_head_stride=dim, scale=0.125,
+                window=0, q_dtype=fe.DTYPE_BF16, output_dtype=fe.DTYPE_F32)
+
+
+def ok(op, **kw):
+    fe.check_args(op, fe.make_args(op, **kw))
+
+
+ALL = [("kv_cache_append_v1", rows), ("kv_cache_read_v1", rows), ("paged_attention_v1", queries)]
+
+
+@pytest.mark.parametrize("op,more", ALL)
+@pytest.mark.parametrize("form", [fe.KV_BF16, fe.KV_E4M3, fe.KV_I8])
+def test_the_cache(op, more, form):
+    kw = {**cache(form), **more()}
+    ok(op, **kw)
+    for bad in (dict(dim=0), dict(dim=24), dict(dim=272), dict(kv_heads=0), dict(page_size=0), dict(format=3),
+                dict(kv_heads=1 << 20, page_size=1 << 20)):
+        assert err(op, **{**kw, **bad}) == "UnsupportedShape", bad
+    assert err(op, **{**kw, "k_cache": sl(0, 10 * 2 * 16 * 64, 8)}) == "Alignment"
+    assert err(op, **{**kw, "v_cache": sl(8, 10 * 2 * 16 * 64, 2)}) == "Alignment"
+    assert err(op, **{**kw, "k_cache": sl(0, 10 * 2 * 16 * 64 - 1)}) == "Length"       # not whole pages
+    assert err(op, **{**kw, "v_cache": sl(8, 9 * 2 * 16 * 64)}) == "Length"
+    assert err(op, **{**kw, "k_cache": (0, 10 * 2 * 16 * 64)}) == "NullAddress"
+    assert err(op, **{**kw, "k_scales": sl(16, 5)}) == "Length"                         # none for bf16, one a row otherwise
+    assert err(op, **{**kw, "page_table": sl(18, 11)}) == "Length"
+    assert err(op, **{**kw, "lengths": sl(19, 4)}) == "Length"
+    assert err(op, **{**kw, "lengths": sl(19, 3, 2)}) == "Alignment"
+
+
+@pytest.mark.parametrize("op", ["kv_cache_append_v1", "kv_cache_read_v1"])
+def test_rows_of_new_tokens(op):
+    kw = {**cache(), **rows()}
+    dtype = "input_dtype" if op == "kv_cache_append_v1" else "output_dtype"
+    assert err(op, **{**kw, dtype: 2}) == "UnsupportedShape"
+    assert err(op, **{**kw, **rows(4)}) == "UnsupportedShape"                            # one token a sequence without offsets
+    more = {**kw, **rows(4), "token_offsets": sl(20, 4)}
+    ok(op, **more)
+    assert err(op, **{**more, "token_offsets": sl(20, 3)}) == "Length"
+    assert err(op, **{**kw, "k": sl(24, 3 * 2 * 64 - 1)}) == "Length"
+    assert err(op, **{**kw, "k": sl(24, 3 * 2 * 64, 1), dtype: 1}) == "Alignment"
+    assert err(op, **{**kw, "k": sl(24, 3 * 2 * 64, 2), dtype: 0}) == "Alignment"
+    ok(op, **{**kw, "k": sl(24, 3 * 2 * 64, 2), dtype: 1})
+    # strided rows: (tokens - 1) * token_stride + (kv_heads - 1) * head_stride + dim elements
+    ok(op, **{**kw, "k": sl(24, 2 * 1000 + 100 + 64), "k_token_stride": 1000, "k_head_stride": 100})
+    ok(op, **{**kw, "k": sl(24, 2 * 64 + 500 + 64), "k_token_stride": 64, "k_head_stride": 500})
+    overlapping = {**kw, "v": sl(32, 2 * 60 + 500 + 64), "v_token_stride": 60, "v_head_stride": 500}
+    if op == "kv_cache_append_v1":
+        ok(op, **overlapping)
+    else:
+        assert err(op, **overlapping) == "UnsupportedShape"
+    empty = {**cache(batch=0), **rows(0)}
+    ok(op, **empty)
+    # what is written lies apart from what is read
+    inside = {**kw, "k": sl(0, 3 * 2 * 64, 4096)}
+    assert err(op, **inside) == "OutputAliasesInput"
+    assert err(op, **{**kw, "v_cache": sl(0, 10 * 2 * 16 * 64)}) == "OutputAliasesInput" if op == "kv_cache_append_v1" else True
+
+
+def test_attention_arguments():
+    kw = {**cache(), **queries()}
+    op = "paged_attention_v1"
+    for bad in (dict(heads=0), dict(heads=3), dict(q_dtype=2), dict(output_dtype=2), dict(scale=math.nan), dict(scale=math.inf)):
+        assert err(op, **{**kw, **bad}) == "UnsupportedShape", bad
+    ok(op, **{**kw, "lse": None})
+    ok(op, **{**kw, "scale": -3.0, "window": 0xffffffff})
+    assert err(op, **{**kw, "lse": sl(56, 11)}) == "Length"
+    assert err(op, **{**kw, "q": sl(40, 3 * 4 * 64 + 1)}) == "Length"
+    assert err(op, **{**kw, "output": sl(48, 3 * 4 * 64 - 1)}) == "Length"
+    ok(op, **{**kw, "q": sl(40, 64), "q_stride": 0, "q_head_stride": 0})
+    ok(op, **{**kw, "q": sl(40, 2 * 5000 + 3 * 70 + 64), "q_stride": 5000, "q_head_stride": 70})
+    assert err(op, **{**kw, "output": sl(40, 3 * 4 * 64)}) == "OutputAliasesInput"
+    assert err(op, **{**kw, "output": sl(48, 3 * 4 * 64), "lse": sl(48, 12)}) == "OutputAliasesInput"
+    assert err(op, **{**kw, "output": sl(0, 3 * 4 * 64)}) == "OutputAliasesInput"
+    big = cache(batch=1 << 20, width=0)
+    many = {**big, "lengths": sl(64, 1 << 20), "page_table": (0, 0), "heads": 4096, "kv_heads": 2, "scale": 1.0}
+    assert err(op, **many) == "UnsupportedShape"
