@@ -37,7 +37,6 @@ int32_t launch_moe_combine(fe2o3_ctx *, cudaStream_t, const void *, fe2o3_geomet
 int32_t launch_moe_ep_exchange(fe2o3_ctx *, cudaStream_t, const void *, fe2o3_geometry *, bool);
 int32_t launch_kv_cache_append(fe2o3_ctx *, cudaStream_t, const void *, fe2o3_geometry *, bool);
 int32_t launch_kv_cache_read(fe2o3_ctx *, cudaStream_t, const void *, fe2o3_geometry *, bool);
-int32_t launch_paged_attention(fe2o3_ctx *, cudaStream_t, const void *, fe2o3_geometry *, bool);
 int32_t launch_moe_compact(cudaStream_t, uint64_t x, uint64_t perm, uint64_t compact_x, uint32_t rows,
                            uint32_t d_model, uint32_t tokens);
 int32_t launch_gemm_exact(fe2o3_ctx *, cudaStream_t, uint32_t dtype, bool epilogue, uint64_t a, uint64_t b, uint64_t c, uint32_t M,
@@ -63,6 +62,11 @@ int32_t attention_split_launch(const AttnSplitPlan *, cudaStream_t);
 void attention_split_geometry(const AttnSplitPlan *, fe2o3_geometry *);
 void attention_split_free(AttnSplitPlan *);
 int32_t attention_split_init_device();
+struct PagedPlan;
+int32_t paged_attention_plan(fe2o3_ctx *, const fe2o3_paged_attention_v1_args *, PagedPlan **);
+int32_t paged_attention_launch(const PagedPlan *, cudaStream_t);
+void paged_attention_geometry(const PagedPlan *, fe2o3_geometry *);
+void paged_attention_free(PagedPlan *);
 int32_t moe_gate_init_device();
 int32_t gemm_exact_init_device();
 int32_t device_scan_init_device();
@@ -139,7 +143,7 @@ static const OpInfo kOps[OP_COUNT] = {
     {"moe_expert_ffn_combine_v1", sizeof(fe2o3_moe_expert_ffn_combine_v1_args), nullptr},
     {"kv_cache_append_v1", sizeof(fe2o3_kv_cache_append_v1_args), launch_kv_cache_append},
     {"kv_cache_read_v1", sizeof(fe2o3_kv_cache_read_v1_args), launch_kv_cache_read},
-    {"paged_attention_v1", sizeof(fe2o3_paged_attention_v1_args), launch_paged_attention},
+    {"paged_attention_v1", sizeof(fe2o3_paged_attention_v1_args), nullptr},
 };
 
 struct fe2o3_prepared {
@@ -150,6 +154,7 @@ struct fe2o3_prepared {
     GemmTcPlan gemm[2];  // tcgen05 plans (FFN uses both)
     AttnTcPlan *attn;    // head size 64
     AttnSplitPlan *attn_split;   // the other head sizes the tensor cores take
+    PagedPlan *paged;
     void *scratch[2];    // device workspace owned by the prepared object (split bf16 operands of the f32 GEMM)
     fe2o3_geometry geo;
 };
@@ -794,6 +799,7 @@ int32_t prepare_common(fe2o3_ctx *ctx, uint32_t op, const void *args, fe2o3_prep
     p->op = op;
     p->attn = nullptr;
     p->attn_split = nullptr;
+    p->paged = nullptr;
     p->scratch[0] = p->scratch[1] = nullptr;
     p->schedule = 0;
     memset(p->kernarg, 0, sizeof p->kernarg);
@@ -836,6 +842,7 @@ int32_t launch_prepared(fe2o3_prepared *p, cudaStream_t s) {
             return launch_attention_simt(ctx, s, reinterpret_cast<const fe2o3_flash_attention_v1_args *>(p->kernarg),
                                          nullptr, false);
         }
+        case OP_PAGED_ATTENTION: return paged_attention_launch(p->paged, s);
         case OP_MOE_EXPERT_FFN: {
             const fe2o3_moe_expert_ffn_v1_args *a = reinterpret_cast<const fe2o3_moe_expert_ffn_v1_args *>(p->kernarg);
             const uint32_t rows = (uint32_t)(a->compact_output.len / a->d_model);
@@ -1468,7 +1475,6 @@ DEFINE_SIMPLE_PREPARE(moe_route_weights_v1, OP_MOE_ROUTE_WEIGHTS)
 DEFINE_SIMPLE_PREPARE(moe_expert_combine_v1, OP_MOE_COMBINE)
 DEFINE_SIMPLE_PREPARE(kv_cache_append_v1, OP_KV_APPEND)
 DEFINE_SIMPLE_PREPARE(kv_cache_read_v1, OP_KV_READ)
-DEFINE_SIMPLE_PREPARE(paged_attention_v1, OP_PAGED_ATTENTION)
 DEFINE_SIMPLE_PREPARE(masked_reduce_u32, OP_MASKED_REDUCE)
 DEFINE_SIMPLE_PREPARE(masked_reduce_u32_packed, OP_MASKED_REDUCE_PACKED)
 DEFINE_SIMPLE_PREPARE(device_scan_u32, OP_DEVICE_SCAN_U32)
@@ -1529,6 +1535,14 @@ int32_t fe2o3_flash_attention_v1_prepare(fe2o3_ctx *ctx, const fe2o3_flash_atten
         return FE2O3_OK;
     }
     return launch_attention_simt(ctx, nullptr, a, &(*out)->geo, true);
+}
+int32_t fe2o3_paged_attention_v1_prepare(fe2o3_ctx *ctx, const fe2o3_paged_attention_v1_args *a, fe2o3_prepared **out) {
+    int32_t st = prepare_common(ctx, OP_PAGED_ATTENTION, a, out);
+    if (st != FE2O3_OK) return st;
+    st = paged_attention_plan(ctx, a, &(*out)->paged);
+    if (st != FE2O3_OK) return fail_prepare(out, st);
+    paged_attention_geometry((*out)->paged, &(*out)->geo);
+    return FE2O3_OK;
 }
 int32_t fe2o3_moe_expert_ffn_v1_prepare(fe2o3_ctx *ctx, const fe2o3_moe_expert_ffn_v1_args *a, fe2o3_prepared **out) {
     int32_t st = prepare_common(ctx, OP_MOE_EXPERT_FFN, a, out);
@@ -1731,6 +1745,7 @@ int32_t fe2o3_prepared_destroy(fe2o3_prepared *p) {
     if (!p) return FE2O3_OK;
     if (p->attn) attention_tc_free(p->attn);
     if (p->attn_split) attention_split_free(p->attn_split);
+    paged_attention_free(p->paged);
     // the workspace may still be read by a launch in flight: freeing synchronises with the device (cudaFree does)
     for (void *w : p->scratch)
         if (w) cudaFree(w);
@@ -1824,6 +1839,7 @@ int32_t fe2o3_launch_and_wait(fe2o3_executable *exe, uint32_t kernel_id, const f
         case OP_TILED_GEMM: st = fe2o3_tiled_gemm_v1_prepare(exe->ctx, (const fe2o3_tiled_gemm_v1_args *)kernarg, FE2O3_GEMM_SCHEDULE_AUTO, &p); break;
         case OP_TILED_GEMM_GENERAL: st = fe2o3_tiled_gemm_general_v1_prepare(exe->ctx, (const fe2o3_tiled_gemm_general_v1_args *)kernarg, FE2O3_GEMM_SCHEDULE_AUTO, &p); break;
         case OP_FLASH_ATTENTION: st = fe2o3_flash_attention_v1_prepare(exe->ctx, (const fe2o3_flash_attention_v1_args *)kernarg, &p); break;
+        case OP_PAGED_ATTENTION: st = fe2o3_paged_attention_v1_prepare(exe->ctx, (const fe2o3_paged_attention_v1_args *)kernarg, &p); break;
         case OP_MOE_EXPERT_FFN: st = fe2o3_moe_expert_ffn_v1_prepare(exe->ctx, (const fe2o3_moe_expert_ffn_v1_args *)kernarg, &p); break;
         case OP_MOE_COMPACT: st = fe2o3_moe_compact_v1_prepare(exe->ctx, (const fe2o3_moe_compact_v1_args *)kernarg, &p); break;
         case OP_MOE_GROUPED_FFN: st = fe2o3_moe_grouped_ffn_v1_prepare(exe->ctx, (const fe2o3_moe_grouped_ffn_v1_args *)kernarg, &p); break;

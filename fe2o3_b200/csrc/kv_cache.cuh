@@ -30,8 +30,10 @@ static inline KvCache kv_cache_of(const fe2o3_ctx *ctx, const Args *a) {
                    ctx->status_word};
 }
 
-// Whether a sequence of n positions fits its row of the page table.
-__device__ __forceinline__ bool kv_fits(const KvCache &c, uint32_t n) { return n <= (uint64_t)c.table_width * c.page_size; }
+// Whether a sequence of n positions fits its row of the page table (and 31 bits).
+__device__ __forceinline__ bool kv_fits(const KvCache &c, uint32_t n) {
+    return n <= 0x7fffffffu && n <= (uint64_t)c.table_width * c.page_size;
+}
 
 // Row number of (sequence, head, position); ~0 and a report where the table names a page outside the cache.
 // The table's entry is read only for positions that fit it.
