@@ -367,7 +367,7 @@ int kv_cache_regions(const Args *a, Region *r, int n, bool writes, int32_t *stat
         return 0;
     }
     const uint64_t page = rows * a->dim, pages = a->k_cache.len / page;
-    if (pages > 0xffffffffu) { *status = unsupported("page numbers are u32"); return 0; }
+    if (pages > 0xffffffffull / rows) { *status = unsupported("a key-value cache has fewer than 2^32 rows"); return 0; }
     if ((a->k_cache.ptr | a->v_cache.ptr) & 15u) {
         fe2o3_set_error("Alignment{role=%s}: the caches start on 16 bytes", a->k_cache.ptr & 15u ? "KeyCache" : "ValueCache");
         *status = FE2O3_ERR_ALIGNMENT;

@@ -48,8 +48,8 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(KvCache c, KvRows r
     if (!place_of(c, r, t, b, position)) return;
     for (uint32_t w = threadIdx.x >> 5; w < 2 * c.kv_heads; w += kThreads / 32) {
         const uint32_t side = w & 1, h = w >> 1;
-        const uint64_t row = kv_row(c, b, h, position);
-        if (row == ~0ull) continue;
+        const uint32_t row = kv_row(c, b, h, position);
+        if (row == ~0u) continue;
         const uint64_t from = (uint64_t)t * r.token_stride[side] + (uint64_t)h * r.head_stride[side];
         float x[8], top = 0.f;
         bool finite = true;
@@ -61,7 +61,7 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(KvCache c, KvRows r
             finite = finite && isfinite(x[i]);
             top = fmaxf(top, fabsf(x[i]));
         }
-        uint8_t *to = (side ? c.v : c.k) + row * c.dim * kKvBytes<FORMAT>;
+        uint8_t *to = (side ? c.v : c.k) + (uint64_t)row * c.dim * kKvBytes<FORMAT>;
         if constexpr (FORMAT == FE2O3_KV_BF16) {
             for (uint32_t i = 0; i < 8; ++i)
                 if (lane + 32 * i < c.dim) reinterpret_cast<uint16_t *>(to)[lane + 32 * i] = f32_to_bf16_bits(x[i]);
@@ -87,12 +87,12 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(KvCache c, KvRows r) 
     if (!place_of(c, r, t, b, position)) return;
     for (uint32_t w = threadIdx.x >> 5; w < 2 * c.kv_heads; w += kThreads / 32) {
         const uint32_t side = w & 1, h = w >> 1;
-        const uint64_t row = kv_row(c, b, h, position);
+        const uint32_t row = kv_row(c, b, h, position);
         const uint64_t to = (uint64_t)t * r.token_stride[side] + (uint64_t)h * r.head_stride[side];
-        const uint8_t *from = (side ? c.v : c.k) + (row == ~0ull ? 0 : row) * c.dim * kKvBytes<FORMAT>;
-        const float scale = FORMAT == FE2O3_KV_BF16 ? 1.f : row == ~0ull ? 0.f : (side ? c.v_scales : c.k_scales)[row];
+        const uint8_t *from = (side ? c.v : c.k) + (uint64_t)(row == ~0u ? 0 : row) * c.dim * kKvBytes<FORMAT>;
+        const float scale = FORMAT == FE2O3_KV_BF16 ? 1.f : row == ~0u ? 0.f : (side ? c.v_scales : c.k_scales)[row];
         for (uint32_t i = lane; i < c.dim; i += 32) {
-            const float v = row == ~0ull ? 0.f : __fmul_rn(kv_element<FORMAT>(from, i), scale);
+            const float v = row == ~0u ? 0.f : __fmul_rn(kv_element<FORMAT>(from, i), scale);
             if (r.f32) static_cast<float *>(r.p[side])[to + i] = v;
             else static_cast<uint16_t *>(r.p[side])[to + i] = f32_to_bf16_bits(v);
         }

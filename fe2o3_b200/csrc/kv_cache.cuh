@@ -36,15 +36,15 @@ __device__ __forceinline__ bool kv_fits(const KvCache &c, uint32_t n) {
 }
 
 // Row number of (sequence, head, position); ~0 and a report where the table names a page outside the cache.
-// The table's entry is read only for positions that fit it.
-__device__ __forceinline__ uint64_t kv_row(const KvCache &c, uint32_t b, uint32_t h, uint32_t position) {
-    const uint32_t in_table = position / c.page_size, slot = position - in_table * c.page_size;
+// `shift`: log2 of the page size, or negative.
+__device__ __forceinline__ uint32_t kv_row(const KvCache &c, uint32_t b, uint32_t h, uint32_t position, int32_t shift = -1) {
+    const uint32_t in_table = shift >= 0 ? position >> shift : position / c.page_size, slot = position - in_table * c.page_size;
     const uint32_t page = c.page_table[(uint64_t)b * c.table_width + in_table];
     if (page >= c.pages) {
         kstatus_set(c.status, FE2O3_KSTATUS_SLOT_RANGE);
-        return ~0ull;
+        return ~0u;
     }
-    return ((uint64_t)page * c.kv_heads + h) * c.page_size + slot;
+    return (page * c.kv_heads + h) * c.page_size + slot;
 }
 
 // Exact value of an e4m3 code (both formats are halves of f16's range).

@@ -1,0 +1,959 @@
+// Attention of one new token a sequence over a paged key-value cache: the kernel (paged_attention.cu plans and
+// launches it, one source a format builds it); the formulas stand at fe2o3_paged_attention_v1_args.
+//
+// HBM-bound: the K and V rows of a (sequence, key head) are read once, for all query heads that share them (4 * group
+// flop a byte of a bf16 cache, 8 * group of an 8-bit one).
+//   Work.  An item is a (sequence, key head, up to 8 * NT query heads); its keys fall into tiles of KT.  The tiles of all
+//   items form one line, an item's behind kEnd places that stand for what its end costs, and the line is cut into equal
+//   shares, one a warp: the lengths are known on the device only, and a launch is the same whatever they are.  A warp
+//   writes the results of items that lie in its share by itself.  Others meet twice: the warps of a block when all
+//   have done their share, through shared memory, and the blocks in the workspace, where the one that comes last to an
+//   item (a counter) joins the pieces.  Both go by the pieces' order: the same bits whoever is last.
+//   Tiles.  Each warp has a ring of stages of its own, filled by 16-byte asynchronous copies row by row through the
+//   page table (any page size; rows outside the sequence are filled with zeros and never read), so that nothing but
+//   its own copies stops a warp.  It keeps the maximum, the sum and the output of what it has seen (one pass, f32).
+//   Products.  mma.sync with the keys (and then the output's columns) as rows and the query heads as columns: of
+//   the 8 columns of a tile few are wasted for small groups, and P is turned into an operand by movmatrix.  The
+//   tensor unit's own sums span one tile, longer ones are f32 additions.  A bf16 cache is multiplied as it is, with the
+//   probabilities as three bf16 terms that add up to the f32 value exactly (two for a bf16 output) and an f32 query as
+//   three as well.  Terms are cut off, not rounded, and held above 0, so that an infinity in V stays one.  8-bit
+//   codes become f16 exactly; the probabilities then carry the row's scale, against a power of two that follows the
+//   largest scale seen, and are two f16 terms (22 bits); queries are brought to f16's range by a power of two a row.
+#pragma once
+#include "kv_cache.cuh"
+
+constexpr int kPagedWarps = 4, kPagedThreads = 32 * kPagedWarps;
+
+struct PagedArgs {
+    KvCache c;
+    const void *q;
+    void *o;
+    float *lse;
+    float4 *slots;        // kPagedSlots partial results a block
+    uint32_t *arrived;    // pieces that have come in, by the block where the item begins; zero between launches
+    uint32_t group, chunks, q_stride, q_head_stride, window, stages;
+    int32_t page_shift;   // log2 of page_size, or -1
+    float scale;
+    bool q_f32, o_f32, q_whole;   // q_whole: rows of the queries start on 16 bytes
+};
+// Of a block in the workspace: the end of an item that began in an earlier block; the ends that its warps 1 to 3 found of
+// items that began in an earlier warp; the beginning of an item that goes on in the next block.
+constexpr uint32_t kPagedSlots = 5, kSlotFirst = 0, kSlotLast = 4;
+
+using PagedKernel = void (*)(PagedArgs);
+struct PagedBuild {
+    PagedKernel kernel;
+    uint32_t stage, part, query;   // bytes: a stage of one warp, a partial result, one term of the queries of one warp
+};
+PagedBuild paged_build_bf16(uint32_t dim, uint32_t nt);
+PagedBuild paged_build_e4m3(uint32_t dim, uint32_t nt);
+PagedBuild paged_build_i8(uint32_t dim, uint32_t nt);
+
+namespace {
+
+constexpr int kQueryExponent = 14;   // f16 queries: the largest of a row lies in [2^14, 2^15)
+
+
+template <uint32_t FORMAT, int DP, int NT>
+struct Shape {
+    static constexpr bool kF16 = FORMAT != FE2O3_KV_BF16;
+    static constexpr int kRow = DP * (kF16 ? 1 : 2);                                        // bytes of a row in a stage
+    static constexpr int kKeys = kF16 ? (DP == 256 ? 16 : 32) : (DP == 64 ? 32 : 16);       // of a tile
+    static constexpr int kStage = 2 * kKeys * kRow + (kF16 ? 8 * kKeys : 0);                // K, V, their scales
+    static constexpr int kHeads = 8 * NT;
+    static constexpr int kQueryRow = 2 * DP + 16;                                           // bytes, padded against bank conflicts
+    static constexpr int kPart = (DP / 16 + 1) * NT;                                        // float4 a lane of a partial result
+};
+
+__device__ __forceinline__ void copy16(uint32_t to, const void *from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copy16(uint32_t to, const void *from, bool there) {   // or zeros
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16u : 0u) : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t to, const void *from, bool there) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(there ? 4u : 0u) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// All but the youngest `behind` groups of this thread's copies have landed.
+__device__ __forceinline__ void copies_wait(uint32_t behind) {
+    if (behind == 2) asm volatile("cp.async.wait_group 2;" ::: "memory");
+    else if (behind == 1) asm volatile("cp.async.wait_group 1;" ::: "memory");
+    else if (behind == 3) asm volatile("cp.async.wait_group 3;" ::: "memory");
+    else asm volatile("cp.async.wait_group 0;" ::: "memory");
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void ldsm4_trans(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ uint4 lds128(uint32_t at) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t at) {
+    uint2 v;
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ float lds_f32(uint32_t at) {
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+    return v;
+}
+// The 8x8 matrix of 16-bit values that a warp holds (row lane / 4, columns 2 (lane % 4) and the next), transposed.
+__device__ __forceinline__ uint32_t turned(uint32_t v) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+template <bool F16>
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (F16)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// The same with nothing to add to.
+template <bool F16>
+__device__ __forceinline__ void mma_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (F16)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+                     : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+                     : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+__device__ __forceinline__ uint32_t f16_pair(float lo, float hi) {   // both rounded to nearest even
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ float2 f16_values(uint32_t p) {
+    float2 r;
+    asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\tcvt.f32.f16 %0, lo;\n\tcvt.f32.f16 %1, hi;\n\t}" : "=f"(r.x), "=f"(r.y) : "r"(p));
+    return r;
+}
+__device__ __forceinline__ float cut_bf16(float v) { return __uint_as_float(__float_as_uint(v) & 0xffff0000u); }
+__device__ __forceinline__ uint32_t bf16_pair_cut(float lo, float hi) { return __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x7632); }
+
+__device__ __forceinline__ uint16_t bf16_of(float v) {   // to nearest even
+    uint16_t r;
+    asm("cvt.rn.bf16.f32 %0, %1;" : "=h"(r) : "f"(v));
+    return r;
+}
+
+// Two 8-bit codes, byte BYTE of `a` and byte BYTE + STEP of `b`, as an f16 pair (both formats exactly).  With STEP 1, a and b are one word.
+template <uint32_t FORMAT, int BYTE, int STEP>
+__device__ __forceinline__ uint32_t codes_f16(uint32_t a, uint32_t b) {
+    if constexpr (FORMAT == FE2O3_KV_I8) {
+        // 1024 + (code + 128) has the code in its low bits: f16's step is 1 there
+        const uint32_t x = __byte_perm(a, b, BYTE | (4 + BYTE + STEP) << 8);
+        uint32_t r = (x & 0x00ff00ffu) ^ 0x64806480u;
+        asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(r) : "r"(0x64806480u));
+        return r;
+    } else {
+        const uint32_t x = STEP == 1 && BYTE == 0 ? a : __byte_perm(a, b, BYTE | (4 + BYTE + STEP) << 4);
+        uint32_t r;
+        asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(r) : "r"(x));
+        return r;
+    }
+}
+
+// Where 16-byte piece c of row r lies in a stage's K or V part.  Rows that the lanes of one shared-memory access touch
+// fall on different banks: 8 rows a matrix for ldmatrix; rows g, g + 1 (K) or 2t (V) for the 8-bit formats.
+template <uint32_t FORMAT, int DP, bool VALUES>
+__device__ __forceinline__ uint32_t piece_at(uint32_t r, uint32_t c) {
+    if constexpr (FORMAT == FE2O3_KV_BF16) return r * (2 * DP) + ((c ^ (r & 7)) << 4);
+    else if constexpr (DP == 64) return (r >> 1) * 128 + ((((r & 1) << 2 | c) ^ (r >> 1 & 3) << 1) << 4);
+    else return r * DP + ((c ^ (VALUES ? r & 6 : (r & 1) << 2)) << 4);
+}
+
+// Column of the output that row m of tile i of the second product stands for.
+template <uint32_t FORMAT, int DP>
+__device__ __forceinline__ uint32_t column_of(uint32_t i, uint32_t m) {
+    if constexpr (FORMAT == FE2O3_KV_BF16) return 16 * i + m;
+    else return (DP == 64 ? 8 * (m & 7) : 16 * (m & 7)) + (DP == 256 ? 128 * (i >> 3) + 2 * (i & 7) : 2 * i) + (m >> 3);
+}
+
+constexpr uint32_t kEnd = 1;     // places on the line in front of an item's tiles
+constexpr uint32_t kLeast = 3;   // places a warp has at least, where there are enough
+constexpr uint32_t kInvalid = ~0u;
+// What a warp's share ends in: whole items only; an item that begins in the share and goes on; one that goes on on both sides; no places.
+enum : uint32_t { kNone, kBegun, kWithin, kEmpty };
+struct Job {
+    uint32_t seq, item, n, block, pieces;   // pieces 0: none
+};
+struct Yes { static constexpr bool value = true; };
+struct No { static constexpr bool value = false; };
+// A sequence's keys as tiles.  One that does not fit its table is reported and has none.
+template <int KT>
+struct Span {
+    uint32_t first, n, tiles;
+    bool valid;
+    __device__ __forceinline__ Span() : first(0), n(0), tiles(0), valid(false) {}
+    __device__ __forceinline__ Span(const PagedArgs &a, uint32_t b) {
+        n = a.c.lengths[b];
+        valid = kv_fits(a.c, n);
+        if (!valid) {
+            kstatus_set(a.c.status, FE2O3_KSTATUS_LENGTH);
+            n = 0;
+        }
+        first = a.window && n > a.window ? n - a.window : 0;
+        tiles = (n - first + KT - 1) / KT;
+    }
+    __device__ __forceinline__ uint32_t places() const { return tiles + kEnd; }
+};
+
+// Running result of one warp over some of an item's keys: output columns (rows of tile i) by two heads a lane.
+template <int MD, int NT>
+struct Part {
+    float m[NT][2], l[NT][2], o[MD][NT][4];
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            m[t][0] = m[t][1] = -INFINITY;
+            l[t][0] = l[t][1] = 0.f;
+#pragma unroll
+            for (int i = 0; i < MD; ++i) o[i][t][0] = o[i][t][1] = o[i][t][2] = o[i][t][3] = 0.f;
+        }
+    }
+    // Adds another part, one float4 a lane at `at`, `at` + 32, ...
+    template <typename Load>
+    __device__ __forceinline__ void add(Load load) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const float4 ml = load(MD * NT + t);
+            const float om[2] = {ml.x, ml.y}, ol[2] = {ml.z, ml.w};
+            float keep[2], take[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const float top = fmaxf(m[t][e], om[e]), base = top == -INFINITY ? 0.f : top;
+                keep[e] = ex2_approx(m[t][e] - base);
+                take[e] = ex2_approx(om[e] - base);
+                l[t][e] = l[t][e] * keep[e] + ol[e] * take[e];
+                m[t][e] = top;
+            }
+#pragma unroll
+            for (int i = 0; i < MD; ++i) {
+                const float4 v = load(i * NT + t);
+                o[i][t][0] = o[i][t][0] * keep[0] + v.x * take[0];
+                o[i][t][1] = o[i][t][1] * keep[1] + v.y * take[1];
+                o[i][t][2] = o[i][t][2] * keep[0] + v.z * take[0];
+                o[i][t][3] = o[i][t][3] * keep[1] + v.w * take[1];
+            }
+        }
+    }
+    template <typename Store>
+    __device__ __forceinline__ void leave(Store store) const {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            store(MD * NT + t, make_float4(m[t][0], m[t][1], l[t][0], l[t][1]));
+#pragma unroll
+            for (int i = 0; i < MD; ++i) store(i * NT + t, make_float4(o[i][t][0], o[i][t][1], o[i][t][2], o[i][t][3]));
+        }
+    }
+};
+
+template <uint32_t FORMAT, int DP, int NT>
+__global__ void __launch_bounds__(kPagedThreads) paged_attention_kernel(const PagedArgs a) {
+    using S = Shape<FORMAT, DP, NT>;
+    using P = Part<DP / 16, NT>;
+    constexpr int KT = S::kKeys, MT = KT / 16, MD = DP / 16, kPieces = S::kRow / 16, kRowsAtOnce = 32 / kPieces;
+    constexpr bool F16 = S::kF16;
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ float head_scales[kPagedWarps][S::kHeads];
+    __shared__ uint32_t kinds[kPagedWarps], ends[kPagedWarps];
+    __shared__ Job jobs[2];
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t4 = lane & 3;
+    uint8_t *const my_ring = smem + warp * a.stages * S::kStage;
+    const uint32_t ring = smem_u32(my_ring);
+    const uint32_t terms = a.q_f32 ? (F16 ? 2 : 3) : 1;
+    uint8_t *const query = smem + kPagedWarps * a.stages * S::kStage + warp * terms * S::kHeads * S::kQueryRow;
+    const uint32_t query_s = smem_u32(query);
+    float *const head_scale = head_scales[warp];
+    const uint32_t row_bytes = a.c.dim * (F16 ? 1 : 2);
+    const uint32_t per_seq = a.c.kv_heads * a.chunks;   // items of a sequence
+
+    if (threadIdx.x < 2) jobs[threadIdx.x].pieces = 0;
+    if (a.c.dim < DP) {   // the columns past the head's: zeros, which no copy goes over
+        for (uint32_t i = lane; i < 2 * KT * a.stages * kPieces; i += 32) {
+            const uint32_t c = i % kPieces, row = i / kPieces, r = row % KT, side = row / KT % 2, stage = row / (2 * KT);
+            if (16 * c < row_bytes) continue;
+            const uint32_t at = stage * S::kStage + side * KT * S::kRow + (side ? piece_at<FORMAT, DP, true>(r, c) : piece_at<FORMAT, DP, false>(r, c));
+            *reinterpret_cast<uint4 *>(my_ring + at) = make_uint4(0, 0, 0, 0);
+        }
+    }
+    begin_after_previous();
+
+    // ---- this warp's share of the line: every warp adds up the sequences for itself ----
+    uint64_t total = 0;
+    constexpr uint32_t kHeld = 4;   // sequences a lane keeps the places of: one trip to memory for 128
+    uint32_t held[kHeld];
+#pragma unroll
+    for (uint32_t i = 0; i < kHeld; ++i) {
+        held[i] = 32 * i + lane < a.c.batch ? Span<KT>(a, 32 * i + lane).places() : 0;
+        total += held[i];
+    }
+    for (uint32_t b = 32 * kHeld + lane; b < a.c.batch; b += 32) total += Span<KT>(a, b).places();
+#pragma unroll
+    for (int d = 16; d; d >>= 1) total += __shfl_xor_sync(~0u, total, d);
+    total *= per_seq;
+    const uint64_t wanted = (total + kLeast * kPagedWarps - 1) / (kLeast * kPagedWarps);
+    uint32_t blocks = wanted < gridDim.x ? (uint32_t)wanted : gridDim.x;
+    // as many blocks an item for all, where that leaves few idle or there is little to do: items of one length then end with a block
+    const uint32_t items = a.c.batch * per_seq;
+    if (items <= blocks && (wanted < gridDim.x || blocks % items * 16 <= blocks)) blocks -= blocks % items;
+    if (blockIdx.x >= blocks) return;
+    const uint64_t me = (uint64_t)blockIdx.x * kPagedWarps + warp, all = (uint64_t)blocks * kPagedWarps;
+    const uint64_t begin = total * me / all;
+    const uint32_t share = (uint32_t)(total * (me + 1) / all - begin);
+    Span<KT> span;
+    uint32_t seq = 0, item = 0, place = 0;   // where the share begins
+    {
+        uint64_t base = 0;
+        for (uint32_t b0 = 0;; b0 += 32) {
+            const uint32_t places = b0 == 0 ? held[0] : b0 == 32 ? held[1] : b0 == 64 ? held[2] : b0 == 96 ? held[3]
+                                    : b0 + lane < a.c.batch ? Span<KT>(a, b0 + lane).places() : 0;
+            const uint64_t mine = (uint64_t)places * per_seq;
+            uint64_t upto = mine;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const uint64_t v = __shfl_up_sync(~0u, upto, d);
+                if (lane >= d) upto += v;
+            }
+            const uint32_t past = __ballot_sync(~0u, base + upto > begin);
+            if (past) {
+                const int at = __ffs(past) - 1;
+                seq = b0 + at;
+                base += __shfl_sync(~0u, upto - mine, at);
+                span = Span<KT>(a, seq);
+                const uint64_t in = begin - base;
+                item = (uint32_t)(in / span.places());
+                place = (uint32_t)(in - (uint64_t)item * span.places());
+                break;
+            }
+            base += __shfl_sync(~0u, upto, 31);
+            if (b0 + 32 >= a.c.batch) break;   // not reached while the lengths stay as they are
+        }
+    }
+
+    // ---- copies: a cursor of its own runs ahead over this warp's tiles ----
+    Span<KT> lspan = span;
+    uint32_t lseq = seq, litem = item, lslot = 0, lrest = share;   // places of the share from its present item's on
+    uint32_t ltile, lend;
+    auto enter = [&](uint32_t from) {   // the cursor's item, from this place on
+        const uint32_t take = min(lspan.places() - from, lrest);
+        ltile = max(from, kEnd) - kEnd;
+        lend = max(from + take, kEnd) - kEnd;
+        lrest -= take;
+    };
+    enter(place);
+    uint32_t entry = 0, entries_from = 0, entries_of = ~0u;   // 32 entries of a sequence's table, a lane each
+    const uint32_t lrow = lane / kPieces, lpiece = lane % kPieces;
+    const bool copies = 16 * lpiece < row_bytes;
+    const uint8_t *const from_k = a.c.k + 16 * lpiece, *const from_v = a.c.v + 16 * lpiece;
+    const uint32_t to_k = piece_at<FORMAT, DP, false>(lrow, lpiece), to_v = KT * S::kRow + piece_at<FORMAT, DP, true>(lrow, lpiece);
+    auto copy_tile = [&] {
+        while (ltile == lend && lrest) {
+            if (++litem == per_seq) {
+                litem = 0;
+                if (++lseq >= a.c.batch) {
+                    lrest = 0;
+                    break;
+                }
+                lspan = Span<KT>(a, lseq);
+            }
+            enter(0);
+        }
+        if (ltile < lend) {
+            const uint32_t key = lspan.first + ltile * KT + lane, head = litem / a.chunks;
+            const uint32_t at = a.page_shift >= 0 ? key >> a.page_shift : key / a.c.page_size;   // in the table
+            const uint32_t first_at = __shfl_sync(~0u, at, 0), last_at = __shfl_sync(~0u, at, KT - 1);
+            if (entries_of != lseq || first_at < entries_from || last_at >= entries_from + 32) {
+                entries_of = lseq;
+                entries_from = first_at;
+                entry = ~0u;
+                if (entries_from + lane < a.c.table_width) entry = a.c.page_table[(uint64_t)lseq * a.c.table_width + entries_from + lane];
+            }
+            const uint32_t page = __shfl_sync(~0u, entry, at - entries_from);
+            uint32_t row = ~0u;
+            if (lane < KT && key < lspan.n) {
+                if (page < a.c.pages) row = (page * a.c.kv_heads + head) * a.c.page_size + (key - at * a.c.page_size);
+                else kstatus_set(a.c.status, FE2O3_KSTATUS_SLOT_RANGE);
+            }
+            const uint32_t to = ring + lslot * S::kStage;
+            if constexpr (F16) {
+                if (lane < KT) {
+                    copy4(to + 2 * KT * S::kRow + 4 * lane, a.c.k_scales + (row == ~0u ? 0 : row), row != ~0u);
+                    copy4(to + 2 * KT * S::kRow + 4 * KT + 4 * lane, a.c.v_scales + (row == ~0u ? 0 : row), row != ~0u);
+                }
+            }
+            const bool full = __all_sync(~0u, lane >= KT || row != ~0u);
+#pragma unroll
+            for (uint32_t i = 0; i < KT / kRowsAtOnce; ++i) {
+                // (the rows of one step and of another differ in bits of their own, so the swizzle falls apart)
+                constexpr uint32_t kBits = F16 ? (DP == 64 ? 0 : 6) : 7;
+                const uint32_t x = (i * kRowsAtOnce & kBits) << 4, down = i * kRowsAtOnce * S::kRow;
+                const uint32_t at_k = F16 ? to + to_k + down : ((to + to_k) ^ x) + down, at_v = ((to + to_v) ^ x) + down;
+                const uint32_t r = __shfl_sync(~0u, row, i * kRowsAtOnce + lrow);
+                if (full) {
+                    const uint64_t at = (uint64_t)r * row_bytes;
+                    if (copies) {
+                        copy16(at_k, from_k + at);
+                        copy16(at_v, from_v + at);
+                    }
+                } else {
+                    const uint64_t at = r == ~0u ? 0 : (uint64_t)r * row_bytes;
+                    if (copies) {
+                        copy16(at_k, r == ~0u ? a.c.k : from_k + at, r != ~0u);
+                        copy16(at_v, r == ~0u ? a.c.v : from_v + at, r != ~0u);
+                    }
+                }
+            }
+            lslot = lslot + 1 == a.stages ? 0 : lslot + 1;
+            ++ltile;
+        }
+        copies_commit();
+    };
+    for (uint32_t s = 0; s < a.stages; ++s) copy_tile();
+
+    // ---- the queries of an item, as 16-bit terms: a lane takes eight columns of a row at a time ----
+    auto lay_query = [&] {
+        constexpr int kLanes = DP / 8, kAtOnce = 32 / kLanes, kPasses = S::kHeads / kAtOnce;
+        const uint32_t head = item / a.chunks, chunk = item % a.chunks, d = lane % kLanes * 8, r0 = lane / kLanes;
+        const uint64_t base = (uint64_t)seq * a.q_stride + (uint64_t)(head * a.group) * a.q_head_stride + d;
+        uint4 raw[kPasses][2];
+#pragma unroll
+        for (int x = 0; x < kPasses; ++x) {
+            raw[x][0] = raw[x][1] = make_uint4(0, 0, 0, 0);
+            const uint32_t in_group = chunk * S::kHeads + x * kAtOnce + r0;
+            if (in_group >= a.group || d >= a.c.dim) continue;
+            const uint64_t from = base + (uint64_t)in_group * a.q_head_stride;
+            const uint8_t *const at = static_cast<const uint8_t *>(a.q) + from * (a.q_f32 ? 4 : 2);
+            if (a.q_whole) {   // rows start on 16 bytes
+                raw[x][0] = *reinterpret_cast<const uint4 *>(at);
+                if (a.q_f32) raw[x][1] = *reinterpret_cast<const uint4 *>(at + 16);
+            } else if (a.q_f32) {
+                const uint32_t *const v = reinterpret_cast<const uint32_t *>(at);
+                raw[x][0] = make_uint4(v[0], v[1], v[2], v[3]);
+                raw[x][1] = make_uint4(v[4], v[5], v[6], v[7]);
+            } else {
+                const uint16_t *const v = reinterpret_cast<const uint16_t *>(at);
+                raw[x][0] = make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
+            }
+        }
+#pragma unroll
+        for (int x = 0; x < kPasses; ++x) {
+            const uint32_t row = x * kAtOnce + r0;
+            uint8_t *const to = query + row * S::kQueryRow + 2 * d;
+            float back = 1.f;
+            if constexpr (!F16) {
+                if (!a.q_f32) *reinterpret_cast<uint4 *>(to) = raw[x][0];
+            }
+            if (F16 || a.q_f32) {
+                float v[8];
+                const uint32_t w[8] = {raw[x][0].x, raw[x][0].y, raw[x][0].z, raw[x][0].w, raw[x][1].x, raw[x][1].y, raw[x][1].z, raw[x][1].w};
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(a.q_f32 ? w[i] : i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+                if constexpr (F16) {
+                    float top = 0.f;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[i]) < INFINITY ? fabsf(v[i]) : 0.f);
+#pragma unroll
+                    for (int i = 1; i < kLanes; i <<= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, i));
+                    const int e = min(120, max(-100, (int)(__float_as_uint(top) >> 23) - 127 - kQueryExponent));
+                    const float by = __uint_as_float((uint32_t)(127 - e) << 23);
+                    back = __uint_as_float((uint32_t)(127 + e) << 23);
+                    uint32_t hi[4], lo[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float v0 = v[2 * i] * by, v1 = v[2 * i + 1] * by;
+                        hi[i] = f16_pair(v0, v1);
+                        const float2 h = f16_values(hi[i]);
+                        lo[i] = f16_pair(fabsf(v0) < INFINITY ? v0 - h.x : 0.f, fabsf(v1) < INFINITY ? v1 - h.y : 0.f);
+                    }
+                    *reinterpret_cast<uint4 *>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                    if (terms > 1) *reinterpret_cast<uint4 *>(to + S::kHeads * S::kQueryRow) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                } else {
+                    // cut off; what is left of 0 is the smallest number of the value's sign, so that an infinity in K stays one
+#pragma unroll
+                    for (int term = 0; term < 3; ++term) {
+                        *reinterpret_cast<uint4 *>(to + term * S::kHeads * S::kQueryRow) =
+                            make_uint4(bf16_pair_cut(v[0], v[1]), bf16_pair_cut(v[2], v[3]), bf16_pair_cut(v[4], v[5]), bf16_pair_cut(v[6], v[7]));
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const float left = v[i] - cut_bf16(v[i]);
+                            if (fabsf(v[i]) < INFINITY && v[i] != 0.f) v[i] = fabsf(left) < 1.1754944e-38f ? copysignf(1.1754944e-38f, v[i]) : left;
+                        }
+                    }
+                }
+            }
+            if (lane % kLanes == 0) head_scale[row] = a.scale * 1.4426950408889634f * back;
+        }
+        __syncwarp();
+    };
+
+    // Writes an item's result.
+    auto write = [&](const P &p, uint32_t seq, uint32_t item, uint32_t n) {
+        const uint32_t head = item / a.chunks, chunk = item % a.chunks;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const uint32_t in_group = chunk * S::kHeads + 8 * nt + 2 * t4 + e;
+                if (in_group >= a.group) continue;
+                const uint64_t row = (uint64_t)seq * a.c.kv_heads * a.group + head * a.group + in_group;
+                const float l = p.l[nt][e], inv = n ? 1.f / l : 0.f;
+                const uint32_t g_at = column_of<FORMAT, DP>(0, g);
+                float *const o32 = static_cast<float *>(a.o) + row * a.c.dim + g_at;
+                uint16_t *const o16 = static_cast<uint16_t *>(a.o) + row * a.c.dim + g_at;
+#pragma unroll
+                for (int i = 0; i < MD; ++i) {
+                    const float v0 = p.o[i][nt][e] * inv, v1 = p.o[i][nt][2 + e] * inv;
+                    if constexpr (F16) {   // columns in a row of their own
+                        if (g_at + (DP == 256 ? 128 * (i >> 3) : 0) >= a.c.dim) continue;
+                        if (a.o_f32) {
+                            o32[column_of<FORMAT, DP>(i, 0)] = v0;
+                            o32[column_of<FORMAT, DP>(i, 0) + 1] = v1;
+                        } else {
+                            o16[column_of<FORMAT, DP>(i, 0)] = bf16_of(v0);
+                            o16[column_of<FORMAT, DP>(i, 0) + 1] = bf16_of(v1);
+                        }
+                    } else {
+                        if (16 * i >= a.c.dim) continue;
+                        if (a.o_f32) {
+                            o32[16 * i] = v0;
+                            o32[16 * i + 8] = v1;
+                        } else {
+                            o16[16 * i] = bf16_of(v0);
+                            o16[16 * i + 8] = bf16_of(v1);
+                        }
+                    }
+                }
+                if (a.lse && g == 0) a.lse[row] = n ? (p.m[nt][e] + log2f(l)) * 0.6931471805599453f : -INFINITY;
+            }
+    };
+    float4 *const slots = a.slots + (uint64_t)blockIdx.x * kPagedSlots * S::kPart * 32 + lane;
+    auto to_slot = [&](const P &p, uint32_t slot) { p.leave([&](int i, float4 v) { slots[(slot * S::kPart + i) * 32] = v; }); };
+
+    // where a lane reads K and V in a stage; a lane's offsets for further steps differ by constants
+    uint32_t k_off[4], v_off[4];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+        if constexpr (!F16) {
+            k_off[x] = piece_at<FORMAT, DP, false>(lane & 15, 2 * x + (lane >> 4));
+            v_off[x] = KT * S::kRow + piece_at<FORMAT, DP, true>((lane & 7) + (lane >> 4) * 8, 2 * x + (lane >> 3 & 1));
+        } else if constexpr (DP == 64) {
+            k_off[x] = piece_at<FORMAT, DP, false>(g, t4);
+            v_off[x] = KT * S::kRow + piece_at<FORMAT, DP, true>(2 * t4 + (x & 1), g >> 1) + 8 * (g & 1);
+        } else {
+            k_off[x] = piece_at<FORMAT, DP, false>(g, 4 * (x & 1) + t4);
+            v_off[x] = KT * S::kRow + piece_at<FORMAT, DP, true>(2 * t4 + (x & 1), g);
+        }
+    }
+
+    // ---- the share, item by item ----
+    const Span<KT> first_span = span;
+    const uint32_t first_seq = seq, first_item = item, first_place = place;
+    P p;
+    uint32_t kind = share ? kNone : kEmpty, slot = 0;
+    uint64_t i0 = 0;        // where on the line the last item begins
+    uint32_t end_of_first = 0;
+    for (uint32_t at = 0; at < share;) {
+        const uint32_t here = min(span.places() - place, share - at);
+        const uint32_t last_tile = max(place + here, kEnd) - kEnd;
+        p.clear();
+        lay_query();
+        float vref = 1.1754944e-38f;   // a power of two above every scale of V so far
+        for (uint32_t tile = max(place, kEnd) - kEnd; tile < last_tile; ++tile) {
+            copies_wait(a.stages - 1);
+            __syncwarp();
+            const uint32_t from = ring + slot * S::kStage;
+            const uint32_t left = span.n - span.first - tile * KT;   // keys from here on
+
+            // scores: rows are keys, columns heads
+            float s[MT][NT][4];
+            if constexpr (!F16) {
+                float odd[MT][NT][4];   // every other step: two chains
+                auto scores = [&](uint32_t term, auto first) {
+#pragma unroll
+                    for (int ks = 0; ks < MD; ks += 2) {
+                        uint32_t ka[MT][2][4];
+#pragma unroll
+                        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) ldsm4(ka[mt][e], from + k_off[(ks + e) & 3] + (ks >> 2) * 128 + mt * 16 * S::kRow);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            uint32_t qb[4];
+                            ldsm4(qb, query_s + (term * S::kHeads + 8 * nt + (lane & 7)) * S::kQueryRow + (2 * ks + (lane >> 3)) * 16);
+#pragma unroll
+                            for (int mt = 0; mt < MT; ++mt) {
+                                if (decltype(first)::value && ks == 0) {
+                                    mma_first<false>(s[mt][nt], ka[mt][0], qb[0], qb[1]);
+                                    mma_first<false>(odd[mt][nt], ka[mt][1], qb[2], qb[3]);
+                                } else {
+                                    mma<false>(s[mt][nt], ka[mt][0], qb[0], qb[1]);
+                                    mma<false>(odd[mt][nt], ka[mt][1], qb[2], qb[3]);
+                                }
+                            }
+                        }
+                    }
+                };
+                scores(0, Yes{});
+                for (uint32_t term = 1; term < terms; ++term) scores(term, No{});
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) s[mt][nt][e] += odd[mt][nt][e];
+            } else {
+#pragma unroll
+                for (int j = 0; j < DP / 64; ++j) {   // 64 columns: the lanes of a row hold 16 each, four a step
+                    uint4 ka[MT][2];
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) ka[mt][e] = lds128(from + k_off[j & 1] + (j >> 1) * 128 + (16 * mt + 8 * e) * S::kRow);
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        uint32_t kf[MT][2][4];
+#pragma unroll
+                        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                const uint32_t w0 = half ? (e ? ka[mt][0].w : ka[mt][0].z) : (e ? ka[mt][0].y : ka[mt][0].x);
+                                const uint32_t w1 = half ? (e ? ka[mt][1].w : ka[mt][1].z) : (e ? ka[mt][1].y : ka[mt][1].x);
+                                kf[mt][e][0] = codes_f16<FORMAT, 0, 1>(w0, w0);
+                                kf[mt][e][1] = codes_f16<FORMAT, 0, 1>(w1, w1);
+                                kf[mt][e][2] = codes_f16<FORMAT, 2, 1>(w0, w0);
+                                kf[mt][e][3] = codes_f16<FORMAT, 2, 1>(w1, w1);
+                            }
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            const uint32_t at_q = query_s + (8 * nt + g) * S::kQueryRow + 128 * j + 32 * t4 + 16 * half;
+                            const uint4 qb = lds128(at_q);
+#pragma unroll
+                            for (int mt = 0; mt < MT; ++mt) {
+                                if (j == 0 && half == 0) mma_first<true>(s[mt][nt], kf[mt][0], qb.x, qb.y);
+                                else mma<true>(s[mt][nt], kf[mt][0], qb.x, qb.y);
+                                mma<true>(s[mt][nt], kf[mt][1], qb.z, qb.w);
+                            }
+                            if (terms > 1) {
+                                const uint4 ql = lds128(at_q + S::kHeads * S::kQueryRow);
+#pragma unroll
+                                for (int mt = 0; mt < MT; ++mt) {
+                                    mma<true>(s[mt][nt], kf[mt][0], ql.x, ql.y);
+                                    mma<true>(s[mt][nt], kf[mt][1], ql.z, ql.w);
+                                }
+                            }
+                        }
+                    }
+                }
+            }
+
+            // the running maximum, in units of log2; weights
+            float vs[MT][2];
+            float grow = 1.f;   // of the output's unit
+            if constexpr (F16) {
+                const uint32_t scales = from + 2 * KT * S::kRow + 4 * g;
+                float top = 0.f;
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const float ks = lds_f32(scales + 4 * (16 * mt + 8 * e));
+                        vs[mt][e] = lds_f32(scales + 4 * KT + 4 * (16 * mt + 8 * e));
+                        top = fmaxf(top, vs[mt][e]);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            s[mt][nt][2 * e] *= ks;
+                            s[mt][nt][2 * e + 1] *= ks;
+                        }
+                    }
+                if (__any_sync(~0u, top >= vref)) {
+#pragma unroll
+                    for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
+                    const float next = __uint_as_float((__float_as_uint(top) & 0x7f800000u) + 0x00800000u);
+                    grow = vref / next;
+                    vref = next;
+                }
+                const float inv = __uint_as_float(0x7f000000u - __float_as_uint(vref));   // 1 / vref: powers of two
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) vs[mt][0] *= inv, vs[mt][1] *= inv;
+            }
+            uint32_t pb[MT][NT][3][2];   // weights as the second product's operand, by terms
+            uint64_t scale_o[NT];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                const float c[2] = {head_scale[8 * nt + 2 * t4], head_scale[8 * nt + 2 * t4 + 1]};
+                float top[2] = {p.m[nt][0], p.m[nt][1]};
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[mt][nt][e] *= c[e & 1];
+                if (left < KT) {
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (16 * mt + 8 * (e >> 1) + g >= left) s[mt][nt][e] = -INFINITY;
+                }
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) top[e] = max3(top[e], s[mt][nt][e], s[mt][nt][e + 2]);
+                float base[2], keep[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+#pragma unroll
+                    for (int d = 4; d < 32; d <<= 1) top[e] = fmaxf(top[e], __shfl_xor_sync(~0u, top[e], d));
+                    base[e] = top[e] == -INFINITY ? 0.f : top[e];
+                    keep[e] = ex2_approx(p.m[nt][e] - base[e]);
+                    p.m[nt][e] = top[e];
+                    p.l[nt][e] *= keep[e];
+                }
+                scale_o[nt] = F16 ? pack_f32x2(keep[0] * grow, keep[1] * grow) : pack_f32x2(keep[0], keep[1]);
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                    float w[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        w[e] = ex2_approx(s[mt][nt][e] - base[e & 1]);
+                        p.l[nt][e & 1] += w[e];
+                    }
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float w0 = w[2 * e], w1 = w[2 * e + 1];
+                        if constexpr (F16) {
+                            w0 *= vs[mt][e];
+                            w1 *= vs[mt][e];
+                            const uint32_t hi = f16_pair(w0, w1);
+                            pb[mt][nt][0][e] = turned(hi);
+                            const float2 h = f16_values(hi);
+                            pb[mt][nt][1][e] = turned(f16_pair(w0 - h.x, w1 - h.y));
+                        } else {
+                            pb[mt][nt][0][e] = turned(bf16_pair_cut(w0, w1));
+                            const float m0 = fmaxf(w0 - cut_bf16(w0), 1.1754944e-38f), m1 = fmaxf(w1 - cut_bf16(w1), 1.1754944e-38f);
+                            if (a.o_f32) {
+                                pb[mt][nt][1][e] = turned(bf16_pair_cut(m0, m1));
+                                pb[mt][nt][2][e] = turned(bf16_pair_cut(fmaxf(m0 - cut_bf16(m0), 1.1754944e-38f), fmaxf(m1 - cut_bf16(m1), 1.1754944e-38f)));
+                            } else {
+                                uint32_t r;
+                                asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(m1), "f"(m0));
+                                pb[mt][nt][1][e] = turned(r);
+                            }
+                        }
+                    }
+                }
+            }
+
+            // output: rows are its columns, columns heads; the tile's sum is the tensor unit's, the rest f32
+            uint4 v4[MT][4][F16 && DP == 256 ? 2 : 1];
+            if constexpr (F16) {
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        if constexpr (DP == 64) {
+                            const uint2 v = lds64(from + v_off[e & 1] + (16 * mt + 8 * (e >> 1)) * S::kRow);
+                            v4[mt][e][0] = make_uint4(v.x, v.y, 0, 0);
+                        } else {
+#pragma unroll
+                            for (int x = 0; x < DP / 128; ++x) v4[mt][e][x] = lds128(from + v_off[e & 1] + 128 * x + (16 * mt + 8 * (e >> 1)) * S::kRow);
+                        }
+                    }
+            }
+#pragma unroll
+            for (int i = 0; i < MD; ++i) {
+                uint32_t va[MT][4];
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                    if constexpr (F16) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const uint4 v = v4[mt][e][DP == 256 ? i >> 3 : 0];
+                            const int word = (DP == 256 ? i & 7 : i) >> 1;
+                            w[e] = word == 0 ? v.x : word == 1 ? v.y : word == 2 ? v.z : v.w;
+                        }
+                        if (i & 1) {
+                            va[mt][0] = codes_f16<FORMAT, 2, 0>(w[0], w[1]);
+                            va[mt][1] = codes_f16<FORMAT, 3, 0>(w[0], w[1]);
+                            va[mt][2] = codes_f16<FORMAT, 2, 0>(w[2], w[3]);
+                            va[mt][3] = codes_f16<FORMAT, 3, 0>(w[2], w[3]);
+                        } else {
+                            va[mt][0] = codes_f16<FORMAT, 0, 0>(w[0], w[1]);
+                            va[mt][1] = codes_f16<FORMAT, 1, 0>(w[0], w[1]);
+                            va[mt][2] = codes_f16<FORMAT, 0, 0>(w[2], w[3]);
+                            va[mt][3] = codes_f16<FORMAT, 1, 0>(w[2], w[3]);
+                        }
+                    } else {
+                        ldsm4_trans(va[mt], from + v_off[i & 3] + (i >> 2) * 128 + mt * 16 * S::kRow);
+                    }
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    float d[4];
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt) {
+                        if (mt == 0) mma_first<F16>(d, va[mt], pb[mt][nt][1][0], pb[mt][nt][1][1]);
+                        else mma<F16>(d, va[mt], pb[mt][nt][1][0], pb[mt][nt][1][1]);
+                        if constexpr (!F16) {
+                            if (a.o_f32) mma<false>(d, va[mt], pb[mt][nt][2][0], pb[mt][nt][2][1]);
+                        }
+                        mma<F16>(d, va[mt], pb[mt][nt][0][0], pb[mt][nt][0][1]);
+                    }
+                    float (&o)[4] = p.o[i][nt];
+                    unpack_f32x2(fma_f32x2(pack_f32x2(o[0], o[1]), scale_o[nt], pack_f32x2(d[0], d[1])), o[0], o[1]);
+                    unpack_f32x2(fma_f32x2(pack_f32x2(o[2], o[3]), scale_o[nt], pack_f32x2(d[2], d[3])), o[2], o[3]);
+                }
+            }
+            slot = slot + 1 == a.stages ? 0 : slot + 1;
+            __syncwarp();   // every lane has read the stage
+            copy_tile();
+        }
+
+        // the lanes of a row add up
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) p.l[nt][e] += __shfl_xor_sync(~0u, p.l[nt][e], d);
+            if constexpr (F16) {
+                const float unit = vref;
+#pragma unroll
+                for (int i = 0; i < MD; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) p.o[i][nt][e] *= unit;
+            }
+        }
+        const bool begins = place == 0, ended = place + here == span.places();
+        i0 = begin + at - place;
+        if (ended) {
+            if (!begins) {
+                to_slot(p, kSlotFirst + warp);
+                end_of_first = 1;
+            } else if (span.valid) {
+                write(p, seq, item, span.n);
+            }
+        } else {
+            kind = begins ? kBegun : kWithin;
+        }
+        at += here;
+        if (at < share) {
+            place = 0;
+            if (++item == per_seq) {
+                item = 0;
+                if (++seq >= a.c.batch) break;   // not reached while the lengths stay as they are
+                span = Span<KT>(a, seq);
+            }
+        }
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+
+    // ---- the block: what a warp left open, the next ones continue ----
+    __syncwarp();
+    float4 *const my_part = reinterpret_cast<float4 *>(my_ring) + lane;   // the ring is free now
+    if (kind == kWithin && warp) p.leave([&](int i, float4 v) { my_part[i * 32] = v; });
+    if (lane == 0) {
+        kinds[warp] = kind;
+        ends[warp] = end_of_first;
+    }
+    __threadfence_block();
+    __syncthreads();
+    auto arrive = [&](uint32_t role, uint64_t i0, uint32_t places, uint32_t seq, uint32_t item, uint32_t n) {   // this block's piece lies in its slot
+        const uint32_t c0 = (uint32_t)(((i0 + 1) * blocks - 1) / total), c1 = (uint32_t)(((i0 + places) * blocks - 1) / total);
+        __threadfence();
+        __syncwarp();
+        if (lane == 0 && atomicAdd(&a.arrived[c0], 1u) == c1 - c0) {
+            a.arrived[c0] = 0;
+            jobs[role] = Job{seq, item, n, c0, c1 - c0 + 1};
+        }
+    };
+    const bool owner = kind == kBegun || (kind == kWithin && warp == 0);
+    bool went_on = owner;   // past the block's end
+    if (owner) {
+        for (uint32_t w = warp + 1; w < kPagedWarps && went_on; ++w) {
+            const float4 *const theirs = reinterpret_cast<const float4 *>(smem + w * a.stages * S::kStage) + lane;
+            if (kinds[w] == kWithin) {
+                p.add([&](int i) { return theirs[i * 32]; });
+            } else if (ends[w]) {
+                p.add([&](int i) { return __ldcg(slots + (w * S::kPart + i) * 32); });
+                went_on = false;
+            }
+        }
+    }
+    // an item that an earlier block began (warp 0 has it), and one that goes on in the next
+    if (warp == 0 && end_of_first) {
+        const uint64_t first = begin - first_place;
+        arrive(0, first, first_span.places(), first_seq, first_item, first_span.valid ? first_span.n : kInvalid);
+    }
+    if (owner) {
+        const uint32_t n = span.valid ? span.n : kInvalid;
+        if (kind == kBegun && !went_on) {
+            if (span.valid) write(p, seq, item, span.n);
+        } else {
+            to_slot(p, kind == kBegun ? kSlotLast : kSlotFirst);
+            arrive(kind == kBegun, i0, span.places(), seq, item, n);
+        }
+    }
+
+    // ---- the blocks: the last one to come joins the pieces, its warps some each ----
+    __syncthreads();
+#pragma unroll 1
+    for (int role = 0; role < 2; ++role) {
+        const Job job = jobs[role];
+        if (!job.pieces) continue;
+        __threadfence();
+        if (role) __syncthreads();   // warp 0 has read the rings
+        p.clear();
+        // (copied into the ring, as many as fit, so that a round costs one trip to the workspace)
+        const uint32_t at_once = a.stages * S::kStage / (S::kPart * 512);
+#pragma unroll 1
+        for (uint32_t i0 = warp; i0 < job.pieces; i0 += kPagedWarps * at_once) {
+            const uint32_t n = min(at_once, (job.pieces - i0 + kPagedWarps - 1) / kPagedWarps);
+#pragma unroll 1
+            for (uint32_t k = 0; k < n; ++k) {
+                const uint32_t i = i0 + kPagedWarps * k;
+                const float4 *const from = a.slots + ((uint64_t)(job.block + i) * kPagedSlots + (i ? kSlotFirst : kSlotLast)) * S::kPart * 32 + lane;
+#pragma unroll
+                for (int x = 0; x < S::kPart; ++x) copy16(ring + ((k * S::kPart + x) * 32 + lane) * 16, from + x * 32);
+            }
+            asm volatile("cp.async.wait_all;" ::: "memory");
+#pragma unroll 1
+            for (uint32_t k = 0; k < n; ++k) p.add([&](int x) { return my_part[(k * S::kPart + x) * 32]; });
+        }
+        if (warp) p.leave([&](int i, float4 v) { my_part[i * 32] = v; });
+        __syncthreads();
+        if (warp == 0) {
+#pragma unroll 1
+            for (uint32_t w = 1; w < kPagedWarps; ++w) {
+                const float4 *const theirs = reinterpret_cast<const float4 *>(smem + w * a.stages * S::kStage) + lane;
+                p.add([&](int i) { return theirs[i * 32]; });
+            }
+            if (job.n != kInvalid) write(p, job.seq, job.item, job.n);
+        }
+    }
+}
+
+template <uint32_t FORMAT, int DP, int NT>
+PagedBuild paged_build() {
+    using S = Shape<FORMAT, DP, NT>;
+    return PagedBuild{paged_attention_kernel<FORMAT, DP, NT>, (uint32_t)S::kStage, (uint32_t)S::kPart * 512u, (uint32_t)(S::kHeads * S::kQueryRow)};
+}
+template <uint32_t FORMAT>
+PagedBuild paged_build_for(uint32_t dim, uint32_t nt) {
+    if (dim <= 64) return nt == 1 ? paged_build<FORMAT, 64, 1>() : paged_build<FORMAT, 64, 2>();
+    if (dim <= 128) return nt == 1 ? paged_build<FORMAT, 128, 1>() : paged_build<FORMAT, 128, 2>();
+    return nt == 1 ? paged_build<FORMAT, 256, 1>() : paged_build<FORMAT, 256, 2>();
+}
+
+}  // namespace
