@@ -1,9 +1,65 @@
 // Plans and launches of attention over a paged key-value cache (the kernel: paged_attention.cuh).
+#include <mutex>
 #include <new>
 
 #include "paged_attention.cuh"
 
+// Workspaces of one device: pieces of slabs that stay until the process ends, so that preparing a launch seldom waits for
+// the allocator (half a millisecond to tens of them); what is given back goes to the next plan of the same size.
+namespace {
+
+struct Workspaces {
+    struct Piece {
+        void *at;
+        size_t bytes;
+        Piece *next;
+    };
+    std::mutex lock;
+    Piece *returned = nullptr;
+    uint8_t *slab = nullptr;
+    size_t left = 0;
+
+    cudaError_t take(size_t bytes, void **out) {
+        std::lock_guard<std::mutex> held(lock);
+        for (Piece **p = &returned; *p; p = &(*p)->next) {
+            if ((*p)->bytes != bytes) continue;
+            Piece *const found = *p;
+            *out = found->at;
+            *p = found->next;
+            delete found;
+            return cudaSuccess;
+        }
+        if (bytes > left) {
+            const size_t size = bytes > (64u << 20) ? bytes : 64u << 20;
+            void *fresh = nullptr;
+            const cudaError_t e = cudaMalloc(&fresh, size);
+            if (e != cudaSuccess) return e;
+            slab = static_cast<uint8_t *>(fresh);   // (what was left of the last one is not used any more)
+            left = size;
+        }
+        *out = slab;
+        slab += bytes;
+        left -= bytes;
+        return cudaSuccess;
+    }
+    void give(void *at, size_t bytes) {   // no launch uses it any more
+        Piece *const p = new (std::nothrow) Piece{at, bytes, nullptr};
+        if (!p) return;
+        std::lock_guard<std::mutex> held(lock);
+        p->next = returned;
+        returned = p;
+    }
+};
+Workspaces *workspaces_of(int device) {
+    static Workspaces all[64];
+    return device >= 0 && device < 64 ? &all[device] : nullptr;
+}
+
+}  // namespace
+
 struct PagedPlan {
+    int device;
+    size_t bytes;
     PagedKernel kernel;
     PagedArgs args;
     uint32_t grid, shared;
@@ -12,7 +68,14 @@ struct PagedPlan {
 
 void paged_attention_free(PagedPlan *p) {
     if (!p) return;
-    if (p->workspace) cudaFree(p->workspace);   // (waits for launches in flight)
+    if (p->workspace) {
+        // a launch in flight may still use it; when the device cannot say, the workspace is not used again
+        int current = -1;
+        cudaGetDevice(&current);
+        if (current != p->device) cudaSetDevice(p->device);
+        if (cudaDeviceSynchronize() == cudaSuccess) workspaces_of(p->device)->give(p->workspace, p->bytes);
+        if (current >= 0 && current != p->device) cudaSetDevice(current);
+    }
     delete p;
 }
 void paged_attention_geometry(const PagedPlan *p, fe2o3_geometry *geo) {
@@ -49,7 +112,10 @@ int32_t paged_attention_plan(fe2o3_ctx *ctx, const fe2o3_paged_attention_v1_args
     if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, b.kernel, kPagedThreads, p->shared);
     p->grid = (uint32_t)(per_sm > 0 ? per_sm : 1) * ctx->sm_count;
     const size_t slots = (size_t)kPagedSlots * p->grid * b.part;
-    if (e == cudaSuccess) e = cudaMalloc(&p->workspace, slots + p->grid * sizeof(uint32_t));
+    p->device = ctx->device;
+    p->bytes = (slots + p->grid * sizeof(uint32_t) + 65535) / 65536 * 65536;
+    Workspaces *const workspaces = workspaces_of(ctx->device);
+    if (e == cudaSuccess) e = workspaces ? workspaces->take(p->bytes, &p->workspace) : cudaErrorInvalidDevice;
     if (e == cudaSuccess) e = cudaMemset(static_cast<uint8_t *>(p->workspace) + slots, 0, p->grid * sizeof(uint32_t));
     if (e == cudaSuccess) e = cudaStreamSynchronize(cudaStreamLegacy);   // no other stream is ordered behind the clear
     if (e != cudaSuccess) {
