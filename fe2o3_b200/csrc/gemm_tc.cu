@@ -952,10 +952,11 @@ EncodeTiledFn encode_fn() {
 
 }  // namespace
 
-// Encodes a tensor map with 128-byte swizzle.  dims/strides innermost first;
+// Encodes a tensor map with 128-byte swizzle (unless told otherwise).  dims/strides innermost first;
 // strides in bytes for dimensions 1..rank-1.
 static int32_t make_tmap(CUtensorMap *out, CUtensorMapDataType dtype, uint64_t base, uint32_t rank, const uint64_t *dims,
-                         const uint64_t *strides_bytes, const uint32_t *box) {
+                         const uint64_t *strides_bytes, const uint32_t *box,
+                         CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B) {
     EncodeTiledFn fn = encode_fn();
     if (!fn) {
         fe2o3_set_error("cuTensorMapEncodeTiled is not available from the driver");
@@ -967,7 +968,7 @@ static int32_t make_tmap(CUtensorMap *out, CUtensorMapDataType dtype, uint64_t b
     for (uint32_t i = 0; i < rank; ++i) { d[i] = dims[i]; b[i] = box[i]; es[i] = 1; }
     for (uint32_t i = 0; i + 1 < rank; ++i) st[i] = strides_bytes[i];
     CUresult r = fn(out, dtype, rank, reinterpret_cast<void *>(base), d, st, b, es,
-                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) {
         fe2o3_set_error("cuTensorMapEncodeTiled failed with CUresult %d", (int)r);
@@ -983,6 +984,13 @@ int32_t fe2o3_make_tmap_bf16(CUtensorMap *out, uint64_t base, uint32_t rank, con
 int32_t fe2o3_make_tmap_f32(CUtensorMap *out, uint64_t base, uint32_t rank, const uint64_t *dims,
                             const uint64_t *strides_bytes, const uint32_t *box) {
     return make_tmap(out, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, base, rank, dims, strides_bytes, box);
+}
+
+// Bytes; a box of 64 columns is swizzled by 64 bytes, a wider one by 128.
+int32_t fe2o3_make_tmap_u8(CUtensorMap *out, uint64_t base, uint32_t rank, const uint64_t *dims, const uint64_t *strides_bytes,
+                           const uint32_t *box) {
+    return make_tmap(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, rank, dims, strides_bytes, box,
+                     box[0] == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 // The tensor-core schedule needs 16-byte aligned bases and leading dimensions

@@ -2,6 +2,7 @@
 #include <mutex>
 #include <new>
 
+#include "gemm_tc.h"
 #include "paged_attention.cuh"
 
 // Workspaces of one device: pieces of slabs that stay until the process ends, so that preparing a launch seldom waits for
@@ -58,6 +59,7 @@ Workspaces *workspaces_of(int device) {
 }  // namespace
 
 struct PagedPlan {
+    CUtensorMap map_k, map_v;
     int device;
     size_t bytes;
     PagedKernel kernel;
@@ -93,20 +95,20 @@ int32_t paged_attention_plan(fe2o3_ctx *ctx, const fe2o3_paged_attention_v1_args
     FE2O3_CUDA(cudaFuncGetAttributes(&attr, reinterpret_cast<const void *>(b.kernel)));
     // as many blocks an SM as registers and two stages a warp allow (131071 tokens: three blocks of two stages 178 us, two of
     // three 186), then as many stages as fit; a partial result has to fit a warp's ring
-    const uint32_t fixed = kPagedWarps * terms * b.query, least = b.part > 2 * b.stage ? (b.part + b.stage - 1) / b.stage : 2;
+    const uint32_t fixed = kPagedWarps * terms * b.query + kPagedMeeting, least = b.part > 2 * b.stage ? (b.part + b.stage - 1) / b.stage : 2;
     uint32_t stages = 0;
     for (uint32_t blocks = 3; blocks && !stages; --blocks) {
-        const uint32_t room = 233472 / blocks - 1024 - (uint32_t)attr.sharedSizeBytes;   // an SM's, less what the system keeps of each block's
+        const uint32_t room = 233472 / blocks - 1024;   // an SM's, less what the system keeps of each block's
         if (blocks > 1 && (uint32_t)attr.numRegs * kPagedThreads * blocks > 65536) continue;
-        if (room < fixed + kPagedWarps * least * b.stage) continue;
-        stages = (room - fixed) / (kPagedWarps * b.stage);
+        if (room < fixed + kPagedWarps * least * (b.stage + b.scales)) continue;
+        stages = (room - fixed) / (kPagedWarps * (b.stage + b.scales));
     }
     if (!stages) return FE2O3_ERR_UNSUPPORTED_SHAPE;   // (not reached: one block fits for every build)
-    if (stages > 4) stages = 4;
+    if (stages > kPagedMaxStages) stages = kPagedMaxStages;
     PagedPlan *p = new (std::nothrow) PagedPlan();
     if (!p) return FE2O3_ERR_SIZE_OVERFLOW;
     p->kernel = b.kernel;
-    p->shared = kPagedWarps * stages * b.stage + fixed;
+    p->shared = kPagedWarps * stages * (b.stage + b.scales) + fixed;
     int per_sm = 0;
     cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void *>(b.kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, (int)p->shared);
     if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, b.kernel, kPagedThreads, p->shared);
@@ -122,14 +124,27 @@ int32_t paged_attention_plan(fe2o3_ctx *ctx, const fe2o3_paged_attention_v1_args
         paged_attention_free(p);
         return fe2o3_cuda_status(e, "paged_attention_v1 workspace");
     }
+    p->args.c = kv_cache_of(ctx, a);
     const uint32_t qb = a->q_dtype == FE2O3_DTYPE_F32 ? 4 : 2;
     const bool whole = a->q.ptr % 16 == 0 && (uint64_t)a->q_stride * qb % 16 == 0 && (uint64_t)a->q_head_stride * qb % 16 == 0;
+    // boxes of the copy engine: rows that no page's end cuts, of whole swizzle patterns
+    uint32_t box = b.keys;
+    while (a->page_size % box) box /= 2;
+    if (box < 8 || p->args.c.pages == 0 || (a->format != FE2O3_KV_BF16 && ((a->k_scales.ptr | a->v_scales.ptr) & 15u))) box = 1;
+    if (box > 1) {
+        const uint32_t eb = a->format == FE2O3_KV_BF16 ? 2 : 1, columns = eb == 2 ? 64 : a->dim <= 64 ? 64 : 128;
+        const uint64_t dims[3] = {a->dim, a->page_size, (uint64_t)p->args.c.pages * a->kv_heads};
+        const uint64_t strides[2] = {(uint64_t)a->dim * eb, (uint64_t)a->dim * eb * a->page_size};
+        const uint32_t shape[3] = {columns, box, 1};
+        const auto make = eb == 2 ? fe2o3_make_tmap_bf16 : fe2o3_make_tmap_u8;
+        if (make(&p->map_k, a->k_cache.ptr, 3, dims, strides, shape) != FE2O3_OK || make(&p->map_v, a->v_cache.ptr, 3, dims, strides, shape) != FE2O3_OK) box = 1;
+    }
     int32_t shift = -1;
     if ((a->page_size & (a->page_size - 1)) == 0) shift = __builtin_ctz(a->page_size);
     p->args = PagedArgs{kv_cache_of(ctx, a), reinterpret_cast<const void *>(a->q.ptr), reinterpret_cast<void *>(a->output.ptr),
                         reinterpret_cast<float *>(a->lse.ptr), static_cast<float4 *>(p->workspace),
                         reinterpret_cast<uint32_t *>(static_cast<uint8_t *>(p->workspace) + slots), group, (group + 8 * nt - 1) / (8 * nt),
-                        a->q_stride, a->q_head_stride, a->window, stages, shift, a->scale, a->q_dtype == FE2O3_DTYPE_F32,
+                        a->q_stride, a->q_head_stride, a->window, stages, shift, box, a->scale, a->q_dtype == FE2O3_DTYPE_F32,
                         a->output_dtype == FE2O3_DTYPE_F32, whole};
     *out = p;
     return FE2O3_OK;
@@ -137,7 +152,7 @@ int32_t paged_attention_plan(fe2o3_ctx *ctx, const fe2o3_paged_attention_v1_args
 
 int32_t paged_attention_launch(const PagedPlan *p, cudaStream_t s) {
     if (p->args.c.batch == 0) return FE2O3_OK;
-    const cudaError_t e = fe2o3_launch_early(p->kernel, p->grid, kPagedThreads, p->shared, s, 1, p->args);
+    const cudaError_t e = fe2o3_launch_early(p->kernel, p->grid, kPagedThreads, p->shared, s, 1, p->map_k, p->map_v, p->args);
     fe2o3_count_launch(1);
     return fe2o3_cuda_status(e, "paged_attention_v1");
 }

@@ -9,9 +9,10 @@
 //   writes the results of items that lie in its share by itself.  Others meet twice: the warps of a block when all
 //   have done their share, through shared memory, and the blocks in the workspace, where the one that comes last to an
 //   item (a counter) joins the pieces.  Both go by the pieces' order: the same bits whoever is last.
-//   Tiles.  Each warp has a ring of stages of its own, filled by 16-byte asynchronous copies row by row through the
-//   page table (any page size; rows outside the sequence are filled with zeros and never read), so that nothing but
-//   its own copies stops a warp.  It keeps the maximum, the sum and the output of what it has seen (one pass, f32).
+//   Tiles.  Each warp has a ring of stages of its own, so that nothing but its own copies stops a warp, and keeps the
+//   maximum, the sum and the output of what it has seen (one pass, f32).  The copy engine fetches a tile as boxes of
+//   rows that lie in one page (page sizes that are multiples of 8: a few instructions of one lane a tile, where 16-byte copies
+//   take a third of a tile's instructions); other page sizes are copied row by row.  Rows outside the sequence are zeros.
 //   Products.  mma.sync with the keys (and then the output's columns) as rows and the query heads as columns: of
 //   the 8 columns of a tile few are wasted for small groups, and P is turned into an operand by movmatrix.  The
 //   tensor unit's own sums span one tile, longer ones are f32 additions.  A bf16 cache is multiplied as it is, with the
@@ -33,6 +34,7 @@ struct PagedArgs {
     uint32_t *arrived;    // pieces that have come in, by the block where the item begins; zero between launches
     uint32_t group, chunks, q_stride, q_head_stride, window, stages;
     int32_t page_shift;   // log2 of page_size, or -1
+    uint32_t box;         // rows of a page that the copy engine takes at once; 1: rows go by 16-byte copies
     float scale;
     bool q_f32, o_f32, q_whole;   // q_whole: rows of the queries start on 16 bytes
 };
@@ -40,10 +42,13 @@ struct PagedArgs {
 // items that began in an earlier warp; the beginning of an item that goes on in the next block.
 constexpr uint32_t kPagedSlots = 5, kSlotFirst = 0, kSlotLast = 4;
 
-using PagedKernel = void (*)(PagedArgs);
+constexpr uint32_t kPagedMaxStages = 4, kPagedMeeting = 512;
+
+using PagedKernel = void (*)(CUtensorMap, CUtensorMap, PagedArgs);
 struct PagedBuild {
     PagedKernel kernel;
     uint32_t stage, part, query;   // bytes: a stage of one warp, a partial result, one term of the queries of one warp
+    uint32_t scales, keys;         // bytes of a stage's scales; keys of a tile
 };
 PagedBuild paged_build_bf16(uint32_t dim, uint32_t nt);
 PagedBuild paged_build_e4m3(uint32_t dim, uint32_t nt);
@@ -59,7 +64,9 @@ struct Shape {
     static constexpr bool kF16 = FORMAT != FE2O3_KV_BF16;
     static constexpr int kRow = DP * (kF16 ? 1 : 2);                                        // bytes of a row in a stage
     static constexpr int kKeys = kF16 ? (DP == 256 ? 16 : 32) : (DP == 64 ? 32 : 16);       // of a tile
-    static constexpr int kStage = 2 * kKeys * kRow + (kF16 ? 8 * kKeys : 0);                // K, V, their scales
+    static constexpr int kStage = 2 * kKeys * kRow;                                         // K, V: whole swizzle patterns
+    static constexpr int kScales = kF16 ? 8 * kKeys : 0;                                    // of the rows of K, of V
+    static constexpr int kPitch = kRow < 128 ? kRow : 128;                                  // a row lies in parts of at most 128 bytes
     static constexpr int kHeads = 8 * NT;
     static constexpr int kQueryRow = 2 * DP + 16;                                           // bytes, padded against bank conflicts
     static constexpr int kPart = (DP / 16 + 1) * NT;                                        // float4 a lane of a partial result
@@ -71,16 +78,11 @@ __device__ __forceinline__ void copy16(uint32_t to, const void *from) {
 __device__ __forceinline__ void copy16(uint32_t to, const void *from, bool there) {   // or zeros
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16u : 0u) : "memory");
 }
+__device__ __forceinline__ void copies_arrive(uint64_t *bar) {   // this thread's copies so far, when they have landed
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
 __device__ __forceinline__ void copy4(uint32_t to, const void *from, bool there) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(there ? 4u : 0u) : "memory");
-}
-__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-// All but the youngest `behind` groups of this thread's copies have landed.
-__device__ __forceinline__ void copies_wait(uint32_t behind) {
-    if (behind == 2) asm volatile("cp.async.wait_group 2;" ::: "memory");
-    else if (behind == 1) asm volatile("cp.async.wait_group 1;" ::: "memory");
-    else if (behind == 3) asm volatile("cp.async.wait_group 3;" ::: "memory");
-    else asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t at) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
@@ -164,13 +166,13 @@ __device__ __forceinline__ uint32_t codes_f16(uint32_t a, uint32_t b) {
     }
 }
 
-// Where 16-byte piece c of row r lies in a stage's K or V part.  Rows that the lanes of one shared-memory access touch
-// fall on different banks: 8 rows a matrix for ldmatrix; rows g, g + 1 (K) or 2t (V) for the 8-bit formats.
-template <uint32_t FORMAT, int DP, bool VALUES>
+// Where 16-byte piece c of row r lies in a stage's K or V part: as the copy engine's swizzle has it, rows in parts of 128 bytes.
+// Of what the lanes of one access touch, nothing meets on a bank but K of the 8-bit formats, in twos.
+template <uint32_t FORMAT, int DP>
 __device__ __forceinline__ uint32_t piece_at(uint32_t r, uint32_t c) {
-    if constexpr (FORMAT == FE2O3_KV_BF16) return r * (2 * DP) + ((c ^ (r & 7)) << 4);
-    else if constexpr (DP == 64) return (r >> 1) * 128 + ((((r & 1) << 2 | c) ^ (r >> 1 & 3) << 1) << 4);
-    else return r * DP + ((c ^ (VALUES ? r & 6 : (r & 1) << 2)) << 4);
+    using S = Shape<FORMAT, DP, 1>;
+    if constexpr (S::kRow == 64) return r * 64 + ((c ^ (r >> 1 & 3)) << 4);
+    else return (c >> 3) * S::kKeys * 128 + r * 128 + (((c ^ r) & 7) << 4);
 }
 
 // Column of the output that row m of tile i of the second product stands for.
@@ -188,9 +190,17 @@ enum : uint32_t { kNone, kBegun, kWithin, kEmpty };
 struct Job {
     uint32_t seq, item, n, block, pieces;   // pieces 0: none
 };
+// What a block has in shared memory beside rings and queries (all of it in the dynamic part, which then starts on a swizzle pattern).
+struct Meeting {
+    uint64_t arrivals[kPagedWarps][kPagedMaxStages];
+    float head_scales[kPagedWarps][16];
+    uint32_t kinds[kPagedWarps], ends[kPagedWarps];
+    Job jobs[2];
+};
+static_assert(sizeof(Meeting) <= kPagedMeeting, "");
 struct Yes { static constexpr bool value = true; };
 struct No { static constexpr bool value = false; };
-// A sequence's keys as tiles.  One that does not fit its table is reported and has none.
+// A sequence's keys as tiles, counted from a multiple of KT.  One that does not fit its table is reported and has none.
 template <int KT>
 struct Span {
     uint32_t first, n, tiles;
@@ -204,9 +214,10 @@ struct Span {
             n = 0;
         }
         first = a.window && n > a.window ? n - a.window : 0;
-        tiles = (n - first + KT - 1) / KT;
+        tiles = (n + KT - 1) / KT - first / KT;
     }
     __device__ __forceinline__ uint32_t places() const { return tiles + kEnd; }
+    __device__ __forceinline__ uint32_t key(uint32_t tile) const { return (first / KT + tile) * KT; }
 };
 
 // Running result of one warp over some of an item's keys: output columns (rows of tile i) by two heads a lane.
@@ -260,34 +271,44 @@ struct Part {
 };
 
 template <uint32_t FORMAT, int DP, int NT>
-__global__ void __launch_bounds__(kPagedThreads) paged_attention_kernel(const PagedArgs a) {
+__global__ void __launch_bounds__(kPagedThreads)
+paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ PagedArgs a) {
     using S = Shape<FORMAT, DP, NT>;
     using P = Part<DP / 16, NT>;
     constexpr int KT = S::kKeys, MT = KT / 16, MD = DP / 16, kPieces = S::kRow / 16, kRowsAtOnce = 32 / kPieces;
     constexpr bool F16 = S::kF16;
-    extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ float head_scales[kPagedWarps][S::kHeads];
-    __shared__ uint32_t kinds[kPagedWarps], ends[kPagedWarps];
-    __shared__ Job jobs[2];
+    extern __shared__ __align__(1024) uint8_t smem[];   // (swizzle patterns are 1 KiB)
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t4 = lane & 3;
     uint8_t *const my_ring = smem + warp * a.stages * S::kStage;
     const uint32_t ring = smem_u32(my_ring);
     const uint32_t terms = a.q_f32 ? (F16 ? 2 : 3) : 1;
-    uint8_t *const query = smem + kPagedWarps * a.stages * S::kStage + warp * terms * S::kHeads * S::kQueryRow;
+    uint8_t *const my_scales = smem + kPagedWarps * a.stages * S::kStage + warp * a.stages * S::kScales;
+    uint8_t *const queries = smem + kPagedWarps * a.stages * (S::kStage + S::kScales);
+    uint8_t *const query = queries + warp * terms * S::kHeads * S::kQueryRow;
+    Meeting &meeting = *reinterpret_cast<Meeting *>(queries + kPagedWarps * terms * S::kHeads * S::kQueryRow);
+    uint32_t (&kinds)[kPagedWarps] = meeting.kinds, (&ends)[kPagedWarps] = meeting.ends;
+    Job (&jobs)[2] = meeting.jobs;
     const uint32_t query_s = smem_u32(query);
-    float *const head_scale = head_scales[warp];
+    float *const head_scale = meeting.head_scales[warp];
     const uint32_t row_bytes = a.c.dim * (F16 ? 1 : 2);
     const uint32_t per_seq = a.c.kv_heads * a.chunks;   // items of a sequence
 
     if (threadIdx.x < 2) jobs[threadIdx.x].pieces = 0;
-    if (a.c.dim < DP) {   // the columns past the head's: zeros, which no copy goes over
+    uint64_t *const bars = meeting.arrivals[warp];
+    if (lane < a.stages) mbar_init(&bars[lane], a.box > 1 ? 1 : 32);
+    mbar_fence_init();
+    if (a.box > 1) {
+        if (lane == 0) {
+            tma_prefetch_desc(&map_k);
+            tma_prefetch_desc(&map_v);
+        }
+    } else if (a.c.dim < DP) {   // the columns past the head's: zeros, which no copy goes over
         for (uint32_t i = lane; i < 2 * KT * a.stages * kPieces; i += 32) {
             const uint32_t c = i % kPieces, row = i / kPieces, r = row % KT, side = row / KT % 2, stage = row / (2 * KT);
-            if (16 * c < row_bytes) continue;
-            const uint32_t at = stage * S::kStage + side * KT * S::kRow + (side ? piece_at<FORMAT, DP, true>(r, c) : piece_at<FORMAT, DP, false>(r, c));
-            *reinterpret_cast<uint4 *>(my_ring + at) = make_uint4(0, 0, 0, 0);
+            if (16 * c >= row_bytes) *reinterpret_cast<uint4 *>(my_ring + stage * S::kStage + side * KT * S::kRow + piece_at<FORMAT, DP>(r, c)) = make_uint4(0, 0, 0, 0);
         }
     }
+    __syncwarp();
     begin_after_previous();
 
     // ---- this warp's share of the line: every warp adds up the sequences for itself ----
@@ -354,10 +375,14 @@ __global__ void __launch_bounds__(kPagedThreads) paged_attention_kernel(const Pa
     };
     enter(place);
     uint32_t entry = 0, entries_from = 0, entries_of = ~0u;   // 32 entries of a sequence's table, a lane each
-    const uint32_t lrow = lane / kPieces, lpiece = lane % kPieces;
-    const bool copies = 16 * lpiece < row_bytes;
-    const uint8_t *const from_k = a.c.k + 16 * lpiece, *const from_v = a.c.v + 16 * lpiece;
-    const uint32_t to_k = piece_at<FORMAT, DP, false>(lrow, lpiece), to_v = KT * S::kRow + piece_at<FORMAT, DP, true>(lrow, lpiece);
+    const uint32_t lrow = lane / kPieces, lpiece = lane % kPieces, boxes = KT / a.box;
+    // Zeros for a row of a stage: K and V, and their scales.
+    auto no_row = [&](uint32_t slot, uint32_t r, bool k_too) {
+        for (uint32_t i = lane; i < 2 * kPieces; i += 32)
+            if (k_too || i >= kPieces)
+                *reinterpret_cast<uint4 *>(my_ring + slot * S::kStage + (i >= kPieces ? KT * S::kRow : 0) + piece_at<FORMAT, DP>(r, i % kPieces)) = make_uint4(0, 0, 0, 0);
+        if (F16 && lane < 2) reinterpret_cast<float *>(my_scales + slot * S::kScales)[lane * KT + r] = 0.f;
+    };
     auto copy_tile = [&] {
         while (ltile == lend && lrest) {
             if (++litem == per_seq) {
@@ -370,55 +395,69 @@ __global__ void __launch_bounds__(kPagedThreads) paged_attention_kernel(const Pa
             }
             enter(0);
         }
-        if (ltile < lend) {
-            const uint32_t key = lspan.first + ltile * KT + lane, head = litem / a.chunks;
-            const uint32_t at = a.page_shift >= 0 ? key >> a.page_shift : key / a.c.page_size;   // in the table
-            const uint32_t first_at = __shfl_sync(~0u, at, 0), last_at = __shfl_sync(~0u, at, KT - 1);
-            if (entries_of != lseq || first_at < entries_from || last_at >= entries_from + 32) {
-                entries_of = lseq;
-                entries_from = first_at;
-                entry = ~0u;
-                if (entries_from + lane < a.c.table_width) entry = a.c.page_table[(uint64_t)lseq * a.c.table_width + entries_from + lane];
-            }
-            const uint32_t page = __shfl_sync(~0u, entry, at - entries_from);
-            uint32_t row = ~0u;
-            if (lane < KT && key < lspan.n) {
-                if (page < a.c.pages) row = (page * a.c.kv_heads + head) * a.c.page_size + (key - at * a.c.page_size);
-                else kstatus_set(a.c.status, FE2O3_KSTATUS_SLOT_RANGE);
-            }
-            const uint32_t to = ring + lslot * S::kStage;
-            if constexpr (F16) {
-                if (lane < KT) {
-                    copy4(to + 2 * KT * S::kRow + 4 * lane, a.c.k_scales + (row == ~0u ? 0 : row), row != ~0u);
-                    copy4(to + 2 * KT * S::kRow + 4 * KT + 4 * lane, a.c.v_scales + (row == ~0u ? 0 : row), row != ~0u);
+        if (ltile >= lend) return;
+        // a lane a box, or a row
+        const uint32_t key = lspan.key(ltile) + min(lane, boxes - 1) * a.box, head = litem / a.chunks;
+        const uint32_t at = a.page_shift >= 0 ? key >> a.page_shift : key / a.c.page_size;   // in the table
+        const uint32_t first_at = __shfl_sync(~0u, at, 0), last_at = __shfl_sync(~0u, at, 31);
+        if (entries_of != lseq || first_at < entries_from || last_at >= entries_from + 32) {
+            entries_of = lseq;
+            entries_from = first_at;
+            entry = ~0u;
+            if (entries_from + lane < a.c.table_width) entry = a.c.page_table[(uint64_t)lseq * a.c.table_width + entries_from + lane];
+        }
+        const uint32_t page = __shfl_sync(~0u, entry, at - entries_from), in_page = key - at * a.c.page_size;
+        const bool wanted = lane < boxes && key < lspan.n && key + a.box > lspan.first, there = wanted && page < a.c.pages;
+        if (wanted && !there) kstatus_set(a.c.status, FE2O3_KSTATUS_SLOT_RANGE);
+        const uint32_t found = __ballot_sync(~0u, there);
+        uint64_t *const bar = &bars[lslot];
+        const uint32_t row = there ? (page * a.c.kv_heads + head) * a.c.page_size + in_page : ~0u;
+        if (a.box > 1) {
+            if (lane == 0) mbar_arrive_expect_tx(bar, __popc(found) * a.box * (2 * S::kRow + (F16 ? 8 : 0)));
+            __syncwarp();
+            if (there) {
+                uint8_t *const to = my_ring + lslot * S::kStage + lane * a.box * S::kPitch;
+#pragma unroll
+                for (int half = 0; half < S::kRow / S::kPitch; ++half) {
+                    tma_load_3d(to + half * KT * 128, &map_k, bar, half * (F16 ? 128 : 64), in_page, page * a.c.kv_heads + head);
+                    tma_load_3d(to + KT * S::kRow + half * KT * 128, &map_v, bar, half * (F16 ? 128 : 64), in_page, page * a.c.kv_heads + head);
+                }
+                if constexpr (F16) {
+                    uint8_t *const scales = my_scales + lslot * S::kScales + lane * a.box * 4;
+                    bulk_load_1d(scales, a.c.k_scales + row, a.box * 4, bar);
+                    bulk_load_1d(scales + KT * 4, a.c.v_scales + row, a.box * 4, bar);
                 }
             }
-            const bool full = __all_sync(~0u, lane >= KT || row != ~0u);
+            __syncwarp();
+            if (found != (boxes == 32 ? ~0u : (1u << boxes) - 1)) {   // at an end of the sequence, or reported
+                for (uint32_t r = 0; r < KT; ++r)
+                    if (!(found >> r / a.box & 1)) no_row(lslot, r, true);
+                fence_proxy_async_smem();   // before the next box goes there
+            }
+        } else {
+            const uint32_t to = ring + lslot * S::kStage, to_k = to + piece_at<FORMAT, DP>(lrow, lpiece), to_v = to_k + KT * S::kRow;
+            if constexpr (F16) {
+                if (lane < KT) {
+                    const uint32_t scales = smem_u32(my_scales + lslot * S::kScales) + 4 * lane;
+                    copy4(scales, a.c.k_scales + (row == ~0u ? 0 : row), row != ~0u);
+                    copy4(scales + 4 * KT, a.c.v_scales + (row == ~0u ? 0 : row), row != ~0u);
+                }
+            }
 #pragma unroll
             for (uint32_t i = 0; i < KT / kRowsAtOnce; ++i) {
                 // (the rows of one step and of another differ in bits of their own, so the swizzle falls apart)
-                constexpr uint32_t kBits = F16 ? (DP == 64 ? 0 : 6) : 7;
-                const uint32_t x = (i * kRowsAtOnce & kBits) << 4, down = i * kRowsAtOnce * S::kRow;
-                const uint32_t at_k = F16 ? to + to_k + down : ((to + to_k) ^ x) + down, at_v = ((to + to_v) ^ x) + down;
+                const uint32_t x = S::kRow == 64 ? 0 : (i * kRowsAtOnce & 7) << 4, down = i * kRowsAtOnce * S::kPitch;
                 const uint32_t r = __shfl_sync(~0u, row, i * kRowsAtOnce + lrow);
-                if (full) {
-                    const uint64_t at = (uint64_t)r * row_bytes;
-                    if (copies) {
-                        copy16(at_k, from_k + at);
-                        copy16(at_v, from_v + at);
-                    }
-                } else {
-                    const uint64_t at = r == ~0u ? 0 : (uint64_t)r * row_bytes;
-                    if (copies) {
-                        copy16(at_k, r == ~0u ? a.c.k : from_k + at, r != ~0u);
-                        copy16(at_v, r == ~0u ? a.c.v : from_v + at, r != ~0u);
-                    }
+                const uint64_t from = r == ~0u ? 0 : (uint64_t)r * row_bytes + 16 * lpiece;
+                if (16 * lpiece < row_bytes) {
+                    copy16((to_k ^ x) + down, a.c.k + from, r != ~0u);
+                    copy16((to_v ^ x) + down, a.c.v + from, r != ~0u);
                 }
             }
-            lslot = lslot + 1 == a.stages ? 0 : lslot + 1;
-            ++ltile;
+            copies_arrive(bar);
         }
-        copies_commit();
+        lslot = lslot + 1 == a.stages ? 0 : lslot + 1;
+        ++ltile;
     };
     for (uint32_t s = 0; s < a.stages; ++s) copy_tile();
 
@@ -546,14 +585,14 @@ __global__ void __launch_bounds__(kPagedThreads) paged_attention_kernel(const Pa
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
         if constexpr (!F16) {
-            k_off[x] = piece_at<FORMAT, DP, false>(lane & 15, 2 * x + (lane >> 4));
-            v_off[x] = KT * S::kRow + piece_at<FORMAT, DP, true>((lane & 7) + (lane >> 4) * 8, 2 * x + (lane >> 3 & 1));
+            k_off[x] = piece_at<FORMAT, DP>(lane & 15, 2 * x + (lane >> 4));
+            v_off[x] = KT * S::kRow + piece_at<FORMAT, DP>((lane & 7) + (lane >> 4) * 8, 2 * x + (lane >> 3 & 1));
         } else if constexpr (DP == 64) {
-            k_off[x] = piece_at<FORMAT, DP, false>(g, t4);
-            v_off[x] = KT * S::kRow + piece_at<FORMAT, DP, true>(2 * t4 + (x & 1), g >> 1) + 8 * (g & 1);
+            k_off[x] = piece_at<FORMAT, DP>(g, t4);
+            v_off[x] = KT * S::kRow + piece_at<FORMAT, DP>(2 * t4 + (x & 1), g >> 1) + 8 * (g & 1);
         } else {
-            k_off[x] = piece_at<FORMAT, DP, false>(g, 4 * (x & 1) + t4);
-            v_off[x] = KT * S::kRow + piece_at<FORMAT, DP, true>(2 * t4 + (x & 1), g);
+            k_off[x] = piece_at<FORMAT, DP>(g, 4 * (x & 1) + t4);
+            v_off[x] = KT * S::kRow + piece_at<FORMAT, DP>(2 * t4 + (x & 1), g);
         }
     }
 
@@ -561,7 +600,8 @@ __global__ void __launch_bounds__(kPagedThreads) paged_attention_kernel(const Pa
     const Span<KT> first_span = span;
     const uint32_t first_seq = seq, first_item = item, first_place = place;
     P p;
-    uint32_t kind = share ? kNone : kEmpty, slot = 0;
+    uint32_t kind = share ? kNone : kEmpty, slot = 0, phase = 0;
+    bool waiting = true;
     uint64_t i0 = 0;        // where on the line the last item begins
     uint32_t end_of_first = 0;
     for (uint32_t at = 0; at < share;) {
@@ -571,10 +611,22 @@ __global__ void __launch_bounds__(kPagedThreads) paged_attention_kernel(const Pa
         lay_query();
         float vref = 1.1754944e-38f;   // a power of two above every scale of V so far
         for (uint32_t tile = max(place, kEnd) - kEnd; tile < last_tile; ++tile) {
-            copies_wait(a.stages - 1);
-            __syncwarp();
+            if (waiting && !mbar_wait_warp(&bars[slot], phase)) {   // (not seen: a copy that never lands)
+                if (lane == 0) kstatus_set(a.c.status, FE2O3_KSTATUS_WAIT_EXPIRED);
+                waiting = false;
+            }
             const uint32_t from = ring + slot * S::kStage;
-            const uint32_t left = span.n - span.first - tile * KT;   // keys from here on
+            // rows of the tile that are keys of the sequence: [ahead, left)
+            const uint32_t key0 = span.key(tile), left = span.n - key0, ahead = max(span.first, key0) - key0;
+            const bool edge = left < KT || ahead;
+            if (edge) {   // the others count nothing: not even what an infinity times 0 would
+                if (a.box > 1) {
+                    for (uint32_t r = 0; r < KT; ++r)
+                        if (r < ahead || r >= left) no_row(slot, r, false);
+                    fence_proxy_async_smem();
+                }
+                __syncwarp();
+            }
 
             // scores: rows are keys, columns heads
             float s[MT][NT][4];
@@ -587,7 +639,7 @@ __global__ void __launch_bounds__(kPagedThreads) paged_attention_kernel(const Pa
 #pragma unroll
                         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-                            for (int e = 0; e < 2; ++e) ldsm4(ka[mt][e], from + k_off[(ks + e) & 3] + (ks >> 2) * 128 + mt * 16 * S::kRow);
+                            for (int e = 0; e < 2; ++e) ldsm4(ka[mt][e], from + k_off[(ks + e) & 3] + (ks >> 2) * KT * 128 + mt * 16 * S::kPitch);
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {
                             uint32_t qb[4];
@@ -620,7 +672,7 @@ __global__ void __launch_bounds__(kPagedThreads) paged_attention_kernel(const Pa
 #pragma unroll
                     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-                        for (int e = 0; e < 2; ++e) ka[mt][e] = lds128(from + k_off[j & 1] + (j >> 1) * 128 + (16 * mt + 8 * e) * S::kRow);
+                        for (int e = 0; e < 2; ++e) ka[mt][e] = lds128(from + k_off[j & 1] + (j >> 1) * KT * 128 + (16 * mt + 8 * e) * S::kPitch);
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
                         uint32_t kf[MT][2][4];
@@ -662,7 +714,7 @@ __global__ void __launch_bounds__(kPagedThreads) paged_attention_kernel(const Pa
             float vs[MT][2];
             float grow = 1.f;   // of the output's unit
             if constexpr (F16) {
-                const uint32_t scales = from + 2 * KT * S::kRow + 4 * g;
+                const uint32_t scales = smem_u32(my_scales) + slot * S::kScales + 4 * g;
                 float top = 0.f;
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt)
@@ -698,12 +750,12 @@ __global__ void __launch_bounds__(kPagedThreads) paged_attention_kernel(const Pa
                 for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) s[mt][nt][e] *= c[e & 1];
-                if (left < KT) {
+                if (edge) {
 #pragma unroll
                     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
-                            if (16 * mt + 8 * (e >> 1) + g >= left) s[mt][nt][e] = -INFINITY;
+                            if (16 * mt + 8 * (e >> 1) + g - ahead >= left - ahead) s[mt][nt][e] = -INFINITY;
                 }
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt)
@@ -762,11 +814,11 @@ __global__ void __launch_bounds__(kPagedThreads) paged_attention_kernel(const Pa
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         if constexpr (DP == 64) {
-                            const uint2 v = lds64(from + v_off[e & 1] + (16 * mt + 8 * (e >> 1)) * S::kRow);
+                            const uint2 v = lds64(from + v_off[e & 1] + (16 * mt + 8 * (e >> 1)) * S::kPitch);
                             v4[mt][e][0] = make_uint4(v.x, v.y, 0, 0);
                         } else {
 #pragma unroll
-                            for (int x = 0; x < DP / 128; ++x) v4[mt][e][x] = lds128(from + v_off[e & 1] + 128 * x + (16 * mt + 8 * (e >> 1)) * S::kRow);
+                            for (int x = 0; x < DP / 128; ++x) v4[mt][e][x] = lds128(from + v_off[e & 1] + x * KT * 128 + (16 * mt + 8 * (e >> 1)) * S::kPitch);
                         }
                     }
             }
@@ -795,7 +847,7 @@ __global__ void __launch_bounds__(kPagedThreads) paged_attention_kernel(const Pa
                             va[mt][3] = codes_f16<FORMAT, 1, 0>(w[2], w[3]);
                         }
                     } else {
-                        ldsm4_trans(va[mt], from + v_off[i & 3] + (i >> 2) * 128 + mt * 16 * S::kRow);
+                        ldsm4_trans(va[mt], from + v_off[i & 3] + (i >> 2) * KT * 128 + mt * 16 * S::kPitch);
                     }
                 }
 #pragma unroll
@@ -815,9 +867,9 @@ __global__ void __launch_bounds__(kPagedThreads) paged_attention_kernel(const Pa
                     unpack_f32x2(fma_f32x2(pack_f32x2(o[2], o[3]), scale_o[nt], pack_f32x2(d[2], d[3])), o[2], o[3]);
                 }
             }
-            slot = slot + 1 == a.stages ? 0 : slot + 1;
+            if (++slot == a.stages) slot = 0, phase ^= 1;
             __syncwarp();   // every lane has read the stage
-            copy_tile();
+            if (waiting) copy_tile();
         }
 
         // the lanes of a row add up
@@ -857,7 +909,6 @@ __global__ void __launch_bounds__(kPagedThreads) paged_attention_kernel(const Pa
             }
         }
     }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
 
     // ---- the block: what a warp left open, the next ones continue ----
     __syncwarp();
@@ -947,7 +998,8 @@ __global__ void __launch_bounds__(kPagedThreads) paged_attention_kernel(const Pa
 template <uint32_t FORMAT, int DP, int NT>
 PagedBuild paged_build() {
     using S = Shape<FORMAT, DP, NT>;
-    return PagedBuild{paged_attention_kernel<FORMAT, DP, NT>, (uint32_t)S::kStage, (uint32_t)S::kPart * 512u, (uint32_t)(S::kHeads * S::kQueryRow)};
+    return PagedBuild{paged_attention_kernel<FORMAT, DP, NT>, (uint32_t)S::kStage, (uint32_t)S::kPart * 512u, (uint32_t)(S::kHeads * S::kQueryRow),
+                      (uint32_t)S::kScales, (uint32_t)S::kKeys};
 }
 template <uint32_t FORMAT>
 PagedBuild paged_build_for(uint32_t dim, uint32_t nt) {
