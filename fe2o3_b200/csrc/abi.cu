@@ -357,8 +357,8 @@ int32_t check_ctx_device(fe2o3_ctx *ctx, const Region *r, int n) {
 // Appends to r from n on; returns the new count, or 0 with *status set.
 template <typename Args>
 int kv_cache_regions(const Args *a, Region *r, int n, bool writes, int32_t *status) {
-    if (a->kv_heads == 0 || a->dim == 0 || a->dim % 16 || a->dim > 256 || a->page_size == 0 || a->format > FE2O3_KV_I8) {
-        *status = unsupported("a key-value cache has kv_heads >= 1, dim a multiple of 16 up to 256, page_size >= 1, format bf16, e4m3 or i8");
+    if (a->kv_heads == 0 || a->kv_heads > 65536 || a->dim == 0 || a->dim % 16 || a->dim > 256 || a->page_size == 0 || a->format > FE2O3_KV_I8) {
+        *status = unsupported("a key-value cache has 1 to 65536 kv_heads, dim a multiple of 16 up to 256, page_size >= 1, format bf16, e4m3 or i8");
         return 0;
     }
     uint64_t rows;   // of one page
