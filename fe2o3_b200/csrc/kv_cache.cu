@@ -2,18 +2,22 @@
 // fe2o3_kv_cache_append_v1_args and fe2o3_kv_cache_read_v1_args.
 //
 // HBM-bound: each element is read once and written once.  A row is 2 to 32 lanes of eight columns each, so that a
-// row's largest magnitude is a shuffle tree and every access is 8, 16 or 32 bytes a lane; rows that do not start on 16
-// bytes are read or written element by element.  A block takes up to kTokens tokens, all their heads, K and V: it finds
-// their slots once (one look at the offsets and one at the page table), and each lane has kDeep rows in flight.
-// Quantisation needs the quotients as IEEE rounds them.  One division a row gives y, the reciprocal of the scale
-// rounded to nearest; q = x y, corrected twice by q + (x - q scale) y, is the correctly rounded quotient (Markstein,
-// Computation of elementary functions on the IBM RISC System/6000 processor, 1990) while nothing leaves the normal range:
-// scales outside 2^+-60 take the division itself.
+// row's largest magnitude is a shuffle tree and every access is 4 to 16 bytes a lane, without gaps between lanes: of f32 rows a
+// lane has four columns in each half (a store of every other 16 bytes costs half as much again).  Rows that do not
+// start on 16 bytes are read or written element by element.  A block takes up to kTokens tokens, all their heads, K and V: one
+// warp finds their slots (offsets, lengths and page table: three trips to memory a block, not a row), and each
+// lane has kDeep rows in flight.  Blocks are as many as fill the SMs a whole number of times.
+// Quantisation needs the quotients as IEEE rounds them, and is bound by issue slots.  One division a row gives y, the
+// reciprocal of the scale rounded to nearest; q = x y, corrected twice by q + (x - q scale) y, is the correctly rounded
+// quotient (Markstein, Computation of elementary functions on the IBM RISC System/6000 processor, 1990) while nothing
+// leaves the normal range: scales outside 2^+-60 take the division itself.
+#include <atomic>
+
 #include "kv_cache.cuh"
 
 namespace {
 
-constexpr int kThreads = 256, kTokens = 8, kDeep = 4;
+constexpr int kThreads = 256, kTokens = 32, kDeep = 4;
 
 struct KvRows {
     uint8_t *p[2];   // k, v: sources of an append, destinations of a read
@@ -23,75 +27,136 @@ struct KvRows {
     uint32_t whole;                                          // rows start on 16 bytes
 };
 
-// Row numbers of a token's head 0; ~0 where its page lies outside the cache.  false (reported) where the lengths do not allow it.
-__device__ __forceinline__ bool slot_of(const KvCache &c, const KvRows &r, uint32_t t, uint32_t &row) {
+// One warp, a lane a token: row number of its head 0, ~0 where its page lies outside the cache.  false (reported) where the
+// lengths do not allow the token a slot.
+__device__ __forceinline__ bool slot_of(const KvCache &c, const KvRows &r, uint32_t t0, uint32_t n, uint32_t &row) {
+    const uint32_t lane = threadIdx.x & 31, t = t0 + lane;
     uint32_t before = 1, own = 1, b = t;   // new tokens of the sequence: from this one on, and all
+    bool ok = lane < n;
     if (r.offsets) {
-        uint32_t n = 0;   // offsets at or below t: the sequence is the last of them (sequences without tokens share an offset)
-        const uint32_t lane = threadIdx.x & 31;
-        for (uint32_t i = 0; i <= c.batch; i += 32) n += __popc(__ballot_sync(~0u, i + lane <= c.batch && r.offsets[i + lane] <= t));
-        if (n == 0 || n > c.batch) {
-            kstatus_set(c.status, FE2O3_KSTATUS_LENGTH);
-            return false;
+        // offsets at or below a token: its sequence is the last of them (sequences without tokens share an offset)
+        uint32_t low = 0, high = 0;
+        for (uint32_t i = 0; i <= c.batch; i += 32) {
+            const uint32_t offset = i + lane <= c.batch ? r.offsets[i + lane] : ~0u;
+            low += __popc(__ballot_sync(~0u, offset <= t0));
+            high += __popc(__ballot_sync(~0u, offset <= t0 + n - 1));
         }
-        b = n - 1;
-        before = r.offsets[n] - t;
-        own = r.offsets[n] - r.offsets[n - 1];
+        uint32_t at = low;
+        while (ok && at < high && r.offsets[at] <= t) ++at;
+        ok = ok && at != 0 && at <= c.batch;
+        if (ok) {
+            b = at - 1;
+            before = r.offsets[at] - t;
+            own = r.offsets[at] - r.offsets[b];
+        }
     }
-    const uint32_t length = c.lengths[b];
-    if (length < own || !kv_fits(c, length)) {
-        kstatus_set(c.status, FE2O3_KSTATUS_LENGTH);
-        return false;
+    if (ok) {
+        const uint32_t length = c.lengths[b];
+        ok = length >= own && kv_fits(c, length);
+        if (ok) row = kv_row(c, b, 0, length - before);
     }
-    row = kv_row(c, b, 0, length - before);
-    return true;
+    if (!ok && lane < n) kstatus_set(c.status, FE2O3_KSTATUS_LENGTH);
+    return ok;
 }
 
-__device__ __forceinline__ void widen(const uint4 &v, float (&x)[8]) {
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        x[2 * i] = __uint_as_float(w[i] << 16);
-        x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-    }
+// A lane's eight columns: those from 8 l on, or for f32 rows four from 4 l and four from 4 (lanes + l) on.
+struct Columns {
+    uint32_t first, second;   // of the two fours
+    bool one, two;            // inside the row
+};
+__device__ __forceinline__ void widen4(const uint2 &v, float *x) {
+    x[0] = __uint_as_float(v.x << 16);
+    x[1] = __uint_as_float(v.x & 0xffff0000u);
+    x[2] = __uint_as_float(v.y << 16);
+    x[3] = __uint_as_float(v.y & 0xffff0000u);
 }
-__device__ __forceinline__ uint4 narrow(const float (&x)[8]) {
-    return make_uint4(f32_to_bf16_bits(x[0]) | f32_to_bf16_bits(x[1]) << 16, f32_to_bf16_bits(x[2]) | f32_to_bf16_bits(x[3]) << 16,
-                      f32_to_bf16_bits(x[4]) | f32_to_bf16_bits(x[5]) << 16, f32_to_bf16_bits(x[6]) | f32_to_bf16_bits(x[7]) << 16);
+__device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {   // to nearest even
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
 }
-// Eight columns in memory order, as they are: f32 takes both halves.
+__device__ __forceinline__ uint2 narrow4(const float *x) { return make_uint2(bf16_pair(x[0], x[1]), bf16_pair(x[2], x[3])); }
+__device__ __forceinline__ uint4 joined(uint2 a, uint2 b) { return make_uint4(a.x, a.y, b.x, b.y); }
+
+// The caller's rows: f32 bits as two fours, or eight bf16.
 template <bool F32>
-__device__ __forceinline__ void fetch(const uint8_t *at, bool whole, uint4 (&v)[2]) {
-    if (whole) {
-        v[0] = __ldcs(reinterpret_cast<const uint4 *>(at));
-        if constexpr (F32) v[1] = __ldcs(reinterpret_cast<const uint4 *>(at + 16));
-    } else if constexpr (F32) {
-        const uint32_t *const e = reinterpret_cast<const uint32_t *>(at);
-        v[0] = make_uint4(e[0], e[1], e[2], e[3]);
-        v[1] = make_uint4(e[4], e[5], e[6], e[7]);
-    } else {
-        const uint16_t *const e = reinterpret_cast<const uint16_t *>(at);
-        v[0] = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
-    }
-}
-template <bool F32>
-__device__ __forceinline__ void put(uint8_t *at, bool whole, const float (&x)[8]) {
+__device__ __forceinline__ void fetch(const uint8_t *row, const Columns &c, bool whole, uint4 (&v)[2]) {
     if constexpr (F32) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            if (!(half ? c.two : c.one)) continue;
+            const uint32_t *const e = reinterpret_cast<const uint32_t *>(row) + (half ? c.second : c.first);
+            v[half] = whole ? __ldcs(reinterpret_cast<const uint4 *>(e)) : make_uint4(e[0], e[1], e[2], e[3]);
+        }
+    } else if (c.one) {
+        const uint16_t *const e = reinterpret_cast<const uint16_t *>(row) + c.first;
+        v[0] = whole ? __ldcs(reinterpret_cast<const uint4 *>(e))
+                     : make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
+    }
+}
+template <bool F32>
+__device__ __forceinline__ void put(uint8_t *row, const Columns &c, bool whole, const uint4 (&v)[2]) {
+    if constexpr (F32) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            if (!(half ? c.two : c.one)) continue;
+            uint32_t *const e = reinterpret_cast<uint32_t *>(row) + (half ? c.second : c.first);
+            if (whole) __stcs(reinterpret_cast<uint4 *>(e), v[half]);
+            else e[0] = v[half].x, e[1] = v[half].y, e[2] = v[half].z, e[3] = v[half].w;
+        }
+    } else if (c.one) {
+        uint16_t *const e = reinterpret_cast<uint16_t *>(row) + c.first;
+        const uint32_t w[4] = {v[0].x, v[0].y, v[0].z, v[0].w};
         if (whole) {
-            __stcs(reinterpret_cast<float4 *>(at), make_float4(x[0], x[1], x[2], x[3]));
-            __stcs(reinterpret_cast<float4 *>(at + 16), make_float4(x[4], x[5], x[6], x[7]));
+            __stcs(reinterpret_cast<uint4 *>(e), v[0]);
         } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) reinterpret_cast<float *>(at)[i] = x[i];
+            for (int i = 0; i < 8; ++i) e[i] = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
+        }
+    }
+}
+// The cache's rows, which start on 16 bytes: eight elements' bits.
+template <uint32_t FORMAT, bool F32>
+__device__ __forceinline__ uint4 fetch_cached(const uint8_t *row, const Columns &c) {
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if constexpr (FORMAT == FE2O3_KV_BF16) {
+        if constexpr (!F32) {
+            if (c.one) v = __ldcs(reinterpret_cast<const uint4 *>(row + 2 * c.first));
+        } else {
+            uint2 a = make_uint2(0, 0), b = a;
+            if (c.one) a = __ldcs(reinterpret_cast<const uint2 *>(row + 2 * c.first));
+            if (c.two) b = __ldcs(reinterpret_cast<const uint2 *>(row + 2 * c.second));
+            v = joined(a, b);
         }
     } else {
-        const uint4 v = narrow(x);
-        if (whole) {
-            __stcs(reinterpret_cast<uint4 *>(at), v);
+        if constexpr (!F32) {
+            if (c.one) {
+                const uint2 a = __ldcs(reinterpret_cast<const uint2 *>(row + c.first));
+                v.x = a.x;
+                v.y = a.y;
+            }
         } else {
-            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-            for (int i = 0; i < 8; ++i) reinterpret_cast<uint16_t *>(at)[i] = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
+            if (c.one) v.x = __ldcs(reinterpret_cast<const uint32_t *>(row + c.first));
+            if (c.two) v.y = __ldcs(reinterpret_cast<const uint32_t *>(row + c.second));
+        }
+    }
+    return v;
+}
+template <uint32_t FORMAT, bool F32>
+__device__ __forceinline__ void put_cached(uint8_t *row, const Columns &c, const uint4 &v) {
+    if constexpr (FORMAT == FE2O3_KV_BF16) {
+        if constexpr (!F32) {
+            if (c.one) *reinterpret_cast<uint4 *>(row + 2 * c.first) = v;
+        } else {
+            if (c.one) *reinterpret_cast<uint2 *>(row + 2 * c.first) = make_uint2(v.x, v.y);
+            if (c.two) *reinterpret_cast<uint2 *>(row + 2 * c.second) = make_uint2(v.z, v.w);
+        }
+    } else {
+        if constexpr (!F32) {
+            if (c.one) *reinterpret_cast<uint2 *>(row + c.first) = make_uint2(v.x, v.y);
+        } else {
+            if (c.one) *reinterpret_cast<uint32_t *>(row + c.first) = v.x;
+            if (c.two) *reinterpret_cast<uint32_t *>(row + c.second) = v.y;
         }
     }
 }
@@ -113,6 +178,17 @@ __device__ __forceinline__ void quotients(const float (&x)[8], float scale, floa
 #pragma unroll
         for (int i = 0; i < 8; ++i) q[i] = scale > 0.f ? __fdiv_rn(x[i], scale) : 0.f;   // (a NaN scale: codes 0)
     }
+}
+// top / C, rounded to nearest: the same corrections, with 1 / C known beforehand.
+template <uint32_t FORMAT>
+__device__ __forceinline__ float scale_of(float top) {
+    constexpr float kC = kKvTop<FORMAT>, kY = (float)(1.0 / kC);
+    if (top > 8.7e-19f && top < 1.1e18f) {
+        float r = top * kY;
+        r = fmaf(fmaf(-kC, r, top), kY, r);
+        return fmaf(fmaf(-kC, r, top), kY, r);
+    }
+    return __fdiv_rn(top, kC);
 }
 template <uint32_t FORMAT>
 __device__ __forceinline__ uint2 codes_of(const float (&q)[8]) {
@@ -156,88 +232,100 @@ __global__ void __launch_bounds__(kThreads) kv_rows_kernel(KvCache c, KvRows r) 
     constexpr uint32_t kEb = F32 ? 4 : 2;
     begin_after_previous();
     const uint32_t t0 = blockIdx.x * r.per_block, n = min(r.per_block, r.tokens - t0), lane = threadIdx.x & 31;
-    if (threadIdx.x == 0) known = 0;
-    __syncthreads();
-    for (uint32_t i = threadIdx.x >> 5; i < n; i += kThreads / 32) {
+    if (threadIdx.x < 32) {
         uint32_t row = ~0u;
-        const bool ok = slot_of(c, r, t0 + i, row);
-        if (lane == 0) {
-            slots[i] = row;
-            if (ok) atomicOr(&known, 1u << i);
-        }
+        const uint32_t ok = __ballot_sync(~0u, slot_of(c, r, t0, n, row));
+        slots[lane] = row;
+        if (lane == 0) known = ok;
     }
     __syncthreads();
-    const uint32_t lanes = 1u << r.lanes_log2, at_once = kThreads >> r.lanes_log2, column = (threadIdx.x & (lanes - 1)) * 8;
-    const bool inside = column < c.dim;
+    const uint32_t lanes = 1u << r.lanes_log2, at_once = kThreads >> r.lanes_log2, l = threadIdx.x & (lanes - 1);
+    const Columns columns = F32 ? Columns{4 * l, 4 * (lanes + l), 4 * l < c.dim, 4 * (lanes + l) < c.dim} : Columns{8 * l, 0, 8 * l < c.dim, false};
     const uint32_t rows = n * 2 * c.kv_heads;
     for (uint32_t base = 0; base < rows; base += kDeep * at_once) {
         const uint32_t first = base + (threadIdx.x >> r.lanes_log2);
         uint4 raw[kDeep][2];
         float scales[kDeep];
         uint32_t at[kDeep], side[kDeep];
-        uint64_t there[kDeep];
+        uint8_t *there[kDeep];
         bool active[kDeep];
 #pragma unroll
         for (int d = 0; d < kDeep; ++d) {
-            const uint32_t i = min(first + d * at_once, rows - 1), of_side = r.heads_inverse ? __umulhi(i, r.heads_inverse) : i / c.kv_heads, h = i - of_side * c.kv_heads;   // head fastest, then K or V, then the token
-            const uint32_t token = of_side >> 1, slot = slots[token];
+            active[d] = false;
+            if (base + d * at_once >= rows) continue;   // (for the whole block)
+            // head fastest, then K or V, then the token
+            const uint32_t i = min(first + d * at_once, rows - 1), of_side = r.heads_inverse ? __umulhi(i, r.heads_inverse) : i / c.kv_heads;
+            const uint32_t h = i - of_side * c.kv_heads, token = of_side >> 1, slot = slots[token];
             side[d] = of_side & 1;
             at[d] = slot == ~0u ? ~0u : slot + h * c.page_size;
-            active[d] = inside && first + d * at_once < rows && (known >> token & 1) && (slot != ~0u || !WRITE);
-            there[d] = ((uint64_t)(t0 + token) * r.token_stride[side[d]] + (uint64_t)h * r.head_stride[side[d]] + column) * kEb;
+            active[d] = first + d * at_once < rows && (known >> token & 1) && (slot != ~0u || !WRITE);
+            there[d] = r.p[side[d]] + ((uint64_t)(t0 + token) * r.token_stride[side[d]] + (uint64_t)h * r.head_stride[side[d]]) * kEb;
             raw[d][0] = raw[d][1] = make_uint4(0, 0, 0, 0);
             scales[d] = 0.f;
             if (!active[d]) continue;
             if constexpr (WRITE) {
-                fetch<F32>(r.p[side[d]] + there[d], r.whole, raw[d]);
+                fetch<F32>(there[d], columns, r.whole, raw[d]);
             } else if (slot != ~0u) {
-                const uint8_t *const from = (side[d] ? c.v : c.k) + ((uint64_t)at[d] * c.dim + column) * kKvBytes<FORMAT>;
-                if constexpr (FORMAT == FE2O3_KV_BF16) {
-                    raw[d][0] = __ldcs(reinterpret_cast<const uint4 *>(from));
-                } else {
-                    const uint2 v = __ldcs(reinterpret_cast<const uint2 *>(from));
-                    raw[d][0].x = v.x;
-                    raw[d][0].y = v.y;
-                    scales[d] = (side[d] ? c.v_scales : c.k_scales)[at[d]];
-                }
+                raw[d][0] = fetch_cached<FORMAT, F32>((side[d] ? c.v : c.k) + (uint64_t)at[d] * c.dim * kKvBytes<FORMAT>, columns);
+                if constexpr (FORMAT != FE2O3_KV_BF16) scales[d] = (side[d] ? c.v_scales : c.k_scales)[at[d]];
             }
         }
 #pragma unroll
         for (int d = 0; d < kDeep; ++d) {
+            if (base + d * at_once >= rows) break;
+            if constexpr (FORMAT == FE2O3_KV_BF16 && !F32) {   // as it is
+                if (!active[d]) continue;
+                if constexpr (WRITE) put_cached<FORMAT, F32>((side[d] ? c.v : c.k) + (uint64_t)at[d] * c.dim * 2, columns, raw[d][0]);
+                else put<F32>(there[d], columns, r.whole, raw[d]);
+                continue;
+            }
             float x[8];
             if constexpr (WRITE) {
-                uint8_t *const to = (side[d] ? c.v : c.k) + ((uint64_t)at[d] * c.dim + column) * kKvBytes<FORMAT>;
-                if constexpr (FORMAT == FE2O3_KV_BF16 && !F32) {
-                    if (active[d]) *reinterpret_cast<uint4 *>(to) = raw[d][0];
-                } else {
-                    if constexpr (F32) {
-                        const uint32_t w[8] = {raw[d][0].x, raw[d][0].y, raw[d][0].z, raw[d][0].w, raw[d][1].x, raw[d][1].y, raw[d][1].z, raw[d][1].w};
+                uint8_t *const to = (side[d] ? c.v : c.k) + (uint64_t)at[d] * c.dim * kKvBytes<FORMAT>;
+                // the largest magnitude as bits: an infinity or a NaN is above every number
+                uint32_t top = 0;
+                if constexpr (F32) {
+                    const uint32_t w[8] = {raw[d][0].x, raw[d][0].y, raw[d][0].z, raw[d][0].w, raw[d][1].x, raw[d][1].y, raw[d][1].z, raw[d][1].w};
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(w[i]);
-                    } else {
-                        widen(raw[d][0], x);
+                    for (int i = 0; i < 8; ++i) {
+                        x[i] = __uint_as_float(w[i]);
+                        top = max(top, w[i] & 0x7fffffffu);
                     }
-                    if constexpr (FORMAT == FE2O3_KV_BF16) {
-                        if (active[d]) *reinterpret_cast<uint4 *>(to) = narrow(x);
-                    } else {
-                        // the largest magnitude as bits: an infinity or a NaN is above every number
-                        uint32_t top = 0;
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
-                        for (uint32_t o = 1; o < lanes; o <<= 1) top = max(top, __shfl_xor_sync(~0u, top, o));
-                        const float scale = top < 0x7f800000u ? __fdiv_rn(__uint_as_float(top), kKvTop<FORMAT>) : __uint_as_float(0x7fc00000u);
-                        float q[8];
-                        quotients(x, scale, q);
-                        if (active[d]) {
-                            *reinterpret_cast<uint2 *>(to) = codes_of<FORMAT>(q);
-                            if (column == 0) (side[d] ? c.v_scales : c.k_scales)[at[d]] = scale;
-                        }
+                } else {
+                    widen4(make_uint2(raw[d][0].x, raw[d][0].y), x);
+                    widen4(make_uint2(raw[d][0].z, raw[d][0].w), x + 4);
+                    const uint32_t pairs = __vmaxu2(__vmaxu2(raw[d][0].x & 0x7fff7fffu, raw[d][0].y & 0x7fff7fffu),
+                                                    __vmaxu2(raw[d][0].z & 0x7fff7fffu, raw[d][0].w & 0x7fff7fffu));
+                    top = max(pairs << 16, pairs & 0xffff0000u);
+                }
+                if constexpr (FORMAT == FE2O3_KV_BF16) {
+                    if (active[d]) put_cached<FORMAT, F32>(to, columns, joined(narrow4(x), narrow4(x + 4)));
+                } else {
+                    for (uint32_t o = 1; o < lanes; o <<= 1) top = max(top, __shfl_xor_sync(~0u, top, o));
+                    const float scale = top < 0x7f800000u ? scale_of<FORMAT>(__uint_as_float(top)) : __uint_as_float(0x7fc00000u);
+                    float q[8];
+                    quotients(x, scale, q);
+                    if (active[d]) {
+                        const uint2 w = codes_of<FORMAT>(q);
+                        put_cached<FORMAT, F32>(to, columns, make_uint4(w.x, w.y, 0, 0));
+                        if (l == 0) (side[d] ? c.v_scales : c.k_scales)[at[d]] = scale;
                     }
                 }
             } else {
-                if constexpr (FORMAT == FE2O3_KV_BF16) widen(raw[d][0], x);
-                else values_of<FORMAT>(make_uint2(raw[d][0].x, raw[d][0].y), scales[d], x);
-                if (active[d]) put<F32>(r.p[side[d]] + there[d], r.whole, x);
+                if constexpr (FORMAT == FE2O3_KV_BF16) {
+                    widen4(make_uint2(raw[d][0].x, raw[d][0].y), x);
+                    widen4(make_uint2(raw[d][0].z, raw[d][0].w), x + 4);
+                } else {
+                    values_of<FORMAT>(make_uint2(raw[d][0].x, raw[d][0].y), scales[d], x);
+                }
+                uint4 v[2];
+                if constexpr (F32) {
+                    v[0] = make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+                    v[1] = make_uint4(__float_as_uint(x[4]), __float_as_uint(x[5]), __float_as_uint(x[6]), __float_as_uint(x[7]));
+                } else {
+                    v[0] = joined(narrow4(x), narrow4(x + 4));
+                }
+                if (active[d]) put<F32>(there[d], columns, r.whole, v);
             }
         }
     }
@@ -248,9 +336,18 @@ using Kernel = void (*)(KvCache, KvRows);
 template <typename Args>
 int32_t launch_rows(fe2o3_ctx *ctx, cudaStream_t s, const Args *a, uint32_t dtype, fe2o3_geometry *geo, bool plan_only,
                     const Kernel (&kernels)[3][2], const char *what) {
-    // tokens of a block: as many as leave every SM two blocks, up to kTokens
-    uint32_t per_block = a->tokens / (2 * (ctx->sm_count > 0 ? ctx->sm_count : 1));
-    per_block = per_block < 1 ? 1 : per_block > kTokens ? kTokens : per_block;
+    // tokens of a block: up to a warp's lanes, and blocks that fill the SMs a whole number of times
+    static std::atomic<int> per_sm[3][2];   // of each kernel, found once
+    const int i = dtype == FE2O3_DTYPE_F32;
+    int fit = per_sm[a->format][i].load(std::memory_order_relaxed);
+    if (fit == 0) {
+        const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, kernels[a->format][i], kThreads, 0);
+        if (e != cudaSuccess) return fe2o3_cuda_status(e, what);
+        per_sm[a->format][i].store(fit < 1 ? fit = 1 : fit, std::memory_order_relaxed);
+    }
+    const uint64_t resident = (uint64_t)fit * (ctx->sm_count > 0 ? ctx->sm_count : 1);
+    const uint64_t waves = (a->tokens + resident * kTokens - 1) / (resident * kTokens);
+    const uint32_t per_block = a->tokens ? ceil_div_u32(a->tokens, resident * waves) : 1;
     const uint32_t grid = ceil_div_u32(a->tokens, per_block);
     if (geo) *geo = fe2o3_geometry{{grid, 1, 1}, {kThreads, 1, 1}, 0, 1};
     if (plan_only || a->tokens == 0) return FE2O3_OK;
@@ -265,10 +362,10 @@ int32_t launch_rows(fe2o3_ctx *ctx, cudaStream_t s, const Args *a, uint32_t dtyp
                    a->tokens,
                    per_block,
                    lanes_log2,
-                   // exact for the indexes of a block, below 16 kv_heads
-                   a->kv_heads == 1 || a->kv_heads > 8192 ? 0 : (uint32_t)((0x100000000ull + a->kv_heads - 1) / a->kv_heads),
+                   // exact for the indexes of a block, below 64 kv_heads
+                   a->kv_heads == 1 || a->kv_heads > 4096 ? 0 : (uint32_t)((0x100000000ull + a->kv_heads - 1) / a->kv_heads),
                    odd % 16 == 0};
-    const cudaError_t e = fe2o3_launch_early(kernels[a->format][dtype == FE2O3_DTYPE_F32], grid, kThreads, 0, s, 1, kv_cache_of(ctx, a), r);
+    const cudaError_t e = fe2o3_launch_early(kernels[a->format][i], grid, kThreads, 0, s, 1, kv_cache_of(ctx, a), r);
     fe2o3_count_launch(1);
     return fe2o3_cuda_status(e, what);
 }
