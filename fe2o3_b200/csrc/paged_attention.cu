@@ -113,7 +113,7 @@ int32_t paged_attention_plan(fe2o3_ctx *ctx, const fe2o3_paged_attention_v1_args
     cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void *>(b.kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, (int)p->shared);
     if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, b.kernel, kPagedThreads, p->shared);
     p->grid = (uint32_t)(per_sm > 0 ? per_sm : 1) * ctx->sm_count;
-    const size_t slots = (size_t)kPagedSlots * p->grid * b.part;
+    const size_t slots = (size_t)kPagedSlots * p->grid * b.part;   // behind them: counters
     p->device = ctx->device;
     p->bytes = (slots + p->grid * sizeof(uint32_t) + 65535) / 65536 * 65536;
     Workspaces *const workspaces = workspaces_of(ctx->device);
@@ -139,11 +139,12 @@ int32_t paged_attention_plan(fe2o3_ctx *ctx, const fe2o3_paged_attention_v1_args
         const auto make = eb == 2 ? fe2o3_make_tmap_bf16 : fe2o3_make_tmap_u8;
         if (make(&p->map_k, a->k_cache.ptr, 3, dims, strides, shape) != FE2O3_OK || make(&p->map_v, a->v_cache.ptr, 3, dims, strides, shape) != FE2O3_OK) box = 1;
     }
+    uint32_t *const counters = reinterpret_cast<uint32_t *>(static_cast<uint8_t *>(p->workspace) + slots);
     int32_t shift = -1;
     if ((a->page_size & (a->page_size - 1)) == 0) shift = __builtin_ctz(a->page_size);
     p->args = PagedArgs{kv_cache_of(ctx, a), reinterpret_cast<const void *>(a->q.ptr), reinterpret_cast<void *>(a->output.ptr),
                         reinterpret_cast<float *>(a->lse.ptr), static_cast<float4 *>(p->workspace),
-                        reinterpret_cast<uint32_t *>(static_cast<uint8_t *>(p->workspace) + slots), group, (group + 8 * nt - 1) / (8 * nt),
+                        counters, group, (group + 8 * nt - 1) / (8 * nt),
                         a->q_stride, a->q_head_stride, a->window, stages, shift, box, a->scale, a->q_dtype == FE2O3_DTYPE_F32,
                         a->output_dtype == FE2O3_DTYPE_F32, whole};
     *out = p;

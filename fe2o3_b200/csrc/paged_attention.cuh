@@ -38,10 +38,9 @@ struct PagedArgs {
     float scale;
     bool q_f32, o_f32, q_whole;   // q_whole: rows of the queries start on 16 bytes
 };
-// Of a block in the workspace: the end of an item that began in an earlier block; the ends that its warps 1 to 3 found of
-// items that began in an earlier warp; the beginning of an item that goes on in the next block.
-constexpr uint32_t kPagedSlots = 5, kSlotFirst = 0, kSlotLast = 4;
-
+// The partial results of a block in the workspace: the end of an item that began in an earlier block, the beginning of one that
+// goes on in the next, and the ends that its warps 1 to 3 found of items that an earlier warp of the block began.
+constexpr uint32_t kPagedSlots = 5, kSlotFirst = 0, kSlotLast = 1, kSlotEnds = 2;
 constexpr uint32_t kPagedMaxStages = 4, kPagedMeeting = 512;
 
 using PagedKernel = void (*)(CUtensorMap, CUtensorMap, PagedArgs);
@@ -187,14 +186,48 @@ constexpr uint32_t kLeast = 3;   // places a warp has at least, where there are 
 constexpr uint32_t kInvalid = ~0u;
 // What a warp's share ends in: whole items only; an item that begins in the share and goes on; one that goes on on both sides; no places.
 enum : uint32_t { kNone, kBegun, kWithin, kEmpty };
+struct Left {
+    uint32_t kind, end_of_first, seq, item, n, places;   // end_of_first: an item that began before the share ended in it
+    uint64_t i0;                                         // where on the line the open item begins
+};
 struct Job {
-    uint32_t seq, item, n, block, pieces;   // pieces 0: none
+    uint32_t seq, item, n, block, pieces;   // pieces 0: none; before the count: the item's places
+    uint64_t i0;
+};
+__device__ __forceinline__ uint32_t running_sum(uint32_t v, uint32_t lane) {
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const uint32_t u = __shfl_up_sync(~0u, v, d);
+        if (lane >= d) v += u;
+    }
+    return v;
+}
+// How the line is cut: an equal share a warp.
+struct Line {
+    uint64_t total;          // places
+    uint32_t blocks, q, r;   // at work; total / (4 blocks) and what is over
+    __device__ __forceinline__ Line(const PagedArgs &a, uint64_t total, uint32_t per_seq) : total(total) {
+        const uint64_t wanted = (total + kLeast * kPagedWarps - 1) / (kLeast * kPagedWarps);
+        blocks = wanted < gridDim.x ? (uint32_t)wanted : gridDim.x;
+        // as many blocks an item for all, where that leaves few idle or there is little to do: items of one length then end with a block
+        const uint32_t items = a.c.batch * per_seq;
+        if (items <= blocks && (wanted < gridDim.x || blocks % items * 16 <= blocks)) blocks -= blocks % items;
+        const uint32_t warps = blocks * kPagedWarps;
+        const uint64_t each = total >> 32 ? total / warps : (uint32_t)total / warps;
+        q = (uint32_t)each;
+        r = (uint32_t)(total - each * warps);
+    }
+    __device__ __forceinline__ void share(uint32_t me, uint64_t &begin, uint32_t &n) const {
+        const uint32_t warps = blocks * kPagedWarps, over = r * me / warps;
+        begin = (uint64_t)q * me + over;
+        n = q + r * (me + 1) / warps - over;
+    }
+    __device__ __forceinline__ uint32_t block_of(uint64_t place) const { return (uint32_t)(((place + 1) * blocks - 1) / total); }
 };
 // What a block has in shared memory beside rings and queries (all of it in the dynamic part, which then starts on a swizzle pattern).
 struct Meeting {
     uint64_t arrivals[kPagedWarps][kPagedMaxStages];
-    float head_scales[kPagedWarps][16];
-    uint32_t kinds[kPagedWarps], ends[kPagedWarps];
+    Left left[kPagedWarps];
     Job jobs[2];
 };
 static_assert(sizeof(Meeting) <= kPagedMeeting, "");
@@ -271,7 +304,7 @@ struct Part {
 };
 
 template <uint32_t FORMAT, int DP, int NT>
-__global__ void __launch_bounds__(kPagedThreads)
+__global__ void __launch_bounds__(kPagedThreads, DP == 256 || NT == 2 ? 1 : 3)
 paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ PagedArgs a) {
     using S = Shape<FORMAT, DP, NT>;
     using P = Part<DP / 16, NT>;
@@ -286,14 +319,10 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     uint8_t *const queries = smem + kPagedWarps * a.stages * (S::kStage + S::kScales);
     uint8_t *const query = queries + warp * terms * S::kHeads * S::kQueryRow;
     Meeting &meeting = *reinterpret_cast<Meeting *>(queries + kPagedWarps * terms * S::kHeads * S::kQueryRow);
-    uint32_t (&kinds)[kPagedWarps] = meeting.kinds, (&ends)[kPagedWarps] = meeting.ends;
-    Job (&jobs)[2] = meeting.jobs;
     const uint32_t query_s = smem_u32(query);
-    float *const head_scale = meeting.head_scales[warp];
     const uint32_t row_bytes = a.c.dim * (F16 ? 1 : 2);
     const uint32_t per_seq = a.c.kv_heads * a.chunks;   // items of a sequence
 
-    if (threadIdx.x < 2) jobs[threadIdx.x].pieces = 0;
     uint64_t *const bars = meeting.arrivals[warp];
     if (lane < a.stages) mbar_init(&bars[lane], a.box > 1 ? 1 : 32);
     mbar_fence_init();
@@ -311,69 +340,25 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     __syncwarp();
     begin_after_previous();
 
-    // ---- this warp's share of the line: every warp adds up the sequences for itself ----
-    uint64_t total = 0;
-    constexpr uint32_t kHeld = 4;   // sequences a lane keeps the places of: one trip to memory for 128
-    uint32_t held[kHeld];
-#pragma unroll
-    for (uint32_t i = 0; i < kHeld; ++i) {
-        held[i] = 32 * i + lane < a.c.batch ? Span<KT>(a, 32 * i + lane).places() : 0;
-        total += held[i];
-    }
-    for (uint32_t b = 32 * kHeld + lane; b < a.c.batch; b += 32) total += Span<KT>(a, b).places();
-#pragma unroll
-    for (int d = 16; d; d >>= 1) total += __shfl_xor_sync(~0u, total, d);
-    total *= per_seq;
-    const uint64_t wanted = (total + kLeast * kPagedWarps - 1) / (kLeast * kPagedWarps);
-    uint32_t blocks = wanted < gridDim.x ? (uint32_t)wanted : gridDim.x;
-    // as many blocks an item for all, where that leaves few idle or there is little to do: items of one length then end with a block
-    const uint32_t items = a.c.batch * per_seq;
-    if (items <= blocks && (wanted < gridDim.x || blocks % items * 16 <= blocks)) blocks -= blocks % items;
-    if (blockIdx.x >= blocks) return;
-    const uint64_t me = (uint64_t)blockIdx.x * kPagedWarps + warp, all = (uint64_t)blocks * kPagedWarps;
-    const uint64_t begin = total * me / all;
-    const uint32_t share = (uint32_t)(total * (me + 1) / all - begin);
-    Span<KT> span;
-    uint32_t seq = 0, item = 0, place = 0;   // where the share begins
-    {
-        uint64_t base = 0;
-        for (uint32_t b0 = 0;; b0 += 32) {
-            const uint32_t places = b0 == 0 ? held[0] : b0 == 32 ? held[1] : b0 == 64 ? held[2] : b0 == 96 ? held[3]
-                                    : b0 + lane < a.c.batch ? Span<KT>(a, b0 + lane).places() : 0;
-            const uint64_t mine = (uint64_t)places * per_seq;
-            uint64_t upto = mine;
-#pragma unroll
-            for (int d = 1; d < 32; d <<= 1) {
-                const uint64_t v = __shfl_up_sync(~0u, upto, d);
-                if (lane >= d) upto += v;
-            }
-            const uint32_t past = __ballot_sync(~0u, base + upto > begin);
-            if (past) {
-                const int at = __ffs(past) - 1;
-                seq = b0 + at;
-                base += __shfl_sync(~0u, upto - mine, at);
-                span = Span<KT>(a, seq);
-                const uint64_t in = begin - base;
-                item = (uint32_t)(in / span.places());
-                place = (uint32_t)(in - (uint64_t)item * span.places());
-                break;
-            }
-            base += __shfl_sync(~0u, upto, 31);
-            if (b0 + 32 >= a.c.batch) break;   // not reached while the lengths stay as they are
-        }
-    }
+    // ---- the line: every warp adds up the sequences for itself, a run of them a lane ----
+    const uint32_t run = (a.c.batch + 31) / 32;
+    uint32_t own = 0, before;
+    for (uint32_t i = 0; i < run; ++i)
+        if (lane * run + i < a.c.batch) own += Span<KT>(a, lane * run + i).places();
+    const uint64_t total = (uint64_t)__shfl_sync(~0u, before = running_sum(own, lane), 31) * per_seq;
+    before -= own;
+    const Line line(a, total, per_seq);
+    if (blockIdx.x >= line.blocks) return;
 
-    // ---- copies: a cursor of its own runs ahead over this warp's tiles ----
-    Span<KT> lspan = span;
-    uint32_t lseq = seq, litem = item, lslot = 0, lrest = share;   // places of the share from its present item's on
-    uint32_t ltile, lend;
+    // ---- copies: the places of the share, by a cursor that runs ahead over its tiles ----
+    Span<KT> lspan;
+    uint32_t lseq = 0, litem = 0, lslot = 0, lrest = 0, ltile = 0, lend = 0;   // lrest: places of the share behind its present item
     auto enter = [&](uint32_t from) {   // the cursor's item, from this place on
         const uint32_t take = min(lspan.places() - from, lrest);
         ltile = max(from, kEnd) - kEnd;
         lend = max(from + take, kEnd) - kEnd;
         lrest -= take;
     };
-    enter(place);
     uint32_t entry = 0, entries_from = 0, entries_of = ~0u;   // 32 entries of a sequence's table, a lane each
     const uint32_t lrow = lane / kPieces, lpiece = lane % kPieces, boxes = KT / a.box;
     // Zeros for a row of a stage: K and V, and their scales.
@@ -459,8 +444,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         lslot = lslot + 1 == a.stages ? 0 : lslot + 1;
         ++ltile;
     };
-    for (uint32_t s = 0; s < a.stages; ++s) copy_tile();
-
+    uint32_t seq, item;   // at work
     // ---- the queries of an item, as 16-bit terms: a lane takes eight columns of a row at a time ----
     auto lay_query = [&] {
         constexpr int kLanes = DP / 8, kAtOnce = 32 / kLanes, kPasses = S::kHeads / kAtOnce;
@@ -532,13 +516,14 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                     }
                 }
             }
-            if (lane % kLanes == 0) head_scale[row] = a.scale * 1.4426950408889634f * back;
+            if (lane % kLanes == 0) *reinterpret_cast<float *>(query + row * S::kQueryRow + 2 * DP) = a.scale * 1.4426950408889634f * back;   // (in the padding)
         }
         __syncwarp();
     };
 
-    // Writes an item's result.
-    auto write = [&](const P &p, uint32_t seq, uint32_t item, uint32_t n) {
+    // Writes an item's result, or the columns of it from output tile i0 on.
+    auto write = [&](const auto &p, uint32_t seq, uint32_t item, uint32_t n, uint32_t i0) {
+        constexpr int kTiles = sizeof(p.o) / sizeof(p.o[0]);
         const uint32_t head = item / a.chunks, chunk = item % a.chunks;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -548,38 +533,25 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                 if (in_group >= a.group) continue;
                 const uint64_t row = (uint64_t)seq * a.c.kv_heads * a.group + head * a.group + in_group;
                 const float l = p.l[nt][e], inv = n ? 1.f / l : 0.f;
-                const uint32_t g_at = column_of<FORMAT, DP>(0, g);
-                float *const o32 = static_cast<float *>(a.o) + row * a.c.dim + g_at;
-                uint16_t *const o16 = static_cast<uint16_t *>(a.o) + row * a.c.dim + g_at;
+                float *const o32 = static_cast<float *>(a.o) + row * a.c.dim;
+                uint16_t *const o16 = static_cast<uint16_t *>(a.o) + row * a.c.dim;
 #pragma unroll
-                for (int i = 0; i < MD; ++i) {
+                for (int i = 0; i < kTiles; ++i) {
                     const float v0 = p.o[i][nt][e] * inv, v1 = p.o[i][nt][2 + e] * inv;
-                    if constexpr (F16) {   // columns in a row of their own
-                        if (g_at + (DP == 256 ? 128 * (i >> 3) : 0) >= a.c.dim) continue;
-                        if (a.o_f32) {
-                            o32[column_of<FORMAT, DP>(i, 0)] = v0;
-                            o32[column_of<FORMAT, DP>(i, 0) + 1] = v1;
-                        } else {
-                            o16[column_of<FORMAT, DP>(i, 0)] = bf16_of(v0);
-                            o16[column_of<FORMAT, DP>(i, 0) + 1] = bf16_of(v1);
-                        }
+                    const uint32_t d = column_of<FORMAT, DP>(i0 + i, g);   // the other row's column: 8 further, or the next
+                    constexpr uint32_t kNext = F16 ? 1 : 8;
+                    if (d >= a.c.dim) continue;
+                    if (a.o_f32) {
+                        o32[d] = v0;
+                        o32[d + kNext] = v1;
                     } else {
-                        if (16 * i >= a.c.dim) continue;
-                        if (a.o_f32) {
-                            o32[16 * i] = v0;
-                            o32[16 * i + 8] = v1;
-                        } else {
-                            o16[16 * i] = bf16_of(v0);
-                            o16[16 * i + 8] = bf16_of(v1);
-                        }
+                        o16[d] = bf16_of(v0);
+                        o16[d + kNext] = bf16_of(v1);
                     }
                 }
-                if (a.lse && g == 0) a.lse[row] = n ? (p.m[nt][e] + log2f(l)) * 0.6931471805599453f : -INFINITY;
+                if (a.lse && g == 0 && i0 == 0) a.lse[row] = n ? (p.m[nt][e] + log2f(l)) * 0.6931471805599453f : -INFINITY;
             }
     };
-    float4 *const slots = a.slots + (uint64_t)blockIdx.x * kPagedSlots * S::kPart * 32 + lane;
-    auto to_slot = [&](const P &p, uint32_t slot) { p.leave([&](int i, float4 v) { slots[(slot * S::kPart + i) * 32] = v; }); };
-
     // where a lane reads K and V in a stage; a lane's offsets for further steps differ by constants
     uint32_t k_off[4], v_off[4];
 #pragma unroll
@@ -596,12 +568,45 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         }
     }
 
-    // ---- the share, item by item ----
+    uint32_t slot = 0, phase = 0;
+    bool waiting = true;
+    uint64_t begin;
+    uint32_t share;
+    line.share(blockIdx.x * kPagedWarps + warp, begin, share);
+    float4 *const slots = a.slots + (uint64_t)blockIdx.x * kPagedSlots * S::kPart * 32 + lane;
+    uint32_t place = 0;   // of the item, where the share begins
+    {
+        const uint32_t in = __ffs(__ballot_sync(~0u, (uint64_t)(before + own) * per_seq > begin)) - 1;   // the lane whose run it is
+        uint64_t base = (uint64_t)__shfl_sync(~0u, before, in) * per_seq;
+        seq = min(in * run, a.c.batch - 1);
+        for (uint32_t b0 = 0; run > 1 && b0 < run; b0 += 32) {
+            const uint32_t b = in * run + b0 + lane, places = b0 + lane < run && b < a.c.batch ? Span<KT>(a, b).places() : 0;
+            const uint32_t upto = running_sum(places, lane), past = __ballot_sync(~0u, base + (uint64_t)upto * per_seq > begin);
+            if (past) {
+                const int at = __ffs(past) - 1;
+                seq = in * run + b0 + at;
+                base += (uint64_t)__shfl_sync(~0u, upto - places, at) * per_seq;
+                break;
+            }
+            base += (uint64_t)__shfl_sync(~0u, upto, 31) * per_seq;
+        }
+        lspan = Span<KT>(a, seq);
+        const uint64_t into = min(begin - base, (uint64_t)lspan.places() * per_seq - 1);
+        item = into >> 32 ? (uint32_t)(into / lspan.places()) : (uint32_t)into / lspan.places();
+        place = (uint32_t)(into - (uint64_t)item * lspan.places());
+    }
+    Span<KT> span = lspan;
     const Span<KT> first_span = span;
     const uint32_t first_seq = seq, first_item = item, first_place = place;
+    lseq = seq;
+    litem = item;
+    lrest = share;
+    enter(place);
+    for (uint32_t s = 0; s < a.stages; ++s) copy_tile();
+
+    // ---- the share, item by item ----
     P p;
-    uint32_t kind = share ? kNone : kEmpty, slot = 0, phase = 0;
-    bool waiting = true;
+    uint32_t kind = share ? kNone : kEmpty;
     uint64_t i0 = 0;        // where on the line the last item begins
     uint32_t end_of_first = 0;
     for (uint32_t at = 0; at < share;) {
@@ -744,7 +749,8 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
             uint64_t scale_o[NT];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-                const float c[2] = {head_scale[8 * nt + 2 * t4], head_scale[8 * nt + 2 * t4 + 1]};
+                const uint32_t c_at = query_s + (8 * nt + 2 * t4) * S::kQueryRow + 2 * DP;
+                const float c[2] = {lds_f32(c_at), lds_f32(c_at + S::kQueryRow)};
                 float top[2] = {p.m[nt][0], p.m[nt][1]};
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt)
@@ -891,10 +897,11 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         i0 = begin + at - place;
         if (ended) {
             if (!begins) {
-                to_slot(p, kSlotFirst + warp);
+                float4 *const to = slots + (warp ? kSlotEnds + warp - 1 : kSlotFirst) * S::kPart * 32;
+                p.leave([&](int i, float4 v) { to[i * 32] = v; });
                 end_of_first = 1;
             } else if (span.valid) {
-                write(p, seq, item, span.n);
+                write(p, seq, item, span.n, 0);
             }
         } else {
             kind = begins ? kBegun : kWithin;
@@ -910,88 +917,85 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         }
     }
 
-    // ---- the block: what a warp left open, the next ones continue ----
-    __syncwarp();
+    // ---- the block: what its warps left open, each of them a quarter of the columns ----
     float4 *const my_part = reinterpret_cast<float4 *>(my_ring) + lane;   // the ring is free now
-    if (kind == kWithin && warp) p.leave([&](int i, float4 v) { my_part[i * 32] = v; });
-    if (lane == 0) {
-        kinds[warp] = kind;
-        ends[warp] = end_of_first;
+    if (kind == kBegun || kind == kWithin) {
+        __syncwarp();
+        p.leave([&](int i, float4 v) { my_part[i * 32] = v; });
     }
+    if (lane == 0) meeting.left[warp] = Left{kind, end_of_first, seq, item, span.valid ? span.n : kInvalid, span.places(), i0};
+    if (threadIdx.x < 2) meeting.jobs[threadIdx.x].pieces = 0;
     __threadfence_block();
     __syncthreads();
-    auto arrive = [&](uint32_t role, uint64_t i0, uint32_t places, uint32_t seq, uint32_t item, uint32_t n) {   // this block's piece lies in its slot
-        const uint32_t c0 = (uint32_t)(((i0 + 1) * blocks - 1) / total), c1 = (uint32_t)(((i0 + places) * blocks - 1) / total);
-        __threadfence();
-        __syncwarp();
-        if (lane == 0 && atomicAdd(&a.arrived[c0], 1u) == c1 - c0) {
-            a.arrived[c0] = 0;
-            jobs[role] = Job{seq, item, n, c0, c1 - c0 + 1};
-        }
+    constexpr int kQuarter = MD / kPagedWarps;
+    Part<kQuarter, NT> part;
+    auto add = [&](const float4 *from) {   // a whole part lies there
+        part.add([&](int i) { return from[(i < kQuarter * NT ? warp * kQuarter * NT + i : MD * NT + (i - kQuarter * NT)) * 32]; });
     };
-    const bool owner = kind == kBegun || (kind == kWithin && warp == 0);
-    bool went_on = owner;   // past the block's end
-    if (owner) {
-        for (uint32_t w = warp + 1; w < kPagedWarps && went_on; ++w) {
-            const float4 *const theirs = reinterpret_cast<const float4 *>(smem + w * a.stages * S::kStage) + lane;
-            if (kinds[w] == kWithin) {
-                p.add([&](int i) { return theirs[i * 32]; });
-            } else if (ends[w]) {
-                p.add([&](int i) { return __ldcg(slots + (w * S::kPart + i) * 32); });
-                went_on = false;
-            }
+#pragma unroll 1
+    for (uint32_t w = 0; w < kPagedWarps; ++w) {   // an item that warp w was the first of the block to leave open
+        const Left left = meeting.left[w];
+        if (left.kind != kBegun && (left.kind != kWithin || w)) continue;
+        part.clear();
+        add(reinterpret_cast<const float4 *>(smem + w * a.stages * S::kStage) + lane);
+        bool open = true;
+#pragma unroll 1
+        for (uint32_t v = w + 1; v < kPagedWarps && open; ++v) {
+            const Left &other = meeting.left[v];
+            if (other.kind != kWithin && !other.end_of_first) continue;   // (no places)
+            open = other.kind == kWithin;
+            add(open ? reinterpret_cast<const float4 *>(smem + v * a.stages * S::kStage) + lane : slots + (kSlotEnds + v - 1) * S::kPart * 32);
         }
-    }
-    // an item that an earlier block began (warp 0 has it), and one that goes on in the next
-    if (warp == 0 && end_of_first) {
-        const uint64_t first = begin - first_place;
-        arrive(0, first, first_span.places(), first_seq, first_item, first_span.valid ? first_span.n : kInvalid);
-    }
-    if (owner) {
-        const uint32_t n = span.valid ? span.n : kInvalid;
-        if (kind == kBegun && !went_on) {
-            if (span.valid) write(p, seq, item, span.n);
+        if (left.kind == kBegun && !open) {
+            if (left.n != kInvalid) write(part, left.seq, left.item, left.n, warp * kQuarter);
         } else {
-            to_slot(p, kind == kBegun ? kSlotLast : kSlotFirst);
-            arrive(kind == kBegun, i0, span.places(), seq, item, n);
+            float4 *const to = slots + (left.kind == kBegun ? kSlotLast : kSlotFirst) * S::kPart * 32;
+            part.leave([&](int i, float4 v) {
+                if (i < kQuarter * NT) to[(warp * kQuarter * NT + i) * 32] = v;
+                else if (warp == 0) to[(MD * NT + (i - kQuarter * NT)) * 32] = v;
+            });
+            if (threadIdx.x == 0) meeting.jobs[left.kind == kBegun] = Job{left.seq, left.item, left.n, 0, left.places, left.i0};
         }
     }
+    if (threadIdx.x == 0 && end_of_first)   // an item of an earlier block that ended in warp 0: it lies in its slot
+        meeting.jobs[0] = Job{first_seq, first_item, first_span.valid ? first_span.n : kInvalid, 0, first_span.places(), begin - first_place};
 
-    // ---- the blocks: the last one to come joins the pieces, its warps some each ----
+    // ---- the blocks: the last one to come to an item joins its pieces, eight in flight ----
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x < 2) {
+        Job &job = meeting.jobs[threadIdx.x];
+        if (job.pieces) {
+            const uint32_t b0 = line.block_of(job.i0), pieces = line.block_of(job.i0 + job.pieces - 1) - b0 + 1;
+            job.block = b0;
+            job.pieces = pieces;
+            if (atomicAdd(&a.arrived[b0], 1u) == pieces - 1) a.arrived[b0] = 0;
+            else job.pieces = 0;
+        }
+    }
     __syncthreads();
 #pragma unroll 1
     for (int role = 0; role < 2; ++role) {
-        const Job job = jobs[role];
+        const Job job = meeting.jobs[role];
         if (!job.pieces) continue;
         __threadfence();
-        if (role) __syncthreads();   // warp 0 has read the rings
-        p.clear();
-        // (copied into the ring, as many as fit, so that a round costs one trip to the workspace)
-        const uint32_t at_once = a.stages * S::kStage / (S::kPart * 512);
+        part.clear();
+        constexpr int kAtOnce = kQuarter * NT <= 2 ? 8 : kQuarter * NT <= 4 ? 4 : 2, kLoads = (kQuarter + 1) * NT;
 #pragma unroll 1
-        for (uint32_t i0 = warp; i0 < job.pieces; i0 += kPagedWarps * at_once) {
-            const uint32_t n = min(at_once, (job.pieces - i0 + kPagedWarps - 1) / kPagedWarps);
-#pragma unroll 1
-            for (uint32_t k = 0; k < n; ++k) {
-                const uint32_t i = i0 + kPagedWarps * k;
-                const float4 *const from = a.slots + ((uint64_t)(job.block + i) * kPagedSlots + (i ? kSlotFirst : kSlotLast)) * S::kPart * 32 + lane;
+        for (uint32_t i = 0; i < job.pieces; i += kAtOnce) {
+            float4 v[kAtOnce][kLoads];
 #pragma unroll
-                for (int x = 0; x < S::kPart; ++x) copy16(ring + ((k * S::kPart + x) * 32 + lane) * 16, from + x * 32);
+            for (int x = 0; x < kAtOnce; ++x) {   // (beyond the last one: that again, which is not added)
+                const uint32_t piece = min(i + x, job.pieces - 1);
+                const float4 *const from = a.slots + ((uint64_t)(job.block + piece) * kPagedSlots + (piece ? kSlotFirst : kSlotLast)) * S::kPart * 32 + lane;
+#pragma unroll
+                for (int k = 0; k < kLoads; ++k) v[x][k] = __ldcg(from + (k < kQuarter * NT ? warp * kQuarter * NT + k : MD * NT + (k - kQuarter * NT)) * 32);
             }
-            asm volatile("cp.async.wait_all;" ::: "memory");
-#pragma unroll 1
-            for (uint32_t k = 0; k < n; ++k) p.add([&](int x) { return my_part[(k * S::kPart + x) * 32]; });
+#pragma unroll
+            for (int x = 0; x < kAtOnce; ++x)
+                if (i + x < job.pieces) part.add([&](int k) { return v[x][k]; });
         }
-        if (warp) p.leave([&](int i, float4 v) { my_part[i * 32] = v; });
-        __syncthreads();
-        if (warp == 0) {
-#pragma unroll 1
-            for (uint32_t w = 1; w < kPagedWarps; ++w) {
-                const float4 *const theirs = reinterpret_cast<const float4 *>(smem + w * a.stages * S::kStage) + lane;
-                p.add([&](int i) { return theirs[i * 32]; });
-            }
-            if (job.n != kInvalid) write(p, job.seq, job.item, job.n);
-        }
+        if (job.n != kInvalid) write(part, job.seq, job.item, job.n, warp * kQuarter);
     }
 }
 

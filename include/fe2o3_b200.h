@@ -472,7 +472,7 @@ typedef struct fe2o3_kv_cache_read_v1_args {
  *   output[b][h] = sum_j softmax_j(scale * q[b][h] . k_j) v_j,   lse[b][h] = log sum_j exp(scale * q[b][h] . k_j)
  * with the keys and values of head h / (heads / kv_heads).  heads is a multiple of kv_heads.  q row (b, h) starts at
  * element b * q_stride + h * q_head_stride; output [batch][heads][dim] is packed, f32 or bf16; lse
- * [batch][heads] f32 is optional.  A sequence of length 0 gives zeros and -inf.  Sums, maxima and
+ * [batch][heads] f32 is optional.  The page table has at most 2^36 positions, batch * heads is below 2^31.  A sequence of length 0 gives zeros and -inf.  Sums, maxima and
  * probabilities are f32 (for a bf16 output the probabilities have 16 significant bits).  The result does not
  * depend on which blocks finish first.  One launch of a prepared object at a time (it owns a workspace). */
 typedef struct fe2o3_paged_attention_v1_args {
