@@ -181,8 +181,8 @@ __device__ __forceinline__ uint32_t column_of(uint32_t i, uint32_t m) {
     else return (DP == 64 ? 8 * (m & 7) : 16 * (m & 7)) + (DP == 256 ? 128 * (i >> 3) + 2 * (i & 7) : 2 * i) + (m >> 3);
 }
 
-constexpr uint32_t kEnd = 1;     // places on the line in front of an item's tiles
-constexpr uint32_t kLeast = 3;   // places a warp has at least, where there are enough
+constexpr uint32_t kEnd = 2;     // places on the line in front of an item's tiles (ragged e4m3 71 us; 76 with 1, 70 with 3, short items then slower)
+constexpr uint32_t kLeast = 1;   // places a warp has at least (10 to 2000 keys a block: 9.7 us for 16 heads of 512 keys, 11.1 with 2, 11.8 with 3)
 constexpr uint32_t kInvalid = ~0u;
 // What a warp's share ends in: whole items only; an item that begins in the share and goes on; one that goes on on both sides; no places.
 enum : uint32_t { kNone, kBegun, kWithin, kEmpty };
@@ -206,8 +206,10 @@ __device__ __forceinline__ uint32_t running_sum(uint32_t v, uint32_t lane) {
 struct Line {
     uint64_t total;          // places
     uint32_t blocks, q, r;   // at work; total / (4 blocks) and what is over
+    uint32_t whole;          // items of up to so many places are not cut: they go to the warp that would have their larger half
     __device__ __forceinline__ Line(const PagedArgs &a, uint64_t total, uint32_t per_seq) : total(total) {
-        const uint64_t wanted = (total + kLeast * kPagedWarps - 1) / (kLeast * kPagedWarps);
+        // (several blocks: no warp is without a place, so that what an earlier block began is seen by warp 0)
+        const uint64_t wanted = max(total / (kLeast * kPagedWarps), (uint64_t)1);
         blocks = wanted < gridDim.x ? (uint32_t)wanted : gridDim.x;
         // as many blocks an item for all, where that leaves few idle or there is little to do: items of one length then end with a block
         const uint32_t items = a.c.batch * per_seq;
@@ -216,11 +218,16 @@ struct Line {
         const uint64_t each = total >> 32 ? total / warps : (uint32_t)total / warps;
         q = (uint32_t)each;
         r = (uint32_t)(total - each * warps);
+        whole = wanted < gridDim.x ? kEnd + 1 : max(4u, q / 8);   // (SMs to spare: two tiles are sooner done by two warps)
     }
     __device__ __forceinline__ void share(uint32_t me, uint64_t &begin, uint32_t &n) const {
         const uint32_t warps = blocks * kPagedWarps, over = r * me / warps;
         begin = (uint64_t)q * me + over;
         n = q + r * (me + 1) / warps - over;
+    }
+    // Places of an item that a share takes which would end (or begin) behind `some` of its places: none or all where it is not cut.
+    __device__ __forceinline__ uint32_t taken(uint32_t some, uint32_t places) const {
+        return places > whole || some >= places ? min(some, places) : 2 * some >= places ? places : 0;
     }
     __device__ __forceinline__ uint32_t block_of(uint64_t place) const { return (uint32_t)(((place + 1) * blocks - 1) / total); }
 };
@@ -354,10 +361,10 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     Span<KT> lspan;
     uint32_t lseq = 0, litem = 0, lslot = 0, lrest = 0, ltile = 0, lend = 0;   // lrest: places of the share behind its present item
     auto enter = [&](uint32_t from) {   // the cursor's item, from this place on
-        const uint32_t take = min(lspan.places() - from, lrest);
+        const uint32_t take = from ? min(lspan.places() - from, lrest) : line.taken(lrest, lspan.places());
         ltile = max(from, kEnd) - kEnd;
         lend = max(from + take, kEnd) - kEnd;
-        lrest -= take;
+        lrest = take ? lrest - min(take, lrest) : 0;
     };
     uint32_t entry = 0, entries_from = 0, entries_of = ~0u;   // 32 entries of a sequence's table, a lane each
     const uint32_t lrow = lane / kPieces, lpiece = lane % kPieces, boxes = KT / a.box;
@@ -595,6 +602,21 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         item = into >> 32 ? (uint32_t)(into / lspan.places()) : (uint32_t)into / lspan.places();
         place = (uint32_t)(into - (uint64_t)item * lspan.places());
     }
+    if (place && line.taken(place, lspan.places()) != place) {   // an item that is not cut: the last warp has it, or this one
+        if (line.taken(place, lspan.places())) {
+            const uint32_t rest = lspan.places() - place;
+            share = share > rest ? share - rest : 0;
+            begin += rest;
+            if (++item == per_seq && share) {
+                item = 0;
+                lspan = Span<KT>(a, seq = min(seq + 1, a.c.batch - 1));
+            }
+        } else {
+            share += place;
+            begin -= place;
+        }
+        place = 0;
+    }
     Span<KT> span = lspan;
     const Span<KT> first_span = span;
     const uint32_t first_seq = seq, first_item = item, first_place = place;
@@ -610,7 +632,8 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     uint64_t i0 = 0;        // where on the line the last item begins
     uint32_t end_of_first = 0;
     for (uint32_t at = 0; at < share;) {
-        const uint32_t here = min(span.places() - place, share - at);
+        const uint32_t here = place ? min(span.places() - place, share - at) : line.taken(share - at, span.places());
+        if (here == 0) break;   // the next warp has it all
         const uint32_t last_tile = max(place + here, kEnd) - kEnd;
         p.clear();
         lay_query();
