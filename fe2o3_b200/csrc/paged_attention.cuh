@@ -238,8 +238,6 @@ struct Meeting {
     Job jobs[2];
 };
 static_assert(sizeof(Meeting) <= kPagedMeeting, "");
-struct Yes { static constexpr bool value = true; };
-struct No { static constexpr bool value = false; };
 // A sequence's keys as tiles, counted from a multiple of KT.  One that does not fit its table is reported and has none.
 template <int KT>
 struct Span {
@@ -659,41 +657,54 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
             // scores: rows are keys, columns heads
             float s[MT][NT][4];
             if constexpr (!F16) {
-                float odd[MT][NT][4];   // every other step: two chains
-                auto scores = [&](uint32_t term, auto first) {
+                float odd[MT][NT][4], low[MT][NT][4];   // every other step: two chains; the lower terms of f32 queries
 #pragma unroll
-                    for (int ks = 0; ks < MD; ks += 2) {
-                        uint32_t ka[MT][2][4];
+                for (int ks = 0; ks < MD; ks += 2) {
+                    uint32_t ka[MT][2][4];
 #pragma unroll
-                        for (int mt = 0; mt < MT; ++mt)
+                    for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-                            for (int e = 0; e < 2; ++e) ldsm4(ka[mt][e], from + k_off[(ks + e) & 3] + (ks >> 2) * KT * 128 + mt * 16 * S::kPitch);
+                        for (int e = 0; e < 2; ++e) ldsm4(ka[mt][e], from + k_off[(ks + e) & 3] + (ks >> 2) * KT * 128 + mt * 16 * S::kPitch);
 #pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) {
-                            uint32_t qb[4];
-                            ldsm4(qb, query_s + (term * S::kHeads + 8 * nt + (lane & 7)) * S::kQueryRow + (2 * ks + (lane >> 3)) * 16);
+                    for (int nt = 0; nt < NT; ++nt) {
+                        const uint32_t at_q = query_s + (8 * nt + (lane & 7)) * S::kQueryRow + (2 * ks + (lane >> 3)) * 16;
+                        uint32_t qb[4];
+                        ldsm4(qb, at_q);
 #pragma unroll
-                            for (int mt = 0; mt < MT; ++mt) {
-                                if (decltype(first)::value && ks == 0) {
-                                    mma_first<false>(s[mt][nt], ka[mt][0], qb[0], qb[1]);
-                                    mma_first<false>(odd[mt][nt], ka[mt][1], qb[2], qb[3]);
-                                } else {
-                                    mma<false>(s[mt][nt], ka[mt][0], qb[0], qb[1]);
-                                    mma<false>(odd[mt][nt], ka[mt][1], qb[2], qb[3]);
+                        for (int mt = 0; mt < MT; ++mt) {
+                            if (ks == 0) {
+                                mma_first<false>(s[mt][nt], ka[mt][0], qb[0], qb[1]);
+                                mma_first<false>(odd[mt][nt], ka[mt][1], qb[2], qb[3]);
+                            } else {
+                                mma<false>(s[mt][nt], ka[mt][0], qb[0], qb[1]);
+                                mma<false>(odd[mt][nt], ka[mt][1], qb[2], qb[3]);
+                            }
+                        }
+                        if (terms > 1) {
+#pragma unroll
+                            for (int term = 2; term; --term) {
+                                ldsm4(qb, at_q + term * S::kHeads * S::kQueryRow);
+#pragma unroll
+                                for (int mt = 0; mt < MT; ++mt) {
+                                    if (ks == 0 && term == 2) mma_first<false>(low[mt][nt], ka[mt][0], qb[0], qb[1]);
+                                    else mma<false>(low[mt][nt], ka[mt][0], qb[0], qb[1]);
+                                    mma<false>(low[mt][nt], ka[mt][1], qb[2], qb[3]);
                                 }
                             }
                         }
                     }
-                };
-                scores(0, Yes{});
-                for (uint32_t term = 1; term < terms; ++term) scores(term, No{});
+                }
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) s[mt][nt][e] += odd[mt][nt][e];
+                        for (int e = 0; e < 4; ++e) {
+                            s[mt][nt][e] += odd[mt][nt][e];
+                            if (terms > 1) s[mt][nt][e] += low[mt][nt][e];
+                        }
             } else {
+                float low[MT][NT][4];
 #pragma unroll
                 for (int j = 0; j < DP / 64; ++j) {   // 64 columns: the lanes of a row hold 16 each, four a step
                     uint4 ka[MT][2];
@@ -729,12 +740,21 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                                 const uint4 ql = lds128(at_q + S::kHeads * S::kQueryRow);
 #pragma unroll
                                 for (int mt = 0; mt < MT; ++mt) {
-                                    mma<true>(s[mt][nt], kf[mt][0], ql.x, ql.y);
-                                    mma<true>(s[mt][nt], kf[mt][1], ql.z, ql.w);
+                                    if (j == 0 && half == 0) mma_first<true>(low[mt][nt], kf[mt][0], ql.x, ql.y);
+                                    else mma<true>(low[mt][nt], kf[mt][0], ql.x, ql.y);
+                                    mma<true>(low[mt][nt], kf[mt][1], ql.z, ql.w);
                                 }
                             }
                         }
                     }
+                }
+                if (terms > 1) {
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) s[mt][nt][e] += low[mt][nt][e];
                 }
             }
 
