@@ -115,10 +115,10 @@ int32_t paged_attention_plan(fe2o3_ctx *ctx, const fe2o3_paged_attention_v1_args
     p->grid = (uint32_t)(per_sm > 0 ? per_sm : 1) * ctx->sm_count;
     const size_t slots = (size_t)kPagedSlots * p->grid * b.part;   // behind them: counters
     p->device = ctx->device;
-    p->bytes = (slots + p->grid * sizeof(uint32_t) + 65535) / 65536 * 65536;
+    p->bytes = (slots + 3 * p->grid * sizeof(uint32_t) + 65535) / 65536 * 65536;
     Workspaces *const workspaces = workspaces_of(ctx->device);
     if (e == cudaSuccess) e = workspaces ? workspaces->take(p->bytes, &p->workspace) : cudaErrorInvalidDevice;
-    if (e == cudaSuccess) e = cudaMemset(static_cast<uint8_t *>(p->workspace) + slots, 0, p->grid * sizeof(uint32_t));
+    if (e == cudaSuccess) e = cudaMemset(static_cast<uint8_t *>(p->workspace) + slots, 0, 3 * p->grid * sizeof(uint32_t));
     if (e == cudaSuccess) e = cudaStreamSynchronize(cudaStreamLegacy);   // no other stream is ordered behind the clear
     if (e != cudaSuccess) {
         paged_attention_free(p);

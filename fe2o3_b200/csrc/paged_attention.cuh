@@ -31,7 +31,7 @@ struct PagedArgs {
     void *o;
     float *lse;
     float4 *slots;        // kPagedSlots partial results a block
-    uint32_t *arrived;    // pieces that have come in, by the block where the item begins; zero between launches
+    uint32_t *arrived;    // pieces that have come in (see the joins), three counters a block; zero between launches
     uint32_t group, chunks, q_stride, q_head_stride, window, stages;
     int32_t page_shift;   // log2 of page_size, or -1
     uint32_t box;         // rows of a page that the copy engine takes at once; 1: rows go by 16-byte copies
@@ -183,6 +183,7 @@ __device__ __forceinline__ uint32_t column_of(uint32_t i, uint32_t m) {
 
 constexpr uint32_t kEnd = 2;     // places on the line in front of an item's tiles (ragged e4m3 71 us; 76 with 1, 70 with 3, short items then slower)
 constexpr uint32_t kLeast = 1;   // places a warp has at least (10 to 2000 keys a block: 9.7 us for 16 heads of 512 keys, 11.1 with 2, 11.8 with 3)
+constexpr uint32_t kGroup = 16;   // pieces joined by one block
 constexpr uint32_t kInvalid = ~0u;
 // What a warp's share ends in: whole items only; an item that begins in the share and goes on; one that goes on on both sides; no places.
 enum : uint32_t { kNone, kBegun, kWithin, kEmpty };
@@ -191,7 +192,8 @@ struct Left {
     uint64_t i0;                                         // where on the line the open item begins
 };
 struct Job {
-    uint32_t seq, item, n, block, pieces;   // pieces 0: none; before the count: the item's places
+    uint32_t seq, item, n, pieces;   // pieces 0: none; before the count: the item's places
+    uint32_t block, first, groups;   // where the item begins, and the group of pieces; groups of the item
     uint64_t i0;
 };
 __device__ __forceinline__ uint32_t running_sum(uint32_t v, uint32_t lane) {
@@ -236,6 +238,7 @@ struct Meeting {
     uint64_t arrivals[kPagedWarps][kPagedMaxStages];
     Left left[kPagedWarps];
     Job jobs[2];
+    bool goes_on;
 };
 static_assert(sizeof(Meeting) <= kPagedMeeting, "");
 // A sequence's keys as tiles, counted from a multiple of KT.  One that does not fit its table is reported and has none.
@@ -975,6 +978,12 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     auto add = [&](const float4 *from) {   // a whole part lies there
         part.add([&](int i) { return from[(i < kQuarter * NT ? warp * kQuarter * NT + i : MD * NT + (i - kQuarter * NT)) * 32]; });
     };
+    auto leave_quarter = [&](const auto &part, float4 *to) {
+        part.leave([&](int i, float4 v) {
+            if (i < kQuarter * NT) to[(warp * kQuarter * NT + i) * 32] = v;
+            else if (warp == 0) to[(MD * NT + (i - kQuarter * NT)) * 32] = v;
+        });
+    };
 #pragma unroll 1
     for (uint32_t w = 0; w < kPagedWarps; ++w) {   // an item that warp w was the first of the block to leave open
         const Left left = meeting.left[w];
@@ -992,27 +1001,28 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         if (left.kind == kBegun && !open) {
             if (left.n != kInvalid) write(part, left.seq, left.item, left.n, warp * kQuarter);
         } else {
-            float4 *const to = slots + (left.kind == kBegun ? kSlotLast : kSlotFirst) * S::kPart * 32;
-            part.leave([&](int i, float4 v) {
-                if (i < kQuarter * NT) to[(warp * kQuarter * NT + i) * 32] = v;
-                else if (warp == 0) to[(MD * NT + (i - kQuarter * NT)) * 32] = v;
-            });
-            if (threadIdx.x == 0) meeting.jobs[left.kind == kBegun] = Job{left.seq, left.item, left.n, 0, left.places, left.i0};
+            leave_quarter(part, slots + (left.kind == kBegun ? kSlotLast : kSlotFirst) * S::kPart * 32);
+            if (threadIdx.x == 0) meeting.jobs[left.kind == kBegun] = Job{left.seq, left.item, left.n, left.places, 0, 0, 0, left.i0};
         }
     }
     if (threadIdx.x == 0 && end_of_first)   // an item of an earlier block that ended in warp 0: it lies in its slot
-        meeting.jobs[0] = Job{first_seq, first_item, first_span.valid ? first_span.n : kInvalid, 0, first_span.places(), begin - first_place};
+        meeting.jobs[0] = Job{first_seq, first_item, first_span.valid ? first_span.n : kInvalid, first_span.places(), 0, 0, 0, begin - first_place};
 
-    // ---- the blocks: the last one to come to an item joins its pieces, eight in flight ----
+    // ---- the blocks: the last one to come joins the pieces, of many pieces in two steps: 16 neighbours, then those ----
     __threadfence();
     __syncthreads();
     if (threadIdx.x < 2) {
         Job &job = meeting.jobs[threadIdx.x];
         if (job.pieces) {
             const uint32_t b0 = line.block_of(job.i0), pieces = line.block_of(job.i0 + job.pieces - 1) - b0 + 1;
+            const uint32_t group = (blockIdx.x - b0) / kGroup, groups = (pieces + kGroup - 1) / kGroup;
             job.block = b0;
-            job.pieces = pieces;
-            if (atomicAdd(&a.arrived[b0], 1u) == pieces - 1) a.arrived[b0] = 0;
+            job.first = b0 + group * kGroup;
+            job.groups = groups;
+            job.pieces = min(kGroup, pieces - group * kGroup);
+            // (a block may be in the first group of one item and begin the second, or a later, of another)
+            uint32_t *const count = a.arrived + (group ? gridDim.x : 0) + job.first;
+            if (atomicAdd(count, 1u) == job.pieces - 1) *count = 0;
             else job.pieces = 0;
         }
     }
@@ -1021,24 +1031,44 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     for (int role = 0; role < 2; ++role) {
         const Job job = meeting.jobs[role];
         if (!job.pieces) continue;
-        __threadfence();
-        part.clear();
-        constexpr int kAtOnce = kQuarter * NT <= 2 ? 8 : kQuarter * NT <= 4 ? 4 : 2, kLoads = (kQuarter + 1) * NT;
+        uint32_t from = job.first, step = 1, n = job.pieces;
+        auto slot_of = [&](uint32_t block) { return a.slots + ((uint64_t)block * kPagedSlots + (block == job.block ? kSlotLast : kSlotFirst)) * S::kPart * 32 + lane; };
+        for (bool whole = job.groups == 1;; whole = true) {
+            __threadfence();
+            part.clear();
+            constexpr int kAtOnce = kQuarter * NT <= 2 ? 8 : kQuarter * NT <= 4 ? 4 : 2, kLoads = (kQuarter + 1) * NT;
 #pragma unroll 1
-        for (uint32_t i = 0; i < job.pieces; i += kAtOnce) {
-            float4 v[kAtOnce][kLoads];
+            for (uint32_t i = 0; i < n; i += kAtOnce) {
+                float4 v[kAtOnce][kLoads];
 #pragma unroll
-            for (int x = 0; x < kAtOnce; ++x) {   // (beyond the last one: that again, which is not added)
-                const uint32_t piece = min(i + x, job.pieces - 1);
-                const float4 *const from = a.slots + ((uint64_t)(job.block + piece) * kPagedSlots + (piece ? kSlotFirst : kSlotLast)) * S::kPart * 32 + lane;
+                for (int x = 0; x < kAtOnce; ++x) {   // (beyond the last one: that again, which is not added)
+                    const float4 *const at = slot_of(from + min(i + x, n - 1) * step);
 #pragma unroll
-                for (int k = 0; k < kLoads; ++k) v[x][k] = __ldcg(from + (k < kQuarter * NT ? warp * kQuarter * NT + k : MD * NT + (k - kQuarter * NT)) * 32);
+                    for (int k = 0; k < kLoads; ++k) v[x][k] = __ldcg(at + (k < kQuarter * NT ? warp * kQuarter * NT + k : MD * NT + (k - kQuarter * NT)) * 32);
+                }
+#pragma unroll
+                for (int x = 0; x < kAtOnce; ++x)
+                    if (i + x < n) part.add([&](int k) { return v[x][k]; });
             }
-#pragma unroll
-            for (int x = 0; x < kAtOnce; ++x)
-                if (i + x < job.pieces) part.add([&](int k) { return v[x][k]; });
+            if (whole) {
+                if (job.n != kInvalid) write(part, job.seq, job.item, job.n, warp * kQuarter);
+                break;
+            }
+            __syncthreads();   // (all warps have read the first piece's maxima)
+            leave_quarter(part, slot_of(from));
+            __threadfence();
+            __syncthreads();
+            if (threadIdx.x == 0) {
+                uint32_t *const count = a.arrived + 2 * gridDim.x + job.block;
+                meeting.goes_on = atomicAdd(count, 1u) == job.groups - 1;
+                if (meeting.goes_on) *count = 0;
+            }
+            __syncthreads();
+            if (!meeting.goes_on) break;
+            from = job.block;
+            step = kGroup;
+            n = job.groups;
         }
-        if (job.n != kInvalid) write(part, job.seq, job.item, job.n, warp * kQuarter);
     }
 }
 
