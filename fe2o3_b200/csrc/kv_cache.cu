@@ -50,12 +50,14 @@ __device__ __forceinline__ bool slot_of(const KvCache &c, const KvRows &r, uint3
             own = r.offsets[at] - r.offsets[b];
         }
     }
+    bool report = !ok && lane < n;
     if (ok) {
         const uint32_t length = c.lengths[b];
         ok = length >= own && kv_fits(c, length);
+        report = !ok && (r.offsets || length);   // (without offsets a sequence of length 0 has no token)
         if (ok) row = kv_row(c, b, 0, length - before);
     }
-    if (!ok && lane < n) kstatus_set(c.status, FE2O3_KSTATUS_LENGTH);
+    if (report) kstatus_set(c.status, FE2O3_KSTATUS_LENGTH);
     return ok;
 }
 

@@ -448,7 +448,7 @@ typedef struct fe2o3_moe_ep_ffn_v1_args {
 
 /* Writes new tokens into the cache.  Rows token_offsets[b] .. token_offsets[b + 1] - 1 of k and v belong to
  * sequence b and go to its last positions before lengths[b] (lengths count the new tokens); without
- * token_offsets (empty slice) row b is sequence b's one new token, and tokens == batch.  Row (t, h) starts at
+ * token_offsets (empty slice) row b is sequence b's one new token, and tokens == batch; a sequence of length 0 has none.  Row (t, h) starts at
  * element t * token_stride + h * head_stride; k and v hold (tokens - 1) * token_stride +
  * (kv_heads - 1) * head_stride + dim elements.  No two new tokens may share a slot. */
 typedef struct fe2o3_kv_cache_append_v1_args {

@@ -675,3 +675,95 @@ def test_rows_beyond_32_bits(gpu, form):
     p = np.exp(s - s.max(-1, keepdims=True))
     want = np.einsum("hn,nhd->hd", p / p.sum(-1, keepdims=True), held[1])
     assert np.abs(o.cpu().numpy()[0] - want).max() <= 1e-4
+
+
+# ---- the cache as a serving program keeps it ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("form", FORMATS)
+def test_cache_object_serves_prompts_and_steps(gpu, form):
+    """Prompts of unlike lengths, steps over page ends, a request that ends and another that takes its place."""
+    fe, torch, ctx, stream = gpu
+    from fe2o3_b200.kv_cache import DecodeStep, PagedKvCache
+    B, H, KH, D = 4, 6, 2, 48
+    cache = PagedKvCache(ctx, stream, sequences=B, positions=64, kv_heads=KH, dim=D, page_size=8, pages=14, format=CODE[form])
+    rng = np.random.default_rng(11)
+    held = [[np.zeros((0, KH, D)) for _ in range(B)] for _ in range(2)]   # f64 values, by side and sequence
+
+    def keep(side, b, rows):
+        code = to_bf16(rows) if form == "bf16" else quantised(rows, form)
+        values = values_of(code, None, form) if form == "bf16" else values_of(*code, form)
+        held[side][b] = np.concatenate([held[side][b], values])
+
+    def prompt(counts):
+        cache.extend(counts)
+        rows = [rows_in(torch, rng.normal(size=(sum(counts), KH, D)), "f32") for _ in range(2)]
+        torch.cuda.synchronize()
+        cache.append(rows[0][0], rows[1][0])
+        at = np.concatenate([[0], np.cumsum(counts)])
+        for side in range(2):
+            for b in range(B):
+                keep(side, b, rows[side][1][at[b]:at[b + 1]])
+
+    q, k, v = (torch.zeros(B, n, D, dtype=torch.bfloat16, device="cuda") for n in (H, KH, KH))
+    out, lse = torch.zeros(B, H, D, device="cuda"), torch.zeros(B, H, device="cuda")
+    step = DecodeStep(cache, q, k, v, out, heads=H, lse=lse)
+
+    def steps(n):
+        for _ in range(n):
+            new = [rows_in(torch, rng.normal(size=(B, m, D)), "bf16") for m in (H, KH, KH)]
+            for t, (x, _) in zip((q, k, v), new):
+                t.copy_(x)
+            torch.cuda.synchronize()
+            step.run()
+            stream.synchronize()
+            got = out.cpu().numpy()
+            for b in range(B):
+                if len(held[0][b]) == 0:
+                    assert (got[b] == 0).all() and (lse[b].cpu().numpy() == -np.inf).all()
+                    continue
+                for side in range(2):
+                    keep(side, b, new[1 + side][1][b:b + 1])
+                for h in range(H):
+                    s = held[0][b][:, h // 3] @ new[0][1][b, h].astype(np.float64) * D ** -0.5
+                    p = np.exp(s - s.max())
+                    want = p @ held[1][b][:, h // 3] / p.sum()
+                    assert np.abs(got[b, h] - want).max() <= 1e-4
+        assert ctx.take_kernel_status(stream) == 0
+
+    prompt([7, 0, 20, 1])
+    steps(3)
+    cache.release(2)
+    for side in range(2):
+        held[side][2] = np.zeros((0, KH, D))
+    steps(2)
+    prompt([0, 9, 30, 0])
+    steps(9)
+    counts = [len(x) for x in held[0]]
+    assert cache.table.lengths.tolist() == counts
+    back = [torch.zeros(sum(counts), KH, D, device="cuda") for _ in range(2)]
+    torch.cuda.synchronize()
+    cache.read(back[0], back[1], counts)
+    for side in range(2):
+        assert (back[side].cpu().numpy() == np.concatenate(held[side]).astype(np.float32)).all()
+    with pytest.raises(MemoryError):
+        cache.extend([0, 40, 0, 0])
+    once = torch.zeros(B, H, D, device="cuda")
+    torch.cuda.synchronize()
+    cache.attend(q, once, H)
+    stream.synchronize()
+    assert torch.equal(once, out)
+    step.destroy()
+    cache.free()
+
+
+def test_example_runs(gpu):
+    import os
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    sys.path.insert(0, os.path.join(root, "examples"))
+    try:
+        import paged_decode
+    finally:
+        sys.path.pop(0)
+    # bf16 projections and residuals of unit size: two roundings of 2^-9 a step on either side of the comparison
+    assert paged_decode.main(["--sequences", "16", "--prompt", "40", "--steps", "5", "--heads", "4", "--dim", "64", "--format", "bf16"]) <= 2e-2

@@ -1,6 +1,7 @@
 """Admission of the paged key-value cache's operators: pure host checks, no GPU."""
 import math
 
+import numpy as np
 import pytest
 
 import fe2o3_b200 as fe
@@ -111,3 +112,46 @@ def test_attention_arguments():
     big = cache(batch=1 << 20, width=0)
     many = {**big, "lengths": sl(64, 1 << 20), "page_table": (0, 0), "heads": 4096, "kv_heads": 2, "scale": 1.0}
     assert err(op, **many) == "UnsupportedShape"
+
+
+# ---- the host's book of pages ----------------------------------------------------------------------------------------
+
+def test_pages_are_handed_out_and_come_back():
+    from fe2o3_b200.kv_cache import PageTable
+    t = PageTable(sequences=3, positions=50, pages=9, page_size=16)
+    assert t.entries.shape == (3, 4)
+    t.extend([16, 0, 33])
+    assert t.lengths.tolist() == [16, 0, 33] and len(t.free) == 9 - 1 - 3
+    t.extend([1, 15, 15])                                # 17, 15, 48: one page each for the first two
+    assert len(t.free) == 3
+    used = [int(p) for row, n in zip(t.entries, (2, 1, 3)) for p in row[:n]]
+    assert len(set(used)) == 6 and all(0 <= p < 9 for p in used)
+    assert (t.entries[0, 2:] == t.FREE).all() and (t.entries[1, 1:] == t.FREE).all()
+    before = t.entries.copy(), t.lengths.copy(), list(t.free)
+    for bad, error in (([48, 33, 0], ValueError),        # past a sequence's last position
+                       ([33, 33, 0], MemoryError),       # more pages than are free
+                       ([1, 1], ValueError), ([-1, 0, 0], ValueError)):
+        with pytest.raises(error):
+            t.extend(bad)
+        assert (t.entries == before[0]).all() and (t.lengths == before[1]).all() and t.free == before[2]
+    t.release(2)
+    assert t.lengths.tolist() == [17, 15, 0] and len(t.free) == 6 and (t.entries[2] == t.FREE).all()
+    t.extend([0, 0, 64])                                 # 50 positions are whole pages: 64
+    assert len(t.free) == 2 and len(set(t.entries[t.entries != t.FREE].tolist())) == 7
+    t.release(0), t.release(1), t.release(2)
+    assert sorted(t.free) == list(range(9))
+    t.release(1)                                         # an empty one: nothing
+    assert len(t.free) == 9
+    with pytest.raises(ValueError):
+        PageTable(0, 1, 1, 1)
+
+
+def test_row_types():
+    from fe2o3_b200.kv_cache import _float_dtype
+    assert _float_dtype(np.zeros(1, np.float32), None) == fe.DTYPE_F32
+    assert _float_dtype(np.zeros(1, np.uint16), None) == fe.DTYPE_BF16
+    assert _float_dtype((0, 4), fe.DTYPE_F32) == fe.DTYPE_F32
+    with pytest.raises(TypeError):
+        _float_dtype((0, 4), None)
+    with pytest.raises(TypeError):
+        _float_dtype(np.zeros(1, np.int32), None)
