@@ -663,9 +663,10 @@ int regions_for(uint32_t op, const void *args, Region *r, int32_t *status) {
             if (!n) return 0;
             if (a->heads == 0 || a->heads % a->kv_heads || a->q_dtype > FE2O3_DTYPE_BF16 || a->output_dtype > FE2O3_DTYPE_BF16 ||
                 !isfinite(a->scale) || (uint64_t)a->batch * a->heads > 0x7fffffffu ||
-                (a->batch && (uint64_t)a->table_width * a->page_size > (1ull << 36) / a->batch)) {
-                *status = unsupported("paged_attention_v1 needs heads a multiple of kv_heads, batch * heads < 2^31, at most 2^36 positions in "
-                                      "the page table, f32 or bf16 queries and output, a finite scale");
+                (a->batch && (uint64_t)a->table_width * a->page_size > (1ull << 35) / a->batch) ||
+                (uint64_t)a->batch * a->table_width * a->page_size > (1ull << 44) / a->heads) {
+                *status = unsupported("paged_attention_v1 needs heads a multiple of kv_heads, batch * heads < 2^31, at most 2^35 positions in "
+                                      "the page table and 2^44 of all heads, f32 or bf16 queries and output, a finite scale");
                 return 0;
             }
             uint64_t len = 0;

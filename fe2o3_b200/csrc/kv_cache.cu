@@ -20,11 +20,10 @@ namespace {
 constexpr int kThreads = 256, kTokens = 32, kDeep = 4;
 
 struct KvRows {
-    uint8_t *p[2];   // k, v: sources of an append, destinations of a read
-    uint32_t token_stride[2], head_stride[2];
+    uint8_t *k, *v;   // sources of an append, destinations of a read
+    uint32_t k_token_stride, v_token_stride, k_head_stride, v_head_stride;
     const uint32_t *offsets;
     uint32_t tokens, per_block, lanes_log2, heads_inverse;   // lanes of a row; 2^32 / kv_heads rounded up, or 0
-    uint32_t whole;                                          // rows start on 16 bytes
 };
 
 // One warp, a lane a token: row number of its head 0, ~0 where its page lies outside the cache.  false (reported) where the
@@ -48,6 +47,7 @@ __device__ __forceinline__ bool slot_of(const KvCache &c, const KvRows &r, uint3
             b = at - 1;
             before = r.offsets[at] - t;
             own = r.offsets[at] - r.offsets[b];
+            ok = r.offsets[b] <= t && t < r.offsets[at];   // (offsets that rise)
         }
     }
     bool report = !ok && lane < n;
@@ -81,35 +81,36 @@ __device__ __forceinline__ uint2 narrow4(const float *x) { return make_uint2(bf1
 __device__ __forceinline__ uint4 joined(uint2 a, uint2 b) { return make_uint4(a.x, a.y, b.x, b.y); }
 
 // The caller's rows: f32 bits as two fours, or eight bf16.
-template <bool F32>
-__device__ __forceinline__ void fetch(const uint8_t *row, const Columns &c, bool whole, uint4 (&v)[2]) {
+template <bool F32, bool WHOLE>
+__device__ __forceinline__ void fetch(const uint8_t *row, const Columns &c, uint4 (&v)[2]) {
     if constexpr (F32) {
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
             if (!(half ? c.two : c.one)) continue;
             const uint32_t *const e = reinterpret_cast<const uint32_t *>(row) + (half ? c.second : c.first);
-            v[half] = whole ? __ldcs(reinterpret_cast<const uint4 *>(e)) : make_uint4(e[0], e[1], e[2], e[3]);
+            if constexpr (WHOLE) v[half] = __ldcs(reinterpret_cast<const uint4 *>(e));
+            else v[half] = make_uint4(e[0], e[1], e[2], e[3]);
         }
     } else if (c.one) {
         const uint16_t *const e = reinterpret_cast<const uint16_t *>(row) + c.first;
-        v[0] = whole ? __ldcs(reinterpret_cast<const uint4 *>(e))
-                     : make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
+        if constexpr (WHOLE) v[0] = __ldcs(reinterpret_cast<const uint4 *>(e));
+        else v[0] = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
     }
 }
-template <bool F32>
-__device__ __forceinline__ void put(uint8_t *row, const Columns &c, bool whole, const uint4 (&v)[2]) {
+template <bool F32, bool WHOLE>
+__device__ __forceinline__ void put(uint8_t *row, const Columns &c, const uint4 (&v)[2]) {
     if constexpr (F32) {
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
             if (!(half ? c.two : c.one)) continue;
             uint32_t *const e = reinterpret_cast<uint32_t *>(row) + (half ? c.second : c.first);
-            if (whole) __stcs(reinterpret_cast<uint4 *>(e), v[half]);
+            if constexpr (WHOLE) __stcs(reinterpret_cast<uint4 *>(e), v[half]);
             else e[0] = v[half].x, e[1] = v[half].y, e[2] = v[half].z, e[3] = v[half].w;
         }
     } else if (c.one) {
         uint16_t *const e = reinterpret_cast<uint16_t *>(row) + c.first;
         const uint32_t w[4] = {v[0].x, v[0].y, v[0].z, v[0].w};
-        if (whole) {
+        if constexpr (WHOLE) {
             __stcs(reinterpret_cast<uint4 *>(e), v[0]);
         } else {
 #pragma unroll
@@ -161,6 +162,13 @@ __device__ __forceinline__ void put_cached(uint8_t *row, const Columns &c, const
             if (c.two) *reinterpret_cast<uint32_t *>(row + c.second) = v.y;
         }
     }
+}
+
+template <int LANES>
+__device__ __forceinline__ uint32_t highest(uint32_t v) {
+#pragma unroll
+    for (int o = 1; o < LANES; o <<= 1) v = max(v, __shfl_xor_sync(~0u, v, o));
+    return v;
 }
 
 // x / scale for eight columns, each as IEEE division rounds it.
@@ -227,7 +235,8 @@ __device__ __forceinline__ void values_of(const uint2 &c, float scale, float (&x
     for (int i = 0; i < 8; ++i) x[i] = __fmul_rn(x[i], scale);
 }
 
-template <uint32_t FORMAT, bool F32, bool WRITE>
+// WHOLE: the caller's rows start on 16 bytes.
+template <uint32_t FORMAT, bool F32, bool WRITE, bool WHOLE>
 __global__ void __launch_bounds__(kThreads) kv_rows_kernel(KvCache c, KvRows r) {
     __shared__ uint32_t slots[kTokens];
     __shared__ uint32_t known;   // tokens whose lengths allow a slot, a bit each
@@ -261,12 +270,13 @@ __global__ void __launch_bounds__(kThreads) kv_rows_kernel(KvCache c, KvRows r) 
             side[d] = of_side & 1;
             at[d] = slot == ~0u ? ~0u : slot + h * c.page_size;
             active[d] = first + d * at_once < rows && (known >> token & 1) && (slot != ~0u || !WRITE);
-            there[d] = r.p[side[d]] + ((uint64_t)(t0 + token) * r.token_stride[side[d]] + (uint64_t)h * r.head_stride[side[d]]) * kEb;
+            there[d] = (side[d] ? r.v : r.k) + ((uint64_t)(t0 + token) * (side[d] ? r.v_token_stride : r.k_token_stride) +
+                                                (uint64_t)h * (side[d] ? r.v_head_stride : r.k_head_stride)) * kEb;
             raw[d][0] = raw[d][1] = make_uint4(0, 0, 0, 0);
             scales[d] = 0.f;
             if (!active[d]) continue;
             if constexpr (WRITE) {
-                fetch<F32>(there[d], columns, r.whole, raw[d]);
+                fetch<F32, WHOLE>(there[d], columns, raw[d]);
             } else if (slot != ~0u) {
                 raw[d][0] = fetch_cached<FORMAT, F32>((side[d] ? c.v : c.k) + (uint64_t)at[d] * c.dim * kKvBytes<FORMAT>, columns);
                 if constexpr (FORMAT != FE2O3_KV_BF16) scales[d] = (side[d] ? c.v_scales : c.k_scales)[at[d]];
@@ -278,7 +288,7 @@ __global__ void __launch_bounds__(kThreads) kv_rows_kernel(KvCache c, KvRows r) 
             if constexpr (FORMAT == FE2O3_KV_BF16 && !F32) {   // as it is
                 if (!active[d]) continue;
                 if constexpr (WRITE) put_cached<FORMAT, F32>((side[d] ? c.v : c.k) + (uint64_t)at[d] * c.dim * 2, columns, raw[d][0]);
-                else put<F32>(there[d], columns, r.whole, raw[d]);
+                else put<F32, WHOLE>(there[d], columns, raw[d]);
                 continue;
             }
             float x[8];
@@ -303,7 +313,10 @@ __global__ void __launch_bounds__(kThreads) kv_rows_kernel(KvCache c, KvRows r) 
                 if constexpr (FORMAT == FE2O3_KV_BF16) {
                     if (active[d]) put_cached<FORMAT, F32>(to, columns, joined(narrow4(x), narrow4(x + 4)));
                 } else {
-                    for (uint32_t o = 1; o < lanes; o <<= 1) top = max(top, __shfl_xor_sync(~0u, top, o));
+                    if (lanes == 16) top = highest<16>(top);   // (unrolled for the usual rows)
+                    else if (lanes == 8) top = highest<8>(top);
+                    else
+                        for (uint32_t o = 1; o < lanes; o <<= 1) top = max(top, __shfl_xor_sync(~0u, top, o));
                     const float scale = top < 0x7f800000u ? scale_of<FORMAT>(__uint_as_float(top)) : __uint_as_float(0x7fc00000u);
                     float q[8];
                     quotients(x, scale, q);
@@ -327,7 +340,7 @@ __global__ void __launch_bounds__(kThreads) kv_rows_kernel(KvCache c, KvRows r) 
                 } else {
                     v[0] = joined(narrow4(x), narrow4(x + 4));
                 }
-                if (active[d]) put<F32>(there[d], columns, r.whole, v);
+                if (active[d]) put<F32, WHOLE>(there[d], columns, v);
             }
         }
     }
@@ -337,15 +350,18 @@ using Kernel = void (*)(KvCache, KvRows);
 
 template <typename Args>
 int32_t launch_rows(fe2o3_ctx *ctx, cudaStream_t s, const Args *a, uint32_t dtype, fe2o3_geometry *geo, bool plan_only,
-                    const Kernel (&kernels)[3][2], const char *what) {
+                    const Kernel (&kernels)[3][2][2], const char *what) {
     // tokens of a block: up to a warp's lanes, and blocks that fill the SMs a whole number of times
-    static std::atomic<int> per_sm[3][2];   // of each kernel, found once
-    const int i = dtype == FE2O3_DTYPE_F32;
-    int fit = per_sm[a->format][i].load(std::memory_order_relaxed);
+    const uint32_t eb = dtype == FE2O3_DTYPE_F32 ? 4 : 2;
+    const uint64_t odd = a->k.ptr | a->v.ptr | (uint64_t)a->k_token_stride * eb | (uint64_t)a->v_token_stride * eb | (uint64_t)a->k_head_stride * eb | (uint64_t)a->v_head_stride * eb;
+    static std::atomic<int> per_sm[3][2][2];   // of each kernel, found once
+    const int i = dtype == FE2O3_DTYPE_F32, whole = odd % 16 == 0;
+    int fit = per_sm[a->format][i][whole].load(std::memory_order_relaxed);
     if (fit == 0) {
-        const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, kernels[a->format][i], kThreads, 0);
+        const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, kernels[a->format][i][whole], kThreads, 0);
         if (e != cudaSuccess) return fe2o3_cuda_status(e, what);
-        per_sm[a->format][i].store(fit < 1 ? fit = 1 : fit, std::memory_order_relaxed);
+        if (fit < 1) fit = 1;
+        per_sm[a->format][i][whole].store(fit, std::memory_order_relaxed);
     }
     const uint64_t resident = (uint64_t)fit * (ctx->sm_count > 0 ? ctx->sm_count : 1);
     const uint64_t waves = (a->tokens + resident * kTokens - 1) / (resident * kTokens);
@@ -353,41 +369,33 @@ int32_t launch_rows(fe2o3_ctx *ctx, cudaStream_t s, const Args *a, uint32_t dtyp
     const uint32_t grid = ceil_div_u32(a->tokens, per_block);
     if (geo) *geo = fe2o3_geometry{{grid, 1, 1}, {kThreads, 1, 1}, 0, 1};
     if (plan_only || a->tokens == 0) return FE2O3_OK;
-    const uint32_t eb = dtype == FE2O3_DTYPE_F32 ? 4 : 2;
-    const uint64_t odd = a->k.ptr | a->v.ptr | (uint64_t)a->k_token_stride * eb | (uint64_t)a->v_token_stride * eb | (uint64_t)a->k_head_stride * eb | (uint64_t)a->v_head_stride * eb;
     uint32_t lanes_log2 = 1;
     while ((8u << lanes_log2) < a->dim) ++lanes_log2;
-    const KvRows r{{reinterpret_cast<uint8_t *>(a->k.ptr), reinterpret_cast<uint8_t *>(a->v.ptr)},
-                   {a->k_token_stride, a->v_token_stride},
-                   {a->k_head_stride, a->v_head_stride},
-                   reinterpret_cast<const uint32_t *>(a->token_offsets.ptr),
-                   a->tokens,
-                   per_block,
-                   lanes_log2,
+    const KvRows r{reinterpret_cast<uint8_t *>(a->k.ptr), reinterpret_cast<uint8_t *>(a->v.ptr), a->k_token_stride, a->v_token_stride,
+                   a->k_head_stride, a->v_head_stride, reinterpret_cast<const uint32_t *>(a->token_offsets.ptr), a->tokens, per_block, lanes_log2,
                    // exact for the indexes of a block, below 64 kv_heads
-                   a->kv_heads == 1 || a->kv_heads > 4096 ? 0 : (uint32_t)((0x100000000ull + a->kv_heads - 1) / a->kv_heads),
-                   odd % 16 == 0};
-    const cudaError_t e = fe2o3_launch_early(kernels[a->format][i], grid, kThreads, 0, s, 1, kv_cache_of(ctx, a), r);
+                   a->kv_heads == 1 || a->kv_heads > 4096 ? 0 : (uint32_t)((0x100000000ull + a->kv_heads - 1) / a->kv_heads)};
+    const cudaError_t e = fe2o3_launch_early(kernels[a->format][i][whole], grid, kThreads, 0, s, 1, kv_cache_of(ctx, a), r);
     fe2o3_count_launch(1);
     return fe2o3_cuda_status(e, what);
 }
 
 }  // namespace
 
+#define KV_FORMAT(FORMAT, WRITE)                                                                                                     \
+    {{kv_rows_kernel<FORMAT, false, WRITE, false>, kv_rows_kernel<FORMAT, false, WRITE, true>},                                      \
+     {kv_rows_kernel<FORMAT, true, WRITE, false>, kv_rows_kernel<FORMAT, true, WRITE, true>}}
+#define KV_FORMATS(WRITE) {KV_FORMAT(FE2O3_KV_BF16, WRITE), KV_FORMAT(FE2O3_KV_E4M3, WRITE), KV_FORMAT(FE2O3_KV_I8, WRITE)}
 int32_t launch_kv_cache_append(fe2o3_ctx *ctx, cudaStream_t s, const void *args, fe2o3_geometry *geo, bool plan_only) {
-    static const Kernel kernels[3][2] = {{kv_rows_kernel<0, false, true>, kv_rows_kernel<0, true, true>},
-                                         {kv_rows_kernel<1, false, true>, kv_rows_kernel<1, true, true>},
-                                         {kv_rows_kernel<2, false, true>, kv_rows_kernel<2, true, true>}};
+    static const Kernel kernels[3][2][2] = KV_FORMATS(true);
     const fe2o3_kv_cache_append_v1_args *a = static_cast<const fe2o3_kv_cache_append_v1_args *>(args);
     return launch_rows(ctx, s, a, a->input_dtype, geo, plan_only, kernels, "kv_cache_append_v1");
 }
 int32_t launch_kv_cache_read(fe2o3_ctx *ctx, cudaStream_t s, const void *args, fe2o3_geometry *geo, bool plan_only) {
-    static const Kernel kernels[3][2] = {{kv_rows_kernel<0, false, false>, kv_rows_kernel<0, true, false>},
-                                         {kv_rows_kernel<1, false, false>, kv_rows_kernel<1, true, false>},
-                                         {kv_rows_kernel<2, false, false>, kv_rows_kernel<2, true, false>}};
+    static const Kernel kernels[3][2][2] = KV_FORMATS(false);
     const fe2o3_kv_cache_read_v1_args *a = static_cast<const fe2o3_kv_cache_read_v1_args *>(args);
     return launch_rows(ctx, s, a, a->output_dtype, geo, plan_only, kernels, "kv_cache_read_v1");
 }
 
-static Fe2o3KernelRegistration reg_append("kv_cache_append_v1", reinterpret_cast<const void *>(kv_rows_kernel<0, false, true>));
-static Fe2o3KernelRegistration reg_read("kv_cache_read_v1", reinterpret_cast<const void *>(kv_rows_kernel<0, false, false>));
+static Fe2o3KernelRegistration reg_append("kv_cache_append_v1", reinterpret_cast<const void *>(kv_rows_kernel<0, false, true, true>));
+static Fe2o3KernelRegistration reg_read("kv_cache_read_v1", reinterpret_cast<const void *>(kv_rows_kernel<0, false, false, true>));

@@ -434,7 +434,7 @@ typedef struct fe2o3_moe_ep_ffn_v1_args {
  * [pages][kv_heads][page_size].  For a row x and the format's largest code C (448 and 127):
  *   scale = max |x| / C, code = x / scale rounded to the nearest code, ties to even,
  * both quotients rounded to f32; a row of zeros has scale 0, a row with an infinity or a NaN has scale NaN and
- * reads back as NaN.  bf16 elements are rounded to nearest even.
+ * reads back as NaN.  bf16 elements are rounded to nearest even, and a NaN becomes a quiet one.
  * dim is a multiple of 16 up to 256, kv_heads at most 65536, page_size any number from 1, a cache has fewer than 2^32 rows, a sequence has fewer than 2^31 positions; both
  * caches start on 16 bytes.  Lengths and page table stay as they are while a launch runs.
  *
@@ -472,9 +472,10 @@ typedef struct fe2o3_kv_cache_read_v1_args {
  *   output[b][h] = sum_j softmax_j(scale * q[b][h] . k_j) v_j,   lse[b][h] = log sum_j exp(scale * q[b][h] . k_j)
  * with the keys and values of head h / (heads / kv_heads).  heads is a multiple of kv_heads.  q row (b, h) starts at
  * element b * q_stride + h * q_head_stride; output [batch][heads][dim] is packed, f32 or bf16; lse
- * [batch][heads] f32 is optional.  The page table has at most 2^36 positions, batch * heads is below 2^31.  A sequence of length 0 gives zeros and -inf.  Sums, maxima and
+ * [batch][heads] f32 is optional.  The page table has at most 2^35 positions (2^44 times heads), batch * heads is below 2^31.  A sequence of length 0 gives zeros and -inf.  Sums, maxima and
  * probabilities are f32 (for a bf16 output the probabilities have 16 significant bits).  The result does not
- * depend on which blocks finish first.  One launch of a prepared object at a time (it owns a workspace). */
+ * depend on which blocks finish first.   One launch of a prepared object at a time (it owns a workspace); what is patched into
+ * its argument block later has no effect. */
 typedef struct fe2o3_paged_attention_v1_args {
     fe2o3_slice q, k_cache, v_cache, k_scales, v_scales, page_table, lengths, output, lse;
     uint32_t batch, heads, kv_heads, dim, page_size, table_width, q_stride, q_head_stride;
