@@ -112,7 +112,12 @@ int32_t paged_attention_plan(fe2o3_ctx *ctx, const fe2o3_paged_attention_v1_args
     int per_sm = 0;
     cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void *>(b.kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, (int)p->shared);
     if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, b.kernel, kPagedThreads, p->shared);
-    p->grid = (uint32_t)(per_sm > 0 ? per_sm : 1) * ctx->sm_count;
+    const uint32_t at_once = (uint32_t)(per_sm > 0 ? per_sm : 1) * ctx->sm_count;
+    p->grid = at_once;
+    // no more blocks than sequences that fill their rows of the table give work to (kEnd and a tile begun come on top)
+    const double tiles = (double)a->table_width * a->page_size / b.keys + 4;
+    const double most = tiles * a->batch * a->kv_heads * ((group + 8 * nt - 1) / (8 * nt)) / kPagedWarps;
+    if (most < p->grid) p->grid = most < 1 ? 1 : (uint32_t)most;
     const size_t slots = (size_t)kPagedSlots * p->grid * b.part;   // behind them: counters
     p->device = ctx->device;
     p->bytes = (slots + 3 * p->grid * sizeof(uint32_t) + 65535) / 65536 * 65536;
@@ -145,7 +150,7 @@ int32_t paged_attention_plan(fe2o3_ctx *ctx, const fe2o3_paged_attention_v1_args
     p->args = PagedArgs{kv_cache_of(ctx, a), reinterpret_cast<const void *>(a->q.ptr), reinterpret_cast<void *>(a->output.ptr),
                         reinterpret_cast<float *>(a->lse.ptr), static_cast<float4 *>(p->workspace),
                         counters, group, (group + 8 * nt - 1) / (8 * nt),
-                        a->q_stride, a->q_head_stride, a->window, stages, shift, box, a->scale, a->q_dtype == FE2O3_DTYPE_F32,
+                        a->q_stride, a->q_head_stride, a->window, stages, at_once, shift, box, a->scale, a->q_dtype == FE2O3_DTYPE_F32,
                         a->output_dtype == FE2O3_DTYPE_F32, whole};
     *out = p;
     return FE2O3_OK;

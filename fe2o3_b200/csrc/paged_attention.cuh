@@ -33,6 +33,7 @@ struct PagedArgs {
     float4 *slots;        // kPagedSlots partial results a block
     uint32_t *arrived;    // pieces that have come in (see the joins), three counters a block; zero between launches
     uint32_t group, chunks, q_stride, q_head_stride, window, stages;
+    uint32_t room;        // blocks that the GPU holds at once (the grid is smaller where the page table cannot fill it)
     int32_t page_shift;   // log2 of page_size, or -1
     uint32_t box;         // rows of a page that the copy engine takes at once; 1: rows go by 16-byte copies
     float scale;
@@ -215,12 +216,12 @@ struct Line {
         blocks = wanted < gridDim.x ? (uint32_t)wanted : gridDim.x;
         // as many blocks an item for all, where that leaves few idle or there is little to do: items of one length then end with a block
         const uint32_t items = a.c.batch * per_seq;
-        if (items <= blocks && (wanted < gridDim.x || blocks % items * 16 <= blocks)) blocks -= blocks % items;
+        if (items <= blocks && (wanted < a.room || blocks % items * 16 <= blocks)) blocks -= blocks % items;
         const uint32_t warps = blocks * kPagedWarps;
         const uint64_t each = total >> 32 ? total / warps : (uint32_t)total / warps;
         q = (uint32_t)each;
         r = (uint32_t)(total - each * warps);
-        whole = wanted < gridDim.x ? kEnd + 1 : max(4u, q / 8);   // (SMs to spare: two tiles are sooner done by two warps)
+        whole = wanted < a.room ? kEnd + 1 : max(4u, q / 8);   // (SMs to spare: two tiles are sooner done by two warps)
     }
     __device__ __forceinline__ void share(uint32_t me, uint64_t &begin, uint32_t &n) const {
         const uint32_t warps = blocks * kPagedWarps, over = r * me / warps;
