@@ -95,7 +95,8 @@ int32_t paged_attention_plan(fe2o3_ctx *ctx, const fe2o3_paged_attention_v1_args
     FE2O3_CUDA(cudaFuncGetAttributes(&attr, reinterpret_cast<const void *>(b.kernel)));
     // as many blocks an SM as registers and two stages a warp allow (131071 tokens: three blocks of two stages 178 us, two of
     // three 186), then as many stages as fit; a partial result has to fit a warp's ring
-    const uint32_t fixed = kPagedWarps * terms * b.query + kPagedMeeting, least = b.part > 2 * b.stage ? (b.part + b.stage - 1) / b.stage : 2;
+    const uint32_t q_rows = group < 8 * nt ? group + 1 : 8 * nt;
+    const uint32_t fixed = kPagedWarps * terms * q_rows * b.query + kPagedMeeting, least = b.part > 2 * b.stage ? (b.part + b.stage - 1) / b.stage : 2;
     uint32_t stages = 0;
     for (uint32_t blocks = 3; blocks && !stages; --blocks) {
         const uint32_t room = 233472 / blocks - 1024;   // an SM's, less what the system keeps of each block's
@@ -150,7 +151,7 @@ int32_t paged_attention_plan(fe2o3_ctx *ctx, const fe2o3_paged_attention_v1_args
     p->args = PagedArgs{kv_cache_of(ctx, a), reinterpret_cast<const void *>(a->q.ptr), reinterpret_cast<void *>(a->output.ptr),
                         reinterpret_cast<float *>(a->lse.ptr), static_cast<float4 *>(p->workspace),
                         counters, group, (group + 8 * nt - 1) / (8 * nt),
-                        a->q_stride, a->q_head_stride, a->window, stages, at_once, shift, box, a->scale, a->q_dtype == FE2O3_DTYPE_F32,
+                        a->q_stride, a->q_head_stride, a->window, stages, q_rows, at_once, shift, box, a->scale, a->q_dtype == FE2O3_DTYPE_F32,
                         a->output_dtype == FE2O3_DTYPE_F32, whole};
     *out = p;
     return FE2O3_OK;

@@ -33,6 +33,7 @@ struct PagedArgs {
     float4 *slots;        // kPagedSlots partial results a block
     uint32_t *arrived;    // pieces that have come in (see the joins), three counters a block; zero between launches
     uint32_t group, chunks, q_stride, q_head_stride, window, stages;
+    uint32_t q_rows;      // of the queries of a chunk in shared memory: its heads, and a row of zeros that stands for those it lacks
     uint32_t room;        // blocks that the GPU holds at once (the grid is smaller where the page table cannot fill it)
     int32_t page_shift;   // log2 of page_size, or -1
     uint32_t box;         // rows of a page that the copy engine takes at once; 1: rows go by 16-byte copies
@@ -47,7 +48,7 @@ constexpr uint32_t kPagedMaxStages = 4, kPagedMeeting = 512;
 using PagedKernel = void (*)(CUtensorMap, CUtensorMap, PagedArgs);
 struct PagedBuild {
     PagedKernel kernel;
-    uint32_t stage, part, query;   // bytes: a stage of one warp, a partial result, one term of the queries of one warp
+    uint32_t stage, part, query;   // bytes: a stage of one warp, a partial result, a row of the queries
     uint32_t scales, keys;         // bytes of a stage's scales; keys of a tile
 };
 PagedBuild paged_build_bf16(uint32_t dim, uint32_t nt);
@@ -326,13 +327,17 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     const uint32_t terms = a.q_f32 ? (F16 ? 2 : 3) : 1;
     uint8_t *const my_scales = smem + kPagedWarps * a.stages * S::kStage + warp * a.stages * S::kScales;
     uint8_t *const queries = smem + kPagedWarps * a.stages * (S::kStage + S::kScales);
-    uint8_t *const query = queries + warp * terms * S::kHeads * S::kQueryRow;
-    Meeting &meeting = *reinterpret_cast<Meeting *>(queries + kPagedWarps * terms * S::kHeads * S::kQueryRow);
+    const uint32_t term_bytes = a.q_rows * S::kQueryRow;
+    uint8_t *const query = queries + warp * terms * term_bytes;
+    Meeting &meeting = *reinterpret_cast<Meeting *>(queries + kPagedWarps * terms * term_bytes);
     const uint32_t query_s = smem_u32(query);
     const uint32_t row_bytes = a.c.dim * (F16 ? 1 : 2);
     const uint32_t per_seq = a.c.kv_heads * a.chunks;   // items of a sequence
 
     uint64_t *const bars = meeting.arrivals[warp];
+    for (uint32_t term = 0; term < terms; ++term)
+        for (uint32_t i = lane; i < S::kQueryRow / 16; i += 32)
+            *reinterpret_cast<uint4 *>(query + term * term_bytes + (a.q_rows - 1) * S::kQueryRow + 16 * i) = make_uint4(0, 0, 0, 0);
     if (lane < a.stages) mbar_init(&bars[lane], a.box > 1 ? 1 : 32);
     mbar_fence_init();
     if (a.box > 1) {
@@ -459,6 +464,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         constexpr int kLanes = DP / 8, kAtOnce = 32 / kLanes, kPasses = S::kHeads / kAtOnce;
         const uint32_t head = item / a.chunks, chunk = item % a.chunks, d = lane % kLanes * 8, r0 = lane / kLanes;
         const uint64_t base = (uint64_t)seq * a.q_stride + (uint64_t)(head * a.group) * a.q_head_stride + d;
+        const uint32_t stored = min(a.group, (uint32_t)S::kHeads);
         uint4 raw[kPasses][2];
 #pragma unroll
         for (int x = 0; x < kPasses; ++x) {
@@ -481,7 +487,8 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         }
 #pragma unroll
         for (int x = 0; x < kPasses; ++x) {
-            const uint32_t row = x * kAtOnce + r0;
+            if (x * kAtOnce >= stored) continue;
+            const uint32_t row = min(x * kAtOnce + r0, a.q_rows - 1);   // (zeros again, where the rows are odd in number)
             uint8_t *const to = query + row * S::kQueryRow + 2 * d;
             float back = 1.f;
             if constexpr (!F16) {
@@ -510,12 +517,12 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                         lo[i] = f16_pair(fabsf(v0) < INFINITY ? v0 - h.x : 0.f, fabsf(v1) < INFINITY ? v1 - h.y : 0.f);
                     }
                     *reinterpret_cast<uint4 *>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                    if (terms > 1) *reinterpret_cast<uint4 *>(to + S::kHeads * S::kQueryRow) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                    if (terms > 1) *reinterpret_cast<uint4 *>(to + term_bytes) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                 } else {
                     // cut off; what is left of 0 is the smallest number of the value's sign, so that an infinity in K stays one
 #pragma unroll
                     for (int term = 0; term < 3; ++term) {
-                        *reinterpret_cast<uint4 *>(to + term * S::kHeads * S::kQueryRow) =
+                        *reinterpret_cast<uint4 *>(to + term * term_bytes) =
                             make_uint4(bf16_pair_cut(v[0], v[1]), bf16_pair_cut(v[2], v[3]), bf16_pair_cut(v[4], v[5]), bf16_pair_cut(v[6], v[7]));
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {
@@ -628,6 +635,15 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     enter(place);
     for (uint32_t s = 0; s < a.stages; ++s) copy_tile();
 
+    uint32_t q_off[NT], c_off[NT][2];   // and of the queries: rows, and the factors of two heads in their padding
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const uint32_t row = min(8 * nt + (F16 ? g : lane & 7), a.q_rows - 1);
+        q_off[nt] = query_s + row * S::kQueryRow + (F16 ? 32 * t4 : (lane >> 3) * 16);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) c_off[nt][e] = query_s + min(8 * nt + 2 * t4 + e, a.q_rows - 1) * S::kQueryRow + 2 * DP;
+    }
+
     // ---- the share, item by item ----
     P p;
     uint32_t kind = share ? kNone : kEmpty;
@@ -671,7 +687,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                         for (int e = 0; e < 2; ++e) ldsm4(ka[mt][e], from + k_off[(ks + e) & 3] + (ks >> 2) * KT * 128 + mt * 16 * S::kPitch);
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
-                        const uint32_t at_q = query_s + (8 * nt + (lane & 7)) * S::kQueryRow + (2 * ks + (lane >> 3)) * 16;
+                        const uint32_t at_q = q_off[nt] + ks * 32;
                         uint32_t qb[4];
                         ldsm4(qb, at_q);
 #pragma unroll
@@ -687,7 +703,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                         if (terms > 1) {
 #pragma unroll
                             for (int term = 2; term; --term) {
-                                ldsm4(qb, at_q + term * S::kHeads * S::kQueryRow);
+                                ldsm4(qb, at_q + term * term_bytes);
 #pragma unroll
                                 for (int mt = 0; mt < MT; ++mt) {
                                     if (ks == 0 && term == 2) mma_first<false>(low[mt][nt], ka[mt][0], qb[0], qb[1]);
@@ -732,7 +748,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                             }
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {
-                            const uint32_t at_q = query_s + (8 * nt + g) * S::kQueryRow + 128 * j + 32 * t4 + 16 * half;
+                            const uint32_t at_q = q_off[nt] + 128 * j + 16 * half;
                             const uint4 qb = lds128(at_q);
 #pragma unroll
                             for (int mt = 0; mt < MT; ++mt) {
@@ -741,7 +757,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                                 mma<true>(s[mt][nt], kf[mt][1], qb.z, qb.w);
                             }
                             if (terms > 1) {
-                                const uint4 ql = lds128(at_q + S::kHeads * S::kQueryRow);
+                                const uint4 ql = lds128(at_q + term_bytes);
 #pragma unroll
                                 for (int mt = 0; mt < MT; ++mt) {
                                     if (j == 0 && half == 0) mma_first<true>(low[mt][nt], kf[mt][0], ql.x, ql.y);
@@ -796,8 +812,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
             uint64_t scale_o[NT];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-                const uint32_t c_at = query_s + (8 * nt + 2 * t4) * S::kQueryRow + 2 * DP;
-                const float c[2] = {lds_f32(c_at), lds_f32(c_at + S::kQueryRow)};
+                const float c[2] = {lds_f32(c_off[nt][0]), lds_f32(c_off[nt][1])};
                 float top[2] = {p.m[nt][0], p.m[nt][1]};
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt)
@@ -1076,7 +1091,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
 template <uint32_t FORMAT, int DP, int NT>
 PagedBuild paged_build() {
     using S = Shape<FORMAT, DP, NT>;
-    return PagedBuild{paged_attention_kernel<FORMAT, DP, NT>, (uint32_t)S::kStage, (uint32_t)S::kPart * 512u, (uint32_t)(S::kHeads * S::kQueryRow),
+    return PagedBuild{paged_attention_kernel<FORMAT, DP, NT>, (uint32_t)S::kStage, (uint32_t)S::kPart * 512u, (uint32_t)S::kQueryRow,
                       (uint32_t)S::kScales, (uint32_t)S::kKeys};
 }
 template <uint32_t FORMAT>
