@@ -7,6 +7,8 @@
 // start on 16 bytes are read or written element by element.  A block takes up to kTokens tokens, all their heads, K and V: one
 // warp finds their slots (offsets, lengths and page table: three trips to memory a block, not a row), and each
 // lane has kDeep rows in flight.  Blocks are as many as fill the SMs a whole number of times.
+// 131072 tokens of 8 heads of 128 read from bf16 pages 172 us (6.2 TB/s); 16384 tokens bf16 to e4m3 35 us (2.9 TB/s, 55 % of
+// the issue slots: 168 instructions a warp for two rows of K or V) and back to f32 33 us; 256 new tokens 3.0 us, an empty launch's time.
 // Quantisation needs the quotients as IEEE rounds them, and is bound by issue slots.  One division a row gives y, the
 // reciprocal of the scale rounded to nearest; q = x y, corrected twice by q + (x - q scale) y, is the correctly rounded
 // quotient (Markstein, Computation of elementary functions on the IBM RISC System/6000 processor, 1990) while nothing
