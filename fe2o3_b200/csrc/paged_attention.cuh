@@ -177,6 +177,21 @@ __device__ __forceinline__ uint32_t codes_f16(uint32_t a, uint32_t b) {
     }
 }
 
+// The four codes of a word as two f16 pairs: of the first product, whose columns may come in any order that the queries share
+// (lay_query).  i8 takes even and odd bytes: no permutation.
+template <uint32_t FORMAT>
+__device__ __forceinline__ void word_f16(uint32_t w, uint32_t &a, uint32_t &b) {
+    if constexpr (FORMAT == FE2O3_KV_I8) {
+        a = (w & 0x00ff00ffu) ^ 0x64806480u;
+        b = (w >> 8 & 0x00ff00ffu) ^ 0x64806480u;
+        asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(a) : "r"(0x64806480u));
+        asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(b) : "r"(0x64806480u));
+    } else {
+        a = codes_f16<FORMAT, 0, 1>(w, w);
+        b = codes_f16<FORMAT, 2, 1>(w, w);
+    }
+}
+
 // Where 16-byte piece c of row r lies in a stage's K or V part: as the copy engine's swizzle has it, rows in parts of 128 bytes.
 // Of what the lanes of one access touch, nothing meets on a bank but K of the 8-bit formats, in twos.
 template <uint32_t FORMAT, int DP>
@@ -521,7 +536,9 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                     uint32_t hi[4], lo[4];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const float v0 = v[2 * i] * by, v1 = v[2 * i + 1] * by;
+                        // the order of word_f16: of i8 columns 0 and 2, then 1 and 3
+                        constexpr bool kEvenOdd = FORMAT == FE2O3_KV_I8;
+                        const float v0 = v[kEvenOdd ? 4 * (i / 2) + i % 2 : 2 * i] * by, v1 = v[kEvenOdd ? 4 * (i / 2) + i % 2 + 2 : 2 * i + 1] * by;
                         hi[i] = f16_pair(v0, v1);
                         const float2 h = f16_values(hi[i]);
                         lo[i] = f16_pair(fabsf(v0) < INFINITY ? v0 - h.x : 0.f, fabsf(v1) < INFINITY ? v1 - h.y : 0.f);
@@ -751,10 +768,8 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                             for (int e = 0; e < 2; ++e) {
                                 const uint32_t w0 = half ? (e ? ka[mt][0].w : ka[mt][0].z) : (e ? ka[mt][0].y : ka[mt][0].x);
                                 const uint32_t w1 = half ? (e ? ka[mt][1].w : ka[mt][1].z) : (e ? ka[mt][1].y : ka[mt][1].x);
-                                kf[mt][e][0] = codes_f16<FORMAT, 0, 1>(w0, w0);
-                                kf[mt][e][1] = codes_f16<FORMAT, 0, 1>(w1, w1);
-                                kf[mt][e][2] = codes_f16<FORMAT, 2, 1>(w0, w0);
-                                kf[mt][e][3] = codes_f16<FORMAT, 2, 1>(w1, w1);
+                                word_f16<FORMAT>(w0, kf[mt][e][0], kf[mt][e][2]);
+                                word_f16<FORMAT>(w1, kf[mt][e][1], kf[mt][e][3]);
                             }
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {
@@ -803,8 +818,8 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                         top = fmaxf(top, vs[mt][e]);
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {
-                            s[mt][nt][2 * e] *= ks;
-                            s[mt][nt][2 * e + 1] *= ks;
+                            float (&x)[4] = s[mt][nt];
+                            unpack_f32x2(mul_f32x2(pack_f32x2(x[2 * e], x[2 * e + 1]), pack_f32x2(ks, ks)), x[2 * e], x[2 * e + 1]);
                         }
                     }
                 if (__any_sync(~0u, top >= vref)) {
@@ -824,10 +839,13 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
             for (int nt = 0; nt < NT; ++nt) {
                 const float c[2] = {lds_f32(c_off[nt][0]), lds_f32(c_off[nt][1])};
                 float top[2] = {p.m[nt][0], p.m[nt][1]};
+                const uint64_t c2 = pack_f32x2(c[0], c[1]);
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) s[mt][nt][e] *= c[e & 1];
+                for (int mt = 0; mt < MT; ++mt) {
+                    float (&x)[4] = s[mt][nt];
+                    unpack_f32x2(mul_f32x2(pack_f32x2(x[0], x[1]), c2), x[0], x[1]);
+                    unpack_f32x2(mul_f32x2(pack_f32x2(x[2], x[3]), c2), x[2], x[3]);
+                }
                 if (edge) {
 #pragma unroll
                     for (int mt = 0; mt < MT; ++mt)
@@ -853,17 +871,20 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) {
                     float w[4];
+                    const uint64_t minus = pack_f32x2(-base[0], -base[1]);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        w[e] = ex2_approx(s[mt][nt][e] - base[e & 1]);
-                        p.l[nt][e & 1] += w[e];
+                    for (int e = 0; e < 4; e += 2) {
+                        float x0, x1;
+                        unpack_f32x2(add_f32x2(pack_f32x2(s[mt][nt][e], s[mt][nt][e + 1]), minus), x0, x1);
+                        w[e] = ex2_approx(x0);
+                        w[e + 1] = ex2_approx(x1);
+                        unpack_f32x2(add_f32x2(pack_f32x2(p.l[nt][0], p.l[nt][1]), pack_f32x2(w[e], w[e + 1])), p.l[nt][0], p.l[nt][1]);
                     }
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
                         float w0 = w[2 * e], w1 = w[2 * e + 1];
                         if constexpr (F16) {
-                            w0 *= vs[mt][e];
-                            w1 *= vs[mt][e];
+                            unpack_f32x2(mul_f32x2(pack_f32x2(w0, w1), pack_f32x2(vs[mt][e], vs[mt][e])), w0, w1);
                             const uint32_t hi = f16_pair(w0, w1);
                             pb[mt][nt][0][e] = turned(hi);
                             const float2 h = f16_values(hi);
