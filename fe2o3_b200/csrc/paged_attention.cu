@@ -93,17 +93,20 @@ int32_t paged_attention_plan(fe2o3_ctx *ctx, const fe2o3_paged_attention_v1_args
     FE2O3_CUDA(cudaSetDevice(ctx->device));
     cudaFuncAttributes attr;
     FE2O3_CUDA(cudaFuncGetAttributes(&attr, reinterpret_cast<const void *>(b.kernel)));
-    // as many blocks an SM as registers and two stages a warp allow (131071 tokens: three blocks of two stages 178 us, two of
-    // three 186), then as many stages as fit; a partial result has to fit a warp's ring
+    // as many blocks an SM as registers and two stages a warp allow, then as many stages as fit; a partial result has to fit a
+    // warp's ring.  Full stages of bf16 rows: two blocks of three stages (32 sequences of 4096, 32 heads of 128 on 8: 93 us, three
+    // blocks of two 99; 64 ragged ones 98 and 102; two of 131071 186 and 183).  With 96 columns it is 92 us and 78, with
+    // pages that take several boxes a tile 103 and 100, e4m3 131 and 110.
     const uint32_t q_rows = group < 8 * nt ? group + 1 : 8 * nt;
     const uint32_t fixed = kPagedWarps * terms * q_rows * b.query + kPagedMeeting, least = b.part > 2 * b.stage ? (b.part + b.stage - 1) / b.stage : 2;
-    uint32_t stages = 0;
-    for (uint32_t blocks = 3; blocks && !stages; --blocks) {
+    auto stages_of = [&](uint32_t blocks) -> uint32_t {   // 0: not so many blocks
         const uint32_t room = 233472 / blocks - 1024;   // an SM's, less what the system keeps of each block's
-        if (blocks > 1 && (uint32_t)attr.numRegs * kPagedThreads * blocks > 65536) continue;
-        if (room < fixed + kPagedWarps * least * (b.stage + b.scales)) continue;
-        stages = (room - fixed) / (kPagedWarps * (b.stage + b.scales));
-    }
+        if (blocks > 1 && (uint32_t)attr.numRegs * kPagedThreads * blocks > 65536) return 0;
+        const uint32_t fit = room < fixed ? 0 : (room - fixed) / (kPagedWarps * (b.stage + b.scales));
+        return fit < least ? 0 : fit;
+    };
+    uint32_t stages = a->format == FE2O3_KV_BF16 && a->dim == 128 && a->page_size % b.keys == 0 && stages_of(2) >= 3 ? stages_of(2) : 0;
+    for (uint32_t blocks = 3; blocks && !stages; --blocks) stages = stages_of(blocks);
     if (!stages) return FE2O3_ERR_UNSUPPORTED_SHAPE;   // (not reached: one block fits for every build)
     if (stages > kPagedMaxStages) stages = kPagedMaxStages;
     PagedPlan *p = new (std::nothrow) PagedPlan();
@@ -111,7 +114,7 @@ int32_t paged_attention_plan(fe2o3_ctx *ctx, const fe2o3_paged_attention_v1_args
     p->kernel = b.kernel;
     p->shared = kPagedWarps * stages * (b.stage + b.scales) + fixed;
     int per_sm = 0;
-    cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void *>(b.kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, (int)p->shared);
+    cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void *>(b.kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, 232448);   // (all: plans of one kernel differ)
     if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, b.kernel, kPagedThreads, p->shared);
     const uint32_t at_once = (uint32_t)(per_sm > 0 ? per_sm : 1) * ctx->sm_count;
     p->grid = at_once;

@@ -597,6 +597,32 @@ def test_attention_on_other_streams(gpu):
     assert ctx.take_kernel_status(stream) == 0
 
 
+def test_attention_plans_of_one_kernel_stand_side_by_side(gpu):
+    """Prepared launches that share a kernel and differ in types, groups and pages: each works whichever was prepared last,
+    and a workspace that was given back starts again at zero."""
+    fe, torch, ctx, stream = gpu
+    plans = []
+    for form, dim, group, dtype, page in [("bf16", 128, 8, "f32", 16), ("bf16", 128, 1, "bf16", 24), ("bf16", 128, 7, "bf16", 16),
+                                          ("i8", 128, 16, "f32", 64), ("i8", 128, 9, "bf16", 3)]:
+        c = filled(gpu, form, [700, 0, 65], 1, dim, page)
+        q, qv = queries(torch, 3, group, dim, dtype)
+        o = torch.zeros(3, group, dim, device="cuda")
+        p = fe.prepare(ctx, "paged_attention_v1", q=q, output=o, heads=group, q_stride=group * dim, q_head_stride=dim, scale=dim ** -0.5,
+                       window=0, q_dtype=0 if dtype == "f32" else 1, output_dtype=0, **c.args())
+        plans.append((c, q, qv, o, p, attention64(c, qv, np.float32(dim ** -0.5))))
+    for order in (plans, plans[::-1]):
+        for c, q, qv, o, p, want in order:
+            o.fill_(7.0)
+            torch.cuda.synchronize()
+            p.launch_and_wait(stream, 20000)
+            check_attention(c, qv, o.cpu().numpy(), None, want, "f32")
+    for x in plans:
+        x[4].destroy()
+    for c, q, qv, o, _, want in plans:
+        got, lse = attend(c, q, c.dim ** -0.5)
+        check_attention(c, qv, got, lse, want, "f32")
+
+
 def test_decode_steps_replay_from_one_graph(gpu):
     """Append and attention captured once; lengths grow in device memory between replays, over page ends."""
     fe, torch, ctx, stream = gpu
