@@ -69,7 +69,6 @@ namespace {
 
 constexpr int kQueryExponent = 14;   // f16 queries: the largest of a row lies in [2^14, 2^15)
 
-
 template <uint32_t FORMAT, int DP, int NT>
 struct Shape {
     static constexpr bool kF16 = FORMAT != FE2O3_KV_BF16;
@@ -83,9 +82,6 @@ struct Shape {
     static constexpr int kPart = (DP / 16 + 1) * NT;                                        // float4 a lane of a partial result
 };
 
-__device__ __forceinline__ void copy16(uint32_t to, const void *from) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
-}
 __device__ __forceinline__ void copy16(uint32_t to, const void *from, bool there) {   // or zeros
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16u : 0u) : "memory");
 }
@@ -301,7 +297,7 @@ struct Part {
             for (int i = 0; i < MD; ++i) o[i][t][0] = o[i][t][1] = o[i][t][2] = o[i][t][3] = 0.f;
         }
     }
-    // Adds another part, one float4 a lane at `at`, `at` + 32, ...
+    // Adds another part, float4 by float4 in leave()'s order.
     template <typename Load>
     __device__ __forceinline__ void add(Load load) {
 #pragma unroll
@@ -392,6 +388,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     // ---- copies: the places of the share, by a cursor that runs ahead over its tiles ----
     Span<KT> lspan;
     uint32_t lseq = 0, litem = 0, lslot = 0, lrest = 0, ltile = 0, lend = 0;   // lrest: places of the share behind its present item
+    uint32_t flying = 0;                                                       // tiles asked for and not waited for
     auto enter = [&](uint32_t from) {   // the cursor's item, from this place on
         const uint32_t take = from ? min(lspan.places() - from, lrest) : line.taken(lrest, lspan.places());
         ltile = max(from, kEnd) - kEnd;
@@ -482,6 +479,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         }
         lslot = lslot + 1 == a.stages ? 0 : lslot + 1;
         ++ltile;
+        ++flying;
     };
     uint32_t seq, item;   // at work
     // ---- the queries of an item, as 16-bit terms: a lane takes eight columns of a row at a time ----
@@ -687,6 +685,12 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
             if (waiting && !mbar_wait_warp(&bars[slot], phase)) {   // (not seen: a copy that never lands)
                 if (lane == 0) kstatus_set(a.c.status, FE2O3_KSTATUS_WAIT_EXPIRED);
                 waiting = false;
+                for (uint32_t s = slot, p = phase; --flying;) {   // nothing more is asked for; what is under way gets its time
+                    if (++s == a.stages) s = 0, p ^= 1;
+                    mbar_wait_warp(&bars[s], p);
+                }
+            } else if (waiting) {
+                --flying;
             }
             const uint32_t from = ring + slot * S::kStage;
             // rows of the tile that are keys of the sequence: [ahead, left)

@@ -417,7 +417,8 @@ def test_attention_pages_and_windows(gpu, page, window):
 
 @pytest.mark.parametrize("form", FORMATS)
 @pytest.mark.parametrize("lengths,heads,kv_heads", [([30011], 4, 1), ([5000, 3], 8, 8), ([9000, 0, 1, 8999, 20], 10, 2), ([70] * 300, 2, 2),
-                                                    ([1] * 700, 3, 1), (list(range(0, 500, 3)), 4, 2), ([2049] * 9, 8, 1)])
+                                                    ([1] * 700, 3, 1), (list(range(0, 500, 3)), 4, 2), ([2049] * 9, 8, 1),
+                                                    ([i % 7 * 9 for i in range(1500)], 2, 1), ([64] * 33 + [20000] + [0] * 40, 3, 3)])
 def test_attention_split_and_joined(gpu, form, lengths, heads, kv_heads):
     """Few long sequences, many short ones, and both: the pieces that blocks compute meet in every way."""
     c = filled(gpu, form, lengths, kv_heads, 32, 16)
