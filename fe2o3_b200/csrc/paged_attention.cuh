@@ -388,7 +388,6 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     // ---- copies: the places of the share, by a cursor that runs ahead over its tiles ----
     Span<KT> lspan;
     uint32_t lseq = 0, litem = 0, lslot = 0, lrest = 0, ltile = 0, lend = 0;   // lrest: places of the share behind its present item
-    uint32_t flying = 0;                                                       // tiles asked for and not waited for
     auto enter = [&](uint32_t from) {   // the cursor's item, from this place on
         const uint32_t take = from ? min(lspan.places() - from, lrest) : line.taken(lrest, lspan.places());
         ltile = max(from, kEnd) - kEnd;
@@ -479,7 +478,6 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         }
         lslot = lslot + 1 == a.stages ? 0 : lslot + 1;
         ++ltile;
-        ++flying;
     };
     uint32_t seq, item;   // at work
     // ---- the queries of an item, as 16-bit terms: a lane takes eight columns of a row at a time ----
@@ -685,12 +683,11 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
             if (waiting && !mbar_wait_warp(&bars[slot], phase)) {   // (not seen: a copy that never lands)
                 if (lane == 0) kstatus_set(a.c.status, FE2O3_KSTATUS_WAIT_EXPIRED);
                 waiting = false;
-                for (uint32_t s = slot, p = phase; --flying;) {   // nothing more is asked for; what is under way gets its time
+                uint32_t s = slot, p = phase;
+                while ((s + 1 == a.stages ? 0 : s + 1) != lslot) {   // nothing more is asked for; what is under way gets its time
                     if (++s == a.stages) s = 0, p ^= 1;
                     mbar_wait_warp(&bars[s], p);
                 }
-            } else if (waiting) {
-                --flying;
             }
             const uint32_t from = ring + slot * S::kStage;
             // rows of the tile that are keys of the sequence: [ahead, left)
