@@ -67,7 +67,8 @@ PagedBuild paged_build_i8(uint32_t dim, uint32_t nt);
 
 namespace {
 
-constexpr int kQueryExponent = 14;   // f16 queries: the largest of a row lies in [2^14, 2^15)
+constexpr int kWeightExponent = 15;  // f16 weights: below 2^15, the largest key's, so that 2^-40 of it is not yet lost
+constexpr int kQueryExponent = 14;    // f16 queries: the largest of a row lies in [2^14, 2^15)
 
 template <uint32_t FORMAT, int DP, int NT>
 struct Shape {
@@ -678,16 +679,11 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         const uint32_t last_tile = max(place + here, kEnd) - kEnd;
         p.clear();
         lay_query();
-        float vref = 1.1754944e-38f;   // a power of two above every scale of V so far
+        float vref = __uint_as_float((uint32_t)(1 + kWeightExponent) << 23);   // a power of two above every scale of V so far
         for (uint32_t tile = max(place, kEnd) - kEnd; tile < last_tile; ++tile) {
             if (waiting && !mbar_wait_warp(&bars[slot], phase)) {   // (not seen: a copy that never lands)
                 if (lane == 0) kstatus_set(a.c.status, FE2O3_KSTATUS_WAIT_EXPIRED);
                 waiting = false;
-                uint32_t s = slot, p = phase;
-                while ((s + 1 == a.stages ? 0 : s + 1) != lslot) {   // nothing more is asked for; what is under way gets its time
-                    if (++s == a.stages) s = 0, p ^= 1;
-                    mbar_wait_warp(&bars[s], p);
-                }
             }
             const uint32_t from = ring + slot * S::kStage;
             // rows of the tile that are keys of the sequence: [ahead, left)
@@ -830,7 +826,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                     grow = vref / next;
                     vref = next;
                 }
-                const float inv = __uint_as_float(0x7f000000u - __float_as_uint(vref));   // 1 / vref: powers of two
+                const float inv = __uint_as_float(0x7f000000u + (kWeightExponent << 23) - __float_as_uint(vref));   // powers of two
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) vs[mt][0] *= inv, vs[mt][1] *= inv;
             }
@@ -967,9 +963,11 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                     unpack_f32x2(fma_f32x2(pack_f32x2(o[2], o[3]), scale_o[nt], pack_f32x2(d[2], d[3])), o[2], o[3]);
                 }
             }
-            if (++slot == a.stages) slot = 0, phase ^= 1;
             __syncwarp();   // every lane has read the stage
-            if (waiting) copy_tile();
+            if (waiting) {
+                if (++slot == a.stages) slot = 0, phase ^= 1;
+                copy_tile();
+            }
         }
 
         // the lanes of a row add up
@@ -980,7 +978,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
 #pragma unroll
                 for (int d = 4; d < 32; d <<= 1) p.l[nt][e] += __shfl_xor_sync(~0u, p.l[nt][e], d);
             if constexpr (F16) {
-                const float unit = vref;
+                const float unit = __uint_as_float(__float_as_uint(vref) - (kWeightExponent << 23));
 #pragma unroll
                 for (int i = 0; i < MD; ++i)
 #pragma unroll
@@ -1008,6 +1006,12 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                 if (++seq >= a.c.batch) break;   // not reached while the lengths stay as they are
                 span = Span<KT>(a, seq);
             }
+        }
+    }
+    if (!waiting) {   // what was under way when a wait ran out gets its time; nothing was asked for since
+        while ((slot + 1 == a.stages ? 0 : slot + 1) != lslot) {
+            if (++slot == a.stages) slot = 0, phase ^= 1;
+            mbar_wait_warp(&bars[slot], phase);
         }
     }
 

@@ -462,6 +462,27 @@ def test_attention_scales(gpu, scale):
     check_attention(c, qv, got, lse, attention64(c, qv, np.float32(scale)), "f32")
 
 
+@pytest.mark.parametrize("form", FORMATS)
+@pytest.mark.parametrize("octaves", [6, 12, 18])
+def test_attention_one_weight_far_above_the_others(gpu, form, octaves):
+    """A column in which the row of the largest weight is 0 is the small weights' sum, to the same accuracy."""
+    c = Cache(gpu, form, [2, 40, 3000], 1, 64, 16)
+    rng = np.random.default_rng(11)
+    for b, n in enumerate(c.lengths):
+        k, v = np.zeros((n, 1, 64)), rng.normal(size=(n, 1, 64))
+        k[n // 2, 0, 0] = octaves * math.log(2)
+        v[n // 2, 0, 1:] = 0
+        c.put(0, b, np.arange(n), k)
+        c.put(1, b, np.arange(n), v)
+    c.to_gpu()
+    q = c.torch.zeros(3, 2, 64, dtype=c.torch.float32, device="cuda")
+    q[:, 0, 0], q[:, 1, 0] = 1.0, 0.75
+    qv = q.cpu().numpy()
+    for out in ("f32", "bf16"):
+        got, lse = attend(c, q, 1.0, out=out)
+        check_attention(c, qv, got, lse, attention64(c, qv, 1.0), out)
+
+
 def test_attention_rising_scores(gpu):
     """Scores that rise all along (every block moves the maximum) and fall all along."""
     for sign in (1, -1):
