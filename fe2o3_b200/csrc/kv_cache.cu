@@ -1,16 +1,17 @@
 // Paged key-value cache: new rows written (rounded or quantised) and rows read back.  The formulas stand at
 // fe2o3_kv_cache_append_v1_args and fe2o3_kv_cache_read_v1_args.
 //
-// HBM-bound: each element is read once and written once.  A row is 2 to 32 lanes of eight columns each, so that a
-// row's largest magnitude is a shuffle tree and every access is 4 to 16 bytes a lane, without gaps between lanes: of f32 rows a
-// lane has four columns in each half (a store of every other 16 bytes costs half as much again).  Rows that do not
-// start on 16 bytes are read or written element by element.  A block takes up to kTokens tokens, all their heads, K and V: one
-// warp finds their slots (offsets, lengths and page table: three trips to memory a block, not a row), and each
-// lane has kDeep rows in flight.  Blocks are as many as fill the SMs a whole number of times.
-// 131072 tokens of 8 heads of 128 read from bf16 pages 172 us (6.2 TB/s); 16384 tokens bf16 to e4m3 35 us (2.9 TB/s, 55 % of
-// the issue slots: 168 instructions a warp for two rows of K or V) and back to f32 33 us; 256 new tokens 3.0 us, an empty launch's time.
-// Quantisation needs the quotients as IEEE rounds them, and is bound by issue slots.  One division a row gives y, the
-// reciprocal of the scale rounded to nearest; q = x y, corrected twice by q + (x - q scale) y, is the correctly rounded
+// HBM-bound: each element is read once and written once.  A row is pieces of 16 bytes of the caller's, two to each of 2 to 32
+// lanes (the second as far on as there are lanes, so that neither leaves gaps between lanes: a store of every other 16 bytes costs
+// half as much again); a row's largest magnitude is a shuffle tree.  Two pieces and not one: what a row costs a lane by itself
+// (its place, the tree, scale and reciprocal) is shared by 16 bf16 columns and not by 8 (to e4m3 32 -> 24 us, as it is 27 -> 26).
+// Rows that do not start on 16 bytes are read or written element by element.  A block takes up to kTokens tokens, all
+// their heads, K and V: one warp finds their slots (offsets, lengths and page table: three trips to memory a block, not a
+// row), and each lane has kDeep rows in flight.  Blocks are as many as fill the SMs a whole number of times.
+// 131072 tokens of 8 heads of 128 read from bf16 pages 168 us (6.4 TB/s); 16384 tokens bf16 to e4m3 24 us (4.2 TB/s; from f32
+// 36 us, 4.7 TB/s) and back to f32 34 us (4.9 TB/s); 256 new tokens 3.0 us, an empty launch's time.
+// Quantisation needs the quotients as IEEE rounds them, and is bound by issue slots.  One reciprocal a row gives y, that
+// of the scale rounded to nearest; q = x y, corrected twice by q + (x - q scale) y, is the correctly rounded
 // quotient (Markstein, Computation of elementary functions on the IBM RISC System/6000 processor, 1990) while nothing
 // leaves the normal range: scales outside 2^+-60 take the division itself.
 #include <atomic>
@@ -19,7 +20,7 @@
 
 namespace {
 
-constexpr int kThreads = 256, kTokens = 32, kDeep = 4;
+constexpr int kThreads = 256, kTokens = 32;
 
 struct KvRows {
     uint8_t *k, *v;   // sources of an append, destinations of a read
@@ -63,107 +64,62 @@ __device__ __forceinline__ bool slot_of(const KvCache &c, const KvRows &r, uint3
     return ok;
 }
 
-// A lane's eight columns: those from 8 l on, or for f32 rows four from 4 l and four from 4 (lanes + l) on.
+// A lane's columns: two pieces of 16 bytes of the caller's row, piece l and piece lanes + l.
 struct Columns {
-    uint32_t first, second;   // of the two fours
-    bool one, two;            // inside the row
+    uint32_t first[2];
+    bool inside[2];
 };
-__device__ __forceinline__ void widen4(const uint2 &v, float *x) {
-    x[0] = __uint_as_float(v.x << 16);
-    x[1] = __uint_as_float(v.x & 0xffff0000u);
-    x[2] = __uint_as_float(v.y << 16);
-    x[3] = __uint_as_float(v.y & 0xffff0000u);
+__device__ __forceinline__ void widen2(uint32_t v, float *x) {
+    x[0] = __uint_as_float(v << 16);
+    x[1] = __uint_as_float(v & 0xffff0000u);
 }
 __device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {   // to nearest even
     uint32_t r;
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
 }
-__device__ __forceinline__ uint2 narrow4(const float *x) { return make_uint2(bf16_pair(x[0], x[1]), bf16_pair(x[2], x[3])); }
-__device__ __forceinline__ uint4 joined(uint2 a, uint2 b) { return make_uint4(a.x, a.y, b.x, b.y); }
 
-// The caller's rows: f32 bits as two fours, or eight bf16.
+// A piece of the caller's row.
 template <bool F32, bool WHOLE>
-__device__ __forceinline__ void fetch(const uint8_t *row, const Columns &c, uint4 (&v)[2]) {
-    if constexpr (F32) {
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            if (!(half ? c.two : c.one)) continue;
-            const uint32_t *const e = reinterpret_cast<const uint32_t *>(row) + (half ? c.second : c.first);
-            if constexpr (WHOLE) v[half] = __ldcs(reinterpret_cast<const uint4 *>(e));
-            else v[half] = make_uint4(e[0], e[1], e[2], e[3]);
-        }
-    } else if (c.one) {
-        const uint16_t *const e = reinterpret_cast<const uint16_t *>(row) + c.first;
-        if constexpr (WHOLE) v[0] = __ldcs(reinterpret_cast<const uint4 *>(e));
-        else v[0] = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
+__device__ __forceinline__ uint4 fetch(const uint8_t *at) {
+    if constexpr (WHOLE) {
+        return __ldcs(reinterpret_cast<const uint4 *>(at));
+    } else if constexpr (F32) {
+        const uint32_t *const e = reinterpret_cast<const uint32_t *>(at);
+        return make_uint4(e[0], e[1], e[2], e[3]);
+    } else {
+        const uint16_t *const e = reinterpret_cast<const uint16_t *>(at);
+        return make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
     }
 }
 template <bool F32, bool WHOLE>
-__device__ __forceinline__ void put(uint8_t *row, const Columns &c, const uint4 (&v)[2]) {
-    if constexpr (F32) {
+__device__ __forceinline__ void put(uint8_t *at, const uint4 &v) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    if constexpr (WHOLE) {
+        __stcs(reinterpret_cast<uint4 *>(at), v);
+    } else {
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            if (!(half ? c.two : c.one)) continue;
-            uint32_t *const e = reinterpret_cast<uint32_t *>(row) + (half ? c.second : c.first);
-            if constexpr (WHOLE) __stcs(reinterpret_cast<uint4 *>(e), v[half]);
-            else e[0] = v[half].x, e[1] = v[half].y, e[2] = v[half].z, e[3] = v[half].w;
-        }
-    } else if (c.one) {
-        uint16_t *const e = reinterpret_cast<uint16_t *>(row) + c.first;
-        const uint32_t w[4] = {v[0].x, v[0].y, v[0].z, v[0].w};
-        if constexpr (WHOLE) {
-            __stcs(reinterpret_cast<uint4 *>(e), v[0]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) e[i] = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
+        for (int i = 0; i < (F32 ? 4 : 8); ++i) {
+            if constexpr (F32) reinterpret_cast<uint32_t *>(at)[i] = w[i];
+            else reinterpret_cast<uint16_t *>(at)[i] = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
         }
     }
 }
-// The cache's rows, which start on 16 bytes: eight elements' bits.
-template <uint32_t FORMAT, bool F32>
-__device__ __forceinline__ uint4 fetch_cached(const uint8_t *row, const Columns &c) {
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if constexpr (FORMAT == FE2O3_KV_BF16) {
-        if constexpr (!F32) {
-            if (c.one) v = __ldcs(reinterpret_cast<const uint4 *>(row + 2 * c.first));
-        } else {
-            uint2 a = make_uint2(0, 0), b = a;
-            if (c.one) a = __ldcs(reinterpret_cast<const uint2 *>(row + 2 * c.first));
-            if (c.two) b = __ldcs(reinterpret_cast<const uint2 *>(row + 2 * c.second));
-            v = joined(a, b);
-        }
-    } else {
-        if constexpr (!F32) {
-            if (c.one) {
-                const uint2 a = __ldcs(reinterpret_cast<const uint2 *>(row + c.first));
-                v.x = a.x;
-                v.y = a.y;
-            }
-        } else {
-            if (c.one) v.x = __ldcs(reinterpret_cast<const uint32_t *>(row + c.first));
-            if (c.two) v.y = __ldcs(reinterpret_cast<const uint32_t *>(row + c.second));
-        }
+// The same columns in the cache, whose rows start on 16 bytes.
+template <int BYTES>
+__device__ __forceinline__ uint4 fetch_cached(const uint8_t *at) {
+    if constexpr (BYTES == 16) return __ldcs(reinterpret_cast<const uint4 *>(at));
+    if constexpr (BYTES == 8) {
+        const uint2 v = __ldcs(reinterpret_cast<const uint2 *>(at));
+        return make_uint4(v.x, v.y, 0, 0);
     }
-    return v;
+    return make_uint4(__ldcs(reinterpret_cast<const uint32_t *>(at)), 0, 0, 0);
 }
-template <uint32_t FORMAT, bool F32>
-__device__ __forceinline__ void put_cached(uint8_t *row, const Columns &c, const uint4 &v) {
-    if constexpr (FORMAT == FE2O3_KV_BF16) {
-        if constexpr (!F32) {
-            if (c.one) *reinterpret_cast<uint4 *>(row + 2 * c.first) = v;
-        } else {
-            if (c.one) *reinterpret_cast<uint2 *>(row + 2 * c.first) = make_uint2(v.x, v.y);
-            if (c.two) *reinterpret_cast<uint2 *>(row + 2 * c.second) = make_uint2(v.z, v.w);
-        }
-    } else {
-        if constexpr (!F32) {
-            if (c.one) *reinterpret_cast<uint2 *>(row + c.first) = make_uint2(v.x, v.y);
-        } else {
-            if (c.one) *reinterpret_cast<uint32_t *>(row + c.first) = v.x;
-            if (c.two) *reinterpret_cast<uint32_t *>(row + c.second) = v.y;
-        }
-    }
+template <int BYTES>
+__device__ __forceinline__ void put_cached(uint8_t *at, const uint4 &v) {
+    if constexpr (BYTES == 16) *reinterpret_cast<uint4 *>(at) = v;
+    else if constexpr (BYTES == 8) *reinterpret_cast<uint2 *>(at) = make_uint2(v.x, v.y);
+    else *reinterpret_cast<uint32_t *>(at) = v.x;
 }
 
 template <int LANES>
@@ -173,22 +129,23 @@ __device__ __forceinline__ uint32_t highest(uint32_t v) {
     return v;
 }
 
-// x / scale for eight columns, each as IEEE division rounds it.
-__device__ __forceinline__ void quotients(const float (&x)[8], float scale, float (&q)[8]) {
+// x / scale, each as IEEE division rounds it.
+template <int N>
+__device__ __forceinline__ void quotients(float (&x)[N], float scale) {
     if (scale > 8.7e-19f && scale < 1.1e18f) {   // 2^+-60; |x| <= 448 scale, and what is below 2^-60 scale rounds to no code
-        const float y = __fdiv_rn(1.f, scale);
+        const float y = __frcp_rn(scale);
         const uint64_t y2 = pack_f32x2(y, y), minus = pack_f32x2(-scale, -scale);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint64_t v = pack_f32x2(x[2 * i], x[2 * i + 1]);
+        for (int i = 0; i < N; i += 2) {
+            const uint64_t v = pack_f32x2(x[i], x[i + 1]);
             uint64_t r = mul_f32x2(v, y2);
             r = fma_f32x2(fma_f32x2(minus, r, v), y2, r);
             r = fma_f32x2(fma_f32x2(minus, r, v), y2, r);
-            unpack_f32x2(r, q[2 * i], q[2 * i + 1]);
+            unpack_f32x2(r, x[i], x[i + 1]);
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) q[i] = scale > 0.f ? __fdiv_rn(x[i], scale) : 0.f;   // (a NaN scale: codes 0)
+        for (int i = 0; i < N; ++i) x[i] = scale > 0.f ? __fdiv_rn(x[i], scale) : 0.f;   // (a NaN scale: codes 0)
     }
 }
 // top / C, rounded to nearest: the same corrections, with 1 / C known beforehand.
@@ -203,38 +160,34 @@ __device__ __forceinline__ float scale_of(float top) {
     return __fdiv_rn(top, kC);
 }
 template <uint32_t FORMAT>
-__device__ __forceinline__ uint2 codes_of(const float (&q)[8]) {
-    uint32_t w[2];
+__device__ __forceinline__ uint32_t codes_of(const float *q) {   // four of them
+    uint32_t w;
+    if constexpr (FORMAT == FE2O3_KV_E4M3) {
+        asm("{\n\t.reg .b16 lo, hi;\n\tcvt.rn.satfinite.e4m3x2.f32 lo, %2, %1;\n\tcvt.rn.satfinite.e4m3x2.f32 hi, %4, %3;\n\t"
+            "mov.b32 %0, {lo, hi};\n\t}" : "=r"(w) : "f"(q[0]), "f"(q[1]), "f"(q[2]), "f"(q[3]));
+    } else {   // 1.5 2^23 + q is rounded to a whole number, which stands in its low bits (|q| < 127.5)
+        uint32_t e[4];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        if constexpr (FORMAT == FE2O3_KV_E4M3) {
-            asm("{\n\t.reg .b16 lo, hi;\n\tcvt.rn.satfinite.e4m3x2.f32 lo, %2, %1;\n\tcvt.rn.satfinite.e4m3x2.f32 hi, %4, %3;\n\t"
-                "mov.b32 %0, {lo, hi};\n\t}" : "=r"(w[i]) : "f"(q[4 * i]), "f"(q[4 * i + 1]), "f"(q[4 * i + 2]), "f"(q[4 * i + 3]));
-        } else {   // 1.5 2^23 + q is rounded to a whole number, which stands in its low bits (|q| < 127.5)
-            uint32_t e[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) e[j] = __float_as_uint(q[4 * i + j] + 12582912.f);
-            w[i] = __byte_perm(__byte_perm(e[0], e[1], 0x0040), __byte_perm(e[2], e[3], 0x0040), 0x5410);
-        }
+        for (int j = 0; j < 4; ++j) e[j] = __float_as_uint(q[j] + 12582912.f);
+        w = __byte_perm(__byte_perm(e[0], e[1], 0x0040), __byte_perm(e[2], e[3], 0x0040), 0x5410);
     }
-    return make_uint2(w[0], w[1]);
+    return w;
 }
 template <uint32_t FORMAT>
-__device__ __forceinline__ void values_of(const uint2 &c, float scale, float (&x)[8]) {
-    const uint32_t w[2] = {c.x, c.y};
+__device__ __forceinline__ void values_of(uint32_t w, float scale, float *x) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < 4; ++i) {
         if constexpr (FORMAT == FE2O3_KV_I8) {
             // the code's bits + 128 below 2^23's: the sum with -(2^23 + 128) is the code
-            x[i] = __uint_as_float(__byte_perm(w[i / 4] ^ 0x80808080u, 0x4b000000u, 0x7440 | (i & 3))) - 8388736.f;
+            x[i] = __uint_as_float(__byte_perm(w ^ 0x80808080u, 0x4b000000u, 0x7440 | i)) - 8388736.f;
         } else if (!(i & 1)) {
             uint32_t h;
-            asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(h) : "r"(w[i / 4] >> (8 * (i & 3))));
+            asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(h) : "r"(w >> (8 * i)));
             asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\tcvt.f32.f16 %0, lo;\n\tcvt.f32.f16 %1, hi;\n\t}" : "=f"(x[i]), "=f"(x[i + 1]) : "r"(h));
         }
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = __fmul_rn(x[i], scale);
+    for (int i = 0; i < 4; ++i) x[i] = __fmul_rn(x[i], scale);
 }
 
 // WHOLE: the caller's rows start on 16 bytes.
@@ -242,7 +195,9 @@ template <uint32_t FORMAT, bool F32, bool WRITE, bool WHOLE>
 __global__ void __launch_bounds__(kThreads) kv_rows_kernel(KvCache c, KvRows r) {
     __shared__ uint32_t slots[kTokens];
     __shared__ uint32_t known;   // tokens whose lengths allow a slot, a bit each
-    constexpr uint32_t kEb = F32 ? 4 : 2;
+    constexpr int kEb = F32 ? 4 : 2, kPiece = 16 / kEb, kCached = kPiece * kKvBytes<FORMAT>;   // a piece: columns, bytes in the cache
+    // rows a lane has in flight: two where it quantises (registers: three take 55 us where two take 52, to e4m3 and back), else four
+    constexpr int kDeep = WRITE && FORMAT != FE2O3_KV_BF16 ? 2 : 4;
     begin_after_previous();
     const uint32_t t0 = blockIdx.x * r.per_block, n = min(r.per_block, r.tokens - t0), lane = threadIdx.x & 31;
     if (threadIdx.x < 32) {
@@ -253,7 +208,7 @@ __global__ void __launch_bounds__(kThreads) kv_rows_kernel(KvCache c, KvRows r) 
     }
     __syncthreads();
     const uint32_t lanes = 1u << r.lanes_log2, at_once = kThreads >> r.lanes_log2, l = threadIdx.x & (lanes - 1);
-    const Columns columns = F32 ? Columns{4 * l, 4 * (lanes + l), 4 * l < c.dim, 4 * (lanes + l) < c.dim} : Columns{8 * l, 0, 8 * l < c.dim, false};
+    const Columns columns{{kPiece * l, kPiece * (lanes + l)}, {kPiece * l < c.dim, kPiece * (lanes + l) < c.dim}};
     const uint32_t rows = n * 2 * c.kv_heads;
     for (uint32_t base = 0; base < rows; base += kDeep * at_once) {
         const uint32_t first = base + (threadIdx.x >> r.lanes_log2);
@@ -277,72 +232,74 @@ __global__ void __launch_bounds__(kThreads) kv_rows_kernel(KvCache c, KvRows r) 
             raw[d][0] = raw[d][1] = make_uint4(0, 0, 0, 0);
             scales[d] = 0.f;
             if (!active[d]) continue;
-            if constexpr (WRITE) {
-                fetch<F32, WHOLE>(there[d], columns, raw[d]);
-            } else if (slot != ~0u) {
-                raw[d][0] = fetch_cached<FORMAT, F32>((side[d] ? c.v : c.k) + (uint64_t)at[d] * c.dim * kKvBytes<FORMAT>, columns);
-                if constexpr (FORMAT != FE2O3_KV_BF16) scales[d] = (side[d] ? c.v_scales : c.k_scales)[at[d]];
+            const uint8_t *const from = WRITE ? there[d] : (side[d] ? c.v : c.k) + (uint64_t)at[d] * c.dim * kKvBytes<FORMAT>;
+            if (!WRITE && slot == ~0u) continue;
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                if (!columns.inside[half]) continue;
+                if constexpr (WRITE) raw[d][half] = fetch<F32, WHOLE>(from + columns.first[half] * kEb);
+                else raw[d][half] = fetch_cached<kCached>(from + columns.first[half] * kKvBytes<FORMAT>);
             }
+            if constexpr (!WRITE && FORMAT != FE2O3_KV_BF16) scales[d] = (side[d] ? c.v_scales : c.k_scales)[at[d]];
         }
 #pragma unroll
         for (int d = 0; d < kDeep; ++d) {
             if (base + d * at_once >= rows) break;
-            if constexpr (FORMAT == FE2O3_KV_BF16 && !F32) {   // as it is
-                if (!active[d]) continue;
-                if constexpr (WRITE) put_cached<FORMAT, F32>((side[d] ? c.v : c.k) + (uint64_t)at[d] * c.dim * 2, columns, raw[d][0]);
-                else put<F32, WHOLE>(there[d], columns, raw[d]);
-                continue;
-            }
-            float x[8];
-            if constexpr (WRITE) {
-                uint8_t *const to = (side[d] ? c.v : c.k) + (uint64_t)at[d] * c.dim * kKvBytes<FORMAT>;
-                // the largest magnitude as bits: an infinity or a NaN is above every number
-                uint32_t top = 0;
-                if constexpr (F32) {
-                    const uint32_t w[8] = {raw[d][0].x, raw[d][0].y, raw[d][0].z, raw[d][0].w, raw[d][1].x, raw[d][1].y, raw[d][1].z, raw[d][1].w};
+            uint8_t *const to = WRITE ? (side[d] ? c.v : c.k) + (uint64_t)at[d] * c.dim * kKvBytes<FORMAT> : there[d];
+            if constexpr (WRITE && FORMAT != FE2O3_KV_BF16) {
+                float x[2 * kPiece];
+                uint32_t top = 0;   // the largest magnitude as bits: an infinity or a NaN is above every number
+                uint32_t pairs = 0;
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        x[i] = __uint_as_float(w[i]);
-                        top = max(top, w[i] & 0x7fffffffu);
-                    }
-                } else {
-                    widen4(make_uint2(raw[d][0].x, raw[d][0].y), x);
-                    widen4(make_uint2(raw[d][0].z, raw[d][0].w), x + 4);
-                    const uint32_t pairs = __vmaxu2(__vmaxu2(raw[d][0].x & 0x7fff7fffu, raw[d][0].y & 0x7fff7fffu),
-                                                    __vmaxu2(raw[d][0].z & 0x7fff7fffu, raw[d][0].w & 0x7fff7fffu));
-                    top = max(pairs << 16, pairs & 0xffff0000u);
-                }
-                if constexpr (FORMAT == FE2O3_KV_BF16) {
-                    if (active[d]) put_cached<FORMAT, F32>(to, columns, joined(narrow4(x), narrow4(x + 4)));
-                } else {
-                    if (lanes == 16) top = highest<16>(top);   // (unrolled for the usual rows)
-                    else if (lanes == 8) top = highest<8>(top);
-                    else
-                        for (uint32_t o = 1; o < lanes; o <<= 1) top = max(top, __shfl_xor_sync(~0u, top, o));
-                    const float scale = top < 0x7f800000u ? scale_of<FORMAT>(__uint_as_float(top)) : __uint_as_float(0x7fc00000u);
-                    float q[8];
-                    quotients(x, scale, q);
-                    if (active[d]) {
-                        const uint2 w = codes_of<FORMAT>(q);
-                        put_cached<FORMAT, F32>(to, columns, make_uint4(w.x, w.y, 0, 0));
-                        if (l == 0) (side[d] ? c.v_scales : c.k_scales)[at[d]] = scale;
+                for (int i = 0; i < 8; ++i) {
+                    const uint4 &v = raw[d][i / 4];
+                    const uint32_t w = i % 4 == 0 ? v.x : i % 4 == 1 ? v.y : i % 4 == 2 ? v.z : v.w;
+                    if constexpr (F32) {
+                        x[i] = __uint_as_float(w);
+                        top = max(top, w & 0x7fffffffu);
+                    } else {
+                        widen2(w, x + 2 * i);
+                        pairs = __vmaxu2(pairs, w & 0x7fff7fffu);
                     }
                 }
+                if constexpr (!F32) top = max(pairs << 16, pairs & 0xffff0000u);
+                if (lanes == 16) top = highest<16>(top);   // (unrolled for the usual rows)
+                else if (lanes == 8) top = highest<8>(top);
+                else
+                    for (uint32_t o = 1; o < lanes; o <<= 1) top = max(top, __shfl_xor_sync(~0u, top, o));
+                const float scale = top < 0x7f800000u ? scale_of<FORMAT>(__uint_as_float(top)) : __uint_as_float(0x7fc00000u);
+                quotients(x, scale);
+                if (!active[d]) continue;
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    if (!columns.inside[half]) continue;
+                    const float *const q = x + half * kPiece;
+                    put_cached<kCached>(to + columns.first[half], make_uint4(codes_of<FORMAT>(q), F32 ? 0 : codes_of<FORMAT>(q + kPiece - 4), 0, 0));
+                }
+                if (l == 0) (side[d] ? c.v_scales : c.k_scales)[at[d]] = scale;
             } else {
-                if constexpr (FORMAT == FE2O3_KV_BF16) {
-                    widen4(make_uint2(raw[d][0].x, raw[d][0].y), x);
-                    widen4(make_uint2(raw[d][0].z, raw[d][0].w), x + 4);
-                } else {
-                    values_of<FORMAT>(make_uint2(raw[d][0].x, raw[d][0].y), scales[d], x);
+                if (!active[d]) continue;
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    if (!columns.inside[half]) continue;
+                    uint4 v = raw[d][half];   // (bf16 as it is)
+                    if constexpr (FORMAT == FE2O3_KV_BF16 && F32 && WRITE) {
+                        v = make_uint4(bf16_pair(__uint_as_float(v.x), __uint_as_float(v.y)), bf16_pair(__uint_as_float(v.z), __uint_as_float(v.w)), 0, 0);
+                    } else if constexpr (FORMAT != FE2O3_KV_BF16 || F32) {
+                        float x[8];
+                        if constexpr (FORMAT == FE2O3_KV_BF16) {
+                            widen2(v.x, x);
+                            widen2(v.y, x + 2);
+                        } else {
+                            values_of<FORMAT>(v.x, scales[d], x);
+                            if constexpr (!F32) values_of<FORMAT>(v.y, scales[d], x + 4);
+                        }
+                        if constexpr (F32) v = make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+                        else v = make_uint4(bf16_pair(x[0], x[1]), bf16_pair(x[2], x[3]), bf16_pair(x[4], x[5]), bf16_pair(x[6], x[7]));
+                    }
+                    if constexpr (WRITE) put_cached<kCached>(to + columns.first[half] * kKvBytes<FORMAT>, v);
+                    else put<F32, WHOLE>(to + columns.first[half] * kEb, v);
                 }
-                uint4 v[2];
-                if constexpr (F32) {
-                    v[0] = make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
-                    v[1] = make_uint4(__float_as_uint(x[4]), __float_as_uint(x[5]), __float_as_uint(x[6]), __float_as_uint(x[7]));
-                } else {
-                    v[0] = joined(narrow4(x), narrow4(x + 4));
-                }
-                if (active[d]) put<F32, WHOLE>(there[d], columns, v);
             }
         }
     }
@@ -372,7 +329,7 @@ int32_t launch_rows(fe2o3_ctx *ctx, cudaStream_t s, const Args *a, uint32_t dtyp
     if (geo) *geo = fe2o3_geometry{{grid, 1, 1}, {kThreads, 1, 1}, 0, 1};
     if (plan_only || a->tokens == 0) return FE2O3_OK;
     uint32_t lanes_log2 = 1;
-    while ((8u << lanes_log2) < a->dim) ++lanes_log2;
+    while ((32u / eb << lanes_log2) < a->dim) ++lanes_log2;
     const KvRows r{reinterpret_cast<uint8_t *>(a->k.ptr), reinterpret_cast<uint8_t *>(a->v.ptr), a->k_token_stride, a->v_token_stride,
                    a->k_head_stride, a->v_head_stride, reinterpret_cast<const uint32_t *>(a->token_offsets.ptr), a->tokens, per_block, lanes_log2,
                    // exact for the indexes of a block, below 64 kv_heads
