@@ -9,11 +9,11 @@
 //   writes the results of items that lie in its share by itself.  Others meet twice: the warps of a block when all
 //   have done their share, through shared memory, and the blocks in the workspace, where the one that comes last to an
 //   item (a counter) joins the pieces.  Both go by the pieces' order: the same bits whoever is last.  A share a warp and not
-//   a block: with a block at every item's end, 64 sequences of 1 to 4096 tokens took 167 us and not 99.
+//   a block: with a block at every item's end, 64 sequences of 1 to 4096 tokens took 167 us where warps took 99.
 //   Tiles.  Each warp has a ring of stages of its own, so that nothing but its own copies stops a warp, and keeps the
 //   maximum, the sum and the output of what it has seen (one pass, f32).  The copy engine fetches a tile as boxes of
 //   rows that lie in one page (page sizes that are multiples of 8); other page sizes go row by row in 16-byte copies (i8, 64
-//   sequences of 4096: 133 us, and 171 with pages of one row; bf16 the same time).  Rows outside the sequence are zeros.
+//   sequences of 4096: 128 us, and 169 with pages of one row; 32 of bf16 94 and 99).  Rows outside the sequence are zeros.
 //   Products.  mma.sync with the keys (and then the output's columns) as rows and the query heads as columns: of
 //   the 8 columns of a tile few are wasted for small groups, and P is turned into an operand by movmatrix.  (The tensor unit
 //   is 20 % busy: tcgen05, whose tiles are 128 rows, would have nothing to give but its rate.)  The tensor unit's own
@@ -23,8 +23,8 @@
 //   an infinity in V stays one.  8-bit codes become f16 exactly; the probabilities then carry the row's scale, against a power of
 //   two that follows the largest scale seen, and are two f16 terms (22 bits); queries are brought to f16's range by a
 //   power of two a row.  Error against 64 bits, f32 output: 1e-7 to 5e-7, as plain f32 arithmetic has.
-// Measured (32 query heads of 128 on 8, on 4 for e4m3): 64 ragged sequences of up to 4096 tokens 99 us, 5.5 TB/s; two of 131071
-// 179 us, 6.0 TB/s; 96 ragged ones of up to 6000, e4m3, 73 us, 4.2 TB/s; 16 heads of 64 on 512 tokens 9.6 us.  In
+// Measured (32 query heads of 128 on 8, on 4 for e4m3): 64 ragged sequences of up to 4096 tokens 98 us, 5.6 TB/s; two of 131071
+// 177 to 189 us, 5.7 to 6.1 TB/s by machine; 96 ragged ones of up to 6000, e4m3, 74 us, 4.2 TB/s; 16 heads of 64 on 512 tokens 9.6 us.  In
 // the middle of a launch bf16 and e4m3 tiles come at 7.1 TB/s.  What is left: 4 us until the first tile is there (lengths,
 // page table, rows: three trips to memory), 3 us of ends and joins, and that some SMs (40 of 148 here) end a tenth later than
 // the others; a share drawn from a counter by those that are done was tried and costs more than it gives (a drawn share pays
