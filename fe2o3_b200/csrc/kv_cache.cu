@@ -129,8 +129,8 @@ __device__ __forceinline__ uint32_t highest(uint32_t v) {
     return v;
 }
 
-// x / scale, each as IEEE division rounds it.
-template <int N>
+// x / scale, each as IEEE division rounds it; up to the largest code, which a subnormal scale's few bits let it pass.
+template <uint32_t FORMAT, int N>
 __device__ __forceinline__ void quotients(float (&x)[N], float scale) {
     if (scale > 8.7e-19f && scale < 1.1e18f) {   // 2^+-60; |x| <= 448 scale, and what is below 2^-60 scale rounds to no code
         const float y = __frcp_rn(scale);
@@ -145,7 +145,7 @@ __device__ __forceinline__ void quotients(float (&x)[N], float scale) {
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < N; ++i) x[i] = scale > 0.f ? __fdiv_rn(x[i], scale) : 0.f;   // (a NaN scale: codes 0)
+        for (int i = 0; i < N; ++i) x[i] = scale > 0.f ? fminf(fmaxf(__fdiv_rn(x[i], scale), -kKvTop<FORMAT>), kKvTop<FORMAT>) : 0.f;   // (a NaN scale: codes 0)
     }
 }
 // top / C, rounded to nearest: the same corrections, with 1 / C known beforehand.
@@ -268,7 +268,7 @@ __global__ void __launch_bounds__(kThreads) kv_rows_kernel(KvCache c, KvRows r) 
                 else
                     for (uint32_t o = 1; o < lanes; o <<= 1) top = max(top, __shfl_xor_sync(~0u, top, o));
                 const float scale = top < 0x7f800000u ? scale_of<FORMAT>(__uint_as_float(top)) : __uint_as_float(0x7fc00000u);
-                quotients(x, scale);
+                quotients<FORMAT>(x, scale);
                 if (!active[d]) continue;
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {

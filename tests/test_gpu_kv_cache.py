@@ -237,6 +237,20 @@ def test_append_special_rows(gpu, form):
         assert np.isnan(got[6, 0]).all() and np.isnan(got[7, 1]).all() and np.isnan(got[8, 0]).all() and np.isfinite(got[6, 1]).all()
 
 
+@pytest.mark.parametrize("form", ["e4m3", "i8"])
+def test_append_rows_of_subnormal_scales(gpu, form):
+    """A scale of few bits may be a third below max / C: its quotients go up to the largest code, with their sign."""
+    top = np.arange(1, 1200)                       # times the smallest number
+    x = np.zeros((len(top), 1, 16), np.float32)
+    x[:, 0, 0], x[:, 0, 1], x[:, 0, 2] = top * 2.0 ** -149, -top * 2.0 ** -149, top // 2 * 2.0 ** -149
+    c = Cache(gpu, form, [len(top)], 1, 16, 16).to_gpu()
+    rows = c.up(x)
+    c.launch("kv_cache_append_v1", k=rows, v=rows, input_dtype=0, token_offsets=c.up(np.array([0, len(top)], np.uint32)), tokens=len(top), **contiguous(1, 16))
+    for side in range(2):
+        c.put(side, 0, np.arange(len(top)), x)
+    c.assert_same()
+
+
 @pytest.mark.parametrize("form", FORMATS)
 @pytest.mark.parametrize("layout", ["token_major", "head_major", "fused", "odd"])
 def test_strided_rows(gpu, form, layout):
