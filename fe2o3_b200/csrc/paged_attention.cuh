@@ -18,8 +18,9 @@
 //   the 8 columns of a tile few are wasted for small groups, and P is turned into an operand by movmatrix.  (The tensor unit
 //   is 20 % busy: tcgen05, whose tiles are 128 rows, would have nothing to give but its rate.)  The tensor unit's own
 //   sums span one tile, longer ones are f32 additions.  A bf16 cache is multiplied as it is, with the
-//   probabilities as three bf16 terms that add up to the f32 value exactly (two, 16 bits, for a bf16 output) and an f32
-//   query as three as well, the lower two in a sum of their own.  Terms are cut off, not rounded, and held above 0, so that
+//   probabilities as three bf16 terms that add up to the f32 value exactly, whatever the output's type (two terms, 16 bits, take
+//   64 ragged sequences from 100.7 to 99.4 us and put four bf16 outputs in a thousand on another side of their rounding), and an
+//   f32 query as three as well, the lower two in a sum of their own.  Terms are cut off, not rounded, and held above 0, so that
 //   an infinity in V stays one.  8-bit codes become f16 exactly; the probabilities then carry the row's scale, against a power of
 //   two that follows the largest scale seen, and are two f16 terms (22 bits); queries are brought to f16's range by a
 //   power of two a row.  Error against 64 bits, f32 output: 1e-7 to 5e-7, as plain f32 arithmetic has.
@@ -889,14 +890,8 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                         } else {
                             pb[mt][nt][0][e] = turned(bf16_pair_cut(w0, w1));
                             const float m0 = fmaxf(w0 - cut_bf16(w0), 1.1754944e-38f), m1 = fmaxf(w1 - cut_bf16(w1), 1.1754944e-38f);
-                            if (a.o_f32) {
-                                pb[mt][nt][1][e] = turned(bf16_pair_cut(m0, m1));
-                                pb[mt][nt][2][e] = turned(bf16_pair_cut(fmaxf(m0 - cut_bf16(m0), 1.1754944e-38f), fmaxf(m1 - cut_bf16(m1), 1.1754944e-38f)));
-                            } else {
-                                uint32_t r;
-                                asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(m1), "f"(m0));
-                                pb[mt][nt][1][e] = turned(r);
-                            }
+                            pb[mt][nt][1][e] = turned(bf16_pair_cut(m0, m1));
+                            pb[mt][nt][2][e] = turned(bf16_pair_cut(fmaxf(m0 - cut_bf16(m0), 1.1754944e-38f), fmaxf(m1 - cut_bf16(m1), 1.1754944e-38f)));
                         }
                     }
                 }
@@ -953,9 +948,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                     for (int mt = 0; mt < MT; ++mt) {
                         if (mt == 0) mma_first<F16>(d, va[mt], pb[mt][nt][1][0], pb[mt][nt][1][1]);
                         else mma<F16>(d, va[mt], pb[mt][nt][1][0], pb[mt][nt][1][1]);
-                        if constexpr (!F16) {
-                            if (a.o_f32) mma<false>(d, va[mt], pb[mt][nt][2][0], pb[mt][nt][2][1]);
-                        }
+                        if constexpr (!F16) mma<false>(d, va[mt], pb[mt][nt][2][0], pb[mt][nt][2][1]);
                         mma<F16>(d, va[mt], pb[mt][nt][0][0], pb[mt][nt][0][1]);
                     }
                     float (&o)[4] = p.o[i][nt];

@@ -419,6 +419,18 @@ def test_attention_head_sizes_and_types(gpu, form, dim, dtype, out):
     check_attention(c, qv, got, lse, attention64(c, qv, np.float32(scale)), out)
 
 
+@pytest.mark.parametrize("form", FORMATS)
+@pytest.mark.parametrize("dim,group", [(64, 4), (128, 1), (128, 9), (80, 16)])
+def test_attention_bf16_output_is_the_f32_one_rounded(gpu, form, dim, group):
+    """The output's type changes its last rounding and nothing before it: bit for bit."""
+    c = filled(gpu, form, EDGES + [1000, 3000], 2, dim, 16)
+    for dtype in ("bf16", "f32"):
+        q, _ = queries(c.torch, len(EDGES) + 2, 2 * group, dim, dtype, by=0.5)
+        whole, lse = attend(c, q, dim ** -0.5)
+        short, lse2 = attend(c, q, dim ** -0.5, out="bf16")
+        assert (short == from_bf16(to_bf16(whole))).all() and (lse == lse2).all()
+
+
 @pytest.mark.parametrize("page", [1, 3, 8, 16, 40, 64, 256])
 @pytest.mark.parametrize("window", [0, 1, 5, 16, 50, 128, 1000])
 def test_attention_pages_and_windows(gpu, page, window):
