@@ -21,9 +21,11 @@
 //   probabilities as three bf16 terms that add up to the f32 value exactly, whatever the output's type (two terms, 16 bits, take
 //   64 ragged sequences from 100.7 to 99.4 us and put four bf16 outputs in a thousand on another side of their rounding), and an
 //   f32 query as three as well, the lower two in a sum of their own.  Terms are cut off, not rounded, and held above 0, so that
-//   an infinity in V stays one.  8-bit codes become f16 exactly; the probabilities then carry the row's scale, against a power of
-//   two that follows the largest scale seen, and are two f16 terms (22 bits); queries are brought to f16's range by a
-//   power of two a row.  Error against 64 bits, f32 output: 1e-7 to 5e-7, as plain f32 arithmetic has.
+//   an infinity in V stays one.  8-bit codes become f16 exactly; the probabilities then carry the row's scale and are two f16
+//   terms (22 bits), in units of a power of two a head that follows the largest product of the two.  (One unit for all heads, of
+//   the largest scale: e4m3 73.8 us for 74.1, 16 heads on one i8 head 53.2 for 53.7; but a large row of no weight takes the
+//   others' bits, all of them from 2^40 on.)  f32 queries are two f16 terms, bf16 ones a single one, in units of a power of two
+//   a row.  Error against 64 bits, f32 output: 1e-7 to 5e-7, as plain f32 arithmetic has.
 // Measured (32 query heads of 128 on 8, on 4 for e4m3): 64 ragged sequences of up to 4096 tokens 98 us, 5.6 TB/s; two of 131071
 // 177 to 189 us, 5.7 to 6.1 TB/s by machine; 96 ragged ones of up to 6000, e4m3, 74 us, 4.2 TB/s; 16 heads of 64 on 512 tokens 9.6 us.  In
 // the middle of a launch bf16 and e4m3 tiles come at 7.1 TB/s.  What is left: 4 us until the first tile is there (lengths,
@@ -68,7 +70,10 @@ PagedBuild paged_build_i8(uint32_t dim, uint32_t nt);
 
 namespace {
 
-constexpr int kWeightExponent = 15;  // f16 weights: below 2^15, the largest key's, so that 2^-40 of it is not yet lost
+// f16 weights (probability times the row's scale): the largest of a head so far lies in [2^14, 2^15), what is rounded away is at most
+// 2^-25, half of f16's smallest number: weights from 2^-17 of the largest have 22 bits, those below 2^-39 are lost.
+constexpr int kWeightExponent = 15;
+constexpr float kLeastWeight = 0x1p-112f, kMostWeight = 0x1.fffffep125f;   // the largest weight is held in between: powers of two and their reciprocals stay normal numbers
 constexpr int kQueryExponent = 14;    // f16 queries: the largest of a row lies in [2^14, 2^15)
 
 template <uint32_t FORMAT, int DP, int NT>
@@ -152,6 +157,13 @@ __device__ __forceinline__ float2 f16_values(uint32_t p) {
 __device__ __forceinline__ float cut_bf16(float v) { return __uint_as_float(__float_as_uint(v) & 0xffff0000u); }
 __device__ __forceinline__ uint32_t bf16_pair_cut(float lo, float hi) { return __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x7632); }
 
+// The next power of two above v.
+__device__ __forceinline__ float above(float v) { return __uint_as_float((__float_as_uint(v) & 0x7f800000u) + 0x00800000u); }
+__device__ __forceinline__ float lg2_approx(float v) {
+    float r;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
 __device__ __forceinline__ uint16_t bf16_of(float v) {   // to nearest even
     uint16_t r;
     asm("cvt.rn.bf16.f32 %0, %1;" : "=h"(r) : "f"(v));
@@ -680,7 +692,9 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         const uint32_t last_tile = max(place + here, kEnd) - kEnd;
         p.clear();
         lay_query();
-        float vref = __uint_as_float((uint32_t)(1 + kWeightExponent) << 23);   // a power of two above every scale of V so far
+        float heaviest[NT][2];   // 8-bit caches: the largest weight of a head so far, as p.m is the largest score
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) heaviest[nt][0] = heaviest[nt][1] = kLeastWeight;
         for (uint32_t tile = max(place, kEnd) - kEnd; tile < last_tile; ++tile) {
             if (waiting && !mbar_wait_warp(&bars[slot], phase)) {   // (not seen: a copy that never lands)
                 if (lane == 0) kstatus_set(a.c.status, FE2O3_KSTATUS_WAIT_EXPIRED);
@@ -802,34 +816,22 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
             }
 
             // the running maximum, in units of log2; weights
-            float vs[MT][2];
-            float grow = 1.f;   // of the output's unit
+            float vs[MT][2], vs_log[MT][2];
             if constexpr (F16) {
                 const uint32_t scales = smem_u32(my_scales) + slot * S::kScales + 4 * g;
-                float top = 0.f;
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
                         const float ks = lds_f32(scales + 4 * (16 * mt + 8 * e));
                         vs[mt][e] = lds_f32(scales + 4 * KT + 4 * (16 * mt + 8 * e));
-                        top = fmaxf(top, vs[mt][e]);
+                        vs_log[mt][e] = lg2_approx(vs[mt][e]);   // (of 0 the lowest there is: such a row weighs nothing)
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {
                             float (&x)[4] = s[mt][nt];
                             unpack_f32x2(mul_f32x2(pack_f32x2(x[2 * e], x[2 * e + 1]), pack_f32x2(ks, ks)), x[2 * e], x[2 * e + 1]);
                         }
                     }
-                if (__any_sync(~0u, top >= vref)) {
-#pragma unroll
-                    for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
-                    const float next = __uint_as_float((__float_as_uint(top) & 0x7f800000u) + 0x00800000u);
-                    grow = vref / next;
-                    vref = next;
-                }
-                const float inv = __uint_as_float(0x7f000000u + (kWeightExponent << 23) - __float_as_uint(vref));   // powers of two
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt) vs[mt][0] *= inv, vs[mt][1] *= inv;
             }
             uint32_t pb[MT][NT][3][2];   // weights as the second product's operand, by terms
             uint64_t scale_o[NT];
@@ -855,17 +857,44 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                 for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) top[e] = max3(top[e], s[mt][nt][e], s[mt][nt][e + 2]);
-                float base[2], keep[2];
+                float weight[2] = {-INFINITY, -INFINITY};   // the tile's largest score with the row's scale in it
+                if constexpr (F16) {
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt) {
+                        float x[4];
+#pragma unroll
+                        for (int e = 0; e < 2; ++e)
+                            unpack_f32x2(add_f32x2(pack_f32x2(s[mt][nt][2 * e], s[mt][nt][2 * e + 1]), pack_f32x2(vs_log[mt][e], vs_log[mt][e])), x[2 * e], x[2 * e + 1]);
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) weight[e] = max3(weight[e], x[e], x[e + 2]);
+                    }
+                }
+                float base[2], keep[2], unit[2];
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
 #pragma unroll
-                    for (int d = 4; d < 32; d <<= 1) top[e] = fmaxf(top[e], __shfl_xor_sync(~0u, top[e], d));
+                    for (int d = 4; d < 32; d <<= 1) {
+                        top[e] = fmaxf(top[e], __shfl_xor_sync(~0u, top[e], d));
+                        if constexpr (F16) weight[e] = fmaxf(weight[e], __shfl_xor_sync(~0u, weight[e], d));
+                    }
                     base[e] = top[e] == -INFINITY ? 0.f : top[e];
                     keep[e] = ex2_approx(p.m[nt][e] - base[e]);
                     p.m[nt][e] = top[e];
                     p.l[nt][e] *= keep[e];
                 }
-                scale_o[nt] = F16 ? pack_f32x2(keep[0] * grow, keep[1] * grow) : pack_f32x2(keep[0], keep[1]);
+                scale_o[nt] = pack_f32x2(keep[0], keep[1]);
+                if constexpr (F16) {   // the output counts in units of a power of two just above the largest weight
+                    float by[2];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const float before = keep[e] * above(heaviest[nt][e]);
+                        heaviest[nt][e] = fminf(fmaxf(fmaxf(heaviest[nt][e] * keep[e], ex2_approx(weight[e] - base[e])), kLeastWeight), kMostWeight);
+                        const uint32_t inverse = 0x7f000000u - __float_as_uint(above(heaviest[nt][e]));
+                        by[e] = before * __uint_as_float(inverse);
+                        unit[e] = __uint_as_float(inverse + (kWeightExponent << 23));
+                    }
+                    scale_o[nt] = pack_f32x2(by[0], by[1]);
+                }
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) {
                     float w[4];
@@ -882,7 +911,8 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                     for (int e = 0; e < 2; ++e) {
                         float w0 = w[2 * e], w1 = w[2 * e + 1];
                         if constexpr (F16) {
-                            unpack_f32x2(mul_f32x2(pack_f32x2(w0, w1), pack_f32x2(vs[mt][e], vs[mt][e])), w0, w1);
+                            // (in this order: a scale of no weight may be beyond f32 in these units)
+                            unpack_f32x2(mul_f32x2(mul_f32x2(pack_f32x2(w0, w1), pack_f32x2(unit[0], unit[1])), pack_f32x2(vs[mt][e], vs[mt][e])), w0, w1);
                             const uint32_t hi = f16_pair(w0, w1);
                             pb[mt][nt][0][e] = turned(hi);
                             const float2 h = f16_values(hi);
@@ -971,11 +1001,12 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
 #pragma unroll
                 for (int d = 4; d < 32; d <<= 1) p.l[nt][e] += __shfl_xor_sync(~0u, p.l[nt][e], d);
             if constexpr (F16) {
-                const float unit = __uint_as_float(__float_as_uint(vref) - (kWeightExponent << 23));
 #pragma unroll
-                for (int i = 0; i < MD; ++i)
+                for (int e = 0; e < 4; ++e) {
+                    const float unit = __uint_as_float(__float_as_uint(above(heaviest[nt][e & 1])) - (kWeightExponent << 23));
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) p.o[i][nt][e] *= unit;
+                    for (int i = 0; i < MD; ++i) p.o[i][nt][e] *= unit;
+                }
             }
         }
         const bool begins = place == 0, ended = place + here == span.places();

@@ -473,7 +473,9 @@ typedef struct fe2o3_kv_cache_read_v1_args {
  * with the keys and values of head h / (heads / kv_heads).  heads is a multiple of kv_heads.  q row (b, h) starts at
  * element b * q_stride + h * q_head_stride; output [batch][heads][dim] is packed, f32 or bf16; lse
  * [batch][heads] f32 is optional.  The page table has at most 2^35 positions (2^44 times heads), batch * heads is below 2^31.  A sequence of length 0 gives zeros and -inf.  Sums, maxima and
- * probabilities are f32, and a bf16 output is the f32 one rounded to nearest even.  The result does not
+ * probabilities are f32, and a bf16 output is the f32 one rounded to nearest even.  Over 8-bit caches a probability
+ * times its row's scale has 22 significant bits from 2^-17 of the head's largest such product on, fewer below, and counts as
+ * nothing below 2^-39 of it; the elements of a query likewise against the largest of their row (bf16 ones are exact from 2^-31 on).  The result does not
  * depend on which blocks finish first.  One launch of a prepared object at a time (it owns a workspace); what is patched into
  * its argument block later has no effect. */
 typedef struct fe2o3_paged_attention_v1_args {

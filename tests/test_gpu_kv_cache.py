@@ -509,6 +509,58 @@ def test_attention_one_weight_far_above_the_others(gpu, form, octaves):
         check_attention(c, qv, got, lse, attention64(c, qv, 1.0), out)
 
 
+@pytest.mark.parametrize("form", FORMATS)
+@pytest.mark.parametrize("octaves", [10, 20, 30, 45, 60])
+def test_attention_values_of_unlike_size(gpu, form, octaves):
+    """A row of values far larger than the others, which one head of a pair gives next to no weight and the other next to all
+    of it: each head has the accuracy that its own products of probability and value allow, wherever the row lies.  (i8 rounds a
+    small value of a row to 0, and what lies under a 0 of the heaviest row is held as the next test says: here no value is small.)"""
+    lengths = [2, 20, 40, 333, 3000] + [300] * 200
+    c = Cache(gpu, form, lengths, 1, 16, 16)
+    rng = np.random.default_rng(12)
+    for b, n in enumerate(c.lengths):
+        big = [0, n - 1, n // 2, n // 3][b % 4]
+        k, v = rng.normal(size=(n, 1, 16)) * 0.01, rng.normal(size=(n, 1, 16)) * 2.0 ** -octaves
+        k[:, 0, 0], v[big] = 0.0, rng.choice([-1, 1], (1, 16)) * rng.uniform(0.5, 1, (1, 16)) if form == "i8" else rng.normal(size=(1, 16))
+        k[big, 0, 0] = (octaves + 6) * math.log(2)
+        if b % 3 == 0:
+            v[(big + 1) % n] = 0                    # and a row of zeros
+        c.put(0, b, np.arange(n), k)
+        c.put(1, b, np.arange(n), v)
+    c.to_gpu()
+    q = rng.normal(size=(len(lengths), 4, 16))
+    q[:, :, 0] = [-1.0, 1.0, -1.5, 0.0]
+    for dtype, out in (("f32", "f32"), ("bf16", "f32"), ("bf16", "bf16")):
+        qt, qv = rows_in(c.torch, q, dtype)
+        got, lse = attend(c, qt, 1.0, out=out)
+        check_attention(c, qv, got, lse, attention64(c, qv, 1.0), out)
+
+
+@pytest.mark.parametrize("form", ["e4m3", "i8"])
+@pytest.mark.parametrize("octaves", [24, 30, 36, 50])
+def test_attention_small_weights_of_8_bit_caches(gpu, form, octaves):
+    """Weights are held to 2^-25 where the head's largest, probability times scale, lies in [2^14, 2^15): to 2^-39 of it, times the
+    largest code for each key.  A column in which the row of the largest weight is 0 shows it."""
+    c = Cache(gpu, form, [2, 40, 3000], 1, 64, 16)
+    rng = np.random.default_rng(13)
+    for b, n in enumerate(c.lengths):
+        k, v = np.zeros((n, 1, 64)), rng.normal(size=(n, 1, 64))
+        k[n // 2, 0, 0] = octaves * math.log(2)
+        v[n // 2, 0, 1:] = 0
+        c.put(0, b, np.arange(n), k)
+        c.put(1, b, np.arange(n), v)
+    c.to_gpu()
+    q = c.torch.zeros(3, 1, 64, dtype=c.torch.float32, device="cuda")
+    q[:, :, 0] = 1.0
+    got, lse = attend(c, q, 1.0)
+    o, l64, mag, big = attention64(c, q.cpu().numpy(), 1.0)
+    n = np.asarray(c.lengths, np.float64)[:, None, None]
+    d = (72 * 2.0 ** -23 + 2.0 ** -22) * big[..., None]
+    largest = mag.max(-1, keepdims=True)            # the largest weight times the largest code, at least
+    assert (np.abs(got - o) <= (2 * d + 2.0 ** -19 + n * 2.0 ** -24) * mag + n * 2.0 ** -39 * largest).all()
+    assert octaves > 30 or (np.abs(got - o)[1:, :, 1:] <= 0.1 * mag[1:, :, 1:]).all()   # (some bits of them are still there)
+
+
 def test_attention_rising_scores(gpu):
     """Scores that rise all along (every block moves the maximum) and fall all along."""
     for sign in (1, -1):
