@@ -11,7 +11,7 @@
 // 131072 tokens of 8 heads of 128 read from bf16 pages 168 us (6.4 TB/s); 16384 tokens bf16 to e4m3 24 us (4.2 TB/s; from f32
 // 36 us, 4.7 TB/s) and back to f32 34 us (4.9 TB/s); 256 new tokens 3.0 us, an empty launch's time.
 // Quantisation needs the quotients as IEEE rounds them, and is bound by issue slots.  One reciprocal a row gives y, that
-// of the scale rounded to nearest; q = x y, corrected twice by q + (x - q scale) y, is the correctly rounded
+// of the scale rounded to nearest; q = x y, corrected twice by q + (x - q scale) y (both with a minus), is the correctly rounded
 // quotient (Markstein, Computation of elementary functions on the IBM RISC System/6000 processor, 1990) while nothing
 // leaves the normal range: scales outside 2^+-60 take the division itself.
 #include <atomic>
@@ -129,23 +129,24 @@ __device__ __forceinline__ uint32_t highest(uint32_t v) {
     return v;
 }
 
-// x / scale, each as IEEE division rounds it; up to the largest code, which a subnormal scale's few bits let it pass.
+// -x / scale, each as IEEE division rounds it; up to the largest code, which a subnormal scale's few bits let it pass.  (With a
+// minus, because the corrections of a quotient of 0 are then zeros of the opposite sign and leave it its own.)
 template <uint32_t FORMAT, int N>
-__device__ __forceinline__ void quotients(float (&x)[N], float scale) {
+__device__ __forceinline__ void minus_quotients(float (&x)[N], float scale) {
     if (scale > 8.7e-19f && scale < 1.1e18f) {   // 2^+-60; |x| <= 448 scale, and what is below 2^-60 scale rounds to no code
-        const float y = __frcp_rn(scale);
-        const uint64_t y2 = pack_f32x2(y, y), minus = pack_f32x2(-scale, -scale);
+        const float y = -__frcp_rn(scale);
+        const uint64_t y2 = pack_f32x2(y, y), scale2 = pack_f32x2(scale, scale);
 #pragma unroll
         for (int i = 0; i < N; i += 2) {
             const uint64_t v = pack_f32x2(x[i], x[i + 1]);
             uint64_t r = mul_f32x2(v, y2);
-            r = fma_f32x2(fma_f32x2(minus, r, v), y2, r);
-            r = fma_f32x2(fma_f32x2(minus, r, v), y2, r);
+            r = fma_f32x2(fma_f32x2(scale2, r, v), y2, r);
+            r = fma_f32x2(fma_f32x2(scale2, r, v), y2, r);
             unpack_f32x2(r, x[i], x[i + 1]);
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < N; ++i) x[i] = scale > 0.f ? fminf(fmaxf(__fdiv_rn(x[i], scale), -kKvTop<FORMAT>), kKvTop<FORMAT>) : 0.f;   // (a NaN scale: codes 0)
+        for (int i = 0; i < N; ++i) x[i] = scale > 0.f ? fminf(fmaxf(-__fdiv_rn(x[i], scale), -kKvTop<FORMAT>), kKvTop<FORMAT>) : -0.f;   // (a NaN scale: codes 0)
     }
 }
 // top / C, rounded to nearest: the same corrections, with 1 / C known beforehand.
@@ -160,15 +161,16 @@ __device__ __forceinline__ float scale_of(float top) {
     return __fdiv_rn(top, kC);
 }
 template <uint32_t FORMAT>
-__device__ __forceinline__ uint32_t codes_of(const float *q) {   // four of them
+__device__ __forceinline__ uint32_t codes_of(const float *q) {   // four of them, of -q
     uint32_t w;
     if constexpr (FORMAT == FE2O3_KV_E4M3) {
         asm("{\n\t.reg .b16 lo, hi;\n\tcvt.rn.satfinite.e4m3x2.f32 lo, %2, %1;\n\tcvt.rn.satfinite.e4m3x2.f32 hi, %4, %3;\n\t"
             "mov.b32 %0, {lo, hi};\n\t}" : "=r"(w) : "f"(q[0]), "f"(q[1]), "f"(q[2]), "f"(q[3]));
-    } else {   // 1.5 2^23 + q is rounded to a whole number, which stands in its low bits (|q| < 127.5)
+        w ^= 0x80808080u;
+    } else {   // 1.5 2^23 - q is rounded to a whole number, which stands in its low bits (|q| < 127.5)
         uint32_t e[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) e[j] = __float_as_uint(q[j] + 12582912.f);
+        for (int j = 0; j < 4; ++j) e[j] = __float_as_uint(12582912.f - q[j]);
         w = __byte_perm(__byte_perm(e[0], e[1], 0x0040), __byte_perm(e[2], e[3], 0x0040), 0x5410);
     }
     return w;
@@ -268,7 +270,7 @@ __global__ void __launch_bounds__(kThreads) kv_rows_kernel(KvCache c, KvRows r) 
                 else
                     for (uint32_t o = 1; o < lanes; o <<= 1) top = max(top, __shfl_xor_sync(~0u, top, o));
                 const float scale = top < 0x7f800000u ? scale_of<FORMAT>(__uint_as_float(top)) : __uint_as_float(0x7fc00000u);
-                quotients<FORMAT>(x, scale);
+                minus_quotients<FORMAT>(x, scale);
                 if (!active[d]) continue;
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {

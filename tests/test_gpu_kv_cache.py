@@ -252,6 +252,28 @@ def test_append_rows_of_subnormal_scales(gpu, form):
 
 
 @pytest.mark.parametrize("form", FORMATS)
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_append_keeps_the_sign_of_zero(gpu, form, dtype):
+    """-0 among ordinary numbers is e4m3's code 0x80, 0 its code 0; so are numbers that round to 0, at every size of the scale."""
+    rng = np.random.default_rng(15)
+    size = np.array([2.0 ** -120, 2.0 ** -70, 2.0 ** -61, 2.0 ** -59, 1e-6, 1.0, 300.0, 2.0 ** 50, 2.0 ** 70, 2.0 ** 110])
+    x = (rng.normal(size=(len(size), 2, 48)) * size[:, None, None]).astype(np.float32)
+    x[:, :, 0:48:5], x[:, :, 1:48:5] = -0.0, 0.0
+    x[:, :, 2:48:5] *= np.float32(2.0 ** -20)
+    c = Cache(gpu, form, [len(size)], 2, 48, 4).to_gpu()
+    t, xv = rows_in(c.torch, x, dtype)
+    kw = dict(token_offsets=c.up(np.array([0, len(size)], np.uint32)), tokens=len(size), **contiguous(2, 48))
+    c.launch("kv_cache_append_v1", k=t, v=t, input_dtype=int(dtype == "bf16"), **kw)
+    for side in range(2):
+        c.put(side, 0, np.arange(len(size)), xv)
+    c.assert_same()
+    out = [c.torch.zeros(len(size), 2, 48, device="cuda") for _ in range(2)]
+    c.launch("kv_cache_read_v1", k=out[0], v=out[1], output_dtype=0, **kw)
+    if form != "i8":
+        assert (np.signbit(out[0].cpu().numpy()) == np.signbit(xv)).all()
+
+
+@pytest.mark.parametrize("form", FORMATS)
 @pytest.mark.parametrize("layout", ["token_major", "head_major", "fused", "odd"])
 def test_strided_rows(gpu, form, layout):
     """One new token a sequence without offsets; rows inside wider storage, heads before tokens, starts on odd elements."""
