@@ -442,6 +442,58 @@ def test_attention_head_sizes_and_types(gpu, form, dim, dtype, out):
 
 
 @pytest.mark.parametrize("form", FORMATS)
+@pytest.mark.parametrize("dim", [48, 112, 128, 144, 256])
+@pytest.mark.parametrize("group", [9, 16, 20])
+def test_attention_groups_above_eight(gpu, form, dim, group):
+    """Sixteen query heads at once, and more than one chunk of them, at every build's width of a row."""
+    lengths = [0, 1, 17, 90, 260]
+    c = filled(gpu, form, lengths, 2, dim, 16)
+    for dtype, out in (("bf16", "f32"), ("f32", "f32"), ("f32", "bf16")):
+        q, qv = queries(c.torch, len(lengths), 2 * group, dim, dtype)
+        got, lse = attend(c, q, dim ** -0.5, out=out)
+        check_attention(c, qv, got, lse, attention64(c, qv, np.float32(dim ** -0.5)), out)
+
+
+@pytest.mark.parametrize("form", FORMATS)
+@pytest.mark.parametrize("dim", [16, 48, 80, 96, 144, 208, 256])
+@pytest.mark.parametrize("page", [1, 3, 20])
+def test_attention_row_by_row(gpu, form, dim, page):
+    """Pages that take no boxes, with rows narrower than their build's: the columns past a head's are zeros that no copy touches."""
+    lengths = [0, 1, 33, 100, 301, 64]
+    c = filled(gpu, form, lengths, 2, dim, page)
+    for group in (3, 11):
+        q, qv = queries(c.torch, len(lengths), 2 * group, dim, "bf16")
+        for window in (0, 50):
+            got, lse = attend(c, q, dim ** -0.5, window=window)
+            check_attention(c, qv, got, lse, attention64(c, qv, np.float32(dim ** -0.5), window), "f32")
+
+
+@pytest.mark.parametrize("form", ["e4m3", "i8"])
+@pytest.mark.parametrize("dim", [64, 96, 256])
+def test_attention_scales_that_start_on_any_float(gpu, form, dim):
+    """Scales off 16 bytes go row by row too, and the rows of an append and a read find them."""
+    lengths = [5, 0, 70, 200]
+    c = filled(gpu, form, lengths, 3, dim, 32)
+    q, qv = queries(c.torch, len(lengths), 12, dim, "bf16")
+    n = c.pages * 3 * 32
+    for off in (1, 2, 3):
+        held = [c.torch.full((n + 8,), math.nan, device="cuda") for _ in range(2)]
+        for t, name in zip(held, ("k_scales", "v_scales")):
+            t[off:off + n] = c.d[name].reshape(-1)
+        scales = dict(k_scales=(held[0].data_ptr() + 4 * off, n), v_scales=(held[1].data_ptr() + 4 * off, n))
+        got, lse = attend(c, q, dim ** -0.5, **scales)
+        check_attention(c, qv, got, lse, attention64(c, qv, np.float32(dim ** -0.5)), "f32")
+        rows, out = (c.torch.randn(200, 3, dim, device="cuda") for _ in range(2))
+        kw = dict(token_offsets=c.up(np.array([0, 0, 0, 0, 200], np.uint32)), tokens=200, **contiguous(3, dim), **scales)
+        c.launch("kv_cache_append_v1", k=rows, v=rows, input_dtype=0, **kw)
+        c.launch("kv_cache_read_v1", k=out, v=c.torch.empty_like(out), output_dtype=0, **kw)
+        code, scale = quantised(rows.cpu().numpy(), form)
+        assert (out.cpu().numpy() == values_of(code, scale, form).astype(np.float32)).all()
+        assert all(t[:off].isnan().all() and t[off + n:].isnan().all() for t in held)
+        c.to_gpu()
+
+
+@pytest.mark.parametrize("form", FORMATS)
 @pytest.mark.parametrize("dim,group", [(64, 4), (128, 1), (128, 9), (80, 16)])
 def test_attention_bf16_output_is_the_f32_one_rounded(gpu, form, dim, group):
     """The output's type changes its last rounding and nothing before it: bit for bit."""
