@@ -94,6 +94,14 @@ def test_rows_of_new_tokens(op):
     assert err(op, **{**kw, "v_cache": sl(0, 10 * 2 * 16 * 64)}) == "OutputAliasesInput" if op == "kv_cache_append_v1" else True
 
 
+def test_caches_that_are_one_array():
+    """What only reads takes K and V from the same array; what writes does not."""
+    same = {**cache(), "v_cache": sl(0, 10 * 2 * 16 * 64)}
+    ok("kv_cache_read_v1", **{**same, **rows()})
+    ok("paged_attention_v1", **{**same, **queries()})
+    assert err("kv_cache_append_v1", **{**same, **rows()}) == "OutputAliasesInput"
+
+
 def test_attention_arguments():
     kw = {**cache(), **queries()}
     op = "paged_attention_v1"
