@@ -662,10 +662,10 @@ int regions_for(uint32_t op, const void *args, Region *r, int32_t *status) {
             int n = kv_cache_regions(a, r, 0, false, status);
             if (!n) return 0;
             if (a->heads == 0 || a->heads % a->kv_heads || a->q_dtype > FE2O3_DTYPE_BF16 || a->output_dtype > FE2O3_DTYPE_BF16 ||
-                !isfinite(a->scale) || (uint64_t)a->batch * a->heads > 0x7fffffffu ||
+                !isfinite(a->scale) || (uint64_t)a->batch * a->heads > 0x7fffffffu || a->batch > (1u << 29) ||   // (places are counted in 32 bits)
                 (a->batch && (uint64_t)a->table_width * a->page_size > (1ull << 35) / a->batch) ||
                 (uint64_t)a->batch * a->table_width * a->page_size > (1ull << 44) / a->heads) {
-                *status = unsupported("paged_attention_v1 needs heads a multiple of kv_heads, batch * heads < 2^31, at most 2^35 positions in "
+                *status = unsupported("paged_attention_v1 needs heads a multiple of kv_heads, batch * heads < 2^31, batch <= 2^29, at most 2^35 positions in "
                                       "the page table and 2^44 of all heads, f32 or bf16 queries and output, a finite scale");
                 return 0;
             }

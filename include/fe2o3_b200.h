@@ -472,7 +472,7 @@ typedef struct fe2o3_kv_cache_read_v1_args {
  *   output[b][h] = sum_j softmax_j(scale * q[b][h] . k_j) v_j,   lse[b][h] = log sum_j exp(scale * q[b][h] . k_j)
  * with the keys and values of head h / (heads / kv_heads).  heads is a multiple of kv_heads.  q row (b, h) starts at
  * element b * q_stride + h * q_head_stride; output [batch][heads][dim] is packed, f32 or bf16; lse
- * [batch][heads] f32 is optional.  The page table has at most 2^35 positions (2^44 times heads), batch * heads is below 2^31.  A sequence of length 0 gives zeros and -inf.  Sums, maxima and
+ * [batch][heads] f32 is optional.  The page table has at most 2^35 positions (2^44 times heads), batch * heads is below 2^31, batch at most 2^29.  A sequence of length 0 gives zeros and -inf.  Sums, maxima and
  * probabilities are f32, and a bf16 output is the f32 one rounded to nearest even.  Over 8-bit caches a probability
  * times its row's scale has 22 significant bits from 2^-17 of the head's largest such product on, fewer below, and counts as
  * nothing below 2^-39 of it; the elements of a query likewise against the largest of their row (bf16 ones are exact from 2^-31 on).  The result does not

@@ -122,6 +122,19 @@ def test_attention_arguments():
     assert err(op, **many) == "UnsupportedShape"
 
 
+@pytest.mark.parametrize("batch,fits", [(1 << 29, True), ((1 << 29) + 1, False), ((1 << 31) - 1, False)])
+def test_attention_batches_that_can_be_counted(batch, fits):
+    """Two places a sequence beside its tiles (2^31 of those, in all of a page table) fit 32 bits."""
+    far = lambda i: BASE + (i << 40)  # noqa: E731
+    kw = dict(cache(kv_heads=1, dim=16), batch=batch, table_width=1, page_table=(far(1), batch), lengths=(far(2), batch), heads=1,
+              q=(far(3), 16), q_stride=0, q_head_stride=0, output=(far(4), 16 * batch), lse=None, scale=1.0, window=0, q_dtype=1, output_dtype=1,
+              k_cache=sl(0, 10 * 16 * 16), v_cache=sl(8, 10 * 16 * 16))
+    if fits:
+        ok("paged_attention_v1", **kw)
+    else:
+        assert err("paged_attention_v1", **kw) == "UnsupportedShape"
+
+
 # ---- the host's book of pages ----------------------------------------------------------------------------------------
 
 def test_pages_are_handed_out_and_come_back():
