@@ -6,7 +6,8 @@
 #include "paged_attention.cuh"
 
 // Workspaces of one device: pieces of slabs that stay until the process ends, so that preparing a launch seldom waits for
-// the allocator (half a millisecond to tens of them); what is given back goes to the next plan of the same size.
+// the allocator (half a millisecond to tens of them).  Pieces are powers of two from 64 KiB on, and what is given back goes to the next
+// plan of the same power: a program that prepares for many geometries, a few at a time, keeps a few pieces of each.
 namespace {
 
 struct Workspaces {
@@ -20,7 +21,12 @@ struct Workspaces {
     uint8_t *slab = nullptr;
     size_t left = 0;
 
-    cudaError_t take(size_t bytes, void **out) {
+    static size_t size_of(size_t bytes) {
+        size_t size = 65536;
+        while (size < bytes) size *= 2;
+        return size;
+    }
+    cudaError_t take(size_t bytes, void **out) {   // (bytes as size_of gives them)
         std::lock_guard<std::mutex> held(lock);
         for (Piece **p = &returned; *p; p = &(*p)->next) {
             if ((*p)->bytes != bytes) continue;
@@ -35,7 +41,13 @@ struct Workspaces {
             void *fresh = nullptr;
             const cudaError_t e = cudaMalloc(&fresh, size);
             if (e != cudaSuccess) return e;
-            slab = static_cast<uint8_t *>(fresh);   // (what was left of the last one is not used any more)
+            for (size_t part = 64u << 20; part >= 65536; part /= 2)   // what is left of the last one, as pieces
+                while (left >= part) {
+                    put(slab, part);
+                    slab += part;
+                    left -= part;
+                }
+            slab = static_cast<uint8_t *>(fresh);
             left = size;
         }
         *out = slab;
@@ -44,11 +56,14 @@ struct Workspaces {
         return cudaSuccess;
     }
     void give(void *at, size_t bytes) {   // no launch uses it any more
-        Piece *const p = new (std::nothrow) Piece{at, bytes, nullptr};
-        if (!p) return;
         std::lock_guard<std::mutex> held(lock);
-        p->next = returned;
-        returned = p;
+        put(at, bytes);
+    }
+
+private:
+    void put(void *at, size_t bytes) {
+        Piece *const p = new (std::nothrow) Piece{at, bytes, returned};
+        if (p) returned = p;
     }
 };
 Workspaces *workspaces_of(int device) {
@@ -124,7 +139,7 @@ int32_t paged_attention_plan(fe2o3_ctx *ctx, const fe2o3_paged_attention_v1_args
     if (most < p->grid) p->grid = most < 1 ? 1 : (uint32_t)most;
     const size_t slots = (size_t)kPagedSlots * p->grid * b.part;   // behind them: counters
     p->device = ctx->device;
-    p->bytes = (slots + 3 * p->grid * sizeof(uint32_t) + 65535) / 65536 * 65536;
+    p->bytes = Workspaces::size_of(slots + 3 * p->grid * sizeof(uint32_t));
     Workspaces *const workspaces = workspaces_of(ctx->device);
     if (e == cudaSuccess) e = workspaces ? workspaces->take(p->bytes, &p->workspace) : cudaErrorInvalidDevice;
     if (e == cudaSuccess) e = cudaMemset(static_cast<uint8_t *>(p->workspace) + slots, 0, 3 * p->grid * sizeof(uint32_t));

@@ -797,6 +797,21 @@ def test_attention_plans_of_one_kernel_stand_side_by_side(gpu):
         check_attention(c, qv, got, lse, want, "f32")
 
 
+def test_attention_workspaces_of_many_geometries(gpu):
+    """Prepared and destroyed one after another, launches for all sizes of a batch share a few pieces: one of each power of two up to
+    the largest need (16 MiB at most), in one or two slabs of 64 MiB."""
+    fe, torch, ctx, stream = gpu
+    c = Cache(gpu, "bf16", [0], 1, 128, 16, width=16).to_gpu()
+    lengths, table = torch.zeros(100, dtype=torch.int32, device="cuda"), torch.zeros(100 * 16, dtype=torch.int32, device="cuda")
+    q, o = torch.zeros(100, 8, 128, device="cuda"), torch.zeros(100, 8, 128, device="cuda")
+    torch.cuda.synchronize()
+    before = torch.cuda.mem_get_info()[0]
+    for batch in range(1, 101):
+        args = {**c.args(), "batch": batch, "lengths": lengths[:batch], "page_table": table[:batch * 16], "q": q[:batch], "output": o[:batch]}
+        fe.prepare(ctx, "paged_attention_v1", heads=8, q_stride=1024, q_head_stride=128, scale=1.0, window=0, q_dtype=0, output_dtype=0, **args).destroy()
+    assert before - torch.cuda.mem_get_info()[0] <= 130 << 20
+
+
 def test_decode_steps_replay_from_one_graph(gpu):
     """Append and attention captured once; lengths grow in device memory between replays, over page ends."""
     fe, torch, ctx, stream = gpu
