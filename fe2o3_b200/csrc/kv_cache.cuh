@@ -47,27 +47,6 @@ __device__ __forceinline__ uint32_t kv_row(const KvCache &c, uint32_t b, uint32_
     return (page * c.kv_heads + h) * c.page_size + slot;
 }
 
-// Exact value of an e4m3 code (both formats are halves of f16's range).
-__device__ __forceinline__ float e4m3_to_f32(uint8_t code) {
-    uint32_t h;
-    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)code));
-    float f;
-    asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.f32.f16 %0, lo;\n\t}" : "=f"(f) : "r"(h));
-    return f;
-}
-__device__ __forceinline__ uint8_t f32_to_e4m3(float v) {
-    uint16_t c;
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(c) : "f"(0.f), "f"(v));
-    return (uint8_t)c;
-}
-
-// Element i of a row, as the code stands for (scale apart).
-template <uint32_t FORMAT>
-__device__ __forceinline__ float kv_element(const uint8_t *row, uint32_t i) {
-    if constexpr (FORMAT == FE2O3_KV_BF16) return bf16_bits_to_f32(reinterpret_cast<const uint16_t *>(row)[i]);
-    if constexpr (FORMAT == FE2O3_KV_E4M3) return e4m3_to_f32(row[i]);
-    return (float)reinterpret_cast<const int8_t *>(row)[i];
-}
 template <uint32_t FORMAT>
 constexpr uint32_t kKvBytes = FORMAT == FE2O3_KV_BF16 ? 2 : 1;   // of an element
 template <uint32_t FORMAT>
