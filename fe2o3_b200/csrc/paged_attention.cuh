@@ -23,7 +23,7 @@
 //   f32 query as three as well, the lower two in a sum of their own.  Terms are cut off, not rounded, and held above 0, so that
 //   an infinity in V stays one.  8-bit codes become f16 exactly; the probabilities then carry the row's scale and are two f16
 //   terms (22 bits), in units of a power of two a head that follows the largest product of the two.  (One unit for all heads, of
-//   the largest scale: e4m3 73.8 us for 74.1, 16 heads on one i8 head 53.2 for 53.7; but a large row of no weight takes the
+//   the largest scale: e4m3 73.8 us for 73.5, 16 heads on one i8 head 53.2 for 53.8; but a large row of no weight takes the
 //   others' bits, all of them from 2^40 on.)  f32 queries are two f16 terms, bf16 ones a single one, in units of a power of two
 //   a row.  Error against 64 bits, f32 output: 1e-7 to 5e-7, as plain f32 arithmetic has.
 // Measured (32 query heads of 128 on 8, on 4 for e4m3): 64 ragged sequences of up to 4096 tokens 98 us, 5.6 TB/s; two of 131071
@@ -857,38 +857,39 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                 for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) top[e] = max3(top[e], s[mt][nt][e], s[mt][nt][e + 2]);
-                float weight[2] = {-INFINITY, -INFINITY};   // the tile's largest score with the row's scale in it
-                if constexpr (F16) {
-#pragma unroll
-                    for (int mt = 0; mt < MT; ++mt) {
-                        float x[4];
-#pragma unroll
-                        for (int e = 0; e < 2; ++e)
-                            unpack_f32x2(add_f32x2(pack_f32x2(s[mt][nt][2 * e], s[mt][nt][2 * e + 1]), pack_f32x2(vs_log[mt][e], vs_log[mt][e])), x[2 * e], x[2 * e + 1]);
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) weight[e] = max3(weight[e], x[e], x[e + 2]);
-                    }
-                }
                 float base[2], keep[2], unit[2];
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
 #pragma unroll
-                    for (int d = 4; d < 32; d <<= 1) {
-                        top[e] = fmaxf(top[e], __shfl_xor_sync(~0u, top[e], d));
-                        if constexpr (F16) weight[e] = fmaxf(weight[e], __shfl_xor_sync(~0u, weight[e], d));
-                    }
+                    for (int d = 4; d < 32; d <<= 1) top[e] = fmaxf(top[e], __shfl_xor_sync(~0u, top[e], d));
                     base[e] = top[e] == -INFINITY ? 0.f : top[e];
                     keep[e] = ex2_approx(p.m[nt][e] - base[e]);
                     p.m[nt][e] = top[e];
                     p.l[nt][e] *= keep[e];
                 }
                 scale_o[nt] = pack_f32x2(keep[0], keep[1]);
+                const uint64_t minus = pack_f32x2(-base[0], -base[1]);
                 if constexpr (F16) {   // the output counts in units of a power of two just above the largest weight
-                    float by[2];
+                    float weight[2] = {-INFINITY, -INFINITY}, by[2];   // weight: the tile's largest, as a logarithm
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt) {
+                        float (&x)[4] = s[mt][nt];
+                        float y[4];
+#pragma unroll
+                        for (int e = 0; e < 4; e += 2) {
+                            const uint64_t score = add_f32x2(pack_f32x2(x[e], x[e + 1]), minus);
+                            unpack_f32x2(score, x[e], x[e + 1]);
+                            unpack_f32x2(add_f32x2(score, pack_f32x2(vs_log[mt][e / 2], vs_log[mt][e / 2])), y[e], y[e + 1]);
+                        }
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) weight[e] = max3(weight[e], y[e], y[e + 2]);
+                    }
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
+#pragma unroll
+                        for (int d = 4; d < 32; d <<= 1) weight[e] = fmaxf(weight[e], __shfl_xor_sync(~0u, weight[e], d));
                         const float before = keep[e] * above(heaviest[nt][e]);
-                        heaviest[nt][e] = fminf(fmaxf(fmaxf(heaviest[nt][e] * keep[e], ex2_approx(weight[e] - base[e])), kLeastWeight), kMostWeight);
+                        heaviest[nt][e] = fminf(fmaxf(fmaxf(heaviest[nt][e] * keep[e], ex2_approx(weight[e])), kLeastWeight), kMostWeight);
                         const uint32_t inverse = 0x7f000000u - __float_as_uint(above(heaviest[nt][e]));
                         by[e] = before * __uint_as_float(inverse);
                         unit[e] = __uint_as_float(inverse + (kWeightExponent << 23));
@@ -898,11 +899,10 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) {
                     float w[4];
-                    const uint64_t minus = pack_f32x2(-base[0], -base[1]);
 #pragma unroll
                     for (int e = 0; e < 4; e += 2) {
-                        float x0, x1;
-                        unpack_f32x2(add_f32x2(pack_f32x2(s[mt][nt][e], s[mt][nt][e + 1]), minus), x0, x1);
+                        float x0 = s[mt][nt][e], x1 = s[mt][nt][e + 1];
+                        if constexpr (!F16) unpack_f32x2(add_f32x2(pack_f32x2(x0, x1), minus), x0, x1);
                         w[e] = ex2_approx(x0);
                         w[e + 1] = ex2_approx(x1);
                         unpack_f32x2(add_f32x2(pack_f32x2(p.l[nt][0], p.l[nt][1]), pack_f32x2(w[e], w[e + 1])), p.l[nt][0], p.l[nt][1]);

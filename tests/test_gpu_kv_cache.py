@@ -635,6 +635,27 @@ def test_attention_small_weights_of_8_bit_caches(gpu, form, octaves):
     assert octaves > 30 or (np.abs(got - o)[1:, :, 1:] <= 0.1 * mag[1:, :, 1:]).all()   # (some bits of them are still there)
 
 
+@pytest.mark.parametrize("form", FORMATS)
+@pytest.mark.parametrize("score", [2.0 ** 18, 2.0 ** 22, -2.0 ** 24, 2.0 ** 26, 2.0 ** 30, -2.0 ** 34])
+def test_attention_equal_scores_far_from_zero(gpu, form, score):
+    """Every key has the same score, however large: the output is the mean of the values, whose rows are of unlike size."""
+    lengths = [1, 2, 31, 100, 999]
+    c = Cache(gpu, form, lengths, 1, 16, 16)
+    rng = np.random.default_rng(17)
+    for b, n in enumerate(c.lengths):
+        k, v = np.zeros((n, 1, 16)), rng.normal(size=(n, 1, 16)) * 2.0 ** rng.integers(0, 12, (n, 1, 1))
+        k[:, 0, 0] = score
+        c.put(0, b, np.arange(n), k)
+        c.put(1, b, np.arange(n), v)
+    c.to_gpu()
+    q = c.torch.zeros(len(lengths), 3, 16, device="cuda")
+    q[:, 0, 0], q[:, 2, 0] = 1.0, 0.75
+    got, _ = attend(c, q, 1.0)
+    for b, n in enumerate(lengths):
+        v = c.get(1, b, np.arange(n))[:, 0]
+        assert (np.abs(got[b] - v.mean(0)) <= (2.0 ** -19 + n * 2.0 ** -24) * np.abs(v).mean(0) + n * 2.0 ** -39 * np.abs(v).max()).all()
+
+
 def test_attention_rising_scores(gpu):
     """Scores that rise all along (every block moves the maximum) and fall all along."""
     for sign in (1, -1):
