@@ -20,8 +20,8 @@
 //   sums span one tile, longer ones are f32 additions.  A bf16 cache is multiplied as it is, with the
 //   probabilities as three bf16 terms that add up to the f32 value exactly, whatever the output's type (two terms, 16 bits, take
 //   64 ragged sequences from 100.7 to 99.4 us and put four bf16 outputs in a thousand on another side of their rounding), and an
-//   f32 query as three as well, the lower two in a sum of their own.  Terms are cut off, not rounded, and held above 0, so that
-//   an infinity in V stays one.  8-bit codes become f16 exactly; the probabilities then carry the row's scale and are two f16
+//   f32 query as three as well, the lower two in a sum of their own.  Terms are cut off, not rounded, and held above 2^-40
+//   of the number, so that an infinity in V stays one.  8-bit codes become f16 exactly; the probabilities then carry the row's scale and are two f16
 //   terms (22 bits), in units of a power of two a head that follows the largest product of the two.  (One unit for all heads, of
 //   the largest scale: e4m3 73.8 us for 73.5, 16 heads on one i8 head 53.2 for 53.8; but a large row of no weight takes the
 //   others' bits, all of them from 2^40 on.)  f32 queries are two f16 terms, bf16 ones a single one, in units of a power of two
@@ -74,6 +74,7 @@ namespace {
 // 2^-25, half of f16's smallest number: weights from 2^-17 of the largest have 22 bits, those below 2^-39 are lost.
 constexpr int kWeightExponent = 15;
 constexpr float kLeastWeight = 0x1p-112f, kMostWeight = 0x1.fffffep125f;   // the largest weight is held in between: powers of two and their reciprocals stay normal numbers
+constexpr float kLeastTerm = 0x1p-40f;   // of a number, the least that its lower bf16 terms are: far below its last bit, and nothing where it is 0
 constexpr int kQueryExponent = 14;    // f16 queries: the largest of a row lies in [2^14, 2^15)
 
 template <uint32_t FORMAT, int DP, int NT>
@@ -157,6 +158,16 @@ __device__ __forceinline__ float2 f16_values(uint32_t p) {
 __device__ __forceinline__ float cut_bf16(float v) { return __uint_as_float(__float_as_uint(v) & 0xffff0000u); }
 __device__ __forceinline__ uint32_t bf16_pair_cut(float lo, float hi) { return __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x7632); }
 
+__device__ __forceinline__ uint32_t bf16_max(uint32_t a, uint32_t b) {   // of a pair
+    uint32_t r;
+    asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+__device__ __forceinline__ uint32_t bf16_least(uint32_t v) {   // kLeastTerm of a pair
+    uint32_t r;
+    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(v), "r"((__float_as_uint(kLeastTerm) >> 16) * 0x10001u));
+    return r;
+}
 // The next power of two above v.
 __device__ __forceinline__ float above(float v) { return __uint_as_float((__float_as_uint(v) & 0x7f800000u) + 0x00800000u); }
 __device__ __forceinline__ float lg2_approx(float v) {
@@ -556,7 +567,10 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                     *reinterpret_cast<uint4 *>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
                     if (terms > 1) *reinterpret_cast<uint4 *>(to + term_bytes) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                 } else {
-                    // cut off; what is left of 0 is the smallest number of the value's sign, so that an infinity in K stays one
+                    // cut off; where nothing is left it is next to nothing with the value's sign, so that an infinity in K stays one
+                    float least[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) least[i] = fabsf(v[i]) * kLeastTerm;
 #pragma unroll
                     for (int term = 0; term < 3; ++term) {
                         *reinterpret_cast<uint4 *>(to + term * term_bytes) =
@@ -564,7 +578,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {
                             const float left = v[i] - cut_bf16(v[i]);
-                            if (fabsf(v[i]) < INFINITY && v[i] != 0.f) v[i] = fabsf(left) < 1.1754944e-38f ? copysignf(1.1754944e-38f, v[i]) : left;
+                            if (fabsf(v[i]) < INFINITY) v[i] = fabsf(left) < least[i] ? copysignf(least[i], v[i]) : left;
                         }
                     }
                 }
@@ -918,10 +932,11 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                             const float2 h = f16_values(hi);
                             pb[mt][nt][1][e] = turned(f16_pair(w0 - h.x, w1 - h.y));
                         } else {
-                            pb[mt][nt][0][e] = turned(bf16_pair_cut(w0, w1));
-                            const float m0 = fmaxf(w0 - cut_bf16(w0), 1.1754944e-38f), m1 = fmaxf(w1 - cut_bf16(w1), 1.1754944e-38f);
-                            pb[mt][nt][1][e] = turned(bf16_pair_cut(m0, m1));
-                            pb[mt][nt][2][e] = turned(bf16_pair_cut(fmaxf(m0 - cut_bf16(m0), 1.1754944e-38f), fmaxf(m1 - cut_bf16(m1), 1.1754944e-38f)));
+                            const uint32_t hi = bf16_pair_cut(w0, w1), least = bf16_least(hi);
+                            const float m0 = w0 - cut_bf16(w0), m1 = w1 - cut_bf16(w1);
+                            pb[mt][nt][0][e] = turned(hi);
+                            pb[mt][nt][1][e] = turned(bf16_max(bf16_pair_cut(m0, m1), least));
+                            pb[mt][nt][2][e] = turned(bf16_max(bf16_pair_cut(m0 - cut_bf16(m0), m1 - cut_bf16(m1)), least));
                         }
                     }
                 }

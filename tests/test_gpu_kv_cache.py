@@ -656,6 +656,44 @@ def test_attention_equal_scores_far_from_zero(gpu, form, score):
         assert (np.abs(got[b] - v.mean(0)) <= (2.0 ** -19 + n * 2.0 ** -24) * np.abs(v).mean(0) + n * 2.0 ** -39 * np.abs(v).max()).all()
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("gap", [60.0, 95.0, 200.0, math.inf])
+def test_attention_largest_values_without_weight(gpu, dtype, gap):
+    """Rows of the largest numbers that bf16 holds, `gap` below the other keys' scores: they count with their weight and, where that
+    is 0, not at all.  (A weight below f32's normal numbers may be 0: 2^-126 of the value.)"""
+    lengths = [2, 30, 700]
+    c = Cache(gpu, "bf16", lengths, 1, 16, 16)
+    rng = np.random.default_rng(18)
+    for b, n in enumerate(c.lengths):
+        k, v = np.zeros((n, 1, 16)), rng.normal(size=(n, 1, 16))
+        far = [0, n // 2, n - 1][b]
+        k[far, 0, 0], v[far] = -gap, from_bf16(np.full((1, 16), 0x7f7f, np.uint16))
+        c.put(0, b, np.arange(n), k)
+        c.put(1, b, np.arange(n), v)
+    c.to_gpu()
+    q, qv = rows_in(c.torch, np.eye(1, 16)[None].repeat(3, 0), dtype)
+    got, lse = attend(c, q, 1.0)
+    with np.errstate(all="ignore"):
+        o, l64, mag, big = attention64(c, qv, 1.0)
+    n = np.asarray(lengths, np.float64)[:, None]
+    weight = np.exp(-gap)
+    bound = (2 * (24 * 2.0 ** -23 + 2.0 ** -22) * min(gap, 100.0) + 2.0 ** -19 + n * 2.0 ** -24)[..., None] * mag
+    bound = bound + (weight * 3.4e38 if weight < 2.0 ** -126 else 0.0)
+    assert (np.abs(got - o) <= bound).all() and (np.abs(lse - l64) <= 1e-5).all()
+    # a query element far below the others, times the largest keys
+    c = Cache(gpu, "bf16", [50], 1, 16, 16)
+    k, v = np.zeros((50, 1, 16)), rng.normal(size=(50, 1, 16))
+    k[:, 0, 1] = np.linspace(-3e38, 3e38, 50)
+    c.put(0, 0, np.arange(50), k)
+    c.put(1, 0, np.arange(50), v)
+    c.to_gpu()
+    q = np.zeros((1, 1, 16))
+    q[0, 0, 1] = 2.0 ** -124
+    qt, qv = rows_in(c.torch, q, dtype)
+    got, lse = attend(c, qt, 1.0)
+    check_attention(c, qv, got, lse, attention64(c, qv, 1.0), "f32")
+
+
 def test_attention_rising_scores(gpu):
     """Scores that rise all along (every block moves the maximum) and fall all along."""
     for sign in (1, -1):
