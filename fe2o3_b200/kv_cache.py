@@ -3,7 +3,8 @@
 `PageTable` is the host's book of pages (no GPU).  `PagedKvCache` owns the cache's device memory in one of three formats
 and launches the library's operators on it: `append` writes new tokens' keys and values, `attend` lets one new token a
 sequence attend to all its positions, `read` brings rows back.  `DecodeStep` binds the tensors of a step once, so that a
-step is two launches and two small copies.
+step is two launches and the copy of the lengths; a step in which a sequence begins a page copies the whole page table too
+(4 bytes a page that the table has room for), from ordinary memory.
 
     cache = PagedKvCache(ctx, stream, sequences=8, positions=4096, kv_heads=8, dim=128, format=KV_E4M3)
     cache.extend([prompt_length] * 8)           # pages for the prompts' tokens
@@ -12,7 +13,10 @@ step is two launches and two small copies.
     for _ in range(n):                          # fill q, k1, v1 on the stream, then
         step.run()
 
-Everything is enqueued on the cache's stream; nothing waits for the GPU but reading results.
+`append`, `extend`, `release` and the steps are enqueued on the cache's stream and do not wait for its launches (but a copy from
+ordinary memory may hold the host until the stream has come to it, once it is larger than the driver keeps aside).  What waits:
+preparing an attention (`attention`, `DecodeStep`) for the legacy stream, destroying one for the whole device, `attend`, which
+does both, and `read` for the cache's stream.
 """
 import numpy as np
 
@@ -130,7 +134,7 @@ class PagedKvCache:
                      **self._rows(k, v, self.new_tokens, strides))
 
     def read(self, k, v, counts, dtype=None, strides=None):
-        """The last `counts[b]` rows of every sequence b into k and v."""
+        """The last `counts[b]` rows of every sequence b into k and v, which are there when this returns."""
         offsets = np.zeros(self.sequences + 1, np.uint32)
         offsets[1:] = np.cumsum(counts)
         at = DeviceBuffer.from_host(self.stream, offsets)
@@ -146,7 +150,8 @@ class PagedKvCache:
                        output_dtype=_float_dtype(out, out_dtype), **self.args())
 
     def attend(self, q, out, heads, **kw):
-        """One new token a sequence, q and out [sequences][heads][dim]."""
+        """One new token a sequence, q and out [sequences][heads][dim].  Returns when the device is idle, since the launch's workspace
+        goes back: a program that attends again and again keeps an `attention` or a `DecodeStep`."""
         p = self.attention(q, out, heads, **kw)
         try:
             p.launch(self.stream)

@@ -434,7 +434,7 @@ typedef struct fe2o3_moe_ep_ffn_v1_args {
  * [pages][kv_heads][page_size].  For a row x and the format's largest code C (448 and 127):
  *   scale = max |x| / C, code = x / scale rounded to the nearest code, ties to even,
  * both quotients rounded to f32; a row of zeros has scale 0, a row with an infinity or a NaN has scale NaN and
- * reads back as NaN.  bf16 elements are rounded to nearest even, and a NaN becomes a quiet one.
+ * reads back as NaN.  A bf16 cache holds f32 rows rounded to nearest even, a NaN as a quiet one, and bf16 rows bit for bit.
  * dim is a multiple of 16 up to 256, kv_heads at most 65536, page_size any number from 1, a cache has fewer than 2^32 rows, a sequence has fewer than 2^31 positions; both
  * caches start on 16 bytes.  Lengths and page table stay as they are while a launch runs.
  *
