@@ -9,8 +9,9 @@
 // their heads, K and V: one warp finds their slots (offsets, lengths and page table: three trips to memory a block, not a
 // row), and each lane has kDeep rows in flight.  Blocks are as many as fill the SMs a whole number of times.
 // 131072 tokens of 8 heads of 128 read from bf16 pages 168 us (6.4 TB/s); 16384 tokens bf16 to e4m3 24 us (4.2 TB/s; from f32
-// 36 us, 4.7 TB/s) and back to f32 34 us (4.9 TB/s); 256 new tokens 3.0 us, an empty launch's time.
-// Quantisation needs the quotients as IEEE rounds them, and is bound by issue slots.  One reciprocal a row gives y, that
+// 37 us, 4.6 TB/s) and back to f32 34 us (4.9 TB/s); 256 new tokens 3.0 us, an empty launch's time.
+// Quantisation needs the quotients as IEEE rounds them; it fills 59 % of the issue slots and 33 % of the DRAM's cycles, and what lies
+// between is one wave's beginning (slots, then rows) and a row's chain of maximum, scale and quotients.  One reciprocal a row gives y, that
 // of the scale rounded to nearest; q = x y, corrected twice by q + (x - q scale) y (both with a minus), is the correctly rounded
 // quotient (Markstein, Computation of elementary functions on the IBM RISC System/6000 processor, 1990) while nothing
 // leaves the normal range: scales outside 2^+-60 take the division itself.

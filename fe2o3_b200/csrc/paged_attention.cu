@@ -109,9 +109,9 @@ int32_t paged_attention_plan(fe2o3_ctx *ctx, const fe2o3_paged_attention_v1_args
     cudaFuncAttributes attr;
     FE2O3_CUDA(cudaFuncGetAttributes(&attr, reinterpret_cast<const void *>(b.kernel)));
     // as many blocks an SM as registers and two stages a warp allow, then as many stages as fit; a partial result has to fit a
-    // warp's ring.  Full stages of bf16 rows: two blocks of three stages (32 sequences of 4096, 32 heads of 128 on 8: 93 us, three
-    // blocks of two 99; 64 ragged ones 98 and 102; two of 131071 186 and 183).  With 96 columns it is 92 us and 78, with
-    // pages that take several boxes a tile 103 and 100, e4m3 131 and 110.
+    // warp's ring.  Full stages of bf16 rows: two blocks of three stages (32 sequences of 4096, 32 heads of 128 on 8: 95 us, three
+    // blocks of two 101; 64 ragged ones 100 and 105; two of 131071 178 and 181).  Rows of 112 columns take 94 us so and 92 with three
+    // blocks, of 96 columns 94 and 77, pages that take several boxes a tile 101 and 99, e4m3 135 and 113, i8 147 and 131.
     const uint32_t q_rows = group < 8 * nt ? group + 1 : 8 * nt;
     const uint32_t fixed = kPagedWarps * terms * q_rows * b.query + kPagedMeeting, least = b.part > 2 * b.stage ? (b.part + b.stage - 1) / b.stage : 2;
     auto stages_of = [&](uint32_t blocks) -> uint32_t {   // 0: not so many blocks

@@ -9,11 +9,11 @@
 //   writes the results of items that lie in its share by itself.  Others meet twice: the warps of a block when all
 //   have done their share, through shared memory, and the blocks in the workspace, where the one that comes last to an
 //   item (a counter) joins the pieces.  Both go by the pieces' order: the same bits whoever is last.  A share a warp and not
-//   a block: with a block at every item's end, 64 sequences of 1 to 4096 tokens took 167 us where warps took 99.
+//   a block: with a block at every item's end, 64 sequences of 1 to 4096 tokens took 167 us where warps took 99 (of that time).
 //   Tiles.  Each warp has a ring of stages of its own, so that nothing but its own copies stops a warp, and keeps the
 //   maximum, the sum and the output of what it has seen (one pass, f32).  The copy engine fetches a tile as boxes of
 //   rows that lie in one page (page sizes that are multiples of 8); other page sizes go row by row in 16-byte copies (i8, 64
-//   sequences of 4096: 128 us, and 169 with pages of one row; 32 of bf16 94 and 99).  Rows outside the sequence are zeros.
+//   sequences of 4096: 131 us, and 173 with pages of one row; 32 of bf16 95 and 99).  Rows outside the sequence are zeros.
 //   Products.  mma.sync with the keys (and then the output's columns) as rows and the query heads as columns: of
 //   the 8 columns of a tile few are wasted for small groups, and P is turned into an operand by movmatrix.  (The tensor unit
 //   is 20 % busy: tcgen05, whose tiles are 128 rows, would have nothing to give but its rate.)  The tensor unit's own
@@ -23,16 +23,18 @@
 //   f32 query as three as well, the lower two in a sum of their own.  Terms are cut off, not rounded, and held above 2^-40
 //   of the number, so that an infinity in V stays one.  8-bit codes become f16 exactly; the probabilities then carry the row's scale and are two f16
 //   terms (22 bits), in units of a power of two a head that follows the largest product of the two.  (One unit for all heads, of
-//   the largest scale: e4m3 73.8 us for 73.5, 16 heads on one i8 head 53.2 for 53.8; but a large row of no weight takes the
+//   the largest scale: e4m3 74.6 us for 74.7, 16 heads on one i8 head 53.4 for 54.2; but a large row of no weight takes the
 //   others' bits, all of them from 2^40 on.)  f32 queries are two f16 terms, bf16 ones a single one, in units of a power of two
 //   a row.  Error against 64 bits, f32 output: 1e-7 to 5e-7, as plain f32 arithmetic has.
-// Measured (32 query heads of 128 on 8, on 4 for e4m3): 64 ragged sequences of up to 4096 tokens 98 us, 5.6 TB/s; two of 131071
-// 177 to 189 us, 5.7 to 6.1 TB/s by machine; 96 ragged ones of up to 6000, e4m3, 74 us, 4.2 TB/s; 16 heads of 64 on 512 tokens 9.6 us.  In
+// Measured (32 query heads of 128 on 8, on 4 for e4m3): 64 ragged sequences of up to 4096 tokens 98 to 102 us, 5.3 to 5.6 TB/s; two of 131071
+// 178 to 193 us, 5.6 to 6.0 TB/s by machine; 96 ragged ones of up to 6000, e4m3, 73 to 75 us, 4.2 TB/s; 16 heads of 64 on 512 tokens 9.6 us.  In
 // the middle of a launch bf16 and e4m3 tiles come at 7.1 TB/s.  What is left: 4 us until the first tile is there (lengths,
 // page table, rows: three trips to memory), 3 us of ends and joins, and that some SMs (40 of 148 here) end a tenth later than
 // the others; a share drawn from a counter by those that are done was tried and costs more than it gives (a drawn share pays
-// beginning and end again: 98 -> 105 us).  16 query heads on an 8-bit head (NT 2) are bound by instructions: 1100 a tile of 32
-// keys, which no longer fit the first instruction cache; half tiles on three blocks an SM come to the same time.
+// beginning and end again: 98 -> 105 us).  The 8-bit builds of 65 to 128 columns spill (168 registers at three blocks an SM, 178
+// bytes a thread stored and 184 loaded).  16 query heads on an 8-bit head (NT 2, 54 us) are bound by latency: 255 registers leave two warps a
+// scheduler, each one dependent chain of some 1150 instructions a tile of 32 keys, at a third of the issue slots; the loop no longer
+// fits the first instruction cache.  Half tiles on three blocks an SM come to the same time.
 #pragma once
 #include "kv_cache.cuh"
 
@@ -229,8 +231,10 @@ __device__ __forceinline__ uint32_t column_of(uint32_t i, uint32_t m) {
     else return (DP == 64 ? 8 * (m & 7) : 16 * (m & 7)) + (DP == 256 ? 128 * (i >> 3) + 2 * (i & 7) : 2 * i) + (m >> 3);
 }
 
-constexpr uint32_t kEnd = 2;     // places on the line in front of an item's tiles (ragged e4m3 71 us; 76 with 1, 70 with 3, short items then slower)
-constexpr uint32_t kLeast = 1;   // places a warp has at least (10 to 2000 keys a block: 9.7 us for 16 heads of 512 keys, 11.1 with 2, 11.8 with 3)
+// places on the line in front of an item's tiles.  With 1, 2, 3: 96 ragged e4m3 sequences 80, 76, 74 us; 64 ragged ones of bf16 105,
+// 100, 100; 256 of 128 tokens 41.3, 42.0, 42.5 (one box, in turn)
+constexpr uint32_t kEnd = 2;
+constexpr uint32_t kLeast = 1;   // places a warp has at least (10 to 2000 keys a block: 9.9 us for 16 heads of 512 keys, 11.1 with 2, the same 25.3 for 8 sequences of 2048)
 constexpr uint32_t kGroup = 16;   // pieces joined by one block
 constexpr uint32_t kInvalid = ~0u;
 // What a warp's share ends in: whole items only; an item that begins in the share and goes on; one that goes on on both sides; no places.
