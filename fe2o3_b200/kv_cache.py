@@ -72,6 +72,12 @@ def _float_dtype(x, dtype):
     raise TypeError(f"rows are f32 or bf16 (bits as uint16), got {name or type(x)}: say dtype=")
 
 
+def _contiguous(*tensors):
+    for x in tensors:
+        if hasattr(x, "is_contiguous") and not x.is_contiguous():
+            raise ValueError("a tensor is contiguous here; rows inside wider storage come as (address, elements) with their strides")
+
+
 class PagedKvCache:
     def __init__(self, ctx, stream, sequences, positions, kv_heads, dim, page_size=16, pages=None, format=KV_BF16):
         """Room for `sequences` of up to `positions` tokens each in `pages` pages (default: enough for all at their
@@ -116,6 +122,7 @@ class PagedKvCache:
         self._upload()
 
     def _rows(self, k, v, tokens, strides):
+        _contiguous(k, v)
         packed = (self.kv_heads * self.dim, self.dim)
         (kt, kh), (vt, vh) = strides or (packed, packed)
         return dict(k=k, v=v, tokens=tokens, k_token_stride=kt, k_head_stride=kh, v_token_stride=vt, v_head_stride=vh)
@@ -135,15 +142,18 @@ class PagedKvCache:
 
     def read(self, k, v, counts, dtype=None, strides=None):
         """The last `counts[b]` rows of every sequence b into k and v, which are there when this returns."""
+        kw = dict(output_dtype=_float_dtype(k, dtype))
         offsets = np.zeros(self.sequences + 1, np.uint32)
         offsets[1:] = np.cumsum(counts)
+        kw.update(self._rows(k, v, int(offsets[-1]), strides))
         at = DeviceBuffer.from_host(self.stream, offsets)
-        self._launch("kv_cache_read_v1", token_offsets=at, output_dtype=_float_dtype(k, dtype), **self._rows(k, v, int(offsets[-1]), strides))
+        self._launch("kv_cache_read_v1", token_offsets=at, **kw)
         self.stream.synchronize()   # before the offsets go
         at.free()
 
     def attention(self, q, out, heads, lse=None, scale=None, window=0, q_dtype=None, out_dtype=None, q_strides=None):
         """A prepared launch of `paged_attention_v1` over this cache; the caller launches and destroys it."""
+        _contiguous(q, out, lse)
         qs, qh = q_strides or (heads * self.dim, self.dim)
         return prepare(self.ctx, "paged_attention_v1", q=q, output=out, lse=lse, heads=heads, q_stride=qs, q_head_stride=qh,
                        scale=self.dim ** -0.5 if scale is None else scale, window=window, q_dtype=_float_dtype(q, q_dtype),

@@ -176,3 +176,22 @@ def test_row_types():
         _float_dtype((0, 4), None)
     with pytest.raises(TypeError):
         _float_dtype(np.zeros(1, np.int32), None)
+
+
+def test_rows_of_wider_storage():
+    """Tensors say whether they are contiguous; addresses with a length do not."""
+    import torch
+    from fe2o3_b200.kv_cache import PagedKvCache, _contiguous
+    f, h = torch.zeros(4, 2, 16), torch.zeros(4, 2, 16, dtype=torch.bfloat16)
+    _contiguous(f, h, None, (0, 4), np.zeros(3))
+    wide = torch.zeros(4, 3, 2, 16)
+    with pytest.raises(ValueError):
+        _contiguous(wide[:, 1])
+    cache = PagedKvCache.__new__(PagedKvCache)           # (nothing of it is on a GPU before the rows are looked at)
+    cache.kv_heads, cache.dim = 2, 16
+    assert cache._rows(f, f, 4, None)["k_token_stride"] == 32
+    for k, v in ((wide[:, 1], f), (f, wide[:, 2])):
+        with pytest.raises(ValueError):
+            cache._rows(k, v, 4, None)
+    with pytest.raises(ValueError):
+        cache.attention(wide[:, 0], f, 2)
