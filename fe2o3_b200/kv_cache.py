@@ -78,6 +78,14 @@ def _contiguous(*tensors):
             raise ValueError("a tensor is contiguous here; rows inside wider storage come as (address, elements) with their strides")
 
 
+def _pair_dtype(k, v, dtype):
+    """DTYPE_* of k and v, which are of one type."""
+    one = _float_dtype(k, dtype)
+    if hasattr(v, "dtype") and _float_dtype(v, dtype) != one:
+        raise TypeError(f"k and v are of one type, got {k.dtype} and {v.dtype}")
+    return one
+
+
 class PagedKvCache:
     def __init__(self, ctx, stream, sequences, positions, kv_heads, dim, page_size=16, pages=None, format=KV_BF16):
         """Room for `sequences` of up to `positions` tokens each in `pages` pages (default: enough for all at their
@@ -137,12 +145,12 @@ class PagedKvCache:
     def append(self, k, v, dtype=None, strides=None):
         """Rows of the tokens of the last `extend`, sequence after sequence: [tokens][kv_heads][dim], or with `strides`
         ((k token, k head), (v token, v head)) in elements, as slices (address, elements)."""
-        self._launch("kv_cache_append_v1", token_offsets=self.device_offsets, input_dtype=_float_dtype(k, dtype),
+        self._launch("kv_cache_append_v1", token_offsets=self.device_offsets, input_dtype=_pair_dtype(k, v, dtype),
                      **self._rows(k, v, self.new_tokens, strides))
 
     def read(self, k, v, counts, dtype=None, strides=None):
         """The last `counts[b]` rows of every sequence b into k and v, which are there when this returns."""
-        kw = dict(output_dtype=_float_dtype(k, dtype))
+        kw = dict(output_dtype=_pair_dtype(k, v, dtype))
         offsets = np.zeros(self.sequences + 1, np.uint32)
         offsets[1:] = np.cumsum(counts)
         kw.update(self._rows(k, v, int(offsets[-1]), strides))
@@ -182,7 +190,7 @@ class DecodeStep:
     def __init__(self, cache, q, k, v, out, heads, lse=None, scale=None, window=0, dtype=None, out_dtype=None, strides=None, q_strides=None):
         self.cache = cache
         self.attend = cache.attention(q, out, heads, lse, scale, window, dtype, out_dtype, q_strides)
-        self.append = prepare(cache.ctx, "kv_cache_append_v1", input_dtype=_float_dtype(k, dtype),
+        self.append = prepare(cache.ctx, "kv_cache_append_v1", input_dtype=_pair_dtype(k, v, dtype),
                               **cache._rows(k, v, cache.sequences, strides), **cache.args())
 
     def run(self):

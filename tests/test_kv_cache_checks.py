@@ -195,3 +195,15 @@ def test_rows_of_wider_storage():
             cache._rows(k, v, 4, None)
     with pytest.raises(ValueError):
         cache.attention(wide[:, 0], f, 2)
+
+
+def test_keys_and_values_of_unlike_types():
+    import torch
+    from fe2o3_b200.kv_cache import _pair_dtype
+    f, h = torch.zeros(4, 2, 16), torch.zeros(4, 2, 16, dtype=torch.bfloat16)
+    assert _pair_dtype(f, f, None) == fe.DTYPE_F32 and _pair_dtype(h, h, None) == fe.DTYPE_BF16
+    assert _pair_dtype((0, 4), (0, 4), fe.DTYPE_BF16) == fe.DTYPE_BF16 and _pair_dtype(h, (0, 4), None) == fe.DTYPE_BF16
+    with pytest.raises(TypeError):
+        _pair_dtype(h, f, None)
+    with pytest.raises(TypeError):
+        _pair_dtype((0, 4), f, None)
