@@ -83,6 +83,21 @@ PagedAttentionArgs = _struct("PagedAttentionArgs",
                              [("batch", u32), ("heads", u32), ("kv_heads", u32), ("dim", u32), ("page_size", u32), ("table_width", u32),
                               ("q_stride", u32), ("q_head_stride", u32), ("scale", f32), ("window", u32), ("q_dtype", u32),
                               ("output_dtype", u32), ("format", u32), ("reserved", u32)])
+KvPagesArgs = _struct("KvPagesArgs",
+                      ["counts", "release", "lengths", "free_count", "page_table", "free_pages", "next_lengths", "next_free_count",
+                       "token_offsets", "positions", "slots"],
+                      [("batch", u32), ("table_width", u32), ("page_size", u32), ("tokens", u32)])
+RotaryArgs = _struct("RotaryArgs", ["q", "k", "positions", "frequencies", "q_output", "k_output"],
+                     [("tokens", u32), ("heads", u32), ("kv_heads", u32), ("dim", u32), ("rotary_dim", u32), ("layout", u32), ("dtype", u32),
+                      ("backward", u32), ("q_token_stride", u32), ("q_head_stride", u32), ("k_token_stride", u32), ("k_head_stride", u32),
+                      ("q_output_token_stride", u32), ("q_output_head_stride", u32), ("k_output_token_stride", u32),
+                      ("k_output_head_stride", u32), ("scale", f32), ("reserved", u32)])
+KvCacheRotaryAppendArgs = _struct("KvCacheRotaryAppendArgs",
+                                  ["q", "k", "v", "positions", "slots", "frequencies", "q_output", "k_cache", "v_cache", "k_scales", "v_scales"],
+                                  [("tokens", u32), ("heads", u32), ("kv_heads", u32), ("dim", u32), ("page_size", u32), ("rotary_dim", u32),
+                                   ("layout", u32), ("input_dtype", u32), ("format", u32), ("q_token_stride", u32), ("q_head_stride", u32),
+                                   ("k_token_stride", u32), ("k_head_stride", u32), ("v_token_stride", u32), ("v_head_stride", u32),
+                                   ("q_output_token_stride", u32), ("q_output_head_stride", u32), ("scale", f32)])
 MaskedReduceArgs = _struct("MaskedReduceArgs", ["values", "active", "output"])
 MaskedReducePackedArgs = _struct("MaskedReducePackedArgs", ["values", "mask", "output"])
 DeviceScanArgs = _struct("DeviceScanArgs", ["values", "output"], [("exclusive", u32), ("reserved", u32)])
@@ -142,6 +157,9 @@ OPS = {
     "kv_cache_append_v1": (KvCacheAppendArgs, 192, False),
     "kv_cache_read_v1": (KvCacheReadArgs, 192, False),
     "paged_attention_v1": (PagedAttentionArgs, 200, False),
+    "kv_pages_v1": (KvPagesArgs, 192, False),
+    "rotary_v1": (RotaryArgs, 168, False),
+    "kv_cache_rotary_append_v1": (KvCacheRotaryAppendArgs, 248, False),
     "masked_reduce_u32": (MaskedReduceArgs, 48, False),
     "masked_reduce_u32_packed": (MaskedReducePackedArgs, 48, False),
     "device_scan_u32": (DeviceScanArgs, 40, False),

@@ -37,6 +37,9 @@ int32_t launch_moe_combine(fe2o3_ctx *, cudaStream_t, const void *, fe2o3_geomet
 int32_t launch_moe_ep_exchange(fe2o3_ctx *, cudaStream_t, const void *, fe2o3_geometry *, bool);
 int32_t launch_kv_cache_append(fe2o3_ctx *, cudaStream_t, const void *, fe2o3_geometry *, bool);
 int32_t launch_kv_cache_read(fe2o3_ctx *, cudaStream_t, const void *, fe2o3_geometry *, bool);
+int32_t launch_kv_pages(fe2o3_ctx *, cudaStream_t, const void *, fe2o3_geometry *, bool);
+int32_t launch_rotary(fe2o3_ctx *, cudaStream_t, const void *, fe2o3_geometry *, bool);
+int32_t launch_kv_cache_rotary_append(fe2o3_ctx *, cudaStream_t, const void *, fe2o3_geometry *, bool);
 int32_t launch_moe_compact(cudaStream_t, uint64_t x, uint64_t perm, uint64_t compact_x, uint32_t rows,
                            uint32_t d_model, uint32_t tokens);
 int32_t launch_gemm_exact(fe2o3_ctx *, cudaStream_t, uint32_t dtype, bool epilogue, uint64_t a, uint64_t b, uint64_t c, uint32_t M,
@@ -107,7 +110,8 @@ enum OpId : uint32_t {
     OP_MOE_GATE, OP_MOE_ROUTE_WEIGHTS, OP_MOE_EXPERT_FFN, OP_MOE_COMBINE, OP_MASKED_REDUCE, OP_MASKED_REDUCE_PACKED,
     OP_WAVE_LDS, OP_WAVE64_COLLECTIVES, OP_WAVE64_SEGMENTED, OP_LDS_REDUCE_I32, OP_SCOPED_ATOMIC_ADD,
     OP_MOE_COMPACT, OP_MOE_GROUPED_FFN, OP_MOE_EP_EXCHANGE, OP_DEVICE_SCAN_U32, OP_DEVICE_SCAN_F32, OP_MOE_EP_FFN,
-    OP_MOE_FFN_COMBINE, OP_KV_APPEND, OP_KV_READ, OP_PAGED_ATTENTION, OP_COUNT
+    OP_MOE_FFN_COMBINE, OP_KV_APPEND, OP_KV_READ, OP_PAGED_ATTENTION, OP_KV_PAGES, OP_ROTARY,
+    OP_KV_ROTARY_APPEND, OP_COUNT
 };
 
 struct OpInfo {
@@ -144,6 +148,9 @@ static const OpInfo kOps[OP_COUNT] = {
     {"kv_cache_append_v1", sizeof(fe2o3_kv_cache_append_v1_args), launch_kv_cache_append},
     {"kv_cache_read_v1", sizeof(fe2o3_kv_cache_read_v1_args), launch_kv_cache_read},
     {"paged_attention_v1", sizeof(fe2o3_paged_attention_v1_args), nullptr},
+    {"kv_pages_v1", sizeof(fe2o3_kv_pages_v1_args), launch_kv_pages},
+    {"rotary_v1", sizeof(fe2o3_rotary_v1_args), launch_rotary},
+    {"kv_cache_rotary_append_v1", sizeof(fe2o3_kv_cache_rotary_append_v1_args), launch_kv_cache_rotary_append},
 };
 
 struct fe2o3_prepared {
@@ -353,12 +360,17 @@ int32_t check_ctx_device(fe2o3_ctx *ctx, const Region *r, int n) {
 
 #define RGN(role_, slice_, expected_, bytes_, out_) Region{role_, slice_, (uint64_t)(expected_), bytes_, out_}
 
-// The cache's own slices, common to the three operators on it: dims, format, pages, and what a row of the tables holds.
-// Appends to r from n on; returns the new count, or 0 with *status set.
+// The cache's own slices, common to the operators on it: dims, format, pages.  Appends to r from n on; returns the new count, or 0 with
+// *status set.
 template <typename Args>
 int kv_cache_regions(const Args *a, Region *r, int n, bool writes, int32_t *status) {
-    if (a->kv_heads == 0 || a->kv_heads > 65536 || a->dim == 0 || a->dim % 16 || a->dim > 256 || a->page_size == 0 || a->format > FE2O3_KV_I8) {
-        *status = unsupported("a key-value cache has 1 to 65536 kv_heads, dim a multiple of 16 up to 256, page_size >= 1, format bf16, e4m3 or i8");
+    const bool four = a->format == FE2O3_KV_E2M1;
+    if (a->kv_heads == 0 || a->kv_heads > 65536 || a->dim == 0 || a->dim % 16 || a->dim > 256 || a->page_size == 0 || (a->format > FE2O3_KV_I8 && !four)) {
+        *status = unsupported("a key-value cache has 1 to 65536 kv_heads, dim a multiple of 16 up to 256, page_size >= 1, format bf16, e4m3, i8 or e2m1");
+        return 0;
+    }
+    if (four && (a->dim % 32 || a->page_size % 8)) {
+        *status = unsupported("a 4-bit key-value cache has dim a multiple of 32 and page_size one of 8");
         return 0;
     }
     uint64_t rows;   // of one page
@@ -366,10 +378,15 @@ int kv_cache_regions(const Args *a, Region *r, int n, bool writes, int32_t *stat
         *status = unsupported("a page holds fewer than 2^32 rows");
         return 0;
     }
-    const uint64_t page = rows * a->dim, pages = a->k_cache.len / page;
+    const uint64_t page = rows * kv_row_elements(a->format, a->dim), pages = a->k_cache.len / page;
     if (pages > 0xffffffffull / rows) { *status = unsupported("a key-value cache has fewer than 2^32 rows"); return 0; }
     if ((a->k_cache.ptr | a->v_cache.ptr) & 15u) {
         fe2o3_set_error("Alignment{role=%s}: the caches start on 16 bytes", a->k_cache.ptr & 15u ? "KeyCache" : "ValueCache");
+        *status = FE2O3_ERR_ALIGNMENT;
+        return 0;
+    }
+    if (four && ((a->k_scales.ptr | a->v_scales.ptr) & 15u)) {
+        fe2o3_set_error("Alignment{role=%s}: the scales of a 4-bit cache start on 16 bytes", a->k_scales.ptr & 15u ? "KeyScales" : "ValueScales");
         *status = FE2O3_ERR_ALIGNMENT;
         return 0;
     }
@@ -379,10 +396,32 @@ int kv_cache_regions(const Args *a, Region *r, int n, bool writes, int32_t *stat
     r[n++] = RGN("ValueCache", a->v_cache, pages * page, eb, writes);
     r[n++] = RGN("KeyScales", a->k_scales, scales, 4, writes);
     r[n++] = RGN("ValueScales", a->v_scales, scales, 4, writes);
+    return n;
+}
+// And what a row of the tables holds.
+template <typename Args>
+int kv_table_regions(const Args *a, Region *r, int n) {
     r[n++] = RGN("PageTable", a->page_table, (uint64_t)a->batch * a->table_width, 4, false);
     r[n++] = RGN("Lengths", a->lengths, a->batch, 4, false);
     return n;
 }
+
+// Elements that rows (t, h) at t * token_stride + h * head_stride span; false: more than 64 bits count.
+bool rows_extent(uint64_t tokens, uint64_t heads, uint64_t dim, uint64_t token_stride, uint64_t head_stride, uint64_t *len) {
+    *len = 0;
+    if (tokens == 0 || heads == 0) return true;
+    const uint64_t t = (tokens - 1) * token_stride, h = (heads - 1) * head_stride;
+    *len = t + h + dim;
+    return t + h >= t && *len >= t + h;
+}
+// Whether no two of them meet.
+bool rows_apart(uint64_t tokens, uint64_t heads, uint64_t dim, uint64_t token_stride, uint64_t head_stride) {
+    if (tokens == 0 || heads == 0) return true;
+    const uint64_t t = (tokens - 1) * token_stride, h = (heads - 1) * head_stride;
+    return ((heads == 1 || head_stride >= dim) && (tokens == 1 || token_stride >= h + dim)) ||
+           ((tokens == 1 || token_stride >= dim) && (heads == 1 || head_stride >= t + dim));
+}
+bool same_slice(const fe2o3_slice &a, const fe2o3_slice &b) { return a.ptr == b.ptr && a.len == b.len; }
 
 // New tokens' rows (append: inputs, read: outputs) and which sequence they belong to.
 template <typename Args>
@@ -406,6 +445,14 @@ int kv_rows_regions(const Args *a, Region *r, int n, uint32_t dtype, bool writes
         r[n++] = Region{i ? "Value" : "Key", rows[i], len, dtype == FE2O3_DTYPE_F32 ? 4u : 2u, writes};
     }
     return n;
+}
+
+bool rotary_admits(uint32_t dim, uint32_t rotary_dim, uint32_t layout, float scale, uint32_t dtype, int32_t *status) {
+    if (dim != 0 && dim % 16 == 0 && dim <= 256 && rotary_dim % 2 == 0 && rotary_dim <= dim && layout <= FE2O3_ROTARY_INTERLEAVED && isfinite(scale) &&
+        dtype <= FE2O3_DTYPE_BF16)
+        return true;
+    *status = unsupported("rotary rows have dim a multiple of 16 up to 256, an even rotary_dim up to dim, halves or neighbours as pairs, a finite scale, f32 or bf16 elements");
+    return false;
 }
 
 // Per-op region tables.  Returns the number of regions, fills `r`.
@@ -650,17 +697,18 @@ int regions_for(uint32_t op, const void *args, Region *r, int32_t *status) {
         case OP_KV_APPEND: {
             const fe2o3_kv_cache_append_v1_args *a = static_cast<const fe2o3_kv_cache_append_v1_args *>(args);
             const int n = kv_cache_regions(a, r, 0, true, status);
-            return n ? kv_rows_regions(a, r, n, a->input_dtype, false, status) : 0;
+            return n ? kv_rows_regions(a, r, kv_table_regions(a, r, n), a->input_dtype, false, status) : 0;
         }
         case OP_KV_READ: {
             const fe2o3_kv_cache_read_v1_args *a = static_cast<const fe2o3_kv_cache_read_v1_args *>(args);
             const int n = kv_cache_regions(a, r, 0, false, status);
-            return n ? kv_rows_regions(a, r, n, a->output_dtype, true, status) : 0;
+            return n ? kv_rows_regions(a, r, kv_table_regions(a, r, n), a->output_dtype, true, status) : 0;
         }
         case OP_PAGED_ATTENTION: {
             const fe2o3_paged_attention_v1_args *a = static_cast<const fe2o3_paged_attention_v1_args *>(args);
             int n = kv_cache_regions(a, r, 0, false, status);
             if (!n) return 0;
+            n = kv_table_regions(a, r, n);
             if (a->heads == 0 || a->heads % a->kv_heads || a->q_dtype > FE2O3_DTYPE_BF16 || a->output_dtype > FE2O3_DTYPE_BF16 ||
                 !isfinite(a->scale) || (uint64_t)a->batch * a->heads > 0x7fffffffu || a->batch > (1u << 29) ||   // (places are counted in 32 bits)
                 (a->batch && (uint64_t)a->table_width * a->page_size > (1ull << 35) / a->batch) ||
@@ -679,6 +727,88 @@ int regions_for(uint32_t op, const void *args, Region *r, int32_t *status) {
             r[n++] = RGN("Query", a->q, len, a->q_dtype == FE2O3_DTYPE_F32 ? 4u : 2u, false);
             r[n++] = RGN("Output", a->output, out * a->dim, a->output_dtype == FE2O3_DTYPE_F32 ? 4u : 2u, true);
             if (a->lse.ptr || a->lse.len) r[n++] = RGN("LogSumExp", a->lse, out, 4, true);
+            return n;
+        }
+        case OP_KV_PAGES: {
+            const fe2o3_kv_pages_v1_args *a = static_cast<const fe2o3_kv_pages_v1_args *>(args);
+            const uint64_t pages = a->free_pages.len, entries = (uint64_t)a->batch * a->table_width;
+            if (a->batch > 16384 || a->page_size == 0 || entries > 0xffffffffull || pages > 0xffffffffull / a->page_size) {
+                *status = unsupported("kv_pages_v1 needs batch <= 16384, page_size >= 1, batch * table_width and the rows of all pages below 2^32");
+                return 0;
+            }
+            int n = 0;
+            if (a->counts.ptr || a->counts.len) r[n++] = RGN("Counts", a->counts, a->batch, 4, false);
+            if (a->release.ptr || a->release.len) r[n++] = RGN("Release", a->release, a->batch, 4, false);
+            if (!same_slice(a->lengths, a->next_lengths)) r[n++] = RGN("Lengths", a->lengths, a->batch, 4, false);
+            if (!same_slice(a->free_count, a->next_free_count)) r[n++] = RGN("FreeCount", a->free_count, 1, 4, false);
+            r[n++] = RGN("PageTable", a->page_table, entries, 4, true);
+            r[n++] = RGN("FreePages", a->free_pages, pages, 4, true);
+            r[n++] = RGN("NextLengths", a->next_lengths, a->batch, 4, true);
+            r[n++] = RGN("NextFreeCount", a->next_free_count, 1, 4, true);
+            if (a->token_offsets.ptr || a->token_offsets.len) r[n++] = RGN("TokenOffsets", a->token_offsets, (uint64_t)a->batch + 1, 4, true);
+            if (a->positions.ptr || a->positions.len) r[n++] = RGN("Positions", a->positions, a->tokens, 4, true);
+            if (a->slots.ptr || a->slots.len) r[n++] = RGN("Slots", a->slots, a->tokens, 4, true);
+            return n;
+        }
+        case OP_ROTARY: {
+            const fe2o3_rotary_v1_args *a = static_cast<const fe2o3_rotary_v1_args *>(args);
+            if (!rotary_admits(a->dim, a->rotary_dim, a->layout, a->scale, a->dtype, status)) return 0;
+            if (a->backward > 1 || a->heads > 65536 || a->kv_heads > 65536) {
+                *status = unsupported("rotary_v1 needs at most 65536 heads and kv_heads, backward 0 or 1");
+                return 0;
+            }
+            const uint32_t eb = a->dtype == FE2O3_DTYPE_F32 ? 4 : 2;
+            const fe2o3_slice in[2] = {a->q, a->k}, out[2] = {a->q_output, a->k_output};
+            const uint64_t heads[2] = {a->heads, a->kv_heads}, ts[2] = {a->q_token_stride, a->k_token_stride}, hs[2] = {a->q_head_stride, a->k_head_stride};
+            const uint64_t ots[2] = {a->q_output_token_stride, a->k_output_token_stride}, ohs[2] = {a->q_output_head_stride, a->k_output_head_stride};
+            const char *const names[2][2] = {{"Query", "QueryOutput"}, {"Key", "KeyOutput"}};
+            uint64_t len[2];
+            int n = 0;
+            for (int i = 0; i < 2; ++i) {
+                uint64_t from;
+                if (!rows_extent(a->tokens, heads[i], a->dim, ts[i], hs[i], &from) || !rows_extent(a->tokens, heads[i], a->dim, ots[i], ohs[i], &len[i])) {
+                    fe2o3_set_error("ExtentOverflow");
+                    *status = FE2O3_ERR_SIZE_OVERFLOW;
+                    return 0;
+                }
+                if (!rows_apart(a->tokens, heads[i], a->dim, ots[i], ohs[i])) { *status = unsupported("output rows overlap"); return 0; }
+                if (!(in[i].ptr == out[i].ptr && in[i].len == out[i].len && ts[i] == ots[i] && hs[i] == ohs[i])) r[n++] = Region{names[i][0], in[i], from, eb, false};
+            }
+            // outputs whose rows lie between one another's (parts of fused rows): one region
+            const uint64_t span[2] = {heads[0] ? (heads[0] - 1) * ohs[0] + a->dim : 0, heads[1] ? (heads[1] - 1) * ohs[1] + a->dim : 0};
+            const int low = out[0].ptr <= out[1].ptr ? 0 : 1, high = 1 - low;
+            const uint64_t between = out[high].ptr - out[low].ptr, shared_stride = ots[0];
+            if (a->tokens > 1 && heads[0] && heads[1] && ots[0] == ots[1] && out[0].len == len[0] && out[1].len == len[1] && out[low].ptr % eb == 0 &&
+                between % eb == 0 && between / eb >= span[low] && between / eb + span[high] <= shared_stride) {
+                const uint64_t all = between / eb + len[high];
+                r[n++] = Region{"Output", fe2o3_slice{out[low].ptr, all}, all, eb, true};
+            } else {
+                for (int i = 0; i < 2; ++i) r[n++] = Region{names[i][1], out[i], len[i], eb, true};
+            }
+            if (a->positions.ptr || a->positions.len) r[n++] = RGN("Positions", a->positions, a->tokens, 4, false);
+            r[n++] = RGN("Frequencies", a->frequencies, a->rotary_dim / 2, 4, false);
+            return n;
+        }
+        case OP_KV_ROTARY_APPEND: {
+            const fe2o3_kv_cache_rotary_append_v1_args *a = static_cast<const fe2o3_kv_cache_rotary_append_v1_args *>(args);
+            int n = kv_cache_regions(a, r, 0, true, status);
+            if (!n || !rotary_admits(a->dim, a->rotary_dim, a->layout, a->scale, a->input_dtype, status)) return 0;
+            if (a->heads > 65536) { *status = unsupported("kv_cache_rotary_append_v1 needs at most 65536 heads"); return 0; }
+            const uint32_t eb = a->input_dtype == FE2O3_DTYPE_F32 ? 4 : 2;
+            const fe2o3_slice rows[4] = {a->q, a->k, a->v, a->q_output};
+            const uint64_t heads[4] = {a->heads, a->kv_heads, a->kv_heads, a->heads};
+            const uint64_t ts[4] = {a->q_token_stride, a->k_token_stride, a->v_token_stride, a->q_output_token_stride};
+            const uint64_t hs[4] = {a->q_head_stride, a->k_head_stride, a->v_head_stride, a->q_output_head_stride};
+            const char *const names[4] = {"Query", "Key", "Value", "QueryOutput"};
+            for (int i = 0; i < 4; ++i) {
+                uint64_t len;
+                if (!rows_extent(a->tokens, heads[i], a->dim, ts[i], hs[i], &len)) { fe2o3_set_error("ExtentOverflow"); *status = FE2O3_ERR_SIZE_OVERFLOW; return 0; }
+                r[n++] = Region{names[i], rows[i], len, eb, i == 3};
+            }
+            if (!rows_apart(a->tokens, heads[3], a->dim, ts[3], hs[3])) { *status = unsupported("output rows overlap"); return 0; }
+            r[n++] = RGN("Slots", a->slots, a->tokens, 4, false);
+            r[n++] = RGN("Positions", a->positions, a->rotary_dim ? a->tokens : 0, 4, false);
+            r[n++] = RGN("Frequencies", a->frequencies, a->rotary_dim / 2, 4, false);
             return n;
         }
         case OP_DEVICE_SCAN_U32:
@@ -1451,6 +1581,9 @@ DEFINE_CHECK(moe_expert_ffn_v1, OP_MOE_EXPERT_FFN)
 DEFINE_CHECK(moe_expert_combine_v1, OP_MOE_COMBINE)
 DEFINE_CHECK(kv_cache_append_v1, OP_KV_APPEND)
 DEFINE_CHECK(kv_cache_read_v1, OP_KV_READ)
+DEFINE_CHECK(kv_pages_v1, OP_KV_PAGES)
+DEFINE_CHECK(rotary_v1, OP_ROTARY)
+DEFINE_CHECK(kv_cache_rotary_append_v1, OP_KV_ROTARY_APPEND)
 DEFINE_CHECK(paged_attention_v1, OP_PAGED_ATTENTION)
 DEFINE_CHECK(masked_reduce_u32, OP_MASKED_REDUCE)
 DEFINE_CHECK(masked_reduce_u32_packed, OP_MASKED_REDUCE_PACKED)
@@ -1477,6 +1610,9 @@ DEFINE_SIMPLE_PREPARE(moe_route_weights_v1, OP_MOE_ROUTE_WEIGHTS)
 DEFINE_SIMPLE_PREPARE(moe_expert_combine_v1, OP_MOE_COMBINE)
 DEFINE_SIMPLE_PREPARE(kv_cache_append_v1, OP_KV_APPEND)
 DEFINE_SIMPLE_PREPARE(kv_cache_read_v1, OP_KV_READ)
+DEFINE_SIMPLE_PREPARE(kv_pages_v1, OP_KV_PAGES)
+DEFINE_SIMPLE_PREPARE(rotary_v1, OP_ROTARY)
+DEFINE_SIMPLE_PREPARE(kv_cache_rotary_append_v1, OP_KV_ROTARY_APPEND)
 DEFINE_SIMPLE_PREPARE(masked_reduce_u32, OP_MASKED_REDUCE)
 DEFINE_SIMPLE_PREPARE(masked_reduce_u32_packed, OP_MASKED_REDUCE_PACKED)
 DEFINE_SIMPLE_PREPARE(device_scan_u32, OP_DEVICE_SCAN_U32)

@@ -72,6 +72,9 @@ static inline cudaError_t fe2o3_launch_early(void (*kernel)(P...), dim3 grid, di
     return cudaLaunchKernelEx(&cfg, kernel, P(args)...);
 }
 
+// Elements that a row of a key-value cache takes in its array (of a 4-bit cache bytes: codes, and block scales that lie apart from them).
+static inline uint64_t kv_row_elements(uint32_t format, uint32_t dim) { return format == FE2O3_KV_E2M1 ? dim / 16 * 9 : dim; }
+
 static inline uint32_t ceil_div_u32(uint64_t a, uint64_t b) { return (uint32_t)((a + b - 1) / b); }
 
 // Flag block of one rank of the expert-parallel layer, in u32 words (world = W):

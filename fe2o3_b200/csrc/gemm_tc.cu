@@ -990,7 +990,7 @@ int32_t fe2o3_make_tmap_f32(CUtensorMap *out, uint64_t base, uint32_t rank, cons
 int32_t fe2o3_make_tmap_u8(CUtensorMap *out, uint64_t base, uint32_t rank, const uint64_t *dims, const uint64_t *strides_bytes,
                            const uint32_t *box) {
     return make_tmap(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, rank, dims, strides_bytes, box,
-                     box[0] == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B);
+                     box[0] == 32 ? CU_TENSOR_MAP_SWIZZLE_NONE : box[0] == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 // The tensor-core schedule needs 16-byte aligned bases and leading dimensions

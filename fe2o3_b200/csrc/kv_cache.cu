@@ -17,7 +17,7 @@
 // leaves the normal range: scales outside 2^+-60 take the division itself.
 #include <atomic>
 
-#include "kv_cache.cuh"
+#include "kv_rows.cuh"
 
 namespace {
 
@@ -70,135 +70,14 @@ struct Columns {
     uint32_t first[2];
     bool inside[2];
 };
-__device__ __forceinline__ void widen2(uint32_t v, float *x) {
-    x[0] = __uint_as_float(v << 16);
-    x[1] = __uint_as_float(v & 0xffff0000u);
-}
-__device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {   // to nearest even
-    uint32_t r;
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
-}
-
-// A piece of the caller's row.
-template <bool F32, bool WHOLE>
-__device__ __forceinline__ uint4 fetch(const uint8_t *at) {
-    if constexpr (WHOLE) {
-        return __ldcs(reinterpret_cast<const uint4 *>(at));
-    } else if constexpr (F32) {
-        const uint32_t *const e = reinterpret_cast<const uint32_t *>(at);
-        return make_uint4(e[0], e[1], e[2], e[3]);
-    } else {
-        const uint16_t *const e = reinterpret_cast<const uint16_t *>(at);
-        return make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
-    }
-}
-template <bool F32, bool WHOLE>
-__device__ __forceinline__ void put(uint8_t *at, const uint4 &v) {
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-    if constexpr (WHOLE) {
-        __stcs(reinterpret_cast<uint4 *>(at), v);
-    } else {
-#pragma unroll
-        for (int i = 0; i < (F32 ? 4 : 8); ++i) {
-            if constexpr (F32) reinterpret_cast<uint32_t *>(at)[i] = w[i];
-            else reinterpret_cast<uint16_t *>(at)[i] = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
-        }
-    }
-}
-// The same columns in the cache, whose rows start on 16 bytes.
-template <int BYTES>
-__device__ __forceinline__ uint4 fetch_cached(const uint8_t *at) {
-    if constexpr (BYTES == 16) return __ldcs(reinterpret_cast<const uint4 *>(at));
-    if constexpr (BYTES == 8) {
-        const uint2 v = __ldcs(reinterpret_cast<const uint2 *>(at));
-        return make_uint4(v.x, v.y, 0, 0);
-    }
-    return make_uint4(__ldcs(reinterpret_cast<const uint32_t *>(at)), 0, 0, 0);
-}
-template <int BYTES>
-__device__ __forceinline__ void put_cached(uint8_t *at, const uint4 &v) {
-    if constexpr (BYTES == 16) *reinterpret_cast<uint4 *>(at) = v;
-    else if constexpr (BYTES == 8) *reinterpret_cast<uint2 *>(at) = make_uint2(v.x, v.y);
-    else *reinterpret_cast<uint32_t *>(at) = v.x;
-}
-
-template <int LANES>
-__device__ __forceinline__ uint32_t highest(uint32_t v) {
-#pragma unroll
-    for (int o = 1; o < LANES; o <<= 1) v = max(v, __shfl_xor_sync(~0u, v, o));
-    return v;
-}
-
-// -x / scale, each as IEEE division rounds it; up to the largest code, which a subnormal scale's few bits let it pass.  (With a
-// minus, because the corrections of a quotient of 0 are then zeros of the opposite sign and leave it its own.)
-template <uint32_t FORMAT, int N>
-__device__ __forceinline__ void minus_quotients(float (&x)[N], float scale) {
-    if (scale > 8.7e-19f && scale < 1.1e18f) {   // 2^+-60; |x| <= 448 scale, and what is below 2^-60 scale rounds to no code
-        const float y = -__frcp_rn(scale);
-        const uint64_t y2 = pack_f32x2(y, y), scale2 = pack_f32x2(scale, scale);
-#pragma unroll
-        for (int i = 0; i < N; i += 2) {
-            const uint64_t v = pack_f32x2(x[i], x[i + 1]);
-            uint64_t r = mul_f32x2(v, y2);
-            r = fma_f32x2(fma_f32x2(scale2, r, v), y2, r);
-            r = fma_f32x2(fma_f32x2(scale2, r, v), y2, r);
-            unpack_f32x2(r, x[i], x[i + 1]);
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) x[i] = scale > 0.f ? fminf(fmaxf(-__fdiv_rn(x[i], scale), -kKvTop<FORMAT>), kKvTop<FORMAT>) : -0.f;   // (a NaN scale: codes 0)
-    }
-}
-// top / C, rounded to nearest: the same corrections, with 1 / C known beforehand.
-template <uint32_t FORMAT>
-__device__ __forceinline__ float scale_of(float top) {
-    constexpr float kC = kKvTop<FORMAT>, kY = (float)(1.0 / kC);
-    if (top > 8.7e-19f && top < 1.1e18f) {
-        float r = top * kY;
-        r = fmaf(fmaf(-kC, r, top), kY, r);
-        return fmaf(fmaf(-kC, r, top), kY, r);
-    }
-    return __fdiv_rn(top, kC);
-}
-template <uint32_t FORMAT>
-__device__ __forceinline__ uint32_t codes_of(const float *q) {   // four of them, of -q
-    uint32_t w;
-    if constexpr (FORMAT == FE2O3_KV_E4M3) {
-        asm("{\n\t.reg .b16 lo, hi;\n\tcvt.rn.satfinite.e4m3x2.f32 lo, %2, %1;\n\tcvt.rn.satfinite.e4m3x2.f32 hi, %4, %3;\n\t"
-            "mov.b32 %0, {lo, hi};\n\t}" : "=r"(w) : "f"(q[0]), "f"(q[1]), "f"(q[2]), "f"(q[3]));
-        w ^= 0x80808080u;
-    } else {   // 1.5 2^23 - q is rounded to a whole number, which stands in its low bits (|q| < 127.5)
-        uint32_t e[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) e[j] = __float_as_uint(12582912.f - q[j]);
-        w = __byte_perm(__byte_perm(e[0], e[1], 0x0040), __byte_perm(e[2], e[3], 0x0040), 0x5410);
-    }
-    return w;
-}
-template <uint32_t FORMAT>
-__device__ __forceinline__ void values_of(uint32_t w, float scale, float *x) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if constexpr (FORMAT == FE2O3_KV_I8) {
-            // the code's bits + 128 below 2^23's: the sum with -(2^23 + 128) is the code
-            x[i] = __uint_as_float(__byte_perm(w ^ 0x80808080u, 0x4b000000u, 0x7440 | i)) - 8388736.f;
-        } else if (!(i & 1)) {
-            uint32_t h;
-            asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(h) : "r"(w >> (8 * i)));
-            asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\tcvt.f32.f16 %0, lo;\n\tcvt.f32.f16 %1, hi;\n\t}" : "=f"(x[i]), "=f"(x[i + 1]) : "r"(h));
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = __fmul_rn(x[i], scale);
-}
 
 // WHOLE: the caller's rows start on 16 bytes.
 template <uint32_t FORMAT, bool F32, bool WRITE, bool WHOLE>
 __global__ void __launch_bounds__(kThreads) kv_rows_kernel(KvCache c, KvRows r) {
     __shared__ uint32_t slots[kTokens];
     __shared__ uint32_t known;   // tokens whose lengths allow a slot, a bit each
-    constexpr int kEb = F32 ? 4 : 2, kPiece = 16 / kEb, kCached = kPiece * kKvBytes<FORMAT>;   // a piece: columns, bytes in the cache
+    constexpr bool kFour = FORMAT == FE2O3_KV_E2M1;
+    constexpr int kEb = F32 ? 4 : 2, kPiece = 16 / kEb, kCached = kv_bytes<FORMAT>(kPiece);   // a piece: columns, bytes in the cache
     // rows a lane has in flight: two where it quantises (registers: three take 55 us where two take 52, to e4m3 and back), else four
     constexpr int kDeep = WRITE && FORMAT != FE2O3_KV_BF16 ? 2 : 4;
     begin_after_previous();
@@ -217,6 +96,7 @@ __global__ void __launch_bounds__(kThreads) kv_rows_kernel(KvCache c, KvRows r) 
         const uint32_t first = base + (threadIdx.x >> r.lanes_log2);
         uint4 raw[kDeep][2];
         float scales[kDeep];
+        uint32_t blocks[kDeep];   // 4 bits: the scales of the two pieces' blocks, a byte each
         uint32_t at[kDeep], side[kDeep];
         uint8_t *there[kDeep];
         bool active[kDeep];
@@ -234,21 +114,26 @@ __global__ void __launch_bounds__(kThreads) kv_rows_kernel(KvCache c, KvRows r) 
                                                 (uint64_t)h * (side[d] ? r.v_head_stride : r.k_head_stride)) * kEb;
             raw[d][0] = raw[d][1] = make_uint4(0, 0, 0, 0);
             scales[d] = 0.f;
+            blocks[d] = 0;
             if (!active[d]) continue;
-            const uint8_t *const from = WRITE ? there[d] : (side[d] ? c.v : c.k) + (uint64_t)at[d] * c.dim * kKvBytes<FORMAT>;
+            const uint8_t *const from = WRITE ? there[d] : (side[d] ? c.v : c.k) + (uint64_t)at[d] * kv_bytes<FORMAT>(c.dim);
             if (!WRITE && slot == ~0u) continue;
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
                 if (!columns.inside[half]) continue;
                 if constexpr (WRITE) raw[d][half] = fetch<F32, WHOLE>(from + columns.first[half] * kEb);
-                else raw[d][half] = fetch_cached<kCached>(from + columns.first[half] * kKvBytes<FORMAT>);
+                else raw[d][half] = fetch_cached<kCached>(from + kv_bytes<FORMAT>(columns.first[half]));
+                if constexpr (!WRITE && kFour) {
+                    const uint8_t *const scale = (side[d] ? c.v : c.k) + c.blocks + ((uint64_t)at[d] * c.dim + columns.first[half]) / 16;
+                    blocks[d] |= (uint32_t)__ldcs(scale) << (8 * half);
+                }
             }
             if constexpr (!WRITE && FORMAT != FE2O3_KV_BF16) scales[d] = (side[d] ? c.v_scales : c.k_scales)[at[d]];
         }
 #pragma unroll
         for (int d = 0; d < kDeep; ++d) {
             if (base + d * at_once >= rows) break;
-            uint8_t *const to = WRITE ? (side[d] ? c.v : c.k) + (uint64_t)at[d] * c.dim * kKvBytes<FORMAT> : there[d];
+            uint8_t *const to = WRITE ? (side[d] ? c.v : c.k) + (uint64_t)at[d] * kv_bytes<FORMAT>(c.dim) : there[d];
             if constexpr (WRITE && FORMAT != FE2O3_KV_BF16) {
                 float x[2 * kPiece];
                 uint32_t top = 0;   // the largest magnitude as bits: an infinity or a NaN is above every number
@@ -270,16 +155,37 @@ __global__ void __launch_bounds__(kThreads) kv_rows_kernel(KvCache c, KvRows r) 
                 else if (lanes == 8) top = highest<8>(top);
                 else
                     for (uint32_t o = 1; o < lanes; o <<= 1) top = max(top, __shfl_xor_sync(~0u, top, o));
-                const float scale = top < 0x7f800000u ? scale_of<FORMAT>(__uint_as_float(top)) : __uint_as_float(0x7fc00000u);
-                minus_quotients<FORMAT>(x, scale);
-                if (!active[d]) continue;
+                if constexpr (kFour) {
+                    float scale, up;
+                    row_scales4(__uint_as_float(top), scale, up);
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    if (!columns.inside[half]) continue;
-                    const float *const q = x + half * kPiece;
-                    put_cached<kCached>(to + columns.first[half], make_uint4(codes_of<FORMAT>(q), F32 ? 0 : codes_of<FORMAT>(q + kPiece - 4), 0, 0));
+                    for (int half = 0; half < 2; ++half) {   // a block is 2 or 4 neighbouring lanes' pieces
+                        const float *const q = x + half * kPiece;
+                        float m = 0.f;
+#pragma unroll
+                        for (int i = 0; i < kPiece; ++i) m = fmaxf(m, fabsf(q[i]));
+#pragma unroll
+                        for (int o = 1; o < 16 / kPiece; o <<= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+                        float factor;
+                        const uint32_t block = block_scale4(m, scale, up, factor);
+                        if (!active[d] || !columns.inside[half]) continue;
+                        put_cached<kCached>(to + columns.first[half] / 2, make_uint4(codes4(q, factor) | (F32 ? 0 : codes4(q + kPiece - 4, factor) << 16), 0, 0, 0));
+                        if (l % (16 / kPiece) == 0) (side[d] ? c.v : c.k)[c.blocks + ((uint64_t)at[d] * c.dim + columns.first[half]) / 16] = (uint8_t)block;
+                    }
+                    if (active[d] && l == 0) (side[d] ? c.v_scales : c.k_scales)[at[d]] = scale;
+                    continue;
+                } else {
+                    const float scale = top < 0x7f800000u ? scale_of<FORMAT>(__uint_as_float(top)) : __uint_as_float(0x7fc00000u);
+                    minus_quotients<FORMAT>(x, scale);
+                    if (!active[d]) continue;
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        if (!columns.inside[half]) continue;
+                        const float *const q = x + half * kPiece;
+                        put_cached<kCached>(to + columns.first[half], make_uint4(codes_of<FORMAT>(q), F32 ? 0 : codes_of<FORMAT>(q + kPiece - 4), 0, 0));
+                    }
+                    if (l == 0) (side[d] ? c.v_scales : c.k_scales)[at[d]] = scale;
                 }
-                if (l == 0) (side[d] ? c.v_scales : c.k_scales)[at[d]] = scale;
             } else {
                 if (!active[d]) continue;
 #pragma unroll
@@ -293,6 +199,10 @@ __global__ void __launch_bounds__(kThreads) kv_rows_kernel(KvCache c, KvRows r) 
                         if constexpr (FORMAT == FE2O3_KV_BF16) {
                             widen2(v.x, x);
                             widen2(v.y, x + 2);
+                        } else if constexpr (kFour) {
+                            const float block = of_e4m3(blocks[d] >> (8 * half) & 255u);
+                            values4(v.x, block, scales[d], x);
+                            if constexpr (!F32) values4(v.x >> 16, block, scales[d], x + 4);
                         } else {
                             values_of<FORMAT>(v.x, scales[d], x);
                             if constexpr (!F32) values_of<FORMAT>(v.y, scales[d], x + 4);
@@ -300,7 +210,7 @@ __global__ void __launch_bounds__(kThreads) kv_rows_kernel(KvCache c, KvRows r) 
                         if constexpr (F32) v = make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
                         else v = make_uint4(bf16_pair(x[0], x[1]), bf16_pair(x[2], x[3]), bf16_pair(x[4], x[5]), bf16_pair(x[6], x[7]));
                     }
-                    if constexpr (WRITE) put_cached<kCached>(to + columns.first[half] * kKvBytes<FORMAT>, v);
+                    if constexpr (WRITE) put_cached<kCached>(to + kv_bytes<FORMAT>(columns.first[half]), v);
                     else put<F32, WHOLE>(to + columns.first[half] * kEb, v);
                 }
             }
@@ -312,18 +222,19 @@ using Kernel = void (*)(KvCache, KvRows);
 
 template <typename Args>
 int32_t launch_rows(fe2o3_ctx *ctx, cudaStream_t s, const Args *a, uint32_t dtype, fe2o3_geometry *geo, bool plan_only,
-                    const Kernel (&kernels)[3][2][2], const char *what) {
+                    const Kernel (&kernels)[4][2][2], const char *what) {
     // tokens of a block: up to a warp's lanes, and blocks that fill the SMs a whole number of times
     const uint32_t eb = dtype == FE2O3_DTYPE_F32 ? 4 : 2;
     const uint64_t odd = a->k.ptr | a->v.ptr | (uint64_t)a->k_token_stride * eb | (uint64_t)a->v_token_stride * eb | (uint64_t)a->k_head_stride * eb | (uint64_t)a->v_head_stride * eb;
-    static std::atomic<int> per_sm[3][2][2];   // of each kernel, found once
+    static std::atomic<int> per_sm[4][2][2];   // of each kernel, found once
+    const uint32_t format = a->format == FE2O3_KV_E2M1 ? 3 : a->format;   // in the tables
     const int i = dtype == FE2O3_DTYPE_F32, whole = odd % 16 == 0;
-    int fit = per_sm[a->format][i][whole].load(std::memory_order_relaxed);
+    int fit = per_sm[format][i][whole].load(std::memory_order_relaxed);
     if (fit == 0) {
-        const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, kernels[a->format][i][whole], kThreads, 0);
+        const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, kernels[format][i][whole], kThreads, 0);
         if (e != cudaSuccess) return fe2o3_cuda_status(e, what);
         if (fit < 1) fit = 1;
-        per_sm[a->format][i][whole].store(fit, std::memory_order_relaxed);
+        per_sm[format][i][whole].store(fit, std::memory_order_relaxed);
     }
     const uint64_t resident = (uint64_t)fit * (ctx->sm_count > 0 ? ctx->sm_count : 1);
     const uint64_t waves = (a->tokens + resident * kTokens - 1) / (resident * kTokens);
@@ -337,7 +248,7 @@ int32_t launch_rows(fe2o3_ctx *ctx, cudaStream_t s, const Args *a, uint32_t dtyp
                    a->k_head_stride, a->v_head_stride, reinterpret_cast<const uint32_t *>(a->token_offsets.ptr), a->tokens, per_block, lanes_log2,
                    // exact for the indexes of a block, below 64 kv_heads
                    a->kv_heads == 1 || a->kv_heads > 4096 ? 0 : (uint32_t)((0x100000000ull + a->kv_heads - 1) / a->kv_heads)};
-    const cudaError_t e = fe2o3_launch_early(kernels[a->format][i][whole], grid, kThreads, 0, s, 1, kv_cache_of(ctx, a), r);
+    const cudaError_t e = fe2o3_launch_early(kernels[format][i][whole], grid, kThreads, 0, s, 1, kv_cache_of(ctx, a), r);
     fe2o3_count_launch(1);
     return fe2o3_cuda_status(e, what);
 }
@@ -347,14 +258,14 @@ int32_t launch_rows(fe2o3_ctx *ctx, cudaStream_t s, const Args *a, uint32_t dtyp
 #define KV_FORMAT(FORMAT, WRITE)                                                                                                     \
     {{kv_rows_kernel<FORMAT, false, WRITE, false>, kv_rows_kernel<FORMAT, false, WRITE, true>},                                      \
      {kv_rows_kernel<FORMAT, true, WRITE, false>, kv_rows_kernel<FORMAT, true, WRITE, true>}}
-#define KV_FORMATS(WRITE) {KV_FORMAT(FE2O3_KV_BF16, WRITE), KV_FORMAT(FE2O3_KV_E4M3, WRITE), KV_FORMAT(FE2O3_KV_I8, WRITE)}
+#define KV_FORMATS(WRITE) {KV_FORMAT(FE2O3_KV_BF16, WRITE), KV_FORMAT(FE2O3_KV_E4M3, WRITE), KV_FORMAT(FE2O3_KV_I8, WRITE), KV_FORMAT(FE2O3_KV_E2M1, WRITE)}
 int32_t launch_kv_cache_append(fe2o3_ctx *ctx, cudaStream_t s, const void *args, fe2o3_geometry *geo, bool plan_only) {
-    static const Kernel kernels[3][2][2] = KV_FORMATS(true);
+    static const Kernel kernels[4][2][2] = KV_FORMATS(true);
     const fe2o3_kv_cache_append_v1_args *a = static_cast<const fe2o3_kv_cache_append_v1_args *>(args);
     return launch_rows(ctx, s, a, a->input_dtype, geo, plan_only, kernels, "kv_cache_append_v1");
 }
 int32_t launch_kv_cache_read(fe2o3_ctx *ctx, cudaStream_t s, const void *args, fe2o3_geometry *geo, bool plan_only) {
-    static const Kernel kernels[3][2][2] = KV_FORMATS(false);
+    static const Kernel kernels[4][2][2] = KV_FORMATS(false);
     const fe2o3_kv_cache_read_v1_args *a = static_cast<const fe2o3_kv_cache_read_v1_args *>(args);
     return launch_rows(ctx, s, a, a->output_dtype, geo, plan_only, kernels, "kv_cache_read_v1");
 }

@@ -10,24 +10,34 @@ struct KvCache {
     const uint32_t *page_table, *lengths;
     uint32_t pages, page_size, table_width, kv_heads, dim, batch;
     uint32_t *status;
+    uint64_t blocks;   // 4 bits: where in k and v the block scales begin
 };
 
+// Without a page table (places come as slots): neither it nor the lengths are there.
+template <typename Args>
+static inline KvCache kv_storage_of(const fe2o3_ctx *ctx, const Args *a) {
+    const uint64_t page = (uint64_t)a->kv_heads * a->page_size * kv_row_elements(a->format, a->dim), pages = a->k_cache.len / page;
+    KvCache c{};
+    c.k = reinterpret_cast<uint8_t *>(a->k_cache.ptr);
+    c.v = reinterpret_cast<uint8_t *>(a->v_cache.ptr);
+    c.k_scales = reinterpret_cast<float *>(a->k_scales.ptr);
+    c.v_scales = reinterpret_cast<float *>(a->v_scales.ptr);
+    c.pages = (uint32_t)pages;
+    c.page_size = a->page_size;
+    c.kv_heads = a->kv_heads;
+    c.dim = a->dim;
+    c.status = ctx->status_word;
+    c.blocks = pages * a->kv_heads * a->page_size * (a->dim / 2);
+    return c;
+}
 template <typename Args>
 static inline KvCache kv_cache_of(const fe2o3_ctx *ctx, const Args *a) {
-    const uint64_t page = (uint64_t)a->kv_heads * a->page_size * a->dim;
-    return KvCache{reinterpret_cast<uint8_t *>(a->k_cache.ptr),
-                   reinterpret_cast<uint8_t *>(a->v_cache.ptr),
-                   reinterpret_cast<float *>(a->k_scales.ptr),
-                   reinterpret_cast<float *>(a->v_scales.ptr),
-                   reinterpret_cast<const uint32_t *>(a->page_table.ptr),
-                   reinterpret_cast<const uint32_t *>(a->lengths.ptr),
-                   (uint32_t)(a->k_cache.len / page),
-                   a->page_size,
-                   a->table_width,
-                   a->kv_heads,
-                   a->dim,
-                   a->batch,
-                   ctx->status_word};
+    KvCache c = kv_storage_of(ctx, a);
+    c.page_table = reinterpret_cast<const uint32_t *>(a->page_table.ptr);
+    c.lengths = reinterpret_cast<const uint32_t *>(a->lengths.ptr);
+    c.table_width = a->table_width;
+    c.batch = a->batch;
+    return c;
 }
 
 // Whether a sequence of n positions fits its row of the page table (and 31 bits).
@@ -47,8 +57,9 @@ __device__ __forceinline__ uint32_t kv_row(const KvCache &c, uint32_t b, uint32_
     return (page * c.kv_heads + h) * c.page_size + slot;
 }
 
+// Bytes that n columns of a row take, the scales apart (4 bits: n is even).
 template <uint32_t FORMAT>
-constexpr uint32_t kKvBytes = FORMAT == FE2O3_KV_BF16 ? 2 : 1;   // of an element
+__host__ __device__ constexpr uint32_t kv_bytes(uint32_t n) { return FORMAT == FE2O3_KV_BF16 ? 2 * n : FORMAT == FE2O3_KV_E2M1 ? n / 2 : n; }
 template <uint32_t FORMAT>
 constexpr float kKvTop = FORMAT == FE2O3_KV_E4M3 ? 448.f : 127.f;   // the largest code
 

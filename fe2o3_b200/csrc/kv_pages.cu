@@ -1,0 +1,207 @@
+// Page tables and slot maps of a step, planned on the device; the rules stand at fe2o3_kv_pages_v1_args.
+//
+// Latency-bound: a step of some hundred sequences moves a few KB, prompts of 131072 tokens 1 MB of slots and positions.  One launch: a
+// cluster of up to kBlocks blocks.  Every block adds up all sequences for itself (pages that come back, new pages, new tokens: 64-bit
+// running sums), so that each knows whether the step fits before anything is written; blocks meet once, when all have read what is
+// replaced in place and the released pages lie on the stack.  Then pages and tokens are dealt out evenly, whatever sequence
+// they are of: a thread finds the sequence of its first token by bisection in shared memory and goes on from there.  The page
+// of a position comes from the table's row or straight from the stack, so tables and slots are written at the same time.
+#include "common.cuh"
+
+namespace {
+
+constexpr uint32_t kMaxThreads = 1024, kBlocks = 8, kAtOnce = 4;   // tokens a thread writes at once
+
+struct PagesArgs {
+    const uint32_t *counts, *release, *lengths, *free_count;
+    uint32_t *table, *free_pages, *next_lengths, *next_free_count, *offsets, *positions, *slots, *status;
+    uint32_t batch, width, page_size, tokens, pages;
+    int32_t shift;   // log2 of page_size, or negative
+};
+
+// A sequence as it comes in: pages it gives back, its length after that, its new tokens, its pages then and in the end.
+struct Sequence {
+    uint32_t back, length, count, held, need;
+    bool fits;
+};
+
+__device__ __forceinline__ uint32_t page_of(const PagesArgs &a, uint32_t position) { return a.shift >= 0 ? position >> a.shift : position / a.page_size; }
+__device__ __forceinline__ uint32_t pages_for(const PagesArgs &a, uint32_t length) { return length ? page_of(a, length - 1) + 1 : 0; }
+
+__device__ __forceinline__ Sequence sequence_of(const PagesArgs &a, uint32_t b) {
+    Sequence s{0, a.lengths[b], 0, 0, 0, true};
+    uint32_t pages = pages_for(a, s.length);
+    s.fits = s.length <= 0x7fffffffu && pages <= a.width;
+    if (a.release && a.release[b]) {
+        s.back = pages;
+        s.length = pages = 0;
+    }
+    s.held = pages;
+    s.count = a.counts ? a.counts[b] : s.length ? 1 : 0;
+    const uint64_t after = (uint64_t)s.length + s.count;
+    s.fits = s.fits && after <= 0x7fffffffu;
+    s.need = s.fits ? pages_for(a, (uint32_t)after) : 0;
+    s.fits = s.fits && s.need <= a.width;
+    return s;
+}
+
+struct Sums {
+    uint64_t back, fresh, tokens;
+    __device__ __forceinline__ Sums operator+(const Sums &o) const { return {back + o.back, fresh + o.fresh, tokens + o.tokens}; }
+};
+
+// What a sequence's pages and tokens are found by, in shared memory.
+struct Place {
+    uint32_t length, first_page, first_token;
+};
+
+__global__ void __launch_bounds__(kMaxThreads) kv_pages_kernel(PagesArgs a) {
+    extern __shared__ Place places[];   // [batch]
+    __shared__ Sums warps[32];
+    __shared__ Sums carry;
+    __shared__ uint32_t bad;
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, many = blockDim.x >> 5;
+    const uint32_t thread = blockIdx.x * blockDim.x + threadIdx.x, threads = gridDim.x * blockDim.x;
+    if (threadIdx.x == 0) {
+        carry = Sums{0, 0, 0};
+        bad = 0;
+    }
+    begin_after_previous();
+    __syncthreads();
+    const uint32_t count = *a.free_count;
+    for (uint32_t b0 = 0; b0 < a.batch; b0 += blockDim.x) {
+        const uint32_t b = b0 + threadIdx.x;
+        Sequence s{0, 0, 0, 0, 0, true};
+        if (b < a.batch) s = sequence_of(a, b);
+        if (!s.fits) bad = 1;
+        const Sums own{s.back, s.need >= s.held ? s.need - s.held : 0, s.count};
+        Sums sum = own;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const Sums up{__shfl_up_sync(~0u, sum.back, d), __shfl_up_sync(~0u, sum.fresh, d), __shfl_up_sync(~0u, sum.tokens, d)};
+            if (lane >= d) sum = sum + up;
+        }
+        if (lane == 31) warps[warp] = sum;
+        __syncthreads();
+        Sums before = carry;
+        for (uint32_t w = 0; w < warp; ++w) before = before + warps[w];
+        sum = before + sum;
+        if (b < a.batch) places[b] = Place{s.length, (uint32_t)(sum.fresh - own.fresh), (uint32_t)(sum.tokens - own.tokens)};
+        __syncthreads();
+        if (threadIdx.x == blockDim.x - 1) carry = sum;
+    }
+    __syncthreads();
+    const Sums total = carry;
+    const bool too_long = bad || total.tokens > 0xffffffffull || ((a.positions || a.slots) && total.tokens > a.tokens);
+    const uint64_t top = (uint64_t)count + total.back;
+    const bool fits = !too_long && top <= a.pages && total.fresh <= top;
+    if (!fits && thread == 0) kstatus_set(a.status, too_long ? FE2O3_KSTATUS_LENGTH : FE2O3_KSTATUS_PAGES);
+
+    // the released pages, sequence by sequence: one warp each (their places on the stack need the running sums again)
+    if (fits && total.back) {
+        uint64_t behind = count;
+        for (uint32_t b0 = 0; b0 < a.batch; b0 += 32) {   // every warp runs over all of them, 32 at a time
+            const uint32_t b = b0 + lane;
+            const uint32_t back = b < a.batch && a.release[b] ? pages_for(a, a.lengths[b]) : 0;
+            uint32_t upto = back;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const uint32_t u = __shfl_up_sync(~0u, upto, d);
+                if (lane >= d) upto += u;
+            }
+            uint32_t left = __ballot_sync(~0u, back != 0);
+            while (left) {
+                const int l = __ffs(left) - 1;
+                left &= left - 1;
+                const uint32_t n = __shfl_sync(~0u, back, l), end = __shfl_sync(~0u, upto, l);
+                if ((b0 + l) % (threads >> 5) != thread >> 5) continue;
+                const uint32_t *const row = a.table + (uint64_t)(b0 + l) * a.width;
+                uint32_t *const to = a.free_pages + behind + end;   // the last entry first
+                for (uint32_t i = lane; i < n; i += 32) to[-1 - (int64_t)i] = row[i];
+            }
+            behind += __shfl_sync(~0u, upto, 31);
+        }
+    }
+    if (gridDim.x > 1) {
+        __threadfence();
+        cluster_sync();
+    } else {
+        __syncthreads();
+    }
+
+    // what the sequences become
+    if (a.offsets && thread == 0) a.offsets[a.batch] = fits ? (uint32_t)total.tokens : 0;
+    if (thread == 0) *a.next_free_count = fits ? (uint32_t)(top - total.fresh) : count;
+    for (uint32_t b = thread; b < a.batch; b += threads) {
+        const uint32_t end = b + 1 < a.batch ? places[b + 1].first_token : (uint32_t)total.tokens;
+        if (fits) a.next_lengths[b] = places[b].length + (end - places[b].first_token);
+        else if (a.next_lengths != a.lengths) a.next_lengths[b] = a.lengths[b];
+        if (a.offsets) a.offsets[b] = fits ? places[b].first_token : 0;
+    }
+    // the last sequence that begins at or before x
+    auto find = [&](uint32_t x, uint32_t Place::*first) {
+        uint32_t low = 0, high = a.batch;
+        while (high - low > 1) {
+            const uint32_t mid = (low + high) / 2;
+            if (places[mid].*first <= x) low = mid;
+            else high = mid;
+        }
+        return low;
+    };
+    if (fits)
+        for (uint32_t i = thread; i < total.fresh; i += threads) {
+            const uint32_t b = find(i, &Place::first_page);
+            a.table[(uint64_t)b * a.width + pages_for(a, places[b].length) + (i - places[b].first_page)] = a.free_pages[top - 1 - i];
+        }
+    if (!a.positions && !a.slots) return;
+    const uint32_t tokens = fits ? (uint32_t)total.tokens : 0;
+    for (uint64_t t0 = (uint64_t)thread * kAtOnce; t0 < a.tokens; t0 += (uint64_t)threads * kAtOnce) {
+        uint32_t position[kAtOnce], slot[kAtOnce], b = t0 < tokens ? find((uint32_t)t0, &Place::first_token) : 0;
+#pragma unroll
+        for (uint32_t i = 0; i < kAtOnce; ++i) {
+            const uint32_t t = (uint32_t)t0 + i;
+            position[i] = 0;
+            slot[i] = FE2O3_SLOT_NONE;
+            if (t0 + i >= tokens) continue;
+            while (b + 1 < a.batch && places[b + 1].first_token <= t) ++b;
+            const Place p = places[b];
+            position[i] = p.length + (t - p.first_token);
+            const uint32_t page = page_of(a, position[i]), held = pages_for(a, p.length);
+            const uint32_t number = page < held ? a.table[(uint64_t)b * a.width + page] : a.free_pages[top - 1 - p.first_page - (page - held)];
+            if (number < a.pages) slot[i] = number * a.page_size + (position[i] - page * a.page_size);
+            else kstatus_set(a.status, FE2O3_KSTATUS_SLOT_RANGE);
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < kAtOnce; ++i) {
+            if (t0 + i >= a.tokens) continue;
+            if (a.positions) a.positions[t0 + i] = position[i];
+            if (a.slots) a.slots[t0 + i] = slot[i];
+        }
+    }
+}
+
+}  // namespace
+
+int32_t launch_kv_pages(fe2o3_ctx *ctx, cudaStream_t s, const void *args, fe2o3_geometry *geo, bool plan_only) {
+    const fe2o3_kv_pages_v1_args *a = static_cast<const fe2o3_kv_pages_v1_args *>(args);
+    const uint64_t work = (uint64_t)a->batch + a->tokens / kAtOnce;
+    const uint32_t threads = work <= 256 ? 256 : work <= 512 ? 512 : kMaxThreads, grid = work <= kMaxThreads ? 1 : kBlocks;
+    const uint32_t shared = a->batch * (uint32_t)sizeof(Place);
+    if (geo) *geo = fe2o3_geometry{{grid, 1, 1}, {threads, 1, 1}, shared, 1};
+    if (plan_only) {
+        FE2O3_CUDA(cudaSetDevice(ctx->device));
+        FE2O3_CUDA(cudaFuncSetAttribute(reinterpret_cast<const void *>(kv_pages_kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, 16384 * sizeof(Place)));
+        return FE2O3_OK;
+    }
+    int32_t shift = -1;
+    if ((a->page_size & (a->page_size - 1)) == 0) shift = __builtin_ctz(a->page_size);
+    auto at = [](const fe2o3_slice &x) { return reinterpret_cast<uint32_t *>(x.ptr); };
+    const PagesArgs p{at(a->counts), at(a->release), at(a->lengths), at(a->free_count), at(a->page_table), at(a->free_pages), at(a->next_lengths),
+                      at(a->next_free_count), at(a->token_offsets), at(a->positions), at(a->slots), ctx->status_word, a->batch, a->table_width,
+                      a->page_size, a->tokens, (uint32_t)a->free_pages.len, shift};
+    const cudaError_t e = fe2o3_launch_early(kv_pages_kernel, grid, threads, shared, s, grid, p);
+    fe2o3_count_launch(1);
+    return fe2o3_cuda_status(e, "kv_pages_v1");
+}
+
+static Fe2o3KernelRegistration reg_pages("kv_pages_v1", reinterpret_cast<const void *>(kv_pages_kernel));

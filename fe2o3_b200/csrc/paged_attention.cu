@@ -103,7 +103,8 @@ int32_t paged_attention_plan(fe2o3_ctx *ctx, const fe2o3_paged_attention_v1_args
     const uint32_t group = a->heads / a->kv_heads;
     // 16 query heads at once for a group of more than 8 (three terms of f32 queries of such long rows would not fit a block)
     const uint32_t nt = group <= 8 || (a->dim > 128 && a->format == FE2O3_KV_BF16 && a->q_dtype == FE2O3_DTYPE_F32) ? 1 : 2;
-    const PagedBuild b = a->format == FE2O3_KV_BF16 ? paged_build_bf16(a->dim, nt) : a->format == FE2O3_KV_E4M3 ? paged_build_e4m3(a->dim, nt) : paged_build_i8(a->dim, nt);
+    const PagedBuild b = a->format == FE2O3_KV_BF16 ? paged_build_bf16(a->dim, nt) : a->format == FE2O3_KV_E4M3 ? paged_build_e4m3(a->dim, nt)
+                         : a->format == FE2O3_KV_I8 ? paged_build_i8(a->dim, nt) : paged_build_e2m1(a->dim, nt);
     const uint32_t terms = a->q_dtype == FE2O3_DTYPE_BF16 ? 1 : a->format == FE2O3_KV_BF16 ? 3 : 2;
     FE2O3_CUDA(cudaSetDevice(ctx->device));
     cudaFuncAttributes attr;
@@ -156,12 +157,18 @@ int32_t paged_attention_plan(fe2o3_ctx *ctx, const fe2o3_paged_attention_v1_args
     while (a->page_size % box) box /= 2;
     if (box < 8 || p->args.c.pages == 0 || (a->format != FE2O3_KV_BF16 && ((a->k_scales.ptr | a->v_scales.ptr) & 15u))) box = 1;
     if (box > 1) {
-        const uint32_t eb = a->format == FE2O3_KV_BF16 ? 2 : 1, columns = eb == 2 ? 64 : a->dim <= 64 ? 64 : 128;
-        const uint64_t dims[3] = {a->dim, a->page_size, (uint64_t)p->args.c.pages * a->kv_heads};
-        const uint64_t strides[2] = {(uint64_t)a->dim * eb, (uint64_t)a->dim * eb * a->page_size};
-        const uint32_t shape[3] = {columns, box, 1};
+        const uint32_t half = a->format == FE2O3_KV_E2M1 ? 2 : 1, eb = a->format == FE2O3_KV_BF16 ? 2 : 1, columns = a->dim / half;   // (4 bits: bytes)
+        const uint32_t padded = a->dim <= 64 ? 64 : a->dim <= 128 || eb == 2 || half == 1 ? 128 : 256;
+        const uint64_t dims[3] = {columns, a->page_size, (uint64_t)p->args.c.pages * a->kv_heads};
+        const uint64_t strides[2] = {(uint64_t)columns * eb, (uint64_t)columns * eb * a->page_size};
+        const uint32_t shape[3] = {eb == 2 ? 64 : padded / half, box, 1};
         const auto make = eb == 2 ? fe2o3_make_tmap_bf16 : fe2o3_make_tmap_u8;
         if (make(&p->map_k, a->k_cache.ptr, 3, dims, strides, shape) != FE2O3_OK || make(&p->map_v, a->v_cache.ptr, 3, dims, strides, shape) != FE2O3_OK) box = 1;
+        if (box == 1 && half == 2) {   // (not seen: the cache's checks are the map's)
+            paged_attention_free(p);
+            fe2o3_set_error("UnsupportedShape: no tensor map for a 4-bit cache of this shape");
+            return FE2O3_ERR_UNSUPPORTED_SHAPE;
+        }
     }
     uint32_t *const counters = reinterpret_cast<uint32_t *>(static_cast<uint8_t *>(p->workspace) + slots);
     int32_t shift = -1;

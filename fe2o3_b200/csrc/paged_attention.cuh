@@ -58,7 +58,7 @@ struct PagedArgs {
 // The partial results of a block in the workspace: the end of an item that began in an earlier block, the beginning of one that
 // goes on in the next, and the ends that its warps 1 to 3 found of items that an earlier warp of the block began.
 constexpr uint32_t kPagedSlots = 5, kSlotFirst = 0, kSlotLast = 1, kSlotEnds = 2;
-constexpr uint32_t kPagedMaxStages = 4, kPagedMeeting = 512;
+constexpr uint32_t kPagedMaxStages = 6, kPagedMeeting = 640;
 
 using PagedKernel = void (*)(CUtensorMap, CUtensorMap, PagedArgs);
 struct PagedBuild {
@@ -69,6 +69,7 @@ struct PagedBuild {
 PagedBuild paged_build_bf16(uint32_t dim, uint32_t nt);
 PagedBuild paged_build_e4m3(uint32_t dim, uint32_t nt);
 PagedBuild paged_build_i8(uint32_t dim, uint32_t nt);
+PagedBuild paged_build_e2m1(uint32_t dim, uint32_t nt);
 
 namespace {
 
@@ -81,11 +82,12 @@ constexpr int kQueryExponent = 14;    // f16 queries: the largest of a row lies 
 
 template <uint32_t FORMAT, int DP, int NT>
 struct Shape {
-    static constexpr bool kF16 = FORMAT != FE2O3_KV_BF16;
-    static constexpr int kRow = DP * (kF16 ? 1 : 2);                                        // bytes of a row in a stage
+    static constexpr bool kF16 = FORMAT != FE2O3_KV_BF16, kFour = FORMAT == FE2O3_KV_E2M1;
+    static constexpr int kRow = kv_bytes<FORMAT>(DP);                                       // bytes of a row in a stage
     static constexpr int kKeys = kF16 ? (DP == 256 ? 16 : 32) : (DP == 64 ? 32 : 16);       // of a tile
     static constexpr int kStage = 2 * kKeys * kRow;                                         // K, V: whole swizzle patterns
-    static constexpr int kScales = kF16 ? 8 * kKeys : 0;                                    // of the rows of K, of V
+    static constexpr int kBlocks = kFour ? kKeys * DP / 16 : 0;                             // block scales of K, and of V
+    static constexpr int kScales = (kF16 ? 8 * kKeys : 0) + 2 * kBlocks;                    // of the rows of K, of V; then the blocks'
     static constexpr int kPitch = kRow < 128 ? kRow : 128;                                  // a row lies in parts of at most 128 bytes
     static constexpr int kHeads = 8 * NT;
     static constexpr int kQueryRow = 2 * DP + 16;                                           // bytes, padded against bank conflicts
@@ -215,12 +217,57 @@ __device__ __forceinline__ void word_f16(uint32_t w, uint32_t &a, uint32_t &b) {
     }
 }
 
+// ---- 4 bits ----
+// The eight codes of a word as f16 pairs, exactly.
+__device__ __forceinline__ void codes4_f16(uint32_t w, uint32_t (&h)[4]) {
+    asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %4;\n\tcvt.rn.f16x2.e2m1x2 %0, a;\n\tcvt.rn.f16x2.e2m1x2 %1, b;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %2, c;\n\tcvt.rn.f16x2.e2m1x2 %3, d;\n\t}" : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3]) : "r"(w));
+}
+__device__ __forceinline__ uint32_t code4_pair(uint32_t w, int byte) {   // the two of one byte
+    uint32_t h[4];
+    codes4_f16(w, h);   // (what is not asked for falls away)
+    return byte == 0 ? h[0] : byte == 1 ? h[1] : byte == 2 ? h[2] : h[3];
+}
+__device__ __forceinline__ uint32_t scales_f16(uint32_t two) {   // of two blocks, a byte each
+    uint32_t r;
+    asm("{\n\t.reg .b16 t;\n\tcvt.u16.u32 t, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, t;\n\t}" : "=r"(r) : "r"(two));
+    return r;
+}
+__device__ __forceinline__ uint32_t times_f16(uint32_t a, uint32_t b) {   // (a code times its block's scale has 6 bits: exact)
+    uint32_t r;
+    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t at) {
+    uint32_t v;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint32_t lds16(uint32_t at) {
+    uint32_t v;
+    asm volatile("{\n\t.reg .b16 t;\n\tld.shared.u16 t, [%1];\n\tcvt.u32.u16 %0, t;\n\t}" : "=r"(v) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint32_t lds8(uint32_t at) {
+    uint32_t v;
+    asm volatile("{\n\t.reg .b16 t;\n\tld.shared.u8 t, [%1];\n\tcvt.u32.u16 %0, t;\n\t}" : "=r"(v) : "r"(at) : "memory");
+    return v;
+}
+// The key that row r of eight stands for.  With 4 bits two neighbours change places for half of the rows, so that the rows of V that the
+// lanes of one access touch (2 t and its neighbour) lie on banks of their own; K's follow.
+template <uint32_t FORMAT, int DP>
+__device__ __forceinline__ uint32_t key_of(uint32_t r) {
+    if constexpr (FORMAT != FE2O3_KV_E2M1 || DP == 256) return r;
+    else return r ^ (r >> (DP == 64 ? 2 : 1) & 1);
+}
+
 // Where 16-byte piece c of row r lies in a stage's K or V part: as the copy engine's swizzle has it, rows in parts of 128 bytes.
 // Of what the lanes of one access touch, nothing meets on a bank but K of the 8-bit formats, in twos.
 template <uint32_t FORMAT, int DP>
 __device__ __forceinline__ uint32_t piece_at(uint32_t r, uint32_t c) {
     using S = Shape<FORMAT, DP, 1>;
-    if constexpr (S::kRow == 64) return r * 64 + ((c ^ (r >> 1 & 3)) << 4);
+    if constexpr (S::kRow == 32) return r * 32 + (c << 4);
+    else if constexpr (S::kRow == 64) return r * 64 + ((c ^ (r >> 1 & 3)) << 4);
     else return (c >> 3) * S::kKeys * 128 + r * 128 + (((c ^ r) & 7) << 4);
 }
 
@@ -369,7 +416,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     using S = Shape<FORMAT, DP, NT>;
     using P = Part<DP / 16, NT>;
     constexpr int KT = S::kKeys, MT = KT / 16, MD = DP / 16, kPieces = S::kRow / 16, kRowsAtOnce = 32 / kPieces;
-    constexpr bool F16 = S::kF16;
+    constexpr bool F16 = S::kF16, F4 = S::kFour;
     extern __shared__ __align__(1024) uint8_t smem[];   // (swizzle patterns are 1 KiB)
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t4 = lane & 3;
     uint8_t *const my_ring = smem + warp * a.stages * S::kStage;
@@ -381,7 +428,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     uint8_t *const query = queries + warp * terms * term_bytes;
     Meeting &meeting = *reinterpret_cast<Meeting *>(queries + kPagedWarps * terms * term_bytes);
     const uint32_t query_s = smem_u32(query);
-    const uint32_t row_bytes = a.c.dim * (F16 ? 1 : 2);
+    const uint32_t row_bytes = kv_bytes<FORMAT>(a.c.dim), row_blocks = a.c.dim / 16;   // (4 bits: block scales of a row)
     const uint32_t per_seq = a.c.kv_heads * a.chunks;   // items of a sequence
 
     uint64_t *const bars = meeting.arrivals[warp];
@@ -395,6 +442,8 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
             tma_prefetch_desc(&map_k);
             tma_prefetch_desc(&map_v);
         }
+    } else if (F4) {   // (a cache without pages: nothing is ever copied)
+        for (uint32_t i = lane; i < a.stages * S::kScales / 4; i += 32) reinterpret_cast<uint32_t *>(my_scales)[i] = 0;
     } else if (a.c.dim < DP) {   // the columns past the head's: zeros, which no copy goes over
         for (uint32_t i = lane; i < 2 * KT * a.stages * kPieces; i += 32) {
             const uint32_t c = i % kPieces, row = i / kPieces, r = row % KT, side = row / KT % 2, stage = row / (2 * KT);
@@ -431,6 +480,12 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
             if (k_too || i >= kPieces)
                 *reinterpret_cast<uint4 *>(my_ring + slot * S::kStage + (i >= kPieces ? KT * S::kRow : 0) + piece_at<FORMAT, DP>(r, i % kPieces)) = make_uint4(0, 0, 0, 0);
         if (F16 && lane < 2) reinterpret_cast<float *>(my_scales + slot * S::kScales)[lane * KT + r] = 0.f;
+        if constexpr (F4)
+            if (lane < row_blocks) {   // (K's rows that count nothing are never added up: their scales may be what they are)
+                uint8_t *const blocks = my_scales + slot * S::kScales + 8 * KT + r * row_blocks + lane;
+                if (k_too) blocks[0] = 0;
+                blocks[S::kBlocks] = 0;
+            }
     };
     auto copy_tile = [&] {
         while (ltile == lend && lrest) {
@@ -462,7 +517,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         uint64_t *const bar = &bars[lslot];
         const uint32_t row = there ? (page * a.c.kv_heads + head) * a.c.page_size + in_page : ~0u;
         if (a.box > 1) {
-            if (lane == 0) mbar_arrive_expect_tx(bar, __popc(found) * a.box * (2 * S::kRow + (F16 ? 8 : 0)));
+            if (lane == 0) mbar_arrive_expect_tx(bar, __popc(found) * a.box * (2 * S::kRow + (F16 ? 8 : 0) + (F4 ? 2 * row_blocks : 0)));
             __syncwarp();
             if (there) {
                 uint8_t *const to = my_ring + lslot * S::kStage + lane * a.box * S::kPitch;
@@ -475,6 +530,12 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                     uint8_t *const scales = my_scales + lslot * S::kScales + lane * a.box * 4;
                     bulk_load_1d(scales, a.c.k_scales + row, a.box * 4, bar);
                     bulk_load_1d(scales + KT * 4, a.c.v_scales + row, a.box * 4, bar);
+                }
+                if constexpr (F4) {
+                    uint8_t *const blocks = my_scales + lslot * S::kScales + 8 * KT + lane * a.box * row_blocks;
+                    const uint64_t from = a.c.blocks + (uint64_t)row * row_blocks;
+                    bulk_load_1d(blocks, a.c.k + from, a.box * row_blocks, bar);
+                    bulk_load_1d(blocks + S::kBlocks, a.c.v + from, a.box * row_blocks, bar);
                 }
             }
             __syncwarp();
@@ -512,6 +573,11 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     // ---- the queries of an item, as 16-bit terms: a lane takes eight columns of a row at a time ----
     auto lay_query = [&] {
         constexpr int kLanes = DP / 8, kAtOnce = 32 / kLanes, kPasses = S::kHeads / kAtOnce;
+        // where a lane's eight columns go.  4 bits: the lanes of a row of K hold 16 or 32 neighbours each (two runs of them for 256 columns), a
+        // word of eight at a time, and read the queries of two words at 32 bytes from one another
+        const uint32_t chunk_of_row = lane % kLanes, in_run = chunk_of_row & 15;
+        const uint32_t word = DP == 64 ? chunk_of_row & 1 : (in_run & 3) + (chunk_of_row >> 4) * 4, of_lane = DP == 64 ? chunk_of_row >> 1 : in_run >> 2;
+        const uint32_t place_of_chunk = F4 ? 8 * (word >> 1) + 2 * of_lane + (word & 1) : chunk_of_row;
         const uint32_t head = item / a.chunks, chunk = item % a.chunks, d = lane % kLanes * 8, r0 = lane / kLanes;
         const uint64_t base = (uint64_t)seq * a.q_stride + (uint64_t)(head * a.group) * a.q_head_stride + d;
         const uint32_t stored = min(a.group, (uint32_t)S::kHeads);
@@ -539,7 +605,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         for (int x = 0; x < kPasses; ++x) {
             if (x * kAtOnce >= stored) continue;
             const uint32_t row = min(x * kAtOnce + r0, a.q_rows - 1);   // (zeros again, where the rows are odd in number)
-            uint8_t *const to = query + row * S::kQueryRow + 2 * d;
+            uint8_t *const to = query + row * S::kQueryRow + 16 * place_of_chunk;
             float back = 1.f;
             if constexpr (!F16) {
                 if (!a.q_f32) *reinterpret_cast<uint4 *>(to) = raw[x][0];
@@ -623,11 +689,17 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                 if (a.lse && g == 0 && i0 == 0) a.lse[row] = n ? (p.m[nt][e] + log2f(l)) * 0.6931471805599453f : -INFINITY;
             }
     };
+    const uint32_t gk = key_of<FORMAT, DP>(g);
     // where a lane reads K and V in a stage; a lane's offsets for further steps differ by constants
     uint32_t k_off[4], v_off[4];
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
-        if constexpr (!F16) {
+        if constexpr (F4) {
+            const uint32_t row = key_of<FORMAT, DP>(2 * t4 + (x & 1));
+            k_off[x] = piece_at<FORMAT, DP>(gk, DP == 64 ? t4 >> 1 : t4 + 4 * (x & 1)) + (DP == 64 ? 8 * (t4 & 1) : 0);   // (256 columns: two pieces)
+            if constexpr (DP == 64) v_off[x] = KT * S::kRow + piece_at<FORMAT, DP>(row, g >> 2) + 4 * (g & 3);
+            else v_off[x] = KT * S::kRow + piece_at<FORMAT, DP>(row, (g >> 1) + (x >> 1) * 4) + 8 * (g & 1);   // (256 columns: two runs)
+        } else if constexpr (!F16) {
             k_off[x] = piece_at<FORMAT, DP>(lane & 15, 2 * x + (lane >> 4));
             v_off[x] = KT * S::kRow + piece_at<FORMAT, DP>((lane & 7) + (lane >> 4) * 8, 2 * x + (lane >> 3 & 1));
         } else if constexpr (DP == 64) {
@@ -780,6 +852,76 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                             s[mt][nt][e] += odd[mt][nt][e];
                             if (terms > 1) s[mt][nt][e] += low[mt][nt][e];
                         }
+            } else if constexpr (F4) {
+                float low[MT][NT][4];
+                constexpr int kRuns = DP == 256 ? 2 : 1, kWords = DP == 64 ? 2 : 4;   // runs of a lane's columns, words of eight in one
+                const uint32_t blocks = smem_u32(my_scales) + slot * S::kScales + 8 * KT;
+#pragma unroll
+                for (int run = 0; run < kRuns; ++run) {
+                    uint4 ka[MT][2];
+                    uint32_t ks[MT][2];   // scales of the run's blocks (of 64 columns one)
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const uint32_t row = 16 * mt + 8 * e, at = from + k_off[run] + row * S::kPitch, scale = blocks + (row + gk) * row_blocks;
+                            if constexpr (DP == 64) {
+                                const uint2 v = lds64(at);
+                                ka[mt][e] = make_uint4(v.x, v.y, 0, 0);
+                                ks[mt][e] = scales_f16(t4 < row_blocks ? lds8(scale + t4) * 0x101u : 0u);
+                            } else {
+                                ka[mt][e] = lds128(at);
+                                ks[mt][e] = scales_f16(2 * t4 + 8 * run < row_blocks ? lds16(scale + 2 * t4 + 8 * run) : 0u);
+                            }
+                        }
+#pragma unroll
+                    for (int word = 0; word < kWords; ++word) {
+                        uint32_t kf[MT][2][4];
+#pragma unroll
+                        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                const uint4 &v = ka[mt][e];
+                                uint32_t h[4];
+                                codes4_f16(word == 0 ? v.x : word == 1 ? v.y : word == 2 ? v.z : v.w, h);
+                                const uint32_t by = DP == 64 ? ks[mt][e] : __byte_perm(ks[mt][e], 0, word < 2 ? 0x1010 : 0x3232);
+                                kf[mt][0][e] = times_f16(h[0], by);
+                                kf[mt][0][e + 2] = times_f16(h[1], by);
+                                kf[mt][1][e] = times_f16(h[2], by);
+                                kf[mt][1][e + 2] = times_f16(h[3], by);
+                            }
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            const int all = 4 * run + word;
+                            const bool first = all == 0;
+                            const uint32_t at_q = q_off[nt] + 128 * (all >> 1) + 16 * (all & 1);
+                            const uint4 qb = lds128(at_q);
+#pragma unroll
+                            for (int mt = 0; mt < MT; ++mt) {
+                                if (first) mma_first<true>(s[mt][nt], kf[mt][0], qb.x, qb.y);
+                                else mma<true>(s[mt][nt], kf[mt][0], qb.x, qb.y);
+                                mma<true>(s[mt][nt], kf[mt][1], qb.z, qb.w);
+                            }
+                            if (terms > 1) {
+                                const uint4 ql = lds128(at_q + term_bytes);
+#pragma unroll
+                                for (int mt = 0; mt < MT; ++mt) {
+                                    if (first) mma_first<true>(low[mt][nt], kf[mt][0], ql.x, ql.y);
+                                    else mma<true>(low[mt][nt], kf[mt][0], ql.x, ql.y);
+                                    mma<true>(low[mt][nt], kf[mt][1], ql.z, ql.w);
+                                }
+                            }
+                        }
+                    }
+                }
+                if (terms > 1) {
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) s[mt][nt][e] += low[mt][nt][e];
+                }
             } else {
                 float low[MT][NT][4];
 #pragma unroll
@@ -836,7 +978,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
             // the running maximum, in units of log2; weights
             float vs[MT][2], vs_log[MT][2];
             if constexpr (F16) {
-                const uint32_t scales = smem_u32(my_scales) + slot * S::kScales + 4 * g;
+                const uint32_t scales = smem_u32(my_scales) + slot * S::kScales + 4 * gk;
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -869,7 +1011,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
-                            if (16 * mt + 8 * (e >> 1) + g - ahead >= left - ahead) s[mt][nt][e] = -INFINITY;
+                            if (16 * mt + 8 * (e >> 1) + gk - ahead >= left - ahead) s[mt][nt][e] = -INFINITY;
                 }
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt)
@@ -947,8 +1089,31 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
             }
 
             // output: rows are its columns, columns heads; the tile's sum is the tensor unit's, the rest f32
-            uint4 v4[MT][4][F16 && DP == 256 ? 2 : 1];
-            if constexpr (F16) {
+            uint4 v4[F4 ? 1 : MT][4][F16 && DP == 256 ? 2 : 1];
+            constexpr int kRuns4 = DP == 256 ? 2 : 1;
+            uint2 w4[F4 ? MT : 1][4][kRuns4];       // 4 bits: the lane's columns of four keys
+            uint32_t vs4[F4 ? MT : 1][2][kRuns4];   // and the scales of two keys' blocks
+            uint32_t lo4[F4 ? MT : 1][2], hi4[F4 ? MT : 1][2];   // codes of two keys side by side: even columns, odd ones
+            if constexpr (F4) {
+                const uint32_t blocks = smem_u32(my_scales) + slot * S::kScales + 8 * KT + S::kBlocks, k0 = key_of<FORMAT, DP>(2 * t4);
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                    for (int run = 0; run < kRuns4; ++run) {
+                        const uint32_t block = (DP == 64 ? g >> 1 : g) + 8 * run;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const uint32_t at = from + v_off[(e & 1) + 2 * run] + (16 * mt + 8 * (e >> 1)) * S::kPitch;
+                            if constexpr (DP == 64) w4[mt][e][run] = make_uint2(lds32(at), 0);
+                            else w4[mt][e][run] = lds64(at);
+                        }
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const uint32_t at = blocks + (16 * mt + 8 * e) * row_blocks + block;
+                            vs4[mt][e][run] = scales_f16(block < row_blocks ? lds8(at + k0 * row_blocks) | lds8(at + (k0 ^ 1) * row_blocks) << 8 : 0u);
+                        }
+                    }
+            } else if constexpr (F16) {
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -967,7 +1132,21 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                 uint32_t va[MT][4];
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) {
-                    if constexpr (F16) {
+                    if constexpr (F4) {
+                        constexpr int kColumns = DP == 256 ? 8 : MD;   // tiles of a run
+                        const int run = i / kColumns, word = i % kColumns / 4, byte = i % 4;
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            if (byte == 0) {
+                                const uint2 a2 = w4[mt][2 * e][run], b2 = w4[mt][2 * e + 1][run];
+                                const uint32_t w0 = word ? a2.y : a2.x, w1 = word ? b2.y : b2.x;
+                                lo4[mt][e] = (w0 & 0x0f0f0f0fu) | (w1 << 4 & 0xf0f0f0f0u);
+                                hi4[mt][e] = (w0 >> 4 & 0x0f0f0f0fu) | (w1 & 0xf0f0f0f0u);
+                            }
+                            va[mt][2 * e] = times_f16(code4_pair(lo4[mt][e], byte), vs4[mt][e][run]);
+                            va[mt][2 * e + 1] = times_f16(code4_pair(hi4[mt][e], byte), vs4[mt][e][run]);
+                        }
+                    } else if constexpr (F16) {
                         uint32_t w[4];
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {

@@ -1,0 +1,4 @@
+// The paged attention kernels over a cache of this format.
+#include "paged_attention.cuh"
+
+PagedBuild paged_build_e2m1(uint32_t dim, uint32_t nt) { return paged_build_for<FE2O3_KV_E2M1>(dim, nt); }

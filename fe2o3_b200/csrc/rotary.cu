@@ -1,0 +1,339 @@
+// Rotary positions: rows of q and k turned pair by pair (rotary_v1), and new tokens turned and written into the key-value cache in one
+// pass (kv_cache_rotary_append_v1).  The formulas stand at fe2o3_rotary_v1_args and fe2o3_kv_cache_rotary_append_v1_args.
+//
+// HBM-bound: each element is read once and written once.  A block takes some tokens, all their rows or a part of them; it first
+// works out the tokens' sines and cosines, once for all heads, into shared memory.  A row is pieces of 16 bytes, two to each of 2 to 32
+// lanes: with halves as pairs the two pieces that hold them, so that a lane turns its own columns; where half of the turned columns is no
+// whole number of pieces, a lane fetches its columns' partners one by one (they are in the first cache).
+// Angles: position times frequency has up to 56 bits.  The product p and what rounding took from it, e, are 64-bit numbers that add up
+// to it exactly; n whole turns are taken off in two steps (2 pi as two 64-bit numbers), which leaves an angle in [-pi, pi] that is right
+// to some 2^-50.  Its sine and cosine are those of its 32-bit rounding, and the rest of it to first order.
+#include <atomic>
+
+#include "kv_rows.cuh"
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr uint32_t kPlain = ~0u;   // FORMAT: no cache, q and k go to rows like theirs
+constexpr uint32_t kMostTokens = 16;
+
+struct RotaryRows {
+    const uint8_t *from[3];            // q, k, v
+    uint8_t *to[2];                    // of q and k
+    uint32_t token_stride[3], head_stride[3], to_token_stride[2], to_head_stride[2];
+    const uint32_t *positions, *slots;
+    const float *frequencies;
+    uint32_t tokens, heads, rows;      // rows of a token: heads, then kv_heads of k (and of v)
+    uint32_t per_block, parts;         // tokens of a block; blocks that share them
+    uint32_t dim, kv_heads, pairs, lanes_log2, half;   // half: of the turned columns, in pieces; 0: partners one by one
+    uint32_t rows_inverse;             // 2^32 / rows rounded up, or 0
+    bool interleaved;
+    float scale, sign;
+};
+
+// Cosine and sine of position * frequency, times scale.
+__device__ __forceinline__ float2 turn_of(uint32_t position, float frequency, float scale, float sign) {
+    const double x = position, f = frequency, p = x * f, e = fma(x, f, -p);
+    const double n = rint(p * 0.15915494309189535);
+    const double a = fma(-n, 2.4492935982947064e-16, fma(-n, 6.283185307179586, p)) + e;
+    const double h = a * 0.3183098861837907;   // in half turns
+    const float near = (float)h, rest = (float)(h - near) * 3.14159274f;
+    float s, c;
+    sincospif(near, &s, &c);
+    return make_float2(fmaf(-rest, s, c) * scale, fmaf(rest, c, s) * scale * sign);
+}
+
+__device__ __forceinline__ uint32_t word_of(const uint4 &v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+
+// A lane's columns of a row into the cache.  bf16 columns from `turned` on are as they came, bit for bit.
+template <uint32_t FORMAT, int kPiece>
+__device__ __forceinline__ void store_row(const KvCache &c, float (&x)[2 * kPiece], const uint4 (&raw)[2], uint32_t turned, uint32_t side, uint32_t row, const uint32_t (&first)[2], const bool (&inside)[2],
+                                          uint32_t l, uint32_t lanes, bool active) {
+    constexpr int kCached = kv_bytes<FORMAT>(kPiece);
+    uint8_t *const base = side ? c.v : c.k, *const to = base + (uint64_t)row * kv_bytes<FORMAT>(c.dim);
+    float *const scales = side ? c.v_scales : c.k_scales;
+    if constexpr (FORMAT == FE2O3_KV_BF16) {
+        if (!active) return;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            if (!inside[half]) continue;
+            const float *const q = x + half * kPiece;
+            uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < kPiece / 2; ++i) w[i] = kPiece == 8 && first[half] + 2 * i >= turned ? word_of(raw[half], i) : bf16_pair(q[2 * i], q[2 * i + 1]);
+            put_cached<kCached>(to + 2 * first[half], make_uint4(w[0], w[1], w[2], w[3]));
+        }
+    } else {
+        uint32_t top = 0;   // the largest magnitude as bits: an infinity or a NaN is above every number
+#pragma unroll
+        for (int i = 0; i < 2 * kPiece; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+        for (uint32_t o = 1; o < lanes; o <<= 1) top = max(top, __shfl_xor_sync(~0u, top, o));
+        float scale;
+        if constexpr (FORMAT == FE2O3_KV_E2M1) {
+            float up;
+            row_scales4(__uint_as_float(top), scale, up);
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const float *const q = x + half * kPiece;
+                float m = 0.f;
+#pragma unroll
+                for (int i = 0; i < kPiece; ++i) m = fmaxf(m, fabsf(q[i]));
+#pragma unroll
+                for (int o = 1; o < 16 / kPiece; o <<= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+                float factor;
+                const uint32_t block = block_scale4(m, scale, up, factor);
+                if (!active || !inside[half]) continue;
+                put_cached<kCached>(to + first[half] / 2, make_uint4(codes4(q, factor) | (kPiece == 4 ? 0 : codes4(q + kPiece - 4, factor) << 16), 0, 0, 0));
+                if (l % (16 / kPiece) == 0) base[c.blocks + ((uint64_t)row * c.dim + first[half]) / 16] = (uint8_t)block;
+            }
+        } else {
+            scale = top < 0x7f800000u ? scale_of<FORMAT>(__uint_as_float(top)) : __uint_as_float(0x7fc00000u);
+            minus_quotients<FORMAT>(x, scale);
+            if (!active) return;
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                if (!inside[half]) continue;
+                const float *const q = x + half * kPiece;
+                put_cached<kCached>(to + first[half], make_uint4(codes_of<FORMAT>(q), kPiece == 4 ? 0 : codes_of<FORMAT>(q + kPiece - 4), 0, 0));
+            }
+        }
+        if (active && l == 0) scales[row] = scale;
+    }
+}
+
+// WHOLE: the rows start on 16 bytes.
+template <uint32_t FORMAT, bool F32, bool WHOLE>
+__global__ void __launch_bounds__(kThreads) rotary_kernel(KvCache c, RotaryRows r) {
+    constexpr int kEb = F32 ? 4 : 2, kPiece = 16 / kEb, kDeep = 2;
+    constexpr bool kCache = FORMAT != kPlain;
+    extern __shared__ float2 turns[];   // [tokens of the block][pairs]
+    __shared__ uint32_t first_rows[kMostTokens];   // in the cache, of head 0; ~0: a token that is left out
+    begin_after_previous();
+    const uint32_t part = blockIdx.x % r.parts, t0 = blockIdx.x / r.parts * r.per_block, n = min(r.per_block, r.tokens - t0);
+    if (kCache && threadIdx.x < n) {
+        const uint32_t slot = r.slots[t0 + threadIdx.x], page = slot / c.page_size;
+        const bool there = page < c.pages;
+        if (!there && slot != FE2O3_SLOT_NONE) kstatus_set(c.status, FE2O3_KSTATUS_SLOT_RANGE);
+        first_rows[threadIdx.x] = there && slot != FE2O3_SLOT_NONE ? page * c.kv_heads * c.page_size + (slot - page * c.page_size) : ~0u;
+    }
+    for (uint32_t i = threadIdx.x; i < n * r.pairs; i += kThreads) {
+        const uint32_t t = i / r.pairs;
+        turns[i] = turn_of(r.positions ? r.positions[t0 + t] : t0 + t, r.frequencies[i - t * r.pairs], r.scale, r.sign);
+    }
+    __syncthreads();
+
+    const uint32_t lanes = 1u << r.lanes_log2, at_once = kThreads >> r.lanes_log2, l = threadIdx.x & (lanes - 1);
+    // a lane's columns: two pieces, the partners of one another where there are any
+    const uint32_t pieces = r.dim / kPiece, rest = (pieces - 2 * r.half) / 2;   // rest: half of those that are not turned (half 0: of all)
+    uint32_t first[2];
+    const bool pair = l < r.half;
+    first[0] = kPiece * (pair ? l : r.half + l);
+    first[1] = kPiece * (pair ? l + r.half : r.half + l + rest);
+    const bool in = l < pieces / 2, inside[2] = {in, in};
+    const uint32_t total = n * r.rows, share = (total + r.parts - 1) / r.parts, end = min(total, (part + 1) * share);
+    for (uint32_t base = part * share; base < end; base += kDeep * at_once) {
+        const uint32_t mine = base + (threadIdx.x >> r.lanes_log2);
+        uint4 raw[kDeep][2];
+        float others[kDeep][2 * kPiece];
+        uint32_t token[kDeep], head[kDeep], what[kDeep];
+        bool active[kDeep];
+        const uint8_t *at[kDeep];
+#pragma unroll
+        for (int d = 0; d < kDeep; ++d) {
+            const uint32_t i = min(mine + d * at_once, end - 1);
+            token[d] = r.rows_inverse ? __umulhi(i, r.rows_inverse) : i / r.rows;
+            head[d] = i - token[d] * r.rows;
+            what[d] = head[d] < r.heads ? 0 : 1;
+            if (what[d]) head[d] -= r.heads;
+            if (kCache && what[d] && head[d] >= r.kv_heads) {
+                what[d] = 2;
+                head[d] -= r.kv_heads;
+            }
+            active[d] = mine + d * at_once < end && (!kCache || first_rows[token[d]] != ~0u);
+            at[d] = r.from[what[d]] + ((uint64_t)(t0 + token[d]) * r.token_stride[what[d]] + (uint64_t)head[d] * r.head_stride[what[d]]) * kEb;
+            raw[d][0] = raw[d][1] = make_uint4(0, 0, 0, 0);
+            if (active[d] && in) {
+#pragma unroll
+                for (int half = 0; half < 2; ++half) raw[d][half] = fetch<F32, WHOLE>(at[d] + first[half] * kEb);
+                if (!r.half && !r.interleaved && what[d] < 2) {
+#pragma unroll
+                    for (int i = 0; i < 2 * kPiece; ++i) {
+                        const uint32_t column = first[i / kPiece] + i % kPiece;
+                        others[d][i] = 0.f;
+                        if (column >= 2 * r.pairs) continue;
+                        const uint8_t *const e = at[d] + (column < r.pairs ? column + r.pairs : column - r.pairs) * kEb;
+                        if constexpr (F32) others[d][i] = *reinterpret_cast<const float *>(e);
+                        else others[d][i] = bf16_bits_to_f32(*reinterpret_cast<const uint16_t *>(e));
+                    }
+                }
+            }
+        }
+        __syncwarp();   // in place: every lane has its columns and their partners before one writes
+#pragma unroll
+        for (int d = 0; d < kDeep; ++d) {
+            if (base + d * at_once >= end) break;
+            float x[2 * kPiece];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const uint32_t w = word_of(raw[d][i / 4], i % 4);
+                if constexpr (F32) x[i] = __uint_as_float(w);
+                else widen2(w, x + 2 * i);
+            }
+            const uint32_t turned = what[d] < 2 ? 2 * r.pairs : 0;
+            if (what[d] < 2 && in) {
+                const float2 *const cs = turns + token[d] * r.pairs;
+                if (r.interleaved) {
+#pragma unroll
+                    for (int i = 0; i < 2 * kPiece; i += 2) {
+                        const uint32_t column = first[i / kPiece] + i % kPiece;
+                        if (column >= 2 * r.pairs) continue;
+                        const float2 t = cs[column / 2];
+                        const float a = x[i], b = x[i + 1];
+                        x[i] = fmaf(a, t.x, -(b * t.y));
+                        x[i + 1] = fmaf(b, t.x, a * t.y);
+                    }
+                } else if (pair) {
+#pragma unroll
+                    for (int i = 0; i < kPiece; ++i) {
+                        const float2 t = cs[first[0] + i];
+                        const float a = x[i], b = x[kPiece + i];
+                        x[i] = fmaf(a, t.x, -(b * t.y));
+                        x[kPiece + i] = fmaf(b, t.x, a * t.y);
+                    }
+                } else if (!r.half) {
+#pragma unroll
+                    for (int i = 0; i < 2 * kPiece; ++i) {
+                        const uint32_t column = first[i / kPiece] + i % kPiece;
+                        if (column >= 2 * r.pairs) continue;
+                        const bool low = column < r.pairs;
+                        const float2 t = cs[low ? column : column - r.pairs];
+                        x[i] = low ? fmaf(x[i], t.x, -(others[d][i] * t.y)) : fmaf(x[i], t.x, others[d][i] * t.y);
+                    }
+                }
+            }
+            if (kCache && what[d]) {
+                if constexpr (kCache) {
+                    const uint32_t row = first_rows[token[d]] + head[d] * c.page_size;
+                    store_row<FORMAT, kPiece>(c, x, raw[d], turned, what[d] - 1, row, first, inside, l, lanes, active[d]);
+                }
+                continue;
+            }
+            if (!active[d] || !in) continue;
+            uint8_t *const to = r.to[what[d]] + ((uint64_t)(t0 + token[d]) * r.to_token_stride[what[d]] + (uint64_t)head[d] * r.to_head_stride[what[d]]) * kEb;
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const float *const q = x + half * kPiece;
+                uint32_t w[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if constexpr (F32) w[i] = __float_as_uint(q[i]);
+                    else w[i] = first[half] + 2 * i >= turned ? word_of(raw[d][half], i) : bf16_pair(q[2 * i], q[2 * i + 1]);
+                }
+                put<F32, WHOLE>(to + first[half] * kEb, make_uint4(w[0], w[1], w[2], w[3]));
+            }
+        }
+    }
+}
+
+using Kernel = void (*)(KvCache, RotaryRows);
+
+int32_t launch_rows(fe2o3_ctx *ctx, cudaStream_t s, Kernel kernel, uint32_t eb, bool four, const KvCache &c, RotaryRows r, fe2o3_geometry *geo, bool plan_only,
+                    const char *what) {
+    const uint32_t piece = 16 / eb;
+    // Partners lie in pieces of their own where half of the turned columns is a whole number of pieces (4 bits: of blocks, which stay with
+    // neighbouring lanes).
+    r.half = !r.interleaved && r.pairs % (four ? 16 : piece) == 0 ? r.pairs / piece : 0;
+    while ((2 * piece << r.lanes_log2) < r.dim) ++r.lanes_log2;
+    if (r.lanes_log2 == 0) r.lanes_log2 = 1;
+    const uint32_t sms = ctx->sm_count > 0 ? ctx->sm_count : 1, resident = sms * 6;
+    r.per_block = 1;
+    r.parts = 1;
+    if (r.tokens >= resident) {
+        const uint64_t waves = (r.tokens + (uint64_t)resident * kMostTokens - 1) / ((uint64_t)resident * kMostTokens);
+        r.per_block = ceil_div_u32(r.tokens, resident * waves);
+    } else if (r.tokens) {
+        const uint32_t rounds = ceil_div_u32((uint64_t)r.rows << r.lanes_log2, kThreads);   // of a token's rows
+        r.parts = resident / r.tokens < rounds ? resident / r.tokens : rounds;
+        if (r.parts == 0) r.parts = 1;
+    }
+    r.rows_inverse = r.rows <= 1 || (uint64_t)r.per_block * r.rows > 65536 || r.rows > 65536 ? 0 : (uint32_t)((0x100000000ull + r.rows - 1) / r.rows);
+    const uint32_t grid = ceil_div_u32(r.tokens, r.per_block) * r.parts, shared = r.per_block * r.pairs * (uint32_t)sizeof(float2);
+    if (geo) *geo = fe2o3_geometry{{grid, 1, 1}, {kThreads, 1, 1}, shared, 1};
+    if (plan_only || r.tokens == 0 || r.rows == 0) return FE2O3_OK;
+    const cudaError_t e = fe2o3_launch_early(kernel, grid, kThreads, shared, s, 1, c, r);
+    fe2o3_count_launch(1);
+    return fe2o3_cuda_status(e, what);
+}
+
+template <typename... P>
+bool on_16(uint64_t bits, P... strides) { return ((bits | ... | strides) & 15u) == 0; }
+
+}  // namespace
+
+#define ROTARY_FORMAT(FORMAT) \
+    {{rotary_kernel<FORMAT, false, false>, rotary_kernel<FORMAT, false, true>}, {rotary_kernel<FORMAT, true, false>, rotary_kernel<FORMAT, true, true>}}
+
+int32_t launch_rotary(fe2o3_ctx *ctx, cudaStream_t s, const void *args, fe2o3_geometry *geo, bool plan_only) {
+    static const Kernel kernels[2][2] = ROTARY_FORMAT(kPlain);
+    const fe2o3_rotary_v1_args *a = static_cast<const fe2o3_rotary_v1_args *>(args);
+    const uint64_t eb = a->dtype == FE2O3_DTYPE_F32 ? 4 : 2;
+    RotaryRows r{};
+    r.from[0] = reinterpret_cast<const uint8_t *>(a->q.ptr);
+    r.from[1] = reinterpret_cast<const uint8_t *>(a->k.ptr);
+    r.to[0] = reinterpret_cast<uint8_t *>(a->q_output.ptr);
+    r.to[1] = reinterpret_cast<uint8_t *>(a->k_output.ptr);
+    r.token_stride[0] = a->q_token_stride, r.token_stride[1] = a->k_token_stride;
+    r.head_stride[0] = a->q_head_stride, r.head_stride[1] = a->k_head_stride;
+    r.to_token_stride[0] = a->q_output_token_stride, r.to_token_stride[1] = a->k_output_token_stride;
+    r.to_head_stride[0] = a->q_output_head_stride, r.to_head_stride[1] = a->k_output_head_stride;
+    r.positions = reinterpret_cast<const uint32_t *>(a->positions.ptr);
+    r.frequencies = reinterpret_cast<const float *>(a->frequencies.ptr);
+    r.tokens = a->tokens;
+    r.heads = a->heads;
+    r.kv_heads = a->kv_heads;
+    r.rows = a->heads + a->kv_heads;
+    r.dim = a->dim;
+    r.pairs = a->rotary_dim / 2;
+    r.interleaved = a->layout == FE2O3_ROTARY_INTERLEAVED;
+    r.scale = a->scale;
+    r.sign = a->backward ? -1.f : 1.f;
+    bool whole = true;
+    if (a->heads) whole = on_16(a->q.ptr | a->q_output.ptr, eb * a->q_token_stride, eb * a->q_head_stride, eb * a->q_output_token_stride, eb * a->q_output_head_stride);
+    if (a->kv_heads) whole = whole && on_16(a->k.ptr | a->k_output.ptr, eb * a->k_token_stride, eb * a->k_head_stride, eb * a->k_output_token_stride, eb * a->k_output_head_stride);
+    return launch_rows(ctx, s, kernels[eb == 4][whole], (uint32_t)eb, false, KvCache{}, r, geo, plan_only, "rotary_v1");
+}
+
+int32_t launch_kv_cache_rotary_append(fe2o3_ctx *ctx, cudaStream_t s, const void *args, fe2o3_geometry *geo, bool plan_only) {
+    static const Kernel kernels[4][2][2] = {ROTARY_FORMAT(FE2O3_KV_BF16), ROTARY_FORMAT(FE2O3_KV_E4M3), ROTARY_FORMAT(FE2O3_KV_I8), ROTARY_FORMAT(FE2O3_KV_E2M1)};
+    const fe2o3_kv_cache_rotary_append_v1_args *a = static_cast<const fe2o3_kv_cache_rotary_append_v1_args *>(args);
+    const uint64_t eb = a->input_dtype == FE2O3_DTYPE_F32 ? 4 : 2;
+    const bool four = a->format == FE2O3_KV_E2M1;
+    RotaryRows r{};
+    r.from[0] = reinterpret_cast<const uint8_t *>(a->q.ptr);
+    r.from[1] = reinterpret_cast<const uint8_t *>(a->k.ptr);
+    r.from[2] = reinterpret_cast<const uint8_t *>(a->v.ptr);
+    r.to[0] = reinterpret_cast<uint8_t *>(a->q_output.ptr);
+    r.token_stride[0] = a->q_token_stride, r.token_stride[1] = a->k_token_stride, r.token_stride[2] = a->v_token_stride;
+    r.head_stride[0] = a->q_head_stride, r.head_stride[1] = a->k_head_stride, r.head_stride[2] = a->v_head_stride;
+    r.to_token_stride[0] = a->q_output_token_stride;
+    r.to_head_stride[0] = a->q_output_head_stride;
+    r.positions = reinterpret_cast<const uint32_t *>(a->positions.ptr);
+    r.slots = reinterpret_cast<const uint32_t *>(a->slots.ptr);
+    r.frequencies = reinterpret_cast<const float *>(a->frequencies.ptr);
+    r.tokens = a->tokens;
+    r.heads = a->heads;
+    r.kv_heads = a->kv_heads;
+    r.rows = a->heads + 2 * a->kv_heads;
+    r.dim = a->dim;
+    r.pairs = a->rotary_dim / 2;
+    r.interleaved = a->layout == FE2O3_ROTARY_INTERLEAVED;
+    r.scale = a->scale;
+    r.sign = 1.f;
+    bool whole = on_16(a->k.ptr | a->v.ptr, eb * a->k_token_stride, eb * a->k_head_stride, eb * a->v_token_stride, eb * a->v_head_stride);
+    if (a->heads) whole = whole && on_16(a->q.ptr | a->q_output.ptr, eb * a->q_token_stride, eb * a->q_head_stride, eb * a->q_output_token_stride, eb * a->q_output_head_stride);
+    return launch_rows(ctx, s, kernels[four ? 3 : a->format][eb == 4][whole], (uint32_t)eb, four, kv_storage_of(ctx, a), r, geo, plan_only, "kv_cache_rotary_append_v1");
+}
+
+static Fe2o3KernelRegistration reg_rotary("rotary_v1", reinterpret_cast<const void *>(rotary_kernel<kPlain, false, true>));
+static Fe2o3KernelRegistration reg_rotary_append("kv_cache_rotary_append_v1", reinterpret_cast<const void *>(rotary_kernel<FE2O3_KV_BF16, false, true>));

@@ -57,6 +57,7 @@ extern "C" {
 #define FE2O3_KSTATUS_WAIT_EXPIRED 4u
 #define FE2O3_KSTATUS_SLOT_RANGE 5u
 #define FE2O3_KSTATUS_SCAN_STATE 6u
+#define FE2O3_KSTATUS_PAGES 7u
 
 typedef struct fe2o3_ctx fe2o3_ctx;
 typedef struct fe2o3_stream fe2o3_stream;
@@ -430,11 +431,21 @@ typedef struct fe2o3_moe_ep_ffn_v1_args {
  *   FE2O3_KV_BF16   bfloat16 (u16); k_scales and v_scales are empty
  *   FE2O3_KV_E4M3   8-bit floating point, four exponent and three mantissa bits (u8)
  *   FE2O3_KV_I8     8-bit integers, -127 .. 127
+ *   FE2O3_KV_E2M1   4-bit floating point, two exponent bits and one mantissa bit (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives),
+ *                   with a scale for every 16 columns in the format of E4M3
  * 8-bit elements stand for code * scale, one f32 scale a row: k_scales and v_scales are
  * [pages][kv_heads][page_size].  For a row x and the format's largest code C (448 and 127):
  *   scale = max |x| / C, code = x / scale rounded to the nearest code, ties to even,
  * both quotients rounded to f32; a row of zeros has scale 0, a row with an infinity or a NaN has scale NaN and
- * reads back as NaN.  A bf16 cache holds f32 rows rounded to nearest even, a NaN as a quiet one, and bf16 rows bit for bit.
+ * reads back as NaN.
+ * A 4-bit cache is an array of bytes: codes [pages][kv_heads][page_size][dim / 2], the even column in a byte's low half, and
+ * behind all of them block scales [pages][kv_heads][page_size][dim / 16]; it holds dim * 9 / 16 bytes a row, dim is a multiple of 32,
+ * page_size one of 8, and the row scales start on 16 bytes too.  Elements stand for code * block scale * row scale.  For a row x with
+ * m = max |x| and a block of 16 columns with m_g = max |x| in it:
+ *   scale = m / 2688, block scale = m_g * (448 / m) as e4m3, code = x * (1 / (block scale * scale)) as e2m1,
+ * every quotient and product rounded to f32, both conversions to nearest, ties to even; a block scale of 0 has codes 0.  A row whose m is below
+ * 2^-100 is held as zeros with scale 0, a row with an infinity or a NaN has codes and block scales 0 and scale NaN, and reads back as NaN.
+ * A bf16 cache holds f32 rows rounded to nearest even, a NaN as a quiet one, and bf16 rows bit for bit.
  * dim is a multiple of 16 up to 256, kv_heads at most 65536, page_size any number from 1, a cache has fewer than 2^32 rows, a sequence has fewer than 2^31 positions; both
  * caches start on 16 bytes.  Lengths and page table stay as they are while a launch runs.
  *
@@ -445,6 +456,7 @@ typedef struct fe2o3_moe_ep_ffn_v1_args {
 #define FE2O3_KV_BF16 0u
 #define FE2O3_KV_E4M3 1u
 #define FE2O3_KV_I8 2u
+#define FE2O3_KV_E2M1 4u
 
 /* Writes new tokens into the cache.  Rows token_offsets[b] .. token_offsets[b + 1] - 1 of k and v belong to
  * sequence b and go to its last positions before lengths[b] (lengths count the new tokens); without
@@ -459,7 +471,7 @@ typedef struct fe2o3_kv_cache_append_v1_args {
 } fe2o3_kv_cache_append_v1_args;
 
 /* Reads rows back into contiguous storage: the same rows, positions and strides as the append, in the
- * other direction.  code * scale is rounded once to f32, and once more for a bf16 output.  Rows of one output may not overlap. */
+ * other direction.  code * scale (4 bits: code * block scale, which is exact, * scale) is rounded once to f32, and once more for a bf16 output.  Rows of one output may not overlap. */
 typedef struct fe2o3_kv_cache_read_v1_args {
     fe2o3_slice k_cache, v_cache, k_scales, v_scales, page_table, lengths, token_offsets, k, v;
     uint32_t tokens, batch, kv_heads, dim, page_size, table_width;
@@ -473,7 +485,7 @@ typedef struct fe2o3_kv_cache_read_v1_args {
  * with the keys and values of head h / (heads / kv_heads).  heads is a multiple of kv_heads.  q row (b, h) starts at
  * element b * q_stride + h * q_head_stride; output [batch][heads][dim] is packed, f32 or bf16; lse
  * [batch][heads] f32 is optional.  The page table has at most 2^35 positions (2^44 times heads), batch * heads is below 2^31, batch at most 2^29.  A sequence of length 0 gives zeros and -inf.  Sums, maxima and
- * probabilities are f32, and a bf16 output is the f32 one rounded to nearest even.  Over 8-bit caches a probability
+ * probabilities are f32, and a bf16 output is the f32 one rounded to nearest even.  Over 8- and 4-bit caches a probability
  * times its row's scale has 22 significant bits from 2^-17 of the head's largest such product on, fewer below, and counts as
  * nothing below 2^-39 of it; the elements of a query likewise against the largest of their row (bf16 ones are exact from 2^-31 on).  The result does not
  * depend on which blocks finish first.  One launch of a prepared object at a time (it owns a workspace); what is patched into
@@ -484,6 +496,60 @@ typedef struct fe2o3_paged_attention_v1_args {
     float scale;
     uint32_t window, q_dtype, output_dtype, format, reserved;
 } fe2o3_paged_attention_v1_args;
+
+/* Plans a step of a paged cache on the device: which sequences give their pages back, which pages new tokens get, and where every
+ * new token goes.  The free pages are a stack: free_pages[0 .. free_count - 1], the next page is the last one.  In this order:
+ *   release   for every sequence b with release[b] != 0, b rising: the ceil(lengths[b] / page_size) pages of its row of the page table go
+ *             on the stack, the row's last first, and its length becomes 0 (release may be empty: none);
+ *   extend    for every sequence b rising: counts[b] new tokens (counts may be empty: one for every sequence whose length is then not 0); the
+ *             pages that its new length needs and it does not have come off the stack into its row, entry by entry.
+ * next_lengths and next_free_count are what lengths and free_count become (each may be the same slice as the one it follows); page_table and
+ * free_pages change in place, entries that no length reaches stay as they are.  token_offsets [batch + 1] are the running sums of the
+ * counts.  The new tokens, sequence after sequence, have positions[t] in their sequence and slots[t] = page * page_size + position % page_size;
+ * behind the last token, up to `tokens`, positions are 0 and slots FE2O3_SLOT_NONE.  token_offsets, positions and slots may each be empty.  A
+ * token whose page has a number that is none of free_pages.len pages has no slot either, and is FE2O3_KSTATUS_SLOT_RANGE.
+ * All or nothing: where a length or count does not fit its row of the page table (or 31 bits), or there are more tokens than `tokens`
+ * (where positions or slots are asked for) or than 32 bits hold, FE2O3_KSTATUS_LENGTH is reported, where free_pages has too few free pages
+ * (or no room for the released ones) FE2O3_KSTATUS_PAGES; page_table and free_pages then stay as they are, next_lengths and next_free_count are
+ * lengths and free_count, token_offsets 0, positions 0 and slots FE2O3_SLOT_NONE.  A page belongs to one sequence here: a table whose
+ * rows share pages is not to be released from.  batch is at most 16384, batch * table_width and the rows of all pages below 2^32. */
+#define FE2O3_SLOT_NONE 0xffffffffu
+typedef struct fe2o3_kv_pages_v1_args {
+    fe2o3_slice counts, release, lengths, free_count, page_table, free_pages, next_lengths, next_free_count, token_offsets, positions, slots;
+    uint32_t batch, table_width, page_size, tokens;
+} fe2o3_kv_pages_v1_args;
+
+/* Rotary positions: the first rotary_dim columns of every row of q and k, in pairs, are turned by an angle of the row's position,
+ *   angle_i = positions[t] * frequencies[i],   (x, y) -> scale * (x cos - y sin, x sin + y cos),   i < rotary_dim / 2,
+ * and with `backward` by the transpose of that (a gradient's way back); the other columns are copied.  Pair i is columns i and
+ * i + rotary_dim / 2 (FE2O3_ROTARY_HALF) or 2 i and 2 i + 1 (FE2O3_ROTARY_INTERLEAVED).  The product is reduced in 64 bits,
+ * whatever the position; sine, cosine and the rest are f32, rounded once to the output's type, the input's.  Without positions (empty slice) row t has
+ * position t.  Rows (t, h) start at element t * token_stride + h * head_stride; k is optional (kv_heads 0 and empty slices).  An output may be its own
+ * input, in place, with the same strides; rows of one output may not overlap.  dim is a multiple of 16 up to 256, rotary_dim
+ * an even number up to dim. */
+#define FE2O3_ROTARY_HALF 0u
+#define FE2O3_ROTARY_INTERLEAVED 1u
+typedef struct fe2o3_rotary_v1_args {
+    fe2o3_slice q, k, positions, frequencies, q_output, k_output;
+    uint32_t tokens, heads, kv_heads, dim, rotary_dim, layout, dtype, backward;
+    uint32_t q_token_stride, q_head_stride, k_token_stride, k_head_stride;
+    uint32_t q_output_token_stride, q_output_head_stride, k_output_token_stride, k_output_head_stride;
+    float scale;
+    uint32_t reserved;
+} fe2o3_rotary_v1_args;
+
+/* New tokens on their way into attention over the cache: q and k are turned as by rotary_v1 (forward), q goes to q_output, k and v into
+ * the cache as by kv_cache_append_v1, k rounded once, from f32.  Token t's row goes to slot slots[t] = page * page_size + place in the page;
+ * a token whose slot is FE2O3_SLOT_NONE is left out, its row of q_output too, and so is one whose slot lies outside the cache, which is
+ * FE2O3_KSTATUS_SLOT_RANGE.  rotary_dim 0: no rotation (frequencies and positions empty).  heads 0: no queries (empty slices).  No two
+ * tokens may share a slot. */
+typedef struct fe2o3_kv_cache_rotary_append_v1_args {
+    fe2o3_slice q, k, v, positions, slots, frequencies, q_output, k_cache, v_cache, k_scales, v_scales;
+    uint32_t tokens, heads, kv_heads, dim, page_size, rotary_dim, layout, input_dtype, format;
+    uint32_t q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+    uint32_t q_output_token_stride, q_output_head_stride;
+    float scale;
+} fe2o3_kv_cache_rotary_append_v1_args;
 
 /* examples/moe_expert_v1/src/kernel.rs:104-109
  * moe_expert_combine_f32_t8_k2_o16_v1(compact_output, inverse, route_weights,
@@ -591,6 +657,9 @@ int32_t fe2o3_moe_ep_ffn_v1_check(const fe2o3_moe_ep_ffn_v1_args *args);
 int32_t fe2o3_kv_cache_append_v1_check(const fe2o3_kv_cache_append_v1_args *args);
 int32_t fe2o3_kv_cache_read_v1_check(const fe2o3_kv_cache_read_v1_args *args);
 int32_t fe2o3_paged_attention_v1_check(const fe2o3_paged_attention_v1_args *args);
+int32_t fe2o3_kv_pages_v1_check(const fe2o3_kv_pages_v1_args *args);
+int32_t fe2o3_rotary_v1_check(const fe2o3_rotary_v1_args *args);
+int32_t fe2o3_kv_cache_rotary_append_v1_check(const fe2o3_kv_cache_rotary_append_v1_args *args);
 int32_t fe2o3_masked_reduce_u32_check(const fe2o3_masked_reduce_u32_args *args);
 int32_t fe2o3_masked_reduce_u32_packed_check(const fe2o3_masked_reduce_u32_packed_args *args);
 int32_t fe2o3_device_scan_u32_check(const fe2o3_device_scan_u32_args *args);
@@ -632,6 +701,9 @@ int32_t fe2o3_moe_ep_ffn_v1_prepare(fe2o3_ctx *ctx, const fe2o3_moe_ep_ffn_v1_ar
 int32_t fe2o3_kv_cache_append_v1_prepare(fe2o3_ctx *ctx, const fe2o3_kv_cache_append_v1_args *args, fe2o3_prepared **out);
 int32_t fe2o3_kv_cache_read_v1_prepare(fe2o3_ctx *ctx, const fe2o3_kv_cache_read_v1_args *args, fe2o3_prepared **out);
 int32_t fe2o3_paged_attention_v1_prepare(fe2o3_ctx *ctx, const fe2o3_paged_attention_v1_args *args, fe2o3_prepared **out);
+int32_t fe2o3_kv_pages_v1_prepare(fe2o3_ctx *ctx, const fe2o3_kv_pages_v1_args *args, fe2o3_prepared **out);
+int32_t fe2o3_rotary_v1_prepare(fe2o3_ctx *ctx, const fe2o3_rotary_v1_args *args, fe2o3_prepared **out);
+int32_t fe2o3_kv_cache_rotary_append_v1_prepare(fe2o3_ctx *ctx, const fe2o3_kv_cache_rotary_append_v1_args *args, fe2o3_prepared **out);
 int32_t fe2o3_masked_reduce_u32_prepare(fe2o3_ctx *ctx, const fe2o3_masked_reduce_u32_args *args,
                                         fe2o3_prepared **out);
 int32_t fe2o3_masked_reduce_u32_packed_prepare(fe2o3_ctx *ctx, const fe2o3_masked_reduce_u32_packed_args *args,

@@ -1,0 +1,131 @@
+"""Admission of page plans, rotary positions and 4-bit caches: pure host checks, no GPU."""
+import math
+
+import pytest
+
+import fe2o3_b200 as fe
+from test_kv_cache_checks import ALL, err, ok, queries, rows, sl
+
+
+def pages(batch=3, width=4, count=10, tokens=8):
+    return dict(counts=sl(0, batch), release=sl(1, batch), lengths=sl(2, batch), free_count=sl(3, 1), page_table=sl(4, batch * width), free_pages=sl(5, count),
+                next_lengths=sl(6, batch), next_free_count=sl(7, 1), token_offsets=sl(8, batch + 1), positions=sl(9, tokens), slots=sl(10, tokens),
+                batch=batch, table_width=width, page_size=16, tokens=tokens)
+
+
+def test_page_plans():
+    op, kw = "kv_pages_v1", pages()
+    ok(op, **kw)
+    for name in ("counts", "release", "token_offsets", "positions", "slots"):
+        ok(op, **{**kw, name: None})
+    ok(op, **{**kw, "next_lengths": kw["lengths"], "next_free_count": kw["free_count"]})
+    ok(op, **pages(batch=0, width=0, count=0, tokens=0))
+    ok(op, **pages(batch=16384))
+    for bad in (dict(page_size=0), dict(batch=16385), dict(table_width=1 << 31), dict(page_size=1 << 30)):
+        assert err(op, **{**kw, **bad}) == "UnsupportedShape", bad
+    for name, n in (("counts", 2), ("release", 4), ("lengths", 2), ("free_count", 2), ("page_table", 11), ("next_lengths", 4), ("next_free_count", 0),
+                    ("token_offsets", 3), ("positions", 9), ("slots", 7)):
+        assert err(op, **{**kw, name: sl(40, n)}) == "Length", name
+    assert err(op, **{**kw, "lengths": (0, 3)}) == "NullAddress"
+    assert err(op, **{**kw, "slots": sl(10, 8, 2)}) == "Alignment"
+    # outputs lie apart, from each other and from what is read; lengths that are only partly the next ones are neither
+    for a, b in (("next_lengths", "counts"), ("positions", "slots"), ("next_lengths", "page_table"), ("free_pages", "page_table"), ("token_offsets", "release")):
+        assert err(op, **{**kw, a: (kw[b][0], kw[a][1])}) == "OutputAliasesInput", (a, b)
+    assert err(op, **{**kw, "next_lengths": (kw["lengths"][0] + 4, 3)}) == "OutputAliasesInput"
+
+
+def rotary(tokens=5, heads=4, kv_heads=2, dim=64):
+    kw = dict(q=sl(0, tokens * heads * dim), k=sl(1, tokens * kv_heads * dim), positions=sl(2, tokens), frequencies=sl(3, 16),
+              q_output=sl(4, tokens * heads * dim), k_output=sl(5, tokens * kv_heads * dim), tokens=tokens, heads=heads, kv_heads=kv_heads, dim=dim, rotary_dim=32,
+              layout=fe.ROTARY_HALF, dtype=fe.DTYPE_F32, backward=0, scale=1.0)
+    for n in ("q", "k", "q_output", "k_output"):
+        kw.update({n + "_token_stride": (heads if n[0] == "q" else kv_heads) * dim, n + "_head_stride": dim})
+    return kw
+
+
+def test_rotary_rows():
+    op, kw = "rotary_v1", rotary()
+    ok(op, **kw)
+    ok(op, **{**kw, "positions": None})
+    ok(op, **{**kw, "layout": fe.ROTARY_INTERLEAVED, "backward": 1, "scale": -2.0})
+    ok(op, **{**kw, "kv_heads": 0, "k": None, "k_output": None})
+    ok(op, **{**kw, "heads": 0, "q": None, "q_output": None})
+    ok(op, **{**kw, "rotary_dim": 0, "frequencies": None})
+    ok(op, **rotary(tokens=0))
+    for bad in (dict(dim=0), dict(dim=24), dict(dim=272), dict(rotary_dim=31), dict(rotary_dim=66), dict(layout=2), dict(dtype=2), dict(backward=2),
+                dict(scale=math.nan), dict(scale=math.inf), dict(heads=65537)):
+        assert err(op, **{**kw, **bad}) == "UnsupportedShape", bad
+    for name, n in (("q", 5 * 4 * 64 - 1), ("k", 5 * 2 * 64 + 1), ("positions", 4), ("frequencies", 15), ("q_output", 64), ("k_output", 64)):
+        assert err(op, **{**kw, name: sl(20, n)}) == "Length", name
+    assert err(op, **{**kw, "q": sl(0, 5 * 4 * 64, 2)}) == "Alignment"
+    ok(op, **{**kw, "q": sl(0, 5 * 4 * 64, 2), "dtype": fe.DTYPE_BF16})
+    # in place with the same strides, and with no others
+    ok(op, **{**kw, "q_output": kw["q"], "k_output": kw["k"]})
+    head_major = {"q_output_token_stride": 64, "q_output_head_stride": 320}
+    ok(op, **{**kw, **head_major})
+    assert err(op, **{**kw, "q_output": kw["q"], **head_major}) == "OutputAliasesInput"
+    assert err(op, **{**kw, "q_output": kw["k_output"]}) == "Length"
+    assert err(op, **{**kw, "q_output": (kw["k_output"][0], 5 * 4 * 64)}) == "OutputAliasesInput"
+    assert err(op, **{**kw, "q_output_token_stride": 128, "q_output": sl(4, 4 * 128 + 256)}) == "UnsupportedShape"   # rows that meet
+    ok(op, **{**kw, "q_token_stride": 0, "q": sl(0, 256)})                                                          # one row for all tokens
+
+
+def test_rotary_rows_inside_fused_ones():
+    """[q | k | v] in one array: turned where they lie, or one array of turned rows; rows that meet are refused."""
+    op, kw = "rotary_v1", rotary()
+    ts, n = 8 * 64, 4 * 8 * 64
+    strides = {k: ts for k in kw if k.endswith("token_stride")}
+    fused = {**kw, **strides, "q": sl(0, n + 256), "k": sl(0, n + 128, 256 * 4)}
+    ok(op, **{**fused, "q_output": fused["q"], "k_output": fused["k"]})
+    ok(op, **{**fused, "q_output": sl(4, n + 256), "k_output": sl(4, n + 128, 256 * 4)})
+    ok(op, **{**fused, "q_output": sl(4, n + 256, 128 * 4), "k_output": sl(4, n + 128)})             # k first
+    assert err(op, **{**fused, "q_output": sl(4, n + 256), "k_output": sl(4, n + 128, 255 * 4)}) == "OutputAliasesInput"
+    assert err(op, **{**fused, "q_output": sl(4, n + 256), "k_output": sl(4, n + 128, 385 * 4)}) == "OutputAliasesInput"   # into the next token's
+    assert err(op, **{**fused, "q_output": fused["q"], "k_output": sl(5, n + 128)}) == "OutputAliasesInput"   # k is read between rows that are written
+    assert err(op, **{**fused, "q_output": sl(4, n + 256), "k_output": sl(4, n + 128, 256 * 4), "positions": sl(4, 5, 400 * 4)}) == "OutputAliasesInput"
+
+
+def four(pages_=10, kv_heads=2, dim=64, page=16, batch=3, width=4):
+    n = pages_ * kv_heads * page
+    return dict(k_cache=sl(24, n * dim * 9 // 16), v_cache=sl(32, n * dim * 9 // 16), k_scales=sl(40, n), v_scales=sl(41, n), page_table=sl(42, batch * width),
+                lengths=sl(43, batch), batch=batch, kv_heads=kv_heads, dim=dim, page_size=page, table_width=width, format=fe.KV_E2M1)
+
+
+@pytest.mark.parametrize("op,more", ALL)
+def test_four_bit_caches(op, more):
+    rest = {k: (v[0] + (64 << 20), v[1]) if isinstance(v, tuple) else v for k, v in more().items()}
+    kw = {**four(), **rest}
+    ok(op, **kw)
+    n = 10 * 2 * 16
+    for bad in (dict(dim=48), dict(dim=16), dict(dim=288), dict(page_size=12), dict(page_size=1), dict(format=3), dict(format=5)):
+        assert err(op, **{**kw, **bad}) == "UnsupportedShape", bad
+    assert err(op, **{**kw, "k_cache": sl(24, n * 64 // 2)}) == "Length"              # codes without their block scales
+    assert err(op, **{**kw, "v_cache": sl(32, n * 36 - 36 * 32)}) == "Length"
+    assert err(op, **{**kw, "k_scales": sl(40, n - 1)}) == "Length"
+    assert err(op, **{**kw, "k_scales": sl(40, n, 4)}) == "Alignment"
+    assert err(op, **{**kw, "v_scales": sl(41, n, 8)}) == "Alignment"
+    assert err(op, **{**kw, "k_cache": sl(24, n * 36, 8)}) == "Alignment"
+
+
+@pytest.mark.parametrize("cache", ["bf16", "e2m1"])
+def test_rotary_append(cache):
+    op = "kv_cache_rotary_append_v1"
+    base = {k: v for k, v in four().items() if k not in ("page_table", "lengths", "batch", "table_width")}
+    if cache == "bf16":
+        base.update(format=fe.KV_BF16, k_cache=sl(24, 10 * 2 * 16 * 64), v_cache=sl(32, 10 * 2 * 16 * 64), k_scales=None, v_scales=None)
+    r = rotary()
+    kw = {**base, **{k: v for k, v in r.items() if not k.startswith("k_output") and k not in ("dtype", "backward", "kv_heads", "dim")}}
+    kw.update(v=sl(12, 5 * 2 * 64), v_token_stride=128, v_head_stride=64, slots=sl(13, 5), input_dtype=fe.DTYPE_F32)
+    ok(op, **kw)
+    ok(op, **{**kw, "rotary_dim": 0, "frequencies": None, "positions": None})
+    ok(op, **{**kw, "heads": 0, "q": None, "q_output": None})
+    for bad in (dict(rotary_dim=33), dict(rotary_dim=66), dict(layout=2), dict(input_dtype=2), dict(scale=math.nan), dict(format=3), dict(heads=70000), dict(dim=24)):
+        assert err(op, **{**kw, **bad}) == "UnsupportedShape", bad
+    for name, n in (("q", 1), ("k", 1), ("v", 1), ("slots", 4), ("positions", 6), ("frequencies", 17), ("q_output", 1), ("k_cache", 100)):
+        assert err(op, **{**kw, name: sl(50, n)}) == "Length", name
+    assert err(op, **{**kw, "positions": None}) == "Length"
+    for name in ("q", "k", "v", "slots"):
+        assert err(op, **{**kw, "q_output": (kw[name][0], kw["q_output"][1])}) == "OutputAliasesInput", name
+    assert err(op, **{**kw, "v": (kw["k_cache"][0], kw["v"][1])}) == "OutputAliasesInput"
+    assert err(op, **{**kw, "v_cache": kw["k_cache"]}) == "OutputAliasesInput"
+    assert err(op, **{**kw, "q_output_token_stride": 100, "q_output": sl(4, 4 * 100 + 256)}) == "UnsupportedShape"
