@@ -732,8 +732,8 @@ int regions_for(uint32_t op, const void *args, Region *r, int32_t *status) {
         case OP_KV_PAGES: {
             const fe2o3_kv_pages_v1_args *a = static_cast<const fe2o3_kv_pages_v1_args *>(args);
             const uint64_t pages = a->free_pages.len, entries = (uint64_t)a->batch * a->table_width;
-            if (a->batch > 16384 || a->page_size == 0 || entries > 0xffffffffull || pages > 0xffffffffull / a->page_size) {
-                *status = unsupported("kv_pages_v1 needs batch <= 16384, page_size >= 1, batch * table_width and the rows of all pages below 2^32");
+            if (a->batch > 8192 || a->page_size == 0 || entries > 0xffffffffull || pages > 0xffffffffull / a->page_size) {
+                *status = unsupported("kv_pages_v1 needs batch <= 8192, page_size >= 1, batch * table_width and the rows of all pages below 2^32");
                 return 0;
             }
             int n = 0;

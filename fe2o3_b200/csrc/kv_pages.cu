@@ -10,7 +10,7 @@
 
 namespace {
 
-constexpr uint32_t kMaxThreads = 1024, kBlocks = 8, kAtOnce = 4;   // tokens a thread writes at once
+constexpr uint32_t kMostSequences = 8192, kMaxThreads = 1024, kBlocks = 8, kAtOnce = 4;   // tokens a thread writes at once
 
 struct PagesArgs {
     const uint32_t *counts, *release, *lengths, *free_count;
@@ -45,14 +45,15 @@ __device__ __forceinline__ Sequence sequence_of(const PagesArgs &a, uint32_t b) 
     return s;
 }
 
-struct Sums {
-    uint64_t back, fresh, tokens;
+struct Sums {   // (pages of sequences that fit are fewer than the table's entries, which 32 bits count)
+    uint32_t back, fresh;
+    uint64_t tokens;
     __device__ __forceinline__ Sums operator+(const Sums &o) const { return {back + o.back, fresh + o.fresh, tokens + o.tokens}; }
 };
 
 // What a sequence's pages and tokens are found by, in shared memory.
 struct Place {
-    uint32_t length, first_page, first_token;
+    uint32_t length, first_page, first_token, first_back;
 };
 
 __global__ void __launch_bounds__(kMaxThreads) kv_pages_kernel(PagesArgs a) {
@@ -74,7 +75,7 @@ __global__ void __launch_bounds__(kMaxThreads) kv_pages_kernel(PagesArgs a) {
         Sequence s{0, 0, 0, 0, 0, true};
         if (b < a.batch) s = sequence_of(a, b);
         if (!s.fits) bad = 1;
-        const Sums own{s.back, s.need >= s.held ? s.need - s.held : 0, s.count};
+        const Sums own{s.fits ? s.back : 0, s.fits ? s.need - s.held : 0, s.count};
         Sums sum = own;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
@@ -86,7 +87,7 @@ __global__ void __launch_bounds__(kMaxThreads) kv_pages_kernel(PagesArgs a) {
         Sums before = carry;
         for (uint32_t w = 0; w < warp; ++w) before = before + warps[w];
         sum = before + sum;
-        if (b < a.batch) places[b] = Place{s.length, (uint32_t)(sum.fresh - own.fresh), (uint32_t)(sum.tokens - own.tokens)};
+        if (b < a.batch) places[b] = Place{s.length, sum.fresh - own.fresh, (uint32_t)(sum.tokens - own.tokens), sum.back - own.back};
         __syncthreads();
         if (threadIdx.x == blockDim.x - 1) carry = sum;
     }
@@ -97,31 +98,21 @@ __global__ void __launch_bounds__(kMaxThreads) kv_pages_kernel(PagesArgs a) {
     const bool fits = !too_long && top <= a.pages && total.fresh <= top;
     if (!fits && thread == 0) kstatus_set(a.status, too_long ? FE2O3_KSTATUS_LENGTH : FE2O3_KSTATUS_PAGES);
 
-    // the released pages, sequence by sequence: one warp each (their places on the stack need the running sums again)
-    if (fits && total.back) {
-        uint64_t behind = count;
-        for (uint32_t b0 = 0; b0 < a.batch; b0 += 32) {   // every warp runs over all of them, 32 at a time
-            const uint32_t b = b0 + lane;
-            const uint32_t back = b < a.batch && a.release[b] ? pages_for(a, a.lengths[b]) : 0;
-            uint32_t upto = back;
-#pragma unroll
-            for (int d = 1; d < 32; d <<= 1) {
-                const uint32_t u = __shfl_up_sync(~0u, upto, d);
-                if (lane >= d) upto += u;
-            }
-            uint32_t left = __ballot_sync(~0u, back != 0);
-            while (left) {
-                const int l = __ffs(left) - 1;
-                left &= left - 1;
-                const uint32_t n = __shfl_sync(~0u, back, l), end = __shfl_sync(~0u, upto, l);
-                if ((b0 + l) % (threads >> 5) != thread >> 5) continue;
-                const uint32_t *const row = a.table + (uint64_t)(b0 + l) * a.width;
-                uint32_t *const to = a.free_pages + behind + end;   // the last entry first
-                for (uint32_t i = lane; i < n; i += 32) to[-1 - (int64_t)i] = row[i];
-            }
-            behind += __shfl_sync(~0u, upto, 31);
+    // the last sequence that begins at or before x
+    auto find = [&](uint32_t x, uint32_t Place::*first) {
+        uint32_t low = 0, high = a.batch;
+        while (high - low > 1) {
+            const uint32_t mid = (low + high) / 2;
+            if (places[mid].*first <= x) low = mid;
+            else high = mid;
         }
-    }
+        return low;
+    };
+    if (fits)   // the released pages: place i on the stack, of a row of n entries, is its entry n - 1 - i
+        for (uint32_t i = thread; i < total.back; i += threads) {
+            const uint32_t b = find(i, &Place::first_back), end = b + 1 < a.batch ? places[b + 1].first_back : total.back;
+            a.free_pages[count + i] = a.table[(uint64_t)b * a.width + (end - 1 - i)];
+        }
     if (gridDim.x > 1) {
         __threadfence();
         cluster_sync();
@@ -138,16 +129,6 @@ __global__ void __launch_bounds__(kMaxThreads) kv_pages_kernel(PagesArgs a) {
         else if (a.next_lengths != a.lengths) a.next_lengths[b] = a.lengths[b];
         if (a.offsets) a.offsets[b] = fits ? places[b].first_token : 0;
     }
-    // the last sequence that begins at or before x
-    auto find = [&](uint32_t x, uint32_t Place::*first) {
-        uint32_t low = 0, high = a.batch;
-        while (high - low > 1) {
-            const uint32_t mid = (low + high) / 2;
-            if (places[mid].*first <= x) low = mid;
-            else high = mid;
-        }
-        return low;
-    };
     if (fits)
         for (uint32_t i = thread; i < total.fresh; i += threads) {
             const uint32_t b = find(i, &Place::first_page);
@@ -190,7 +171,7 @@ int32_t launch_kv_pages(fe2o3_ctx *ctx, cudaStream_t s, const void *args, fe2o3_
     if (geo) *geo = fe2o3_geometry{{grid, 1, 1}, {threads, 1, 1}, shared, 1};
     if (plan_only) {
         FE2O3_CUDA(cudaSetDevice(ctx->device));
-        FE2O3_CUDA(cudaFuncSetAttribute(reinterpret_cast<const void *>(kv_pages_kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, 16384 * sizeof(Place)));
+        FE2O3_CUDA(cudaFuncSetAttribute(reinterpret_cast<const void *>(kv_pages_kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, kMostSequences * sizeof(Place)));
         return FE2O3_OK;
     }
     int32_t shift = -1;

@@ -78,6 +78,7 @@ namespace {
 constexpr int kWeightExponent = 15;
 constexpr float kLeastWeight = 0x1p-112f, kMostWeight = 0x1.fffffep125f;   // the largest weight is held in between: powers of two and their reciprocals stay normal numbers
 constexpr float kLeastTerm = 0x1p-40f;   // of a number, the least that its lower bf16 terms are: far below its last bit, and nothing where it is 0
+constexpr float kSlack = 8.f;          // 4 bits: what a score may lie above the maximum kept (log2) before that moves: a probability is up to 2^8 then
 constexpr int kQueryExponent = 14;    // f16 queries: the largest of a row lies in [2^14, 2^15)
 
 template <uint32_t FORMAT, int DP, int NT>
@@ -474,6 +475,14 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     };
     uint32_t entry = 0, entries_from = 0, entries_of = ~0u;   // 32 entries of a sequence's table, a lane each
     const uint32_t lrow = lane / kPieces, lpiece = lane % kPieces, boxes = KT / a.box;
+    // 4 bits: six copies a box, of rows, row scales and block scales.  Eight lanes take the boxes, four such sets the kinds: K's and V's row scales
+    // and block scales, and two of them the rows.  (One lane after another, as with the other formats, is 120 instructions a tile more.)
+    const uint32_t lbox = F4 ? lane & 7 : lane, lset = lane >> 3;
+    const uint8_t *const scales_from = !F4 ? nullptr : lset == 0 ? reinterpret_cast<const uint8_t *>(a.c.k_scales) : lset == 1 ? reinterpret_cast<const uint8_t *>(a.c.v_scales)
+                                                     : (lset == 2 ? a.c.k : a.c.v) + a.c.blocks;
+    const uint32_t scales_row = lset < 2 ? 4 : row_blocks;   // bytes
+    const uint32_t scales_to = (lset < 2 ? lset * 4 * KT : 8 * KT + (lset & 1) * S::kBlocks) + lbox * a.box * scales_row;
+    const CUtensorMap *const lmap = lset & 1 ? &map_v : &map_k;
     // Zeros for a row of a stage: K and V, and their scales.
     auto no_row = [&](uint32_t slot, uint32_t r, bool k_too) {
         for (uint32_t i = lane; i < 2 * kPieces; i += 32)
@@ -501,7 +510,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         }
         if (ltile >= lend) return;
         // a lane a box, or a row
-        const uint32_t key = lspan.key(ltile) + min(lane, boxes - 1) * a.box, head = litem / a.chunks;
+        const uint32_t key = lspan.key(ltile) + min(lbox, boxes - 1) * a.box, head = litem / a.chunks;
         const uint32_t at = a.page_shift >= 0 ? key >> a.page_shift : key / a.c.page_size;   // in the table
         const uint32_t first_at = __shfl_sync(~0u, at, 0), last_at = __shfl_sync(~0u, at, 31);
         if (entries_of != lseq || first_at < entries_from || last_at >= entries_from + 32) {
@@ -511,15 +520,21 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
             if (entries_from + lane < a.c.table_width) entry = a.c.page_table[(uint64_t)lseq * a.c.table_width + entries_from + lane];
         }
         const uint32_t page = __shfl_sync(~0u, entry, at - entries_from), in_page = key - at * a.c.page_size;
-        const bool wanted = lane < boxes && key < lspan.n && key + a.box > lspan.first, there = wanted && page < a.c.pages;
+        const bool wanted = lbox < boxes && key < lspan.n && key + a.box > lspan.first, there = wanted && page < a.c.pages;
         if (wanted && !there) kstatus_set(a.c.status, FE2O3_KSTATUS_SLOT_RANGE);
-        const uint32_t found = __ballot_sync(~0u, there);
+        const uint32_t found = __ballot_sync(~0u, there) & (F4 ? 0xffu : ~0u);
         uint64_t *const bar = &bars[lslot];
         const uint32_t row = there ? (page * a.c.kv_heads + head) * a.c.page_size + in_page : ~0u;
         if (a.box > 1) {
             if (lane == 0) mbar_arrive_expect_tx(bar, __popc(found) * a.box * (2 * S::kRow + (F16 ? 8 : 0) + (F4 ? 2 * row_blocks : 0)));
             __syncwarp();
-            if (there) {
+            if (F4) {
+                if (there) {
+                    bulk_load_1d(my_scales + lslot * S::kScales + scales_to, scales_from + (uint64_t)row * scales_row, a.box * scales_row, bar);
+                    if (lset < 2)
+                        tma_load_3d(my_ring + lslot * S::kStage + lset * (KT * S::kRow) + lbox * a.box * S::kPitch, lmap, bar, 0, in_page, page * a.c.kv_heads + head);
+                }
+            } else if (there) {
                 uint8_t *const to = my_ring + lslot * S::kStage + lane * a.box * S::kPitch;
 #pragma unroll
                 for (int half = 0; half < S::kRow / S::kPitch; ++half) {
@@ -530,12 +545,6 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                     uint8_t *const scales = my_scales + lslot * S::kScales + lane * a.box * 4;
                     bulk_load_1d(scales, a.c.k_scales + row, a.box * 4, bar);
                     bulk_load_1d(scales + KT * 4, a.c.v_scales + row, a.box * 4, bar);
-                }
-                if constexpr (F4) {
-                    uint8_t *const blocks = my_scales + lslot * S::kScales + 8 * KT + lane * a.box * row_blocks;
-                    const uint64_t from = a.c.blocks + (uint64_t)row * row_blocks;
-                    bulk_load_1d(blocks, a.c.k + from, a.box * row_blocks, bar);
-                    bulk_load_1d(blocks + S::kBlocks, a.c.v + from, a.box * row_blocks, bar);
                 }
             }
             __syncwarp();
@@ -785,6 +794,13 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         float heaviest[NT][2];   // 8-bit caches: the largest weight of a head so far, as p.m is the largest score
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) heaviest[nt][0] = heaviest[nt][1] = kLeastWeight;
+        float unit4[NT][2];      // 4 bits: of the weights, and the maxima with a minus, as the last tiles left them
+        uint64_t minus4[NT];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            unit4[nt][0] = unit4[nt][1] = __uint_as_float(0x7f000000u - __float_as_uint(above(kLeastWeight)) + (kWeightExponent << 23));
+            minus4[nt] = 0;
+        }
         for (uint32_t tile = max(place, kEnd) - kEnd; tile < last_tile; ++tile) {
             if (waiting && !mbar_wait_warp(&bars[slot], phase)) {   // (not seen: a copy that never lands)
                 if (lane == 0) kstatus_set(a.c.status, FE2O3_KSTATUS_WAIT_EXPIRED);
@@ -976,7 +992,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
             }
 
             // the running maximum, in units of log2; weights
-            float vs[MT][2], vs_log[MT][2];
+            float vs[MT][2], vs_log[MT][2];   // (4 bits: no logarithms)
             if constexpr (F16) {
                 const uint32_t scales = smem_u32(my_scales) + slot * S::kScales + 4 * gk;
 #pragma unroll
@@ -985,7 +1001,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                     for (int e = 0; e < 2; ++e) {
                         const float ks = lds_f32(scales + 4 * (16 * mt + 8 * e));
                         vs[mt][e] = lds_f32(scales + 4 * KT + 4 * (16 * mt + 8 * e));
-                        vs_log[mt][e] = lg2_approx(vs[mt][e]);   // (of 0 the lowest there is: such a row weighs nothing)
+                        if constexpr (!F4) vs_log[mt][e] = lg2_approx(vs[mt][e]);   // (of 0 the lowest there is: such a row weighs nothing)
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {
                             float (&x)[4] = s[mt][nt];
@@ -1017,6 +1033,80 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                 for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) top[e] = max3(top[e], s[mt][nt][e], s[mt][nt][e + 2]);
+                if constexpr (F4) {
+                    // Once some tiles are done, a tile seldom moves a maximum or a unit: the lanes look at what they have themselves, and only where
+                    // one of them finds more do they compare notes.  (The 8-bit order, both trees at every tile: see below.)
+                    float keep[2] = {1.f, 1.f};
+                    const bool higher = __any_sync(~0u, top[0] > p.m[nt][0] + kSlack || top[1] > p.m[nt][1] + kSlack);
+                    if (higher) {
+                        float base[2];
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+#pragma unroll
+                            for (int d = 4; d < 32; d <<= 1) top[e] = fmaxf(top[e], __shfl_xor_sync(~0u, top[e], d));
+                            base[e] = top[e] == -INFINITY ? 0.f : top[e];
+                            keep[e] = ex2_approx(p.m[nt][e] - base[e]);
+                            p.m[nt][e] = top[e];
+                            p.l[nt][e] *= keep[e];
+                        }
+                        minus4[nt] = pack_f32x2(-base[0], -base[1]);
+                    }
+                    float w[MT][4], z[MT][4], largest[2] = {0.f, 0.f};
+                    auto weigh = [&] {   // (in this order: a scale of no weight may be beyond f32 in these units)
+#pragma unroll
+                        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                            for (int e = 0; e < 4; e += 2)
+                                unpack_f32x2(mul_f32x2(mul_f32x2(pack_f32x2(w[mt][e], w[mt][e + 1]), pack_f32x2(unit4[nt][0], unit4[nt][1])), pack_f32x2(vs[mt][e / 2], vs[mt][e / 2])),
+                                             z[mt][e], z[mt][e + 1]);
+                    };
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                        for (int e = 0; e < 4; e += 2) {
+                            float x0, x1;
+                            unpack_f32x2(add_f32x2(pack_f32x2(s[mt][nt][e], s[mt][nt][e + 1]), minus4[nt]), x0, x1);
+                            w[mt][e] = ex2_approx(x0);
+                            w[mt][e + 1] = ex2_approx(x1);
+                            unpack_f32x2(add_f32x2(pack_f32x2(p.l[nt][0], p.l[nt][1]), pack_f32x2(w[mt][e], w[mt][e + 1])), p.l[nt][0], p.l[nt][1]);
+                        }
+                    weigh();
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) largest[e] = max3(largest[e], z[mt][e], z[mt][e + 2]);
+                    constexpr float kFull = 65504.f;   // f16's largest number: an octave above where the largest weight is put
+                    scale_o[nt] = pack_f32x2(1.f, 1.f);
+                    if (higher || __any_sync(~0u, largest[0] >= kFull || largest[1] >= kFull)) {
+                        float by[2];
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            float most = 0.f;
+#pragma unroll
+                            for (int mt = 0; mt < MT; ++mt) most = max3(most, w[mt][e] * vs[mt][0], w[mt][e + 2] * vs[mt][1]);
+#pragma unroll
+                            for (int d = 4; d < 32; d <<= 1) most = fmaxf(most, __shfl_xor_sync(~0u, most, d));
+                            const float before = keep[e] * above(heaviest[nt][e]);
+                            heaviest[nt][e] = fminf(fmaxf(fmaxf(heaviest[nt][e] * keep[e], most), kLeastWeight), kMostWeight);
+                            const uint32_t inverse = 0x7f000000u - __float_as_uint(above(heaviest[nt][e]));
+                            by[e] = before * __uint_as_float(inverse);
+                            unit4[nt][e] = __uint_as_float(inverse + (kWeightExponent << 23));
+                        }
+                        scale_o[nt] = pack_f32x2(by[0], by[1]);
+                        weigh();
+                    }
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const float w0 = z[mt][2 * e], w1 = z[mt][2 * e + 1];
+                            const uint32_t hi = f16_pair(w0, w1);
+                            pb[mt][nt][0][e] = turned(hi);
+                            const float2 h = f16_values(hi);
+                            pb[mt][nt][1][e] = turned(f16_pair(w0 - h.x, w1 - h.y));
+                        }
+                    continue;
+                }
                 float base[2], keep[2], unit[2];
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {

@@ -26,9 +26,9 @@ struct RotaryRows {
     const float *frequencies;
     uint32_t tokens, heads, rows;      // rows of a token: heads, then kv_heads of k (and of v)
     uint32_t per_block, parts;         // tokens of a block; blocks that share them
-    uint32_t dim, kv_heads, pairs, lanes_log2, half;   // half: of the turned columns, in pieces; 0: partners one by one
+    uint32_t dim, kv_heads, pairs, lanes_log2;
+    uint32_t groups, token_turns;      // pieces whose pairs lie together (see turn_at); places of a token's sines and cosines
     uint32_t rows_inverse;             // 2^32 / rows rounded up, or 0
-    bool interleaved;
     float scale, sign;
 };
 
@@ -102,13 +102,25 @@ __device__ __forceinline__ void store_row(const KvCache &c, float (&x)[2 * kPiec
     }
 }
 
+// How pairs lie: halves whose partners lie in pieces of their own (kPieces) or anywhere (kAnywhere), or neighbours.
+enum : int { kPieces, kAnywhere, kNeighbours };
+
+// Where the sine and cosine of pair i lie among those of a token.  A lane takes two at once, its pairs of one piece (PAIRS of them), and the
+// lanes of a row take the same two of theirs at the same time: those lie side by side.
+template <int MODE, int PAIRS>
+__device__ __forceinline__ uint32_t turn_at(uint32_t i, uint32_t groups) {
+    if constexpr (MODE == kAnywhere) return i;
+    else return (i % PAIRS / 2 * groups + i / PAIRS) * 2 + (i & 1);
+}
+
 // WHOLE: the rows start on 16 bytes.
-template <uint32_t FORMAT, bool F32, bool WHOLE>
-__global__ void __launch_bounds__(kThreads) rotary_kernel(KvCache c, RotaryRows r) {
-    constexpr int kEb = F32 ? 4 : 2, kPiece = 16 / kEb, kDeep = 2;
+template <uint32_t FORMAT, bool F32, int MODE, bool WHOLE>
+__global__ void __launch_bounds__(kThreads, FORMAT == kPlain || FORMAT == FE2O3_KV_BF16 ? 4 : 3) rotary_kernel(KvCache c, RotaryRows r) {
+    constexpr int kEb = F32 ? 4 : 2, kPiece = 16 / kEb, kDeep = 2, kPairs = MODE == kNeighbours ? kPiece / 2 : kPiece;
     constexpr bool kCache = FORMAT != kPlain;
-    extern __shared__ float2 turns[];   // [tokens of the block][pairs]
+    extern __shared__ float4 table[];              // [tokens of the block][pairs]; then the rows in flight, where partners lie anywhere
     __shared__ uint32_t first_rows[kMostTokens];   // in the cache, of head 0; ~0: a token that is left out
+    float2 *const turns = reinterpret_cast<float2 *>(table);
     begin_after_previous();
     const uint32_t part = blockIdx.x % r.parts, t0 = blockIdx.x / r.parts * r.per_block, n = min(r.per_block, r.tokens - t0);
     if (kCache && threadIdx.x < n) {
@@ -118,27 +130,24 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(KvCache c, RotaryRows 
         first_rows[threadIdx.x] = there && slot != FE2O3_SLOT_NONE ? page * c.kv_heads * c.page_size + (slot - page * c.page_size) : ~0u;
     }
     for (uint32_t i = threadIdx.x; i < n * r.pairs; i += kThreads) {
-        const uint32_t t = i / r.pairs;
-        turns[i] = turn_of(r.positions ? r.positions[t0 + t] : t0 + t, r.frequencies[i - t * r.pairs], r.scale, r.sign);
+        const uint32_t t = i / r.pairs, pair = i - t * r.pairs;
+        turns[t * r.token_turns + turn_at<MODE, kPairs>(pair, r.groups)] = turn_of(r.positions ? r.positions[t0 + t] : t0 + t, r.frequencies[pair], r.scale, r.sign);
     }
     __syncthreads();
 
     const uint32_t lanes = 1u << r.lanes_log2, at_once = kThreads >> r.lanes_log2, l = threadIdx.x & (lanes - 1);
-    // a lane's columns: two pieces, the partners of one another where there are any
-    const uint32_t pieces = r.dim / kPiece, rest = (pieces - 2 * r.half) / 2;   // rest: half of those that are not turned (half 0: of all)
-    uint32_t first[2];
-    const bool pair = l < r.half;
-    first[0] = kPiece * (pair ? l : r.half + l);
-    first[1] = kPiece * (pair ? l + r.half : r.half + l + rest);
-    const bool in = l < pieces / 2, inside[2] = {in, in};
+    // a lane's columns: two pieces, the partners of one another where pairs allow
+    const uint32_t pieces = r.dim / kPiece, paired = MODE == kPieces ? r.groups : 0, rest = (pieces - 2 * paired) / 2;   // rest: half of the other pieces
+    const bool pair = l < paired, in = l < pieces / 2;
+    const uint32_t first[2] = {kPiece * (pair ? l : paired + l), kPiece * (pair ? l + paired : paired + l + rest)};
+    const bool inside[2] = {in, in};
+    uint8_t *const scratch = reinterpret_cast<uint8_t *>(turns + (uint64_t)r.per_block * r.token_turns) + (threadIdx.x >> r.lanes_log2) * kDeep * r.dim * kEb;
     const uint32_t total = n * r.rows, share = (total + r.parts - 1) / r.parts, end = min(total, (part + 1) * share);
     for (uint32_t base = part * share; base < end; base += kDeep * at_once) {
         const uint32_t mine = base + (threadIdx.x >> r.lanes_log2);
         uint4 raw[kDeep][2];
-        float others[kDeep][2 * kPiece];
         uint32_t token[kDeep], head[kDeep], what[kDeep];
         bool active[kDeep];
-        const uint8_t *at[kDeep];
 #pragma unroll
         for (int d = 0; d < kDeep; ++d) {
             const uint32_t i = min(mine + d * at_once, end - 1);
@@ -151,25 +160,25 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(KvCache c, RotaryRows 
                 head[d] -= r.kv_heads;
             }
             active[d] = mine + d * at_once < end && (!kCache || first_rows[token[d]] != ~0u);
-            at[d] = r.from[what[d]] + ((uint64_t)(t0 + token[d]) * r.token_stride[what[d]] + (uint64_t)head[d] * r.head_stride[what[d]]) * kEb;
             raw[d][0] = raw[d][1] = make_uint4(0, 0, 0, 0);
             if (active[d] && in) {
+                const uint32_t ts = what[d] == 0 ? r.token_stride[0] : what[d] == 1 ? r.token_stride[1] : r.token_stride[2];
+                const uint32_t hs = what[d] == 0 ? r.head_stride[0] : what[d] == 1 ? r.head_stride[1] : r.head_stride[2];
+                const uint8_t *const at = (what[d] == 0 ? r.from[0] : what[d] == 1 ? r.from[1] : r.from[2]) + ((uint64_t)(t0 + token[d]) * ts + (uint64_t)head[d] * hs) * kEb;
 #pragma unroll
-                for (int half = 0; half < 2; ++half) raw[d][half] = fetch<F32, WHOLE>(at[d] + first[half] * kEb);
-                if (!r.half && !r.interleaved && what[d] < 2) {
-#pragma unroll
-                    for (int i = 0; i < 2 * kPiece; ++i) {
-                        const uint32_t column = first[i / kPiece] + i % kPiece;
-                        others[d][i] = 0.f;
-                        if (column >= 2 * r.pairs) continue;
-                        const uint8_t *const e = at[d] + (column < r.pairs ? column + r.pairs : column - r.pairs) * kEb;
-                        if constexpr (F32) others[d][i] = *reinterpret_cast<const float *>(e);
-                        else others[d][i] = bf16_bits_to_f32(*reinterpret_cast<const uint16_t *>(e));
-                    }
-                }
+                for (int half = 0; half < 2; ++half) raw[d][half] = fetch<F32, WHOLE>(at + first[half] * kEb);
             }
         }
-        __syncwarp();   // in place: every lane has its columns and their partners before one writes
+        if constexpr (MODE == kAnywhere) {   // the rows, for partners to be looked up (a row's lanes are of one warp)
+            __syncwarp();
+#pragma unroll
+            for (int d = 0; d < kDeep; ++d)
+                if (in) {
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) *reinterpret_cast<uint4 *>(scratch + d * r.dim * kEb + first[half] * kEb) = raw[d][half];
+                }
+        }
+        __syncwarp();   // (and in place: every lane has its columns before one writes)
 #pragma unroll
         for (int d = 0; d < kDeep; ++d) {
             if (base + d * at_once >= end) break;
@@ -181,46 +190,58 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(KvCache c, RotaryRows 
                 else widen2(w, x + 2 * i);
             }
             const uint32_t turned = what[d] < 2 ? 2 * r.pairs : 0;
-            if (what[d] < 2 && in) {
-                const float2 *const cs = turns + token[d] * r.pairs;
-                if (r.interleaved) {
+            const float2 *const cs = turns + token[d] * r.token_turns;
+            if (MODE == kPieces && turned && pair) {
 #pragma unroll
-                    for (int i = 0; i < 2 * kPiece; i += 2) {
-                        const uint32_t column = first[i / kPiece] + i % kPiece;
-                        if (column >= 2 * r.pairs) continue;
-                        const float2 t = cs[column / 2];
-                        const float a = x[i], b = x[i + 1];
-                        x[i] = fmaf(a, t.x, -(b * t.y));
-                        x[i + 1] = fmaf(b, t.x, a * t.y);
-                    }
-                } else if (pair) {
+                for (int i = 0; i < kPiece; i += 2) {
+                    const float4 t = reinterpret_cast<const float4 *>(cs)[i / 2 * r.groups + l];
+                    const float a = x[i], b = x[kPiece + i], a1 = x[i + 1], b1 = x[kPiece + i + 1];
+                    x[i] = fmaf(a, t.x, -(b * t.y));
+                    x[kPiece + i] = fmaf(b, t.x, a * t.y);
+                    x[i + 1] = fmaf(a1, t.z, -(b1 * t.w));
+                    x[kPiece + i + 1] = fmaf(b1, t.z, a1 * t.w);
+                }
+            }
+            if (MODE == kNeighbours && in) {
 #pragma unroll
-                    for (int i = 0; i < kPiece; ++i) {
-                        const float2 t = cs[first[0] + i];
-                        const float a = x[i], b = x[kPiece + i];
-                        x[i] = fmaf(a, t.x, -(b * t.y));
-                        x[kPiece + i] = fmaf(b, t.x, a * t.y);
-                    }
-                } else if (!r.half) {
+                for (int half = 0; half < 2; ++half)
 #pragma unroll
-                    for (int i = 0; i < 2 * kPiece; ++i) {
-                        const uint32_t column = first[i / kPiece] + i % kPiece;
-                        if (column >= 2 * r.pairs) continue;
-                        const bool low = column < r.pairs;
-                        const float2 t = cs[low ? column : column - r.pairs];
-                        x[i] = low ? fmaf(x[i], t.x, -(others[d][i] * t.y)) : fmaf(x[i], t.x, others[d][i] * t.y);
+                    for (int i = 0; i < kPiece; i += 4) {
+                        if (first[half] + i >= turned) continue;   // (turned columns end with a pair, the second of two or the first)
+                        const float4 t = reinterpret_cast<const float4 *>(cs)[i / 4 * r.groups + first[half] / kPiece];
+                        float *const y = x + half * kPiece + i;
+                        const float a = y[0], b = y[1], a1 = y[2], b1 = y[3];
+                        y[0] = fmaf(a, t.x, -(b * t.y));
+                        y[1] = fmaf(b, t.x, a * t.y);
+                        if (first[half] + i + 2 >= turned) continue;
+                        y[2] = fmaf(a1, t.z, -(b1 * t.w));
+                        y[3] = fmaf(b1, t.z, a1 * t.w);
                     }
+            }
+            if (MODE == kAnywhere && in) {
+#pragma unroll
+                for (int i = 0; i < 2 * kPiece; ++i) {
+                    const uint32_t column = first[i / kPiece] + i % kPiece;
+                    if (column >= turned) continue;
+                    const bool low = column < r.pairs;
+                    const float2 t = cs[low ? column : column - r.pairs];
+                    const uint8_t *const e = scratch + d * r.dim * kEb + (low ? column + r.pairs : column - r.pairs) * kEb;
+                    float other;
+                    if constexpr (F32) other = *reinterpret_cast<const float *>(e);
+                    else other = bf16_bits_to_f32(*reinterpret_cast<const uint16_t *>(e));
+                    x[i] = low ? fmaf(x[i], t.x, -(other * t.y)) : fmaf(x[i], t.x, other * t.y);
                 }
             }
             if (kCache && what[d]) {
                 if constexpr (kCache) {
                     const uint32_t row = first_rows[token[d]] + head[d] * c.page_size;
-                    store_row<FORMAT, kPiece>(c, x, raw[d], turned, what[d] - 1, row, first, inside, l, lanes, active[d]);
+                    store_row<FORMAT, kPiece>(c, x, raw[d], turned, what[d] - 1, row, first, inside, l, lanes, active[d] && in);
                 }
                 continue;
             }
             if (!active[d] || !in) continue;
-            uint8_t *const to = r.to[what[d]] + ((uint64_t)(t0 + token[d]) * r.to_token_stride[what[d]] + (uint64_t)head[d] * r.to_head_stride[what[d]]) * kEb;
+            const uint32_t ts = !kCache && what[d] ? r.to_token_stride[1] : r.to_token_stride[0], hs = !kCache && what[d] ? r.to_head_stride[1] : r.to_head_stride[0];
+            uint8_t *const to = (!kCache && what[d] ? r.to[1] : r.to[0]) + ((uint64_t)(t0 + token[d]) * ts + (uint64_t)head[d] * hs) * kEb;
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
                 const float *const q = x + half * kPiece;
@@ -238,15 +259,25 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(KvCache c, RotaryRows 
 
 using Kernel = void (*)(KvCache, RotaryRows);
 
-int32_t launch_rows(fe2o3_ctx *ctx, cudaStream_t s, Kernel kernel, uint32_t eb, bool four, const KvCache &c, RotaryRows r, fe2o3_geometry *geo, bool plan_only,
-                    const char *what) {
+// kernels: [MODE][WHOLE] of the types at hand.
+int32_t launch_rows(fe2o3_ctx *ctx, cudaStream_t s, const Kernel (&kernels)[3][2], bool whole, bool interleaved, uint32_t eb, bool four, const KvCache &c, RotaryRows r,
+                    std::atomic<int> (&per_sm)[3][2], fe2o3_geometry *geo, bool plan_only, const char *what) {
     const uint32_t piece = 16 / eb;
     // Partners lie in pieces of their own where half of the turned columns is a whole number of pieces (4 bits: of blocks, which stay with
     // neighbouring lanes).
-    r.half = !r.interleaved && r.pairs % (four ? 16 : piece) == 0 ? r.pairs / piece : 0;
+    const int mode = interleaved ? kNeighbours : r.pairs % (four ? 16 : piece) == 0 ? kPieces : kAnywhere;
+    r.groups = mode == kNeighbours ? (2 * r.pairs + piece - 1) / piece : mode == kPieces ? r.pairs / piece : 0;
+    r.token_turns = mode == kNeighbours ? r.groups * (piece / 2) : (r.pairs + 1) & ~1u;
     while ((2 * piece << r.lanes_log2) < r.dim) ++r.lanes_log2;
     if (r.lanes_log2 == 0) r.lanes_log2 = 1;
-    const uint32_t sms = ctx->sm_count > 0 ? ctx->sm_count : 1, resident = sms * 6;
+    int fit = per_sm[mode][whole].load(std::memory_order_relaxed);
+    if (fit == 0) {
+        const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, kernels[mode][whole], kThreads, 16384);
+        if (e != cudaSuccess) return fe2o3_cuda_status(e, what);
+        if (fit < 1) fit = 1;
+        per_sm[mode][whole].store(fit, std::memory_order_relaxed);
+    }
+    const uint32_t resident = (ctx->sm_count > 0 ? ctx->sm_count : 1) * fit;
     r.per_block = 1;
     r.parts = 1;
     if (r.tokens >= resident) {
@@ -258,10 +289,11 @@ int32_t launch_rows(fe2o3_ctx *ctx, cudaStream_t s, Kernel kernel, uint32_t eb, 
         if (r.parts == 0) r.parts = 1;
     }
     r.rows_inverse = r.rows <= 1 || (uint64_t)r.per_block * r.rows > 65536 || r.rows > 65536 ? 0 : (uint32_t)((0x100000000ull + r.rows - 1) / r.rows);
-    const uint32_t grid = ceil_div_u32(r.tokens, r.per_block) * r.parts, shared = r.per_block * r.pairs * (uint32_t)sizeof(float2);
+    const uint32_t in_flight = mode == kAnywhere ? (kThreads >> r.lanes_log2) * 2 * r.dim * eb : 0;   // at most 16 KiB
+    const uint32_t grid = ceil_div_u32(r.tokens, r.per_block) * r.parts, shared = r.per_block * r.token_turns * (uint32_t)sizeof(float2) + in_flight;
     if (geo) *geo = fe2o3_geometry{{grid, 1, 1}, {kThreads, 1, 1}, shared, 1};
     if (plan_only || r.tokens == 0 || r.rows == 0) return FE2O3_OK;
-    const cudaError_t e = fe2o3_launch_early(kernel, grid, kThreads, shared, s, 1, c, r);
+    const cudaError_t e = fe2o3_launch_early(kernels[mode][whole], grid, kThreads, shared, s, 1, c, r);
     fe2o3_count_launch(1);
     return fe2o3_cuda_status(e, what);
 }
@@ -271,11 +303,15 @@ bool on_16(uint64_t bits, P... strides) { return ((bits | ... | strides) & 15u) 
 
 }  // namespace
 
-#define ROTARY_FORMAT(FORMAT) \
-    {{rotary_kernel<FORMAT, false, false>, rotary_kernel<FORMAT, false, true>}, {rotary_kernel<FORMAT, true, false>, rotary_kernel<FORMAT, true, true>}}
+#define ROTARY_MODES(FORMAT, F32)                                                                                        \
+    {{rotary_kernel<FORMAT, F32, kPieces, false>, rotary_kernel<FORMAT, F32, kPieces, true>},                            \
+     {rotary_kernel<FORMAT, F32, kAnywhere, false>, rotary_kernel<FORMAT, F32, kAnywhere, true>},                        \
+     {rotary_kernel<FORMAT, F32, kNeighbours, false>, rotary_kernel<FORMAT, F32, kNeighbours, true>}}
+#define ROTARY_FORMAT(FORMAT) {ROTARY_MODES(FORMAT, false), ROTARY_MODES(FORMAT, true)}
 
 int32_t launch_rotary(fe2o3_ctx *ctx, cudaStream_t s, const void *args, fe2o3_geometry *geo, bool plan_only) {
-    static const Kernel kernels[2][2] = ROTARY_FORMAT(kPlain);
+    static const Kernel kernels[2][3][2] = ROTARY_FORMAT(kPlain);
+    static std::atomic<int> per_sm[2][3][2];
     const fe2o3_rotary_v1_args *a = static_cast<const fe2o3_rotary_v1_args *>(args);
     const uint64_t eb = a->dtype == FE2O3_DTYPE_F32 ? 4 : 2;
     RotaryRows r{};
@@ -295,17 +331,17 @@ int32_t launch_rotary(fe2o3_ctx *ctx, cudaStream_t s, const void *args, fe2o3_ge
     r.rows = a->heads + a->kv_heads;
     r.dim = a->dim;
     r.pairs = a->rotary_dim / 2;
-    r.interleaved = a->layout == FE2O3_ROTARY_INTERLEAVED;
     r.scale = a->scale;
     r.sign = a->backward ? -1.f : 1.f;
     bool whole = true;
     if (a->heads) whole = on_16(a->q.ptr | a->q_output.ptr, eb * a->q_token_stride, eb * a->q_head_stride, eb * a->q_output_token_stride, eb * a->q_output_head_stride);
     if (a->kv_heads) whole = whole && on_16(a->k.ptr | a->k_output.ptr, eb * a->k_token_stride, eb * a->k_head_stride, eb * a->k_output_token_stride, eb * a->k_output_head_stride);
-    return launch_rows(ctx, s, kernels[eb == 4][whole], (uint32_t)eb, false, KvCache{}, r, geo, plan_only, "rotary_v1");
+    return launch_rows(ctx, s, kernels[eb == 4], whole, a->layout == FE2O3_ROTARY_INTERLEAVED, (uint32_t)eb, false, KvCache{}, r, per_sm[eb == 4], geo, plan_only, "rotary_v1");
 }
 
 int32_t launch_kv_cache_rotary_append(fe2o3_ctx *ctx, cudaStream_t s, const void *args, fe2o3_geometry *geo, bool plan_only) {
-    static const Kernel kernels[4][2][2] = {ROTARY_FORMAT(FE2O3_KV_BF16), ROTARY_FORMAT(FE2O3_KV_E4M3), ROTARY_FORMAT(FE2O3_KV_I8), ROTARY_FORMAT(FE2O3_KV_E2M1)};
+    static const Kernel kernels[4][2][3][2] = {ROTARY_FORMAT(FE2O3_KV_BF16), ROTARY_FORMAT(FE2O3_KV_E4M3), ROTARY_FORMAT(FE2O3_KV_I8), ROTARY_FORMAT(FE2O3_KV_E2M1)};
+    static std::atomic<int> per_sm[4][2][3][2];   // of each kernel, found once
     const fe2o3_kv_cache_rotary_append_v1_args *a = static_cast<const fe2o3_kv_cache_rotary_append_v1_args *>(args);
     const uint64_t eb = a->input_dtype == FE2O3_DTYPE_F32 ? 4 : 2;
     const bool four = a->format == FE2O3_KV_E2M1;
@@ -327,13 +363,13 @@ int32_t launch_kv_cache_rotary_append(fe2o3_ctx *ctx, cudaStream_t s, const void
     r.rows = a->heads + 2 * a->kv_heads;
     r.dim = a->dim;
     r.pairs = a->rotary_dim / 2;
-    r.interleaved = a->layout == FE2O3_ROTARY_INTERLEAVED;
     r.scale = a->scale;
     r.sign = 1.f;
     bool whole = on_16(a->k.ptr | a->v.ptr, eb * a->k_token_stride, eb * a->k_head_stride, eb * a->v_token_stride, eb * a->v_head_stride);
     if (a->heads) whole = whole && on_16(a->q.ptr | a->q_output.ptr, eb * a->q_token_stride, eb * a->q_head_stride, eb * a->q_output_token_stride, eb * a->q_output_head_stride);
-    return launch_rows(ctx, s, kernels[four ? 3 : a->format][eb == 4][whole], (uint32_t)eb, four, kv_storage_of(ctx, a), r, geo, plan_only, "kv_cache_rotary_append_v1");
+    const uint32_t format = four ? 3 : a->format;   // in the tables
+    return launch_rows(ctx, s, kernels[format][eb == 4], whole, a->layout == FE2O3_ROTARY_INTERLEAVED, (uint32_t)eb, four, kv_storage_of(ctx, a), r, per_sm[format][eb == 4], geo, plan_only, "kv_cache_rotary_append_v1");
 }
 
-static Fe2o3KernelRegistration reg_rotary("rotary_v1", reinterpret_cast<const void *>(rotary_kernel<kPlain, false, true>));
-static Fe2o3KernelRegistration reg_rotary_append("kv_cache_rotary_append_v1", reinterpret_cast<const void *>(rotary_kernel<FE2O3_KV_BF16, false, true>));
+static Fe2o3KernelRegistration reg_rotary("rotary_v1", reinterpret_cast<const void *>(rotary_kernel<kPlain, false, kPieces, true>));
+static Fe2o3KernelRegistration reg_rotary_append("kv_cache_rotary_append_v1", reinterpret_cast<const void *>(rotary_kernel<FE2O3_KV_BF16, false, kPieces, true>));

@@ -20,8 +20,8 @@ def test_page_plans():
         ok(op, **{**kw, name: None})
     ok(op, **{**kw, "next_lengths": kw["lengths"], "next_free_count": kw["free_count"]})
     ok(op, **pages(batch=0, width=0, count=0, tokens=0))
-    ok(op, **pages(batch=16384))
-    for bad in (dict(page_size=0), dict(batch=16385), dict(table_width=1 << 31), dict(page_size=1 << 30)):
+    ok(op, **pages(batch=8192))
+    for bad in (dict(page_size=0), dict(batch=8193), dict(table_width=1 << 31), dict(page_size=1 << 30)):
         assert err(op, **{**kw, **bad}) == "UnsupportedShape", bad
     for name, n in (("counts", 2), ("release", 4), ("lengths", 2), ("free_count", 2), ("page_table", 11), ("next_lengths", 4), ("next_free_count", 0),
                     ("token_offsets", 3), ("positions", 9), ("slots", 7)):
