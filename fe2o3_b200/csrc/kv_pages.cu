@@ -10,7 +10,7 @@
 
 namespace {
 
-constexpr uint32_t kMostSequences = 8192, kMaxThreads = 1024, kBlocks = 8, kAtOnce = 4;   // tokens a thread writes at once
+constexpr uint32_t kMostSequences = 8192, kMaxThreads = 1024, kBlocks = 16;
 
 struct PagesArgs {
     const uint32_t *counts, *release, *lengths, *free_count;
@@ -56,6 +56,7 @@ struct Place {
     uint32_t length, first_page, first_token, first_back;
 };
 
+template <uint32_t kAtOnce>   // tokens that a thread writes at once
 __global__ void __launch_bounds__(kMaxThreads) kv_pages_kernel(PagesArgs a) {
     extern __shared__ Place places[];   // [batch]
     __shared__ Sums warps[32];
@@ -136,28 +137,59 @@ __global__ void __launch_bounds__(kMaxThreads) kv_pages_kernel(PagesArgs a) {
         }
     if (!a.positions && !a.slots) return;
     const uint32_t tokens = fits ? (uint32_t)total.tokens : 0;
+    const bool whole = ((reinterpret_cast<uint64_t>(a.positions) | reinterpret_cast<uint64_t>(a.slots)) & 15) == 0;
     for (uint64_t t0 = (uint64_t)thread * kAtOnce; t0 < a.tokens; t0 += (uint64_t)threads * kAtOnce) {
-        uint32_t position[kAtOnce], slot[kAtOnce], b = t0 < tokens ? find((uint32_t)t0, &Place::first_token) : 0;
+        uint32_t position[kAtOnce], slot[kAtOnce];
+        const uint32_t *from[kAtOnce];   // the number of the position's page
+        uint32_t b = t0 < tokens ? find((uint32_t)t0, &Place::first_token) : 0;
+        Place p{0, 0, 0, 0};
+        uint32_t end = 0, held = 0;
+        if (t0 < tokens) {
+            p = places[b];
+            end = b + 1 < a.batch ? places[b + 1].first_token : tokens;
+            held = pages_for(a, p.length);
+        }
 #pragma unroll
         for (uint32_t i = 0; i < kAtOnce; ++i) {
             const uint32_t t = (uint32_t)t0 + i;
             position[i] = 0;
             slot[i] = FE2O3_SLOT_NONE;
+            from[i] = nullptr;
             if (t0 + i >= tokens) continue;
-            while (b + 1 < a.batch && places[b + 1].first_token <= t) ++b;
-            const Place p = places[b];
+            while (t >= end) {
+                p = places[++b];
+                end = b + 1 < a.batch ? places[b + 1].first_token : tokens;
+                held = pages_for(a, p.length);
+            }
             position[i] = p.length + (t - p.first_token);
-            const uint32_t page = page_of(a, position[i]), held = pages_for(a, p.length);
-            const uint32_t number = page < held ? a.table[(uint64_t)b * a.width + page] : a.free_pages[top - 1 - p.first_page - (page - held)];
-            if (number < a.pages) slot[i] = number * a.page_size + (position[i] - page * a.page_size);
-            else kstatus_set(a.status, FE2O3_KSTATUS_SLOT_RANGE);
+            const uint32_t page = page_of(a, position[i]);
+            from[i] = page < held ? a.table + (uint64_t)b * a.width + page : a.free_pages + (top - 1 - p.first_page - (page - held));
+            slot[i] = position[i] - page * a.page_size;
         }
 #pragma unroll
         for (uint32_t i = 0; i < kAtOnce; ++i) {
-            if (t0 + i >= a.tokens) continue;
-            if (a.positions) a.positions[t0 + i] = position[i];
-            if (a.slots) a.slots[t0 + i] = slot[i];
+            if (!from[i]) continue;
+            const uint32_t number = *from[i];
+            if (number < a.pages) {
+                slot[i] += number * a.page_size;
+            } else {
+                slot[i] = FE2O3_SLOT_NONE;
+                kstatus_set(a.status, FE2O3_KSTATUS_SLOT_RANGE);
+            }
         }
+        auto put = [&](uint32_t *to, const uint32_t (&v)[kAtOnce]) {
+            if (!to) return;
+            if (kAtOnce % 4 == 0 && whole && t0 + kAtOnce <= a.tokens) {
+#pragma unroll
+                for (uint32_t i = 0; i + 3 < kAtOnce; i += 4) *reinterpret_cast<uint4 *>(to + t0 + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+            } else {
+#pragma unroll
+                for (uint32_t i = 0; i < kAtOnce; ++i)
+                    if (t0 + i < a.tokens) to[t0 + i] = v[i];
+            }
+        };
+        put(a.positions, position);
+        put(a.slots, slot);
     }
 }
 
@@ -165,13 +197,16 @@ __global__ void __launch_bounds__(kMaxThreads) kv_pages_kernel(PagesArgs a) {
 
 int32_t launch_kv_pages(fe2o3_ctx *ctx, cudaStream_t s, const void *args, fe2o3_geometry *geo, bool plan_only) {
     const fe2o3_kv_pages_v1_args *a = static_cast<const fe2o3_kv_pages_v1_args *>(args);
-    const uint64_t work = (uint64_t)a->batch + a->tokens / kAtOnce;
-    const uint32_t threads = work <= 256 ? 256 : work <= 512 ? 512 : kMaxThreads, grid = work <= kMaxThreads ? 1 : kBlocks;
-    const uint32_t shared = a->batch * (uint32_t)sizeof(Place);
+    // one block for as many tokens and sequences as it has threads, a thread each; else a cluster, eight tokens a thread
+    const uint32_t work = a->batch > a->tokens ? a->batch : a->tokens, threads = work <= 256 ? 256 : work <= 512 ? 512 : kMaxThreads;
+    const bool one = work <= kMaxThreads;
+    const uint32_t grid = one ? 1 : kBlocks, shared = a->batch * (uint32_t)sizeof(Place);
+    const auto kernel = one ? kv_pages_kernel<1> : kv_pages_kernel<8>;
     if (geo) *geo = fe2o3_geometry{{grid, 1, 1}, {threads, 1, 1}, shared, 1};
     if (plan_only) {
         FE2O3_CUDA(cudaSetDevice(ctx->device));
-        FE2O3_CUDA(cudaFuncSetAttribute(reinterpret_cast<const void *>(kv_pages_kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, kMostSequences * sizeof(Place)));
+        FE2O3_CUDA(cudaFuncSetAttribute(reinterpret_cast<const void *>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, kMostSequences * sizeof(Place)));
+        FE2O3_CUDA(cudaFuncSetAttribute(reinterpret_cast<const void *>(kernel), cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
         return FE2O3_OK;
     }
     int32_t shift = -1;
@@ -180,9 +215,9 @@ int32_t launch_kv_pages(fe2o3_ctx *ctx, cudaStream_t s, const void *args, fe2o3_
     const PagesArgs p{at(a->counts), at(a->release), at(a->lengths), at(a->free_count), at(a->page_table), at(a->free_pages), at(a->next_lengths),
                       at(a->next_free_count), at(a->token_offsets), at(a->positions), at(a->slots), ctx->status_word, a->batch, a->table_width,
                       a->page_size, a->tokens, (uint32_t)a->free_pages.len, shift};
-    const cudaError_t e = fe2o3_launch_early(kv_pages_kernel, grid, threads, shared, s, grid, p);
+    const cudaError_t e = fe2o3_launch_early(kernel, grid, threads, shared, s, grid, p);
     fe2o3_count_launch(1);
     return fe2o3_cuda_status(e, "kv_pages_v1");
 }
 
-static Fe2o3KernelRegistration reg_pages("kv_pages_v1", reinterpret_cast<const void *>(kv_pages_kernel));
+static Fe2o3KernelRegistration reg_pages("kv_pages_v1", reinterpret_cast<const void *>(kv_pages_kernel<1>));
