@@ -76,7 +76,6 @@ template <uint32_t FORMAT, bool F32, bool WRITE, bool WHOLE>
 __global__ void __launch_bounds__(kThreads) kv_rows_kernel(KvCache c, KvRows r) {
     __shared__ uint32_t slots[kTokens];
     __shared__ uint32_t known;   // tokens whose lengths allow a slot, a bit each
-    constexpr bool kFour = FORMAT == FE2O3_KV_E2M1;
     constexpr int kEb = F32 ? 4 : 2, kPiece = 16 / kEb, kCached = kv_bytes<FORMAT>(kPiece);   // a piece: columns, bytes in the cache
     // rows a lane has in flight: two where it quantises (registers: three take 55 us where two take 52, to e4m3 and back), else four
     constexpr int kDeep = WRITE && FORMAT != FE2O3_KV_BF16 ? 2 : 4;
@@ -96,7 +95,6 @@ __global__ void __launch_bounds__(kThreads) kv_rows_kernel(KvCache c, KvRows r) 
         const uint32_t first = base + (threadIdx.x >> r.lanes_log2);
         uint4 raw[kDeep][2];
         float scales[kDeep];
-        uint32_t blocks[kDeep];   // 4 bits: the scales of the two pieces' blocks, a byte each
         uint32_t at[kDeep], side[kDeep];
         uint8_t *there[kDeep];
         bool active[kDeep];
@@ -114,7 +112,6 @@ __global__ void __launch_bounds__(kThreads) kv_rows_kernel(KvCache c, KvRows r) 
                                                 (uint64_t)h * (side[d] ? r.v_head_stride : r.k_head_stride)) * kEb;
             raw[d][0] = raw[d][1] = make_uint4(0, 0, 0, 0);
             scales[d] = 0.f;
-            blocks[d] = 0;
             if (!active[d]) continue;
             const uint8_t *const from = WRITE ? there[d] : (side[d] ? c.v : c.k) + (uint64_t)at[d] * kv_bytes<FORMAT>(c.dim);
             if (!WRITE && slot == ~0u) continue;
@@ -123,10 +120,6 @@ __global__ void __launch_bounds__(kThreads) kv_rows_kernel(KvCache c, KvRows r) 
                 if (!columns.inside[half]) continue;
                 if constexpr (WRITE) raw[d][half] = fetch<F32, WHOLE>(from + columns.first[half] * kEb);
                 else raw[d][half] = fetch_cached<kCached>(from + kv_bytes<FORMAT>(columns.first[half]));
-                if constexpr (!WRITE && kFour) {
-                    const uint8_t *const scale = (side[d] ? c.v : c.k) + c.blocks + ((uint64_t)at[d] * c.dim + columns.first[half]) / 16;
-                    blocks[d] |= (uint32_t)__ldcs(scale) << (8 * half);
-                }
             }
             if constexpr (!WRITE && FORMAT != FE2O3_KV_BF16) scales[d] = (side[d] ? c.v_scales : c.k_scales)[at[d]];
         }
@@ -155,37 +148,16 @@ __global__ void __launch_bounds__(kThreads) kv_rows_kernel(KvCache c, KvRows r) 
                 else if (lanes == 8) top = highest<8>(top);
                 else
                     for (uint32_t o = 1; o < lanes; o <<= 1) top = max(top, __shfl_xor_sync(~0u, top, o));
-                if constexpr (kFour) {
-                    float scale, up;
-                    row_scales4(__uint_as_float(top), scale, up);
+                const float scale = top < 0x7f800000u ? scale_of<FORMAT>(__uint_as_float(top)) : __uint_as_float(0x7fc00000u);
+                minus_quotients<FORMAT>(x, scale);
+                if (!active[d]) continue;
 #pragma unroll
-                    for (int half = 0; half < 2; ++half) {   // a block is 2 or 4 neighbouring lanes' pieces
-                        const float *const q = x + half * kPiece;
-                        float m = 0.f;
-#pragma unroll
-                        for (int i = 0; i < kPiece; ++i) m = fmaxf(m, fabsf(q[i]));
-#pragma unroll
-                        for (int o = 1; o < 16 / kPiece; o <<= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
-                        float factor;
-                        const uint32_t block = block_scale4(m, scale, up, factor);
-                        if (!active[d] || !columns.inside[half]) continue;
-                        put_cached<kCached>(to + columns.first[half] / 2, make_uint4(codes4(q, factor) | (F32 ? 0 : codes4(q + kPiece - 4, factor) << 16), 0, 0, 0));
-                        if (l % (16 / kPiece) == 0) (side[d] ? c.v : c.k)[c.blocks + ((uint64_t)at[d] * c.dim + columns.first[half]) / 16] = (uint8_t)block;
-                    }
-                    if (active[d] && l == 0) (side[d] ? c.v_scales : c.k_scales)[at[d]] = scale;
-                    continue;
-                } else {
-                    const float scale = top < 0x7f800000u ? scale_of<FORMAT>(__uint_as_float(top)) : __uint_as_float(0x7fc00000u);
-                    minus_quotients<FORMAT>(x, scale);
-                    if (!active[d]) continue;
-#pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        if (!columns.inside[half]) continue;
-                        const float *const q = x + half * kPiece;
-                        put_cached<kCached>(to + columns.first[half], make_uint4(codes_of<FORMAT>(q), F32 ? 0 : codes_of<FORMAT>(q + kPiece - 4), 0, 0));
-                    }
-                    if (l == 0) (side[d] ? c.v_scales : c.k_scales)[at[d]] = scale;
+                for (int half = 0; half < 2; ++half) {
+                    if (!columns.inside[half]) continue;
+                    const float *const q = x + half * kPiece;
+                    put_cached<kCached>(to + columns.first[half], make_uint4(codes_of<FORMAT>(q), F32 ? 0 : codes_of<FORMAT>(q + kPiece - 4), 0, 0));
                 }
+                if (l == 0) (side[d] ? c.v_scales : c.k_scales)[at[d]] = scale;
             } else {
                 if (!active[d]) continue;
 #pragma unroll
@@ -199,10 +171,6 @@ __global__ void __launch_bounds__(kThreads) kv_rows_kernel(KvCache c, KvRows r) 
                         if constexpr (FORMAT == FE2O3_KV_BF16) {
                             widen2(v.x, x);
                             widen2(v.y, x + 2);
-                        } else if constexpr (kFour) {
-                            const float block = of_e4m3(blocks[d] >> (8 * half) & 255u);
-                            values4(v.x, block, scales[d], x);
-                            if constexpr (!F32) values4(v.x >> 16, block, scales[d], x + 4);
                         } else {
                             values_of<FORMAT>(v.x, scales[d], x);
                             if constexpr (!F32) values_of<FORMAT>(v.y, scales[d], x + 4);
@@ -212,6 +180,140 @@ __global__ void __launch_bounds__(kThreads) kv_rows_kernel(KvCache c, KvRows r) 
                     }
                     if constexpr (WRITE) put_cached<kCached>(to + kv_bytes<FORMAT>(columns.first[half]), v);
                     else put<F32, WHOLE>(to + columns.first[half] * kEb, v);
+                }
+            }
+        }
+    }
+}
+
+// ---- 4 bits ----
+// Rows of 32 columns a lane (at least two lanes a row): what a row costs a lane by itself is dear beside 16 bytes of codes.  (With the 16 columns
+// of the other formats, 131072 tokens of 8 heads of 128 are read in 148 us, and 16384 are written in 36.)  A lane that writes takes two
+// blocks of 16 columns, l and l + lanes, whose scales it finds by itself.  One that reads takes four words of eight columns, l and every lanes-th
+// further: the stores of a row's lanes lie side by side.  (f32 ones, 32 bytes a word, by two neighbours that swap halves of their words first.)
+template <bool F32, bool WRITE, bool WHOLE>
+__global__ void __launch_bounds__(kThreads) kv_rows4_kernel(KvCache c, KvRows r) {
+    __shared__ uint32_t slots[kTokens];
+    __shared__ uint32_t known;
+    constexpr int kEb = F32 ? 4 : 2, kDeep = WRITE ? (F32 ? 1 : 2) : 4, kPieces = WRITE ? kEb : 1;   // kPieces: 16 bytes each, of a block that is written
+    begin_after_previous();
+    const uint32_t t0 = blockIdx.x * r.per_block, n = min(r.per_block, r.tokens - t0), lane = threadIdx.x & 31;
+    if (threadIdx.x < 32) {
+        uint32_t row = ~0u;
+        const uint32_t ok = __ballot_sync(~0u, slot_of(c, r, t0, n, row));
+        slots[lane] = row;
+        if (lane == 0) known = ok;
+    }
+    __syncthreads();
+    const uint32_t lanes = 1u << r.lanes_log2, at_once = kThreads >> r.lanes_log2, l = threadIdx.x & (lanes - 1);
+    const uint32_t rows = n * 2 * c.kv_heads, blocks = c.dim / 16, words = c.dim / 8;
+    for (uint32_t base = 0; base < rows; base += kDeep * at_once) {
+        const uint32_t first = base + (threadIdx.x >> r.lanes_log2);
+        uint4 raw[WRITE ? kDeep : 1][2][kPieces];
+        uint32_t code[WRITE ? 1 : kDeep][4], block[WRITE ? 1 : kDeep][4];
+        float scales[kDeep];
+        uint32_t at[kDeep], side[kDeep];
+        uint8_t *there[kDeep];
+        bool active[kDeep];
+#pragma unroll
+        for (int d = 0; d < kDeep; ++d) {
+            active[d] = false;
+            if (base + d * at_once >= rows) continue;   // (for the whole block)
+            // head fastest, then K or V, then the token
+            const uint32_t i = min(first + d * at_once, rows - 1), of_side = r.heads_inverse ? __umulhi(i, r.heads_inverse) : i / c.kv_heads;
+            const uint32_t h = i - of_side * c.kv_heads, token = of_side >> 1, slot = slots[token];
+            side[d] = of_side & 1;
+            at[d] = slot == ~0u ? ~0u : slot + h * c.page_size;
+            active[d] = first + d * at_once < rows && (known >> token & 1) && (slot != ~0u || !WRITE);
+            there[d] = (side[d] ? r.v : r.k) + ((uint64_t)(t0 + token) * (side[d] ? r.v_token_stride : r.k_token_stride) +
+                                                (uint64_t)h * (side[d] ? r.v_head_stride : r.k_head_stride)) * kEb;
+            if constexpr (WRITE) {
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const uint32_t b = l + half * lanes;
+#pragma unroll
+                    for (int x = 0; x < kPieces; ++x)
+                        raw[d][half][x] = active[d] && b < blocks ? fetch<F32, WHOLE>(there[d] + b * 16 * kEb + 16 * x) : make_uint4(0, 0, 0, 0);
+                }
+            } else {
+                const uint8_t *const cache = side[d] ? c.v : c.k;
+                const bool held = active[d] && slot != ~0u;
+                scales[d] = held ? (side[d] ? c.v_scales : c.k_scales)[at[d]] : 0.f;
+                const uint8_t *const codes = cache + (uint64_t)at[d] * (c.dim / 2), *const block_scales = cache + c.blocks + (uint64_t)at[d] * blocks;
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    const uint32_t word = l + x * lanes;
+                    code[d][x] = block[d][x] = 0;
+                    if (!held || word >= words) continue;
+                    code[d][x] = __ldcs(reinterpret_cast<const uint32_t *>(codes) + word);
+                    block[d][x] = __ldcs(block_scales + word / 2);
+                }
+            }
+        }
+#pragma unroll
+        for (int d = 0; d < kDeep; ++d) {
+            if (base + d * at_once >= rows) break;
+            if constexpr (WRITE) {
+                uint32_t tops[2];   // largest magnitudes as bits: an infinity or a NaN is above every number
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    uint32_t top = 0;
+#pragma unroll
+                    for (int x = 0; x < kPieces; ++x) {
+                        const uint4 &v = raw[d][half][x];
+                        if constexpr (F32) top = max(max(top, v.x & 0x7fffffffu), max(max(v.y & 0x7fffffffu, v.z & 0x7fffffffu), v.w & 0x7fffffffu));
+                        else top = __vmaxu2(__vmaxu2(top, v.x & 0x7fff7fffu), __vmaxu2(__vmaxu2(v.y & 0x7fff7fffu, v.z & 0x7fff7fffu), v.w & 0x7fff7fffu));
+                    }
+                    tops[half] = F32 ? top : max(top << 16, top & 0xffff0000u);
+                }
+                uint32_t top = max(tops[0], tops[1]);
+                for (uint32_t o = 1; o < lanes; o <<= 1) top = max(top, __shfl_xor_sync(~0u, top, o));
+                if (!active[d]) continue;
+                float scale, up;
+                row_scales4(__uint_as_float(top), scale, up);
+                uint8_t *const cache = side[d] ? c.v : c.k;
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const uint32_t b = l + half * lanes;
+                    if (b >= blocks) continue;
+                    float factor;
+                    const uint32_t code = block_scale4(__uint_as_float(tops[half]), scale, up, factor);
+                    uint32_t w[2] = {0, 0};
+#pragma unroll
+                    for (int x = 0; x < kPieces; ++x) {
+                        const uint32_t v[4] = {raw[d][half][x].x, raw[d][half][x].y, raw[d][half][x].z, raw[d][half][x].w};
+                        float y[F32 ? 4 : 8];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            if constexpr (F32) y[i] = __uint_as_float(v[i]);
+                            else widen2(v[i], y + 2 * i);
+                        }
+                        if constexpr (F32) w[x / 2] |= codes4(y, factor) << (16 * (x & 1));
+                        else w[x] = codes8(y, factor);
+                    }
+                    __stcs(reinterpret_cast<uint2 *>(cache + (uint64_t)at[d] * (c.dim / 2) + 8 * b), make_uint2(w[0], w[1]));
+                    cache[c.blocks + (uint64_t)at[d] * blocks + b] = (uint8_t)code;
+                }
+                if (l == 0) (side[d] ? c.v_scales : c.k_scales)[at[d]] = scale;
+            } else {
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    const uint32_t word = l + x * lanes;
+                    uint32_t w = code[d][x];
+                    if constexpr (F32) {   // columns 0 to 3 and 8 to 11 of the two words go to the even lane
+                        const uint32_t other = __shfl_xor_sync(~0u, w, 1);
+                        w = l & 1 ? __byte_perm(other, w, 0x7632) : __byte_perm(w, other, 0x5410);
+                    }
+                    if (!active[d] || word >= words) continue;
+                    float v[8];
+                    values8(w, block[d][x], scales[d], v);
+                    if constexpr (F32) {
+                        uint8_t *const to = there[d] + (word & ~1u) * 32 + (l & 1) * 16;
+                        put<F32, WHOLE>(to, make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])));
+                        put<F32, WHOLE>(to + 32, make_uint4(__float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7])));
+                    } else {
+                        put<F32, WHOLE>(there[d] + word * 16, make_uint4(bf16_pair(v[0], v[1]), bf16_pair(v[2], v[3]), bf16_pair(v[4], v[5]), bf16_pair(v[6], v[7])));
+                    }
                 }
             }
         }
@@ -243,7 +345,7 @@ int32_t launch_rows(fe2o3_ctx *ctx, cudaStream_t s, const Args *a, uint32_t dtyp
     if (geo) *geo = fe2o3_geometry{{grid, 1, 1}, {kThreads, 1, 1}, 0, 1};
     if (plan_only || a->tokens == 0) return FE2O3_OK;
     uint32_t lanes_log2 = 1;
-    while ((32u / eb << lanes_log2) < a->dim) ++lanes_log2;
+    while ((format == 3 ? 32u << lanes_log2 : 32u / eb << lanes_log2) < a->dim) ++lanes_log2;
     const KvRows r{reinterpret_cast<uint8_t *>(a->k.ptr), reinterpret_cast<uint8_t *>(a->v.ptr), a->k_token_stride, a->v_token_stride,
                    a->k_head_stride, a->v_head_stride, reinterpret_cast<const uint32_t *>(a->token_offsets.ptr), a->tokens, per_block, lanes_log2,
                    // exact for the indexes of a block, below 64 kv_heads
@@ -258,7 +360,7 @@ int32_t launch_rows(fe2o3_ctx *ctx, cudaStream_t s, const Args *a, uint32_t dtyp
 #define KV_FORMAT(FORMAT, WRITE)                                                                                                     \
     {{kv_rows_kernel<FORMAT, false, WRITE, false>, kv_rows_kernel<FORMAT, false, WRITE, true>},                                      \
      {kv_rows_kernel<FORMAT, true, WRITE, false>, kv_rows_kernel<FORMAT, true, WRITE, true>}}
-#define KV_FORMATS(WRITE) {KV_FORMAT(FE2O3_KV_BF16, WRITE), KV_FORMAT(FE2O3_KV_E4M3, WRITE), KV_FORMAT(FE2O3_KV_I8, WRITE), KV_FORMAT(FE2O3_KV_E2M1, WRITE)}
+#define KV_FORMATS(WRITE) {KV_FORMAT(FE2O3_KV_BF16, WRITE), KV_FORMAT(FE2O3_KV_E4M3, WRITE), KV_FORMAT(FE2O3_KV_I8, WRITE), {{kv_rows4_kernel<false, WRITE, false>, kv_rows4_kernel<false, WRITE, true>}, {kv_rows4_kernel<true, WRITE, false>, kv_rows4_kernel<true, WRITE, true>}}}
 int32_t launch_kv_cache_append(fe2o3_ctx *ctx, cudaStream_t s, const void *args, fe2o3_geometry *geo, bool plan_only) {
     static const Kernel kernels[4][2][2] = KV_FORMATS(true);
     const fe2o3_kv_cache_append_v1_args *a = static_cast<const fe2o3_kv_cache_append_v1_args *>(args);

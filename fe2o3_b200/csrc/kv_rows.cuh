@@ -50,8 +50,7 @@ __device__ __forceinline__ uint4 fetch_cached(const uint8_t *at) {
         const uint2 v = __ldcs(reinterpret_cast<const uint2 *>(at));
         return make_uint4(v.x, v.y, 0, 0);
     }
-    if constexpr (BYTES == 4) return make_uint4(__ldcs(reinterpret_cast<const uint32_t *>(at)), 0, 0, 0);
-    return make_uint4(__ldcs(reinterpret_cast<const uint16_t *>(at)), 0, 0, 0);
+    return make_uint4(__ldcs(reinterpret_cast<const uint32_t *>(at)), 0, 0, 0);
 }
 template <int BYTES>
 __device__ __forceinline__ void put_cached(uint8_t *at, const uint4 &v) {
@@ -143,10 +142,19 @@ __device__ __forceinline__ float of_e4m3(uint32_t code) {
     asm("{\n\t.reg .b32 h;\n\t.reg .b16 t, u;\n\tcvt.u16.u32 t, %1;\n\tcvt.rn.f16x2.e4m3x2 h, t;\n\tmov.b32 {t, u}, h;\n\tcvt.f32.f16 %0, t;\n\t}" : "=f"(v) : "r"(code));
     return v;
 }
+// n / m, rounded to nearest, from y near 1 / m (the corrections of minus_quotients).
+__device__ __forceinline__ float corrected(float n, float m, float y) {
+    float r = n * y;
+    r = fmaf(fmaf(-m, r, n), y, r);
+    return fmaf(fmaf(-m, r, n), y, r);
+}
 // A row's scale and 448 / m of its largest magnitude m (an infinity or a NaN: scale NaN; below 2^-100: both 0, and all codes).
 __device__ __forceinline__ void row_scales4(float m, float &scale, float &up) {
     scale = up = 0.f;
-    if (m >= 0x1p-100f && m < INFINITY) {
+    if (m > 8.7e-19f && m < 1.1e18f) {   // 2^+-60: nothing leaves the normal range
+        scale = corrected(m, 2688.f, (float)(1.0 / 2688.0));
+        up = corrected(448.f, m, __frcp_rn(m));
+    } else if (m >= 0x1p-100f && m < INFINITY) {
         scale = __fdiv_rn(m, 2688.f);
         up = __fdiv_rn(448.f, m);
     } else if (!(m < INFINITY)) {
@@ -161,23 +169,38 @@ __device__ __forceinline__ uint32_t block_scale4(float m, float scale, float up,
     if (code) factor = __frcp_rn(of_e4m3(code) * scale);
     return code;
 }
-// Four elements as codes, the first in the lowest bits.  (With a block of zeros nothing keeps a sign.)
+// Elements as codes, the first in the lowest bits.  (With a block of zeros nothing keeps a sign.)
 __device__ __forceinline__ uint32_t codes4(const float *x, float factor) {
     if (!(factor > 0.f)) return 0;
     uint32_t w;
-    asm("{\n\t.reg .b8 lo, hi, no;\n\tcvt.rn.satfinite.e2m1x2.f32 lo, %2, %1;\n\tcvt.rn.satfinite.e2m1x2.f32 hi, %4, %3;\n\t"
-        "mov.b32 %0, {lo, hi, lo, hi};\n\t}" : "=r"(w) : "f"(x[0] * factor), "f"(x[1] * factor), "f"(x[2] * factor), "f"(x[3] * factor));
+    asm("{\n\t.reg .b8 a, b, no;\n\tcvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\tcvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+        "mov.b32 %0, {a, b, a, b};\n\t}" : "=r"(w) : "f"(x[0] * factor), "f"(x[1] * factor), "f"(x[2] * factor), "f"(x[3] * factor));
     return w & 0xffffu;
 }
-// What four codes stand for.
-__device__ __forceinline__ void values4(uint32_t w, float block, float scale, float *x) {
-    uint32_t h[2];
-    asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %2;\n\tcvt.rn.f16x2.e2m1x2 %0, a;\n\tcvt.rn.f16x2.e2m1x2 %1, b;\n\t}" : "=r"(h[0]), "=r"(h[1]) : "r"(w));
+__device__ __forceinline__ uint32_t codes8(const float *x, float factor) {
+    if (!(factor > 0.f)) return 0;
+    float y[8];
+    const uint64_t by = pack_f32x2(factor, factor);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\tcvt.f32.f16 %0, lo;\n\tcvt.f32.f16 %1, hi;\n\t}" : "=f"(x[2 * i]), "=f"(x[2 * i + 1]) : "r"(h[i]));
-        x[2 * i] = x[2 * i] * block * scale;   // (the first product is exact)
-        x[2 * i + 1] = x[2 * i + 1] * block * scale;
+    for (int i = 0; i < 8; i += 2) unpack_f32x2(mul_f32x2(pack_f32x2(x[i], x[i + 1]), by), y[i], y[i + 1]);
+    uint32_t w;
+    asm("{\n\t.reg .b8 a, b, c, d;\n\tcvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\tcvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\tcvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\tmov.b32 %0, {a, b, c, d};\n\t}"
+        : "=r"(w) : "f"(y[0]), "f"(y[1]), "f"(y[2]), "f"(y[3]), "f"(y[4]), "f"(y[5]), "f"(y[6]), "f"(y[7]));
+    return w;
+}
+// What eight codes of a block stand for; a code times its block's scale has 6 bits, f16's 11 hold it exactly.
+__device__ __forceinline__ void values8(uint32_t w, uint32_t block, float scale, float *x) {
+    uint32_t h[4], by;
+    asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %4;\n\tcvt.rn.f16x2.e2m1x2 %0, a;\n\tcvt.rn.f16x2.e2m1x2 %1, b;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %2, c;\n\tcvt.rn.f16x2.e2m1x2 %3, d;\n\t}" : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3]) : "r"(w));
+    asm("{\n\t.reg .b16 t;\n\tcvt.u16.u32 t, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, t;\n\t}" : "=r"(by) : "r"(block * 0x101u));
+    const uint64_t scale2 = pack_f32x2(scale, scale);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float lo, hi;
+        asm("{\n\t.reg .b32 p;\n\t.reg .b16 a, b;\n\tmul.rn.f16x2 p, %2, %3;\n\tmov.b32 {a, b}, p;\n\tcvt.f32.f16 %0, a;\n\tcvt.f32.f16 %1, b;\n\t}" : "=f"(lo), "=f"(hi) : "r"(h[i]), "r"(by));
+        unpack_f32x2(mul_f32x2(pack_f32x2(lo, hi), scale2), x[2 * i], x[2 * i + 1]);
     }
 }
 

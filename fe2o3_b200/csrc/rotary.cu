@@ -84,7 +84,7 @@ __device__ __forceinline__ void store_row(const KvCache &c, float (&x)[2 * kPiec
                 float factor;
                 const uint32_t block = block_scale4(m, scale, up, factor);
                 if (!active || !inside[half]) continue;
-                put_cached<kCached>(to + first[half] / 2, make_uint4(codes4(q, factor) | (kPiece == 4 ? 0 : codes4(q + kPiece - 4, factor) << 16), 0, 0, 0));
+                put_cached<kCached>(to + first[half] / 2, make_uint4(kPiece == 4 ? codes4(q, factor) : codes8(q, factor), 0, 0, 0));
                 if (l % (16 / kPiece) == 0) base[c.blocks + ((uint64_t)row * c.dim + first[half]) / 16] = (uint8_t)block;
             }
         } else {
