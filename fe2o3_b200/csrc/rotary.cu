@@ -16,7 +16,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr uint32_t kPlain = ~0u;   // FORMAT: no cache, q and k go to rows like theirs
-constexpr uint32_t kMostTokens = 16;
+constexpr uint32_t kMostTokens = 8;
 
 struct RotaryRows {
     const uint8_t *from[3];            // q, k, v
@@ -26,7 +26,7 @@ struct RotaryRows {
     const float *frequencies;
     uint32_t tokens, heads, rows;      // rows of a token: heads, then kv_heads of k (and of v)
     uint32_t per_block, parts;         // tokens of a block; blocks that share them
-    uint32_t dim, kv_heads, pairs, lanes_log2;
+    uint32_t dim, kv_heads, pairs, lanes;
     uint32_t groups, token_turns;      // pieces whose pairs lie together (see turn_at); places of a token's sines and cosines
     uint32_t rows_inverse;             // 2^32 / rows rounded up, or 0
     float scale, sign;
@@ -135,22 +135,22 @@ __global__ void __launch_bounds__(kThreads, FORMAT == kPlain || FORMAT == FE2O3_
     }
     __syncthreads();
 
-    const uint32_t lanes = 1u << r.lanes_log2, at_once = kThreads >> r.lanes_log2, l = threadIdx.x & (lanes - 1);
+    const uint32_t lanes = r.lanes, of_warp = 32 / lanes, at_once = kThreads / 32 * of_warp, in_warp = (threadIdx.x & 31) / lanes, l = (threadIdx.x & 31) - in_warp * lanes;
+    const uint32_t mine = (threadIdx.x >> 5) * of_warp + in_warp;   // of the rows at once
     // a lane's columns: two pieces, the partners of one another where pairs allow
     const uint32_t pieces = r.dim / kPiece, paired = MODE == kPieces ? r.groups : 0, rest = (pieces - 2 * paired) / 2;   // rest: half of the other pieces
-    const bool pair = l < paired, in = l < pieces / 2;
+    const bool pair = l < paired, in = l < pieces / 2 && in_warp < of_warp;   // (lanes left over have none)
     const uint32_t first[2] = {kPiece * (pair ? l : paired + l), kPiece * (pair ? l + paired : paired + l + rest)};
     const bool inside[2] = {in, in};
-    uint8_t *const scratch = reinterpret_cast<uint8_t *>(turns + (uint64_t)r.per_block * r.token_turns) + (threadIdx.x >> r.lanes_log2) * kDeep * r.dim * kEb;
+    float *const scratch = reinterpret_cast<float *>(turns + (uint64_t)r.per_block * r.token_turns) + mine * kDeep * r.dim;
     const uint32_t total = n * r.rows, share = (total + r.parts - 1) / r.parts, end = min(total, (part + 1) * share);
     for (uint32_t base = part * share; base < end; base += kDeep * at_once) {
-        const uint32_t mine = base + (threadIdx.x >> r.lanes_log2);
         uint4 raw[kDeep][2];
         uint32_t token[kDeep], head[kDeep], what[kDeep];
         bool active[kDeep];
 #pragma unroll
         for (int d = 0; d < kDeep; ++d) {
-            const uint32_t i = min(mine + d * at_once, end - 1);
+            const uint32_t i = min(base + mine + d * at_once, end - 1);
             token[d] = r.rows_inverse ? __umulhi(i, r.rows_inverse) : i / r.rows;
             head[d] = i - token[d] * r.rows;
             what[d] = head[d] < r.heads ? 0 : 1;
@@ -159,7 +159,7 @@ __global__ void __launch_bounds__(kThreads, FORMAT == kPlain || FORMAT == FE2O3_
                 what[d] = 2;
                 head[d] -= r.kv_heads;
             }
-            active[d] = mine + d * at_once < end && (!kCache || first_rows[token[d]] != ~0u);
+            active[d] = base + mine + d * at_once < end && (!kCache || first_rows[token[d]] != ~0u);
             raw[d][0] = raw[d][1] = make_uint4(0, 0, 0, 0);
             if (active[d] && in) {
                 const uint32_t ts = what[d] == 0 ? r.token_stride[0] : what[d] == 1 ? r.token_stride[1] : r.token_stride[2];
@@ -169,37 +169,61 @@ __global__ void __launch_bounds__(kThreads, FORMAT == kPlain || FORMAT == FE2O3_
                 for (int half = 0; half < 2; ++half) raw[d][half] = fetch<F32, WHOLE>(at + first[half] * kEb);
             }
         }
-        if constexpr (MODE == kAnywhere) {   // the rows, for partners to be looked up (a row's lanes are of one warp)
-            __syncwarp();
+        __syncwarp();   // in place: every lane has its columns before one writes
+        float x[kDeep][2 * kPiece];
 #pragma unroll
-            for (int d = 0; d < kDeep; ++d)
-                if (in) {
-#pragma unroll
-                    for (int half = 0; half < 2; ++half) *reinterpret_cast<uint4 *>(scratch + d * r.dim * kEb + first[half] * kEb) = raw[d][half];
-                }
-        }
-        __syncwarp();   // (and in place: every lane has its columns before one writes)
-#pragma unroll
-        for (int d = 0; d < kDeep; ++d) {
-            if (base + d * at_once >= end) break;
-            float x[2 * kPiece];
+        for (int d = 0; d < kDeep; ++d)
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const uint32_t w = word_of(raw[d][i / 4], i % 4);
-                if constexpr (F32) x[i] = __uint_as_float(w);
-                else widen2(w, x + 2 * i);
+                if constexpr (F32) x[d][i] = __uint_as_float(w);
+                else widen2(w, x[d] + 2 * i);
             }
+        if constexpr (MODE == kAnywhere) {   // through shared memory, a pair a lane (a row's lanes are of one warp)
+#pragma unroll
+            for (int d = 0; d < kDeep; ++d)
+#pragma unroll
+                for (int half = 0; half < 2; ++half)
+                    if (what[d] < 2 && in && first[half] < 2 * r.pairs)
+#pragma unroll
+                        for (int i = 0; i < kPiece; i += 4)
+                            *reinterpret_cast<float4 *>(scratch + d * r.dim + first[half] + i) = *reinterpret_cast<const float4 *>(x[d] + half * kPiece + i);
+            __syncwarp();
+#pragma unroll
+            for (int d = 0; d < kDeep; ++d) {
+                if (what[d] == 2 || in_warp >= of_warp) continue;
+                float *const row = scratch + d * r.dim;
+                for (uint32_t i = l; i < r.pairs; i += lanes) {
+                    const float2 t = turns[token[d] * r.token_turns + i];
+                    const float a = row[i], b = row[i + r.pairs];
+                    row[i] = fmaf(a, t.x, -(b * t.y));
+                    row[i + r.pairs] = fmaf(b, t.x, a * t.y);
+                }
+            }
+            __syncwarp();
+#pragma unroll
+            for (int d = 0; d < kDeep; ++d)
+#pragma unroll
+                for (int half = 0; half < 2; ++half)
+                    if (what[d] < 2 && in && first[half] < 2 * r.pairs)
+#pragma unroll
+                        for (int i = 0; i < kPiece; i += 4)
+                            *reinterpret_cast<float4 *>(x[d] + half * kPiece + i) = *reinterpret_cast<const float4 *>(scratch + d * r.dim + first[half] + i);
+        }
+#pragma unroll
+        for (int d = 0; d < kDeep; ++d) {
+            if (base + d * at_once >= end) break;
             const uint32_t turned = what[d] < 2 ? 2 * r.pairs : 0;
             const float2 *const cs = turns + token[d] * r.token_turns;
             if (MODE == kPieces && turned && pair) {
 #pragma unroll
                 for (int i = 0; i < kPiece; i += 2) {
                     const float4 t = reinterpret_cast<const float4 *>(cs)[i / 2 * r.groups + l];
-                    const float a = x[i], b = x[kPiece + i], a1 = x[i + 1], b1 = x[kPiece + i + 1];
-                    x[i] = fmaf(a, t.x, -(b * t.y));
-                    x[kPiece + i] = fmaf(b, t.x, a * t.y);
-                    x[i + 1] = fmaf(a1, t.z, -(b1 * t.w));
-                    x[kPiece + i + 1] = fmaf(b1, t.z, a1 * t.w);
+                    const float a = x[d][i], b = x[d][kPiece + i], a1 = x[d][i + 1], b1 = x[d][kPiece + i + 1];
+                    x[d][i] = fmaf(a, t.x, -(b * t.y));
+                    x[d][kPiece + i] = fmaf(b, t.x, a * t.y);
+                    x[d][i + 1] = fmaf(a1, t.z, -(b1 * t.w));
+                    x[d][kPiece + i + 1] = fmaf(b1, t.z, a1 * t.w);
                 }
             }
             if (MODE == kNeighbours && in) {
@@ -209,7 +233,7 @@ __global__ void __launch_bounds__(kThreads, FORMAT == kPlain || FORMAT == FE2O3_
                     for (int i = 0; i < kPiece; i += 4) {
                         if (first[half] + i >= turned) continue;   // (turned columns end with a pair, the second of two or the first)
                         const float4 t = reinterpret_cast<const float4 *>(cs)[i / 4 * r.groups + first[half] / kPiece];
-                        float *const y = x + half * kPiece + i;
+                        float *const y = x[d] + half * kPiece + i;
                         const float a = y[0], b = y[1], a1 = y[2], b1 = y[3];
                         y[0] = fmaf(a, t.x, -(b * t.y));
                         y[1] = fmaf(b, t.x, a * t.y);
@@ -218,24 +242,10 @@ __global__ void __launch_bounds__(kThreads, FORMAT == kPlain || FORMAT == FE2O3_
                         y[3] = fmaf(b1, t.z, a1 * t.w);
                     }
             }
-            if (MODE == kAnywhere && in) {
-#pragma unroll
-                for (int i = 0; i < 2 * kPiece; ++i) {
-                    const uint32_t column = first[i / kPiece] + i % kPiece;
-                    if (column >= turned) continue;
-                    const bool low = column < r.pairs;
-                    const float2 t = cs[low ? column : column - r.pairs];
-                    const uint8_t *const e = scratch + d * r.dim * kEb + (low ? column + r.pairs : column - r.pairs) * kEb;
-                    float other;
-                    if constexpr (F32) other = *reinterpret_cast<const float *>(e);
-                    else other = bf16_bits_to_f32(*reinterpret_cast<const uint16_t *>(e));
-                    x[i] = low ? fmaf(x[i], t.x, -(other * t.y)) : fmaf(x[i], t.x, other * t.y);
-                }
-            }
             if (kCache && what[d]) {
                 if constexpr (kCache) {
                     const uint32_t row = first_rows[token[d]] + head[d] * c.page_size;
-                    store_row<FORMAT, kPiece>(c, x, raw[d], turned, what[d] - 1, row, first, inside, l, lanes, active[d] && in);
+                    store_row<FORMAT, kPiece>(c, x[d], raw[d], turned, what[d] - 1, row, first, inside, l, lanes, active[d] && in);
                 }
                 continue;
             }
@@ -244,7 +254,7 @@ __global__ void __launch_bounds__(kThreads, FORMAT == kPlain || FORMAT == FE2O3_
             uint8_t *const to = (!kCache && what[d] ? r.to[1] : r.to[0]) + ((uint64_t)(t0 + token[d]) * ts + (uint64_t)head[d] * hs) * kEb;
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-                const float *const q = x + half * kPiece;
+                const float *const q = x[d] + half * kPiece;
                 uint32_t w[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -260,7 +270,7 @@ __global__ void __launch_bounds__(kThreads, FORMAT == kPlain || FORMAT == FE2O3_
 using Kernel = void (*)(KvCache, RotaryRows);
 
 // kernels: [MODE][WHOLE] of the types at hand.
-int32_t launch_rows(fe2o3_ctx *ctx, cudaStream_t s, const Kernel (&kernels)[3][2], bool whole, bool interleaved, uint32_t eb, bool four, const KvCache &c, RotaryRows r,
+int32_t launch_rows(fe2o3_ctx *ctx, cudaStream_t s, const Kernel (&kernels)[3][2], bool whole, bool interleaved, uint32_t eb, bool quantised, bool four, const KvCache &c, RotaryRows r,
                     std::atomic<int> (&per_sm)[3][2], fe2o3_geometry *geo, bool plan_only, const char *what) {
     const uint32_t piece = 16 / eb;
     // Partners lie in pieces of their own where half of the turned columns is a whole number of pieces (4 bits: of blocks, which stay with
@@ -268,15 +278,20 @@ int32_t launch_rows(fe2o3_ctx *ctx, cudaStream_t s, const Kernel (&kernels)[3][2
     const int mode = interleaved ? kNeighbours : r.pairs % (four ? 16 : piece) == 0 ? kPieces : kAnywhere;
     r.groups = mode == kNeighbours ? (2 * r.pairs + piece - 1) / piece : mode == kPieces ? r.pairs / piece : 0;
     r.token_turns = mode == kNeighbours ? r.groups * (piece / 2) : (r.pairs + 1) & ~1u;
-    while ((2 * piece << r.lanes_log2) < r.dim) ++r.lanes_log2;
-    if (r.lanes_log2 == 0) r.lanes_log2 = 1;
+    r.lanes = r.dim / (2 * piece);   // 1 to 32; where a row's magnitudes are compared, a power of two
+    if (quantised) {
+        uint32_t lanes = 2;
+        while (lanes < r.lanes) lanes *= 2;
+        r.lanes = lanes;
+    }
     int fit = per_sm[mode][whole].load(std::memory_order_relaxed);
     if (fit == 0) {
-        const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, kernels[mode][whole], kThreads, 16384);
+        const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, kernels[mode][whole], kThreads, mode == kAnywhere ? 20480 : 4096);   // (about)
         if (e != cudaSuccess) return fe2o3_cuda_status(e, what);
         if (fit < 1) fit = 1;
         per_sm[mode][whole].store(fit, std::memory_order_relaxed);
     }
+    const uint32_t at_once = kThreads / 32 * (32 / r.lanes);   // rows
     const uint32_t resident = (ctx->sm_count > 0 ? ctx->sm_count : 1) * fit;
     r.per_block = 1;
     r.parts = 1;
@@ -284,12 +299,12 @@ int32_t launch_rows(fe2o3_ctx *ctx, cudaStream_t s, const Kernel (&kernels)[3][2
         const uint64_t waves = (r.tokens + (uint64_t)resident * kMostTokens - 1) / ((uint64_t)resident * kMostTokens);
         r.per_block = ceil_div_u32(r.tokens, resident * waves);
     } else if (r.tokens) {
-        const uint32_t rounds = ceil_div_u32((uint64_t)r.rows << r.lanes_log2, kThreads);   // of a token's rows
+        const uint32_t rounds = ceil_div_u32(r.rows, at_once);   // of a token's rows
         r.parts = resident / r.tokens < rounds ? resident / r.tokens : rounds;
         if (r.parts == 0) r.parts = 1;
     }
     r.rows_inverse = r.rows <= 1 || (uint64_t)r.per_block * r.rows > 65536 || r.rows > 65536 ? 0 : (uint32_t)((0x100000000ull + r.rows - 1) / r.rows);
-    const uint32_t in_flight = mode == kAnywhere ? (kThreads >> r.lanes_log2) * 2 * r.dim * eb : 0;   // at most 16 KiB
+    const uint32_t in_flight = mode == kAnywhere ? at_once * 2 * r.dim * 4 : 0;   // at most 32 KiB
     const uint32_t grid = ceil_div_u32(r.tokens, r.per_block) * r.parts, shared = r.per_block * r.token_turns * (uint32_t)sizeof(float2) + in_flight;
     if (geo) *geo = fe2o3_geometry{{grid, 1, 1}, {kThreads, 1, 1}, shared, 1};
     if (plan_only || r.tokens == 0 || r.rows == 0) return FE2O3_OK;
@@ -336,7 +351,7 @@ int32_t launch_rotary(fe2o3_ctx *ctx, cudaStream_t s, const void *args, fe2o3_ge
     bool whole = true;
     if (a->heads) whole = on_16(a->q.ptr | a->q_output.ptr, eb * a->q_token_stride, eb * a->q_head_stride, eb * a->q_output_token_stride, eb * a->q_output_head_stride);
     if (a->kv_heads) whole = whole && on_16(a->k.ptr | a->k_output.ptr, eb * a->k_token_stride, eb * a->k_head_stride, eb * a->k_output_token_stride, eb * a->k_output_head_stride);
-    return launch_rows(ctx, s, kernels[eb == 4], whole, a->layout == FE2O3_ROTARY_INTERLEAVED, (uint32_t)eb, false, KvCache{}, r, per_sm[eb == 4], geo, plan_only, "rotary_v1");
+    return launch_rows(ctx, s, kernels[eb == 4], whole, a->layout == FE2O3_ROTARY_INTERLEAVED, (uint32_t)eb, false, false, KvCache{}, r, per_sm[eb == 4], geo, plan_only, "rotary_v1");
 }
 
 int32_t launch_kv_cache_rotary_append(fe2o3_ctx *ctx, cudaStream_t s, const void *args, fe2o3_geometry *geo, bool plan_only) {
@@ -368,7 +383,7 @@ int32_t launch_kv_cache_rotary_append(fe2o3_ctx *ctx, cudaStream_t s, const void
     bool whole = on_16(a->k.ptr | a->v.ptr, eb * a->k_token_stride, eb * a->k_head_stride, eb * a->v_token_stride, eb * a->v_head_stride);
     if (a->heads) whole = whole && on_16(a->q.ptr | a->q_output.ptr, eb * a->q_token_stride, eb * a->q_head_stride, eb * a->q_output_token_stride, eb * a->q_output_head_stride);
     const uint32_t format = four ? 3 : a->format;   // in the tables
-    return launch_rows(ctx, s, kernels[format][eb == 4], whole, a->layout == FE2O3_ROTARY_INTERLEAVED, (uint32_t)eb, four, kv_storage_of(ctx, a), r, per_sm[format][eb == 4], geo, plan_only, "kv_cache_rotary_append_v1");
+    return launch_rows(ctx, s, kernels[format][eb == 4], whole, a->layout == FE2O3_ROTARY_INTERLEAVED, (uint32_t)eb, a->format != FE2O3_KV_BF16, four, kv_storage_of(ctx, a), r, per_sm[format][eb == 4], geo, plan_only, "kv_cache_rotary_append_v1");
 }
 
 static Fe2o3KernelRegistration reg_rotary("rotary_v1", reinterpret_cast<const void *>(rotary_kernel<kPlain, false, kPieces, true>));
