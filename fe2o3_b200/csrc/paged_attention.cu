@@ -103,8 +103,13 @@ int32_t paged_attention_plan(fe2o3_ctx *ctx, const fe2o3_paged_attention_v1_args
     const uint32_t group = a->heads / a->kv_heads;
     // 16 query heads at once for a group of more than 8 (three terms of f32 queries of such long rows would not fit a block)
     const uint32_t nt = group <= 8 || (a->dim > 128 && a->format == FE2O3_KV_BF16 && a->q_dtype == FE2O3_DTYPE_F32) ? 1 : 2;
+    // Tiles of 64 keys for 4-bit rows that may be long: 32 query heads on 4 of 128, pages of 64, 96 ragged sequences of up to 6000 82 us with 32 keys
+    // and 77 with 64, two of 131071 (on 8) 113 and 102, rows of 64 columns 62 and 58; but 256 sequences of up to 500 41 and 49, and pages of 16
+    // (four boxes a tile) 91 and 98, of 32 82 and 92.
+    const uint64_t positions = (uint64_t)a->table_width * a->page_size, seen = a->window && a->window < positions ? a->window : positions;
+    const bool long_rows = a->format == FE2O3_KV_E2M1 && nt == 1 && a->dim <= 128 && a->page_size % 64 == 0 && seen >= 4096;
     const PagedBuild b = a->format == FE2O3_KV_BF16 ? paged_build_bf16(a->dim, nt) : a->format == FE2O3_KV_E4M3 ? paged_build_e4m3(a->dim, nt)
-                         : a->format == FE2O3_KV_I8 ? paged_build_i8(a->dim, nt) : paged_build_e2m1(a->dim, nt);
+                         : a->format == FE2O3_KV_I8 ? paged_build_i8(a->dim, nt) : paged_build_e2m1(a->dim, nt, long_rows);
     const uint32_t terms = a->q_dtype == FE2O3_DTYPE_BF16 ? 1 : a->format == FE2O3_KV_BF16 ? 3 : 2;
     FE2O3_CUDA(cudaSetDevice(ctx->device));
     cudaFuncAttributes attr;
@@ -124,7 +129,8 @@ int32_t paged_attention_plan(fe2o3_ctx *ctx, const fe2o3_paged_attention_v1_args
     uint32_t stages = a->format == FE2O3_KV_BF16 && a->dim == 128 && a->page_size % b.keys == 0 && stages_of(2) >= 3 ? stages_of(2) : 0;
     for (uint32_t blocks = 3; blocks && !stages; --blocks) stages = stages_of(blocks);
     if (!stages) return FE2O3_ERR_UNSUPPORTED_SHAPE;   // (not reached: one block fits for every build)
-    if (stages > kPagedMaxStages) stages = kPagedMaxStages;
+    const uint32_t most_stages = a->format == FE2O3_KV_E2M1 ? kPagedMaxStages4 : kPagedMaxStages;
+    if (stages > most_stages) stages = most_stages;
     PagedPlan *p = new (std::nothrow) PagedPlan();
     if (!p) return FE2O3_ERR_SIZE_OVERFLOW;
     p->kernel = b.kernel;

@@ -58,7 +58,7 @@ struct PagedArgs {
 // The partial results of a block in the workspace: the end of an item that began in an earlier block, the beginning of one that
 // goes on in the next, and the ends that its warps 1 to 3 found of items that an earlier warp of the block began.
 constexpr uint32_t kPagedSlots = 5, kSlotFirst = 0, kSlotLast = 1, kSlotEnds = 2;
-constexpr uint32_t kPagedMaxStages = 6, kPagedMeeting = 640;
+constexpr uint32_t kPagedMaxStages = 4, kPagedMaxStages4 = 6, kPagedMeeting = 512;   // kPagedMaxStages4: of 4-bit rows, whose stages are small
 
 using PagedKernel = void (*)(CUtensorMap, CUtensorMap, PagedArgs);
 struct PagedBuild {
@@ -69,7 +69,7 @@ struct PagedBuild {
 PagedBuild paged_build_bf16(uint32_t dim, uint32_t nt);
 PagedBuild paged_build_e4m3(uint32_t dim, uint32_t nt);
 PagedBuild paged_build_i8(uint32_t dim, uint32_t nt);
-PagedBuild paged_build_e2m1(uint32_t dim, uint32_t nt);
+PagedBuild paged_build_e2m1(uint32_t dim, uint32_t nt, bool long_rows);
 
 namespace {
 
@@ -81,11 +81,12 @@ constexpr float kLeastTerm = 0x1p-40f;   // of a number, the least that its lowe
 constexpr float kSlack = 8.f;          // 4 bits: what a score may lie above the maximum kept (log2) before that moves: a probability is up to 2^8 then
 constexpr int kQueryExponent = 14;    // f16 queries: the largest of a row lies in [2^14, 2^15)
 
-template <uint32_t FORMAT, int DP, int NT>
+// LONG: tiles of 64 keys on two blocks an SM, for long rows of a 4-bit cache (see paged_attention_plan).
+template <uint32_t FORMAT, int DP, int NT, bool LONG = false>
 struct Shape {
     static constexpr bool kF16 = FORMAT != FE2O3_KV_BF16, kFour = FORMAT == FE2O3_KV_E2M1;
     static constexpr int kRow = kv_bytes<FORMAT>(DP);                                       // bytes of a row in a stage
-    static constexpr int kKeys = kF16 ? (DP == 256 ? 16 : 32) : (DP == 64 ? 32 : 16);       // of a tile
+    static constexpr int kKeys = LONG ? 64 : kF16 ? (DP == 256 ? 16 : 32) : (DP == 64 ? 32 : 16);       // of a tile
     static constexpr int kStage = 2 * kKeys * kRow;                                         // K, V: whole swizzle patterns
     static constexpr int kBlocks = kFour ? kKeys * DP / 16 : 0;                             // block scales of K, and of V
     static constexpr int kScales = (kF16 ? 8 * kKeys : 0) + 2 * kBlocks;                    // of the rows of K, of V; then the blocks'
@@ -331,16 +332,20 @@ struct Line {
     __device__ __forceinline__ uint32_t taken(uint32_t some, uint32_t places) const {
         return places > whole || some >= places ? min(some, places) : 2 * some >= places ? places : 0;
     }
-    __device__ __forceinline__ uint32_t block_of(uint64_t place) const { return (uint32_t)(((place + 1) * blocks - 1) / total); }
+    __device__ static __forceinline__ uint32_t block_of(uint64_t place, uint64_t total, uint32_t blocks) { return (uint32_t)(((place + 1) * blocks - 1) / total); }
 };
 // What a block has in shared memory beside rings and queries (all of it in the dynamic part, which then starts on a swizzle pattern).
+template <bool FOUR>
 struct Meeting {
-    uint64_t arrivals[kPagedWarps][kPagedMaxStages];
+    uint64_t arrivals[kPagedWarps][FOUR ? kPagedMaxStages4 : kPagedMaxStages];
     Left left[kPagedWarps];
+    Job first;       // where warp 0 begins, should an item of an earlier block end there
+    uint64_t total;  // of the line (kept here and not in registers through all tiles)
+    uint32_t blocks;
     Job jobs[2];
     bool goes_on;
 };
-static_assert(sizeof(Meeting) <= kPagedMeeting, "");
+static_assert(sizeof(Meeting<false>) <= kPagedMeeting && sizeof(Meeting<true>) <= kPagedMeeting, "");
 // A sequence's keys as tiles, counted from a multiple of KT.  One that does not fit its table is reported and has none.
 template <int KT>
 struct Span {
@@ -411,10 +416,10 @@ struct Part {
     }
 };
 
-template <uint32_t FORMAT, int DP, int NT>
-__global__ void __launch_bounds__(kPagedThreads, DP == 256 || NT == 2 ? 1 : 3)
+template <uint32_t FORMAT, int DP, int NT, bool LONG = false>
+__global__ void __launch_bounds__(kPagedThreads, DP == 256 || NT == 2 ? 1 : LONG ? 2 : 3)
 paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ PagedArgs a) {
-    using S = Shape<FORMAT, DP, NT>;
+    using S = Shape<FORMAT, DP, NT, LONG>;
     using P = Part<DP / 16, NT>;
     constexpr int KT = S::kKeys, MT = KT / 16, MD = DP / 16, kPieces = S::kRow / 16, kRowsAtOnce = 32 / kPieces;
     constexpr bool F16 = S::kF16, F4 = S::kFour;
@@ -427,7 +432,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     uint8_t *const queries = smem + kPagedWarps * a.stages * (S::kStage + S::kScales);
     const uint32_t term_bytes = a.q_rows * S::kQueryRow;
     uint8_t *const query = queries + warp * terms * term_bytes;
-    Meeting &meeting = *reinterpret_cast<Meeting *>(queries + kPagedWarps * terms * term_bytes);
+    Meeting<F4> &meeting = *reinterpret_cast<Meeting<F4> *>(queries + kPagedWarps * terms * term_bytes);
     const uint32_t query_s = smem_u32(query);
     const uint32_t row_bytes = kv_bytes<FORMAT>(a.c.dim), row_blocks = a.c.dim / 16;   // (4 bits: block scales of a row)
     const uint32_t per_seq = a.c.kv_heads * a.chunks;   // items of a sequence
@@ -763,8 +768,14 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         place = 0;
     }
     Span<KT> span = lspan;
+    // (4 bits: what is wanted at the end lies in shared memory until then, and the products have its registers.)
     const Span<KT> first_span = span;
     const uint32_t first_seq = seq, first_item = item, first_place = place;
+    if (F4 && threadIdx.x == 0) {
+        meeting.first = Job{seq, item, span.valid ? span.n : kInvalid, span.places(), 0, 0, 0, begin - place};
+        meeting.total = line.total;
+        meeting.blocks = line.blocks;
+    }
     lseq = seq;
     litem = item;
     lrest = share;
@@ -783,8 +794,9 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     // ---- the share, item by item ----
     P p;
     uint32_t kind = share ? kNone : kEmpty;
-    uint64_t i0 = 0;        // where on the line the last item begins
     uint32_t end_of_first = 0;
+    uint64_t i0 = 0;        // where on the line the last item begins
+    if (F4 && lane == 0) meeting.left[warp].i0 = 0;
     for (uint32_t at = 0; at < share;) {
         const uint32_t here = place ? min(span.places() - place, share - at) : line.taken(share - at, span.places());
         if (here == 0) break;   // the next warp has it all
@@ -870,17 +882,19 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                         }
             } else if constexpr (F4) {
                 float low[MT][NT][4];
-                constexpr int kRuns = DP == 256 ? 2 : 1, kWords = DP == 64 ? 2 : 4;   // runs of a lane's columns, words of eight in one
+                constexpr int kAtOnce = MT < 2 ? MT : 2, kRuns = DP == 256 ? 2 : 1, kWords = DP == 64 ? 2 : 4;   // runs of a lane's columns, words of eight in one
                 const uint32_t blocks = smem_u32(my_scales) + slot * S::kScales + 8 * KT;
 #pragma unroll
-                for (int run = 0; run < kRuns; ++run) {
-                    uint4 ka[MT][2];
-                    uint32_t ks[MT][2];   // scales of the run's blocks (of 64 columns one)
+                for (int m0 = 0; m0 < MT; m0 += kAtOnce)   // (more rows at once cost registers)
 #pragma unroll
-                    for (int mt = 0; mt < MT; ++mt)
+                for (int run = 0; run < kRuns; ++run) {
+                    uint4 ka[kAtOnce][2];
+                    uint32_t ks[kAtOnce][2];   // scales of the run's blocks (of 64 columns one)
+#pragma unroll
+                    for (int mt = 0; mt < kAtOnce; ++mt)
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {
-                            const uint32_t row = 16 * mt + 8 * e, at = from + k_off[run] + row * S::kPitch, scale = blocks + (row + gk) * row_blocks;
+                            const uint32_t row = 16 * (m0 + mt) + 8 * e, at = from + k_off[run] + row * S::kPitch, scale = blocks + (row + gk) * row_blocks;
                             if constexpr (DP == 64) {
                                 const uint2 v = lds64(at);
                                 ka[mt][e] = make_uint4(v.x, v.y, 0, 0);
@@ -892,9 +906,9 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                         }
 #pragma unroll
                     for (int word = 0; word < kWords; ++word) {
-                        uint32_t kf[MT][2][4];
+                        uint32_t kf[kAtOnce][2][4];
 #pragma unroll
-                        for (int mt = 0; mt < MT; ++mt)
+                        for (int mt = 0; mt < kAtOnce; ++mt)
 #pragma unroll
                             for (int e = 0; e < 2; ++e) {
                                 const uint4 &v = ka[mt][e];
@@ -913,18 +927,18 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                             const uint32_t at_q = q_off[nt] + 128 * (all >> 1) + 16 * (all & 1);
                             const uint4 qb = lds128(at_q);
 #pragma unroll
-                            for (int mt = 0; mt < MT; ++mt) {
-                                if (first) mma_first<true>(s[mt][nt], kf[mt][0], qb.x, qb.y);
-                                else mma<true>(s[mt][nt], kf[mt][0], qb.x, qb.y);
-                                mma<true>(s[mt][nt], kf[mt][1], qb.z, qb.w);
+                            for (int mt = 0; mt < kAtOnce; ++mt) {
+                                if (first) mma_first<true>(s[m0 + mt][nt], kf[mt][0], qb.x, qb.y);
+                                else mma<true>(s[m0 + mt][nt], kf[mt][0], qb.x, qb.y);
+                                mma<true>(s[m0 + mt][nt], kf[mt][1], qb.z, qb.w);
                             }
                             if (terms > 1) {
                                 const uint4 ql = lds128(at_q + term_bytes);
 #pragma unroll
-                                for (int mt = 0; mt < MT; ++mt) {
-                                    if (first) mma_first<true>(low[mt][nt], kf[mt][0], ql.x, ql.y);
-                                    else mma<true>(low[mt][nt], kf[mt][0], ql.x, ql.y);
-                                    mma<true>(low[mt][nt], kf[mt][1], ql.z, ql.w);
+                                for (int mt = 0; mt < kAtOnce; ++mt) {
+                                    if (first) mma_first<true>(low[m0 + mt][nt], kf[mt][0], ql.x, ql.y);
+                                    else mma<true>(low[m0 + mt][nt], kf[mt][0], ql.x, ql.y);
+                                    mma<true>(low[m0 + mt][nt], kf[mt][1], ql.z, ql.w);
                                 }
                             }
                         }
@@ -1180,27 +1194,60 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
 
             // output: rows are its columns, columns heads; the tile's sum is the tensor unit's, the rest f32
             uint4 v4[F4 ? 1 : MT][4][F16 && DP == 256 ? 2 : 1];
-            constexpr int kRuns4 = DP == 256 ? 2 : 1;
-            uint2 w4[F4 ? MT : 1][4][kRuns4];       // 4 bits: the lane's columns of four keys
-            uint32_t vs4[F4 ? MT : 1][2][kRuns4];   // and the scales of two keys' blocks
-            uint32_t lo4[F4 ? MT : 1][2], hi4[F4 ? MT : 1][2];   // codes of two keys side by side: even columns, odd ones
             if constexpr (F4) {
+                constexpr int kAtOnce = MT < 2 ? MT : 2, kRuns = DP == 256 ? 2 : 1, kTiles = MD / kRuns;   // kTiles: of a run of the lane's columns
                 const uint32_t blocks = smem_u32(my_scales) + slot * S::kScales + 8 * KT + S::kBlocks, k0 = key_of<FORMAT, DP>(2 * t4);
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
+                for (int m0 = 0; m0 < MT; m0 += kAtOnce)
 #pragma unroll
-                    for (int run = 0; run < kRuns4; ++run) {
+                    for (int run = 0; run < kRuns; ++run) {
                         const uint32_t block = (DP == 64 ? g >> 1 : g) + 8 * run;
+                        uint2 w4[kAtOnce][4];       // the lane's columns of four keys
+                        uint32_t vs4[kAtOnce][2];   // and the scales of two keys' blocks
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const uint32_t at = from + v_off[(e & 1) + 2 * run] + (16 * mt + 8 * (e >> 1)) * S::kPitch;
-                            if constexpr (DP == 64) w4[mt][e][run] = make_uint2(lds32(at), 0);
-                            else w4[mt][e][run] = lds64(at);
+                        for (int mt = 0; mt < kAtOnce; ++mt) {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const uint32_t at = from + v_off[(e & 1) + 2 * run] + (16 * (m0 + mt) + 8 * (e >> 1)) * S::kPitch;
+                                if constexpr (DP == 64) w4[mt][e] = make_uint2(lds32(at), 0);
+                                else w4[mt][e] = lds64(at);
+                            }
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                const uint32_t at = blocks + (16 * (m0 + mt) + 8 * e) * row_blocks + block;
+                                vs4[mt][e] = scales_f16(block < row_blocks ? lds8(at + k0 * row_blocks) | lds8(at + (k0 ^ 1) * row_blocks) << 8 : 0u);
+                            }
                         }
+                        uint32_t lo4[kAtOnce][2], hi4[kAtOnce][2];   // codes of two keys side by side: even columns, odd ones
 #pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const uint32_t at = blocks + (16 * mt + 8 * e) * row_blocks + block;
-                            vs4[mt][e][run] = scales_f16(block < row_blocks ? lds8(at + k0 * row_blocks) | lds8(at + (k0 ^ 1) * row_blocks) << 8 : 0u);
+                        for (int i = 0; i < kTiles; ++i) {
+                            uint32_t va[kAtOnce][4];
+#pragma unroll
+                            for (int mt = 0; mt < kAtOnce; ++mt)
+#pragma unroll
+                                for (int e = 0; e < 2; ++e) {
+                                    if (i % 4 == 0) {
+                                        const uint32_t w0 = i / 4 ? w4[mt][2 * e].y : w4[mt][2 * e].x, w1 = i / 4 ? w4[mt][2 * e + 1].y : w4[mt][2 * e + 1].x;
+                                        lo4[mt][e] = (w0 & 0x0f0f0f0fu) | (w1 << 4 & 0xf0f0f0f0u);
+                                        hi4[mt][e] = (w0 >> 4 & 0x0f0f0f0fu) | (w1 & 0xf0f0f0f0u);
+                                    }
+                                    va[mt][2 * e] = times_f16(code4_pair(lo4[mt][e], i % 4), vs4[mt][e]);
+                                    va[mt][2 * e + 1] = times_f16(code4_pair(hi4[mt][e], i % 4), vs4[mt][e]);
+                                }
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt) {
+                                float d[4];
+#pragma unroll
+                                for (int mt = 0; mt < kAtOnce; ++mt) {
+                                    if (mt == 0) mma_first<true>(d, va[mt], pb[m0 + mt][nt][1][0], pb[m0 + mt][nt][1][1]);
+                                    else mma<true>(d, va[mt], pb[m0 + mt][nt][1][0], pb[m0 + mt][nt][1][1]);
+                                    mma<true>(d, va[mt], pb[m0 + mt][nt][0][0], pb[m0 + mt][nt][0][1]);
+                                }
+                                float (&o)[4] = p.o[run * kTiles + i][nt];
+                                const uint64_t d01 = pack_f32x2(d[0], d[1]), d23 = pack_f32x2(d[2], d[3]), o01 = pack_f32x2(o[0], o[1]), o23 = pack_f32x2(o[2], o[3]);
+                                unpack_f32x2(m0 ? add_f32x2(o01, d01) : fma_f32x2(o01, scale_o[nt], d01), o[0], o[1]);
+                                unpack_f32x2(m0 ? add_f32x2(o23, d23) : fma_f32x2(o23, scale_o[nt], d23), o[2], o[3]);
+                            }
                         }
                     }
             } else if constexpr (F16) {
@@ -1218,25 +1265,11 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                     }
             }
 #pragma unroll
-            for (int i = 0; i < MD; ++i) {
+            for (int i = 0; i < (F4 ? 0 : MD); ++i) {
                 uint32_t va[MT][4];
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) {
-                    if constexpr (F4) {
-                        constexpr int kColumns = DP == 256 ? 8 : MD;   // tiles of a run
-                        const int run = i / kColumns, word = i % kColumns / 4, byte = i % 4;
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            if (byte == 0) {
-                                const uint2 a2 = w4[mt][2 * e][run], b2 = w4[mt][2 * e + 1][run];
-                                const uint32_t w0 = word ? a2.y : a2.x, w1 = word ? b2.y : b2.x;
-                                lo4[mt][e] = (w0 & 0x0f0f0f0fu) | (w1 << 4 & 0xf0f0f0f0u);
-                                hi4[mt][e] = (w0 >> 4 & 0x0f0f0f0fu) | (w1 & 0xf0f0f0f0u);
-                            }
-                            va[mt][2 * e] = times_f16(code4_pair(lo4[mt][e], byte), vs4[mt][e][run]);
-                            va[mt][2 * e + 1] = times_f16(code4_pair(hi4[mt][e], byte), vs4[mt][e][run]);
-                        }
-                    } else if constexpr (F16) {
+                    if constexpr (F16) {
                         uint32_t w[4];
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
@@ -1298,7 +1331,8 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
             }
         }
         const bool begins = place == 0, ended = place + here == span.places();
-        i0 = begin + at - place;
+        if constexpr (!F4) i0 = begin + at - place;
+        else if (lane == 0) meeting.left[warp].i0 = begin + at - place;
         if (ended) {
             if (!begins) {
                 float4 *const to = slots + (warp ? kSlotEnds + warp - 1 : kSlotFirst) * S::kPart * 32;
@@ -1333,7 +1367,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         __syncwarp();
         p.leave([&](int i, float4 v) { my_part[i * 32] = v; });
     }
-    if (lane == 0) meeting.left[warp] = Left{kind, end_of_first, seq, item, span.valid ? span.n : kInvalid, span.places(), i0};
+    if (lane == 0) meeting.left[warp] = Left{kind, end_of_first, seq, item, span.valid ? span.n : kInvalid, span.places(), F4 ? meeting.left[warp].i0 : i0};
     if (threadIdx.x < 2) meeting.jobs[threadIdx.x].pieces = 0;
     __threadfence_block();
     __syncthreads();
@@ -1370,7 +1404,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         }
     }
     if (threadIdx.x == 0 && end_of_first)   // an item of an earlier block that ended in warp 0: it lies in its slot
-        meeting.jobs[0] = Job{first_seq, first_item, first_span.valid ? first_span.n : kInvalid, first_span.places(), 0, 0, 0, begin - first_place};
+        meeting.jobs[0] = F4 ? meeting.first : Job{first_seq, first_item, first_span.valid ? first_span.n : kInvalid, first_span.places(), 0, 0, 0, begin - first_place};
 
     // ---- the blocks: the last one to come joins the pieces, of many pieces in two steps: 16 neighbours, then those ----
     __threadfence();
@@ -1378,7 +1412,9 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     if (threadIdx.x < 2) {
         Job &job = meeting.jobs[threadIdx.x];
         if (job.pieces) {
-            const uint32_t b0 = line.block_of(job.i0), pieces = line.block_of(job.i0 + job.pieces - 1) - b0 + 1;
+            const uint64_t total = F4 ? meeting.total : line.total;
+            const uint32_t blocks = F4 ? meeting.blocks : line.blocks;
+            const uint32_t b0 = Line::block_of(job.i0, total, blocks), pieces = Line::block_of(job.i0 + job.pieces - 1, total, blocks) - b0 + 1;
             const uint32_t group = (blockIdx.x - b0) / kGroup, groups = (pieces + kGroup - 1) / kGroup;
             job.block = b0;
             job.first = b0 + group * kGroup;
@@ -1436,10 +1472,10 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     }
 }
 
-template <uint32_t FORMAT, int DP, int NT>
+template <uint32_t FORMAT, int DP, int NT, bool LONG = false>
 PagedBuild paged_build() {
-    using S = Shape<FORMAT, DP, NT>;
-    return PagedBuild{paged_attention_kernel<FORMAT, DP, NT>, (uint32_t)S::kStage, (uint32_t)S::kPart * 512u, (uint32_t)S::kQueryRow,
+    using S = Shape<FORMAT, DP, NT, LONG>;
+    return PagedBuild{paged_attention_kernel<FORMAT, DP, NT, LONG>, (uint32_t)S::kStage, (uint32_t)S::kPart * 512u, (uint32_t)S::kQueryRow,
                       (uint32_t)S::kScales, (uint32_t)S::kKeys};
 }
 template <uint32_t FORMAT>

@@ -280,6 +280,20 @@ def test_attention_split_and_joined(gpu, lengths, heads, kv_heads, dim):  # noqa
     assert (got == again).all() and (lse == lse2).all()
 
 
+@pytest.mark.parametrize("dim", [32, 64, 96, 128])
+@pytest.mark.parametrize("group,dtype", [(1, "bf16"), (4, "f32"), (8, "bf16")])
+def test_attention_tables_with_room_for_long_rows(gpu, dim, group, dtype):  # noqa: F811
+    """Tables of 4096 positions and more, in pages of whole tiles of 64 keys: lengths around those, empty ones, windows, pieces that blocks join."""
+    for page, lengths in ((64, EDGES + [1000, 4096, 4500]), (128, [9000, 0, 1, 8999, 20]), (192, [64] * 33 + [5000] + [0] * 9)):
+        c = filled(gpu, lengths, 2, dim, page, width=-(-9100 // page))
+        q, qv = queries(c.torch, len(lengths), 2 * group, dim, dtype)
+        for window in (0, 4100):
+            got, lse = attend(c, q, dim ** -0.5, window=window)
+            check_attention(c, qv, got, lse, attention64(c, qv, f32(dim ** -0.5), window), "f32")
+        again, lse2 = attend(c, q, dim ** -0.5, window=4100)
+        assert (got == again).all() and (lse == lse2).all()
+
+
 @pytest.mark.parametrize("octaves", [10, 20, 30, 45, 60])
 def test_attention_values_of_unlike_size(gpu, octaves):  # noqa: F811
     """A row of values far larger than the others, which one head gives next to no weight and another next to all of it.  (No value of it is small
