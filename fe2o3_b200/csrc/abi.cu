@@ -736,8 +736,10 @@ int regions_for(uint32_t op, const void *args, Region *r, int32_t *status) {
                 *status = unsupported("kv_pages_v1 needs batch <= 8192, page_size >= 1, batch * table_width and the rows of all pages below 2^32");
                 return 0;
             }
+            const bool each = !a->counts.ptr && !a->counts.len, mapped = a->positions.ptr || a->positions.len || a->slots.ptr || a->slots.len;
+            if (each && mapped && a->tokens < a->batch) { *status = unsupported("without counts positions and slots have a row for every sequence: tokens >= batch"); return 0; }
             int n = 0;
-            if (a->counts.ptr || a->counts.len) r[n++] = RGN("Counts", a->counts, a->batch, 4, false);
+            if (!each) r[n++] = RGN("Counts", a->counts, a->batch, 4, false);
             if (a->release.ptr || a->release.len) r[n++] = RGN("Release", a->release, a->batch, 4, false);
             if (!same_slice(a->lengths, a->next_lengths)) r[n++] = RGN("Lengths", a->lengths, a->batch, 4, false);
             if (!same_slice(a->free_count, a->next_free_count)) r[n++] = RGN("FreeCount", a->free_count, 1, 4, false);

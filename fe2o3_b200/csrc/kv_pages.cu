@@ -94,7 +94,7 @@ __global__ void __launch_bounds__(kMaxThreads) kv_pages_kernel(PagesArgs a) {
     }
     __syncthreads();
     const Sums total = carry;
-    const bool too_long = bad || total.tokens > 0xffffffffull || ((a.positions || a.slots) && total.tokens > a.tokens);
+    const bool too_long = bad || total.tokens > 0xffffffffull || (a.counts && (a.positions || a.slots) && total.tokens > a.tokens);
     const uint64_t top = (uint64_t)count + total.back;
     const bool fits = !too_long && top <= a.pages && total.fresh <= top;
     if (!fits && thread == 0) kstatus_set(a.status, too_long ? FE2O3_KSTATUS_LENGTH : FE2O3_KSTATUS_PAGES);
@@ -136,17 +136,17 @@ __global__ void __launch_bounds__(kMaxThreads) kv_pages_kernel(PagesArgs a) {
             a.table[(uint64_t)b * a.width + pages_for(a, places[b].length) + (i - places[b].first_page)] = a.free_pages[top - 1 - i];
         }
     if (!a.positions && !a.slots) return;
-    const uint32_t tokens = fits ? (uint32_t)total.tokens : 0;
+    const uint32_t tokens = !fits ? 0 : a.counts ? (uint32_t)total.tokens : a.batch;   // (without counts row b is sequence b's)
     const bool whole = ((reinterpret_cast<uint64_t>(a.positions) | reinterpret_cast<uint64_t>(a.slots)) & 15) == 0;
     for (uint64_t t0 = (uint64_t)thread * kAtOnce; t0 < a.tokens; t0 += (uint64_t)threads * kAtOnce) {
         uint32_t position[kAtOnce], slot[kAtOnce];
         const uint32_t *from[kAtOnce];   // the number of the position's page
-        uint32_t b = t0 < tokens ? find((uint32_t)t0, &Place::first_token) : 0;
+        uint32_t b = t0 >= tokens ? 0 : a.counts ? find((uint32_t)t0, &Place::first_token) : (uint32_t)t0;
         Place p{0, 0, 0, 0};
         uint32_t end = 0, held = 0;
         if (t0 < tokens) {
             p = places[b];
-            end = b + 1 < a.batch ? places[b + 1].first_token : tokens;
+            end = !a.counts ? b + 1 : b + 1 < a.batch ? places[b + 1].first_token : tokens;
             held = pages_for(a, p.length);
         }
 #pragma unroll
@@ -158,10 +158,11 @@ __global__ void __launch_bounds__(kMaxThreads) kv_pages_kernel(PagesArgs a) {
             if (t0 + i >= tokens) continue;
             while (t >= end) {
                 p = places[++b];
-                end = b + 1 < a.batch ? places[b + 1].first_token : tokens;
+                end = !a.counts ? b + 1 : b + 1 < a.batch ? places[b + 1].first_token : tokens;
                 held = pages_for(a, p.length);
             }
-            position[i] = p.length + (t - p.first_token);
+            if (!a.counts && !p.length) continue;
+            position[i] = p.length + (a.counts ? t - p.first_token : 0);
             const uint32_t page = page_of(a, position[i]);
             from[i] = page < held ? a.table + (uint64_t)b * a.width + page : a.free_pages + (top - 1 - p.first_page - (page - held));
             slot[i] = position[i] - page * a.page_size;

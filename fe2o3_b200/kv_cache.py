@@ -1,9 +1,9 @@
 """A paged key-value cache and the decode step over it, for serving.
 
-`PageTable` is the host's book of pages (no GPU).  `PagedKvCache` owns the cache's device memory in one of three formats
-and launches the library's operators on it: `append` writes new tokens' keys and values, `attend` lets one new token a
+`PageTable` is the host's book of pages (no GPU), `DevicePages` one on the device, whose steps need nothing from the host and can be
+captured in a CUDA graph.  `PagedKvCache` owns the cache's device memory in one of four formats and launches the library's operators on it: `append` writes new tokens' keys and values, `attend` lets one new token a
 sequence attend to all its positions, `read` brings rows back.  `DecodeStep` binds the tensors of a step once, so that a
-step is two launches and the copy of the lengths; a step in which a sequence begins a page copies the whole page table too
+step is two launches and the copy of the lengths, or three launches with a book on the device; a step in which a sequence begins a page copies the whole page table too
 (4 bytes a page that the table has room for), from ordinary memory.
 
     cache = PagedKvCache(ctx, stream, sequences=8, positions=4096, kv_heads=8, dim=128, format=KV_E4M3)
@@ -13,6 +13,11 @@ step is two launches and the copy of the lengths; a step in which a sequence beg
     for _ in range(n):                          # fill q, k1, v1 on the stream, then
         step.run()
 
+    cache = PagedKvCache(ctx, stream, 8, 4096, 8, 128, format=KV_E2M1, tokens=8 * prompt_length)   # with a book on the device
+    cache.extend([prompt_length] * 8)
+    cache.append(k, v, q=q, q_out=turned, rotary=rotary)   # rotary positions on the way
+    step = DecodeStep(cache, q1, k1, v1, out, heads=32, rotary=rotary)
+
 `append`, `extend`, `release` and the steps are enqueued on the cache's stream and do not wait for its launches (but a copy from
 ordinary memory may hold the host until the stream has come to it, once it is larger than the driver keeps aside).  What waits:
 preparing an attention (`attention`, `DecodeStep`) for the legacy stream, destroying one for the whole device, `attend`, which
@@ -20,7 +25,7 @@ does both, and `read` for the cache's stream.
 """
 import numpy as np
 
-from . import DTYPE_BF16, DTYPE_F32, KV_BF16, KV_E4M3, KV_I8, DeviceBuffer, prepare
+from . import DTYPE_BF16, DTYPE_F32, KV_BF16, KV_E2M1, KV_E4M3, KV_I8, DeviceBuffer, prepare
 
 
 class PageTable:
@@ -60,6 +65,50 @@ class PageTable:
         self.lengths[sequence] = 0
 
 
+class DevicePages:
+    """The same book on the device (`kv_pages_v1`): pages go out and come back in the same order.  What does not fit is found there too: it is reported
+    (`ctx.take_kernel_status`), and nothing changes.  `tokens`: the most new tokens of an `extend`."""
+
+    def __init__(self, ctx, stream, sequences, positions, pages, page_size, tokens):
+        if min(sequences, positions, pages, page_size, tokens) < 1:
+            raise ValueError("sequences, positions, pages, page_size and tokens are at least 1")
+        self.stream, self.width, self.tokens = stream, -(-positions // page_size), tokens
+        self.table = DeviceBuffer.from_host(stream, np.full((sequences, self.width), PageTable.FREE, np.uint32))
+        self.free_pages = DeviceBuffer.from_host(stream, np.arange(pages - 1, -1, -1, dtype=np.uint32))
+        self.free_count = DeviceBuffer.from_host(stream, np.array([pages], np.uint32))
+        zeros = lambda n: DeviceBuffer.zeroed(stream, n, np.uint32)  # noqa: E731
+        self.lengths, self.counts, self.released, self.offsets = zeros(sequences), zeros(sequences), zeros(sequences), zeros(sequences + 1)
+        # of an extend's new tokens; and of a step's, a row for every sequence
+        self.positions, self.slots, self.step_positions, self.step_slots = zeros(tokens), zeros(tokens), zeros(sequences), zeros(sequences)
+        same = dict(lengths=self.lengths, next_lengths=self.lengths, free_count=self.free_count, next_free_count=self.free_count, page_table=self.table,
+                    free_pages=self.free_pages, batch=sequences, table_width=self.width, page_size=page_size)
+        self._extend = prepare(ctx, "kv_pages_v1", counts=self.counts, release=self.released, token_offsets=self.offsets, positions=self.positions,
+                               slots=self.slots, tokens=tokens, **same)
+        self._step = prepare(ctx, "kv_pages_v1", positions=self.step_positions, slots=self.step_slots, tokens=sequences, **same)
+
+    def extend(self, counts, release=None):
+        """Places for `counts[b]` new tokens of every sequence b, after those of `release` (truth values) have given their pages back."""
+        n = len(self.lengths)
+        counts, release = np.asarray(counts), np.zeros(n, np.uint32) if release is None else np.asarray(release).astype(bool).astype(np.uint32)
+        if counts.shape != (n,) or release.shape != (n,) or (counts < 0).any() or int(counts.astype(np.int64).sum()) > self.tokens:
+            raise ValueError(f"counts has one number, at least 0, for each of the {n} sequences, and no more than {self.tokens} in all")
+        # (arrays in ordinary memory: the copies have read them when the calls return)
+        self.counts.copy_from_host_async(self.stream, counts.astype(np.uint32))
+        self.released.copy_from_host_async(self.stream, release)
+        self._extend.launch(self.stream)
+
+    def step(self, stream=None):
+        """A place for one new token of every sequence at work (of length above 0)."""
+        self._step.launch(stream or self.stream)
+
+    def free(self):
+        self._extend.destroy()
+        self._step.destroy()
+        for b in (self.table, self.free_pages, self.free_count, self.lengths, self.counts, self.released, self.offsets, self.positions, self.slots,
+                  self.step_positions, self.step_slots):
+            b.free()
+
+
 def _float_dtype(x, dtype):
     """DTYPE_* of rows: by the tensor's own type, or as said."""
     if dtype is not None:
@@ -87,27 +136,38 @@ def _pair_dtype(k, v, dtype):
 
 
 class PagedKvCache:
-    def __init__(self, ctx, stream, sequences, positions, kv_heads, dim, page_size=16, pages=None, format=KV_BF16):
+    def __init__(self, ctx, stream, sequences, positions, kv_heads, dim, page_size=16, pages=None, format=KV_BF16, tokens=None):
         """Room for `sequences` of up to `positions` tokens each in `pages` pages (default: enough for all at their
-        longest)."""
+        longest).  With `tokens`, the most new tokens of one `extend`, the book of pages lies on the device."""
+        if format == KV_E2M1 and (dim % 32 or page_size % 8):
+            raise ValueError("a 4-bit cache has dim a multiple of 32 and page_size one of 8")
         self.ctx, self.stream, self.format = ctx, stream, format
         pages = sequences * -(-positions // page_size) if pages is None else pages
-        self.table = PageTable(sequences, positions, pages, page_size)
         self.sequences, self.kv_heads, self.dim, self.page_size = sequences, kv_heads, dim, page_size
         rows = pages * kv_heads * page_size
-        element = {KV_BF16: np.uint16, KV_E4M3: np.uint8, KV_I8: np.int8}[format]
-        self.k_cache, self.v_cache = (DeviceBuffer.zeroed(stream, rows * dim, element) for _ in range(2))
+        element = {KV_BF16: np.uint16, KV_E4M3: np.uint8, KV_I8: np.int8, KV_E2M1: np.uint8}[format]
+        row = dim * 9 // 16 if format == KV_E2M1 else dim   # elements
+        self.k_cache, self.v_cache = (DeviceBuffer.zeroed(stream, rows * row, element) for _ in range(2))
         self.k_scales, self.v_scales = ((DeviceBuffer.zeroed(stream, rows, np.float32) if format != KV_BF16 else None) for _ in range(2))
+        self.new_tokens = 0
+        if tokens is not None:
+            self.table, self.pages = None, DevicePages(ctx, stream, sequences, positions, pages, page_size, tokens)
+            self.device_table, self.device_lengths, self.device_offsets = self.pages.table, self.pages.lengths, self.pages.offsets
+            self.table_width = self.pages.width
+            return
+        self.table, self.pages = PageTable(sequences, positions, pages, page_size), None
+        self.table_width = self.table.entries.shape[1]
         self.device_table = DeviceBuffer.from_host(stream, self.table.entries)
         self.device_lengths = DeviceBuffer.from_host(stream, self.table.lengths)
         self.device_offsets = DeviceBuffer.zeroed(stream, sequences + 1, np.uint32)
-        self.new_tokens = 0
+
+    def _storage(self):
+        return dict(k_cache=self.k_cache, v_cache=self.v_cache, k_scales=self.k_scales, v_scales=self.v_scales, kv_heads=self.kv_heads, dim=self.dim,
+                    page_size=self.page_size, format=self.format)
 
     def args(self):
         """The cache's own arguments of the three operators."""
-        return dict(k_cache=self.k_cache, v_cache=self.v_cache, k_scales=self.k_scales, v_scales=self.v_scales, page_table=self.device_table,
-                    lengths=self.device_lengths, batch=self.sequences, kv_heads=self.kv_heads, dim=self.dim, page_size=self.page_size,
-                    table_width=self.table.entries.shape[1], format=self.format)
+        return dict(page_table=self.device_table, lengths=self.device_lengths, batch=self.sequences, table_width=self.table_width, **self._storage())
 
     def _upload(self, pages_changed=True):
         # (arrays in ordinary memory: the copies have read them when the calls return)
@@ -115,17 +175,29 @@ class PagedKvCache:
             self.device_table.copy_from_host_async(self.stream, self.table.entries)
         self.device_lengths.copy_from_host_async(self.stream, self.table.lengths)
 
-    def extend(self, counts):
-        """Positions for new tokens of every sequence; `append` then writes them."""
+    def extend(self, counts, release=None):
+        """Positions for new tokens of every sequence; `append` then writes them.  (release: with a book on the device, sequences that give their
+        pages back first.)"""
+        if self.pages:
+            self.pages.extend(counts, release)
+            self.new_tokens = int(np.sum(counts))
+            return
+        if release is not None:
+            for b in np.nonzero(np.asarray(release))[0]:
+                self.table.release(int(b))
         before = len(self.table.free)
         self.table.extend(counts)
         offsets = np.zeros(self.sequences + 1, np.uint32)
         offsets[1:] = np.cumsum(counts)
         self.new_tokens = int(offsets[-1])
-        self._upload(len(self.table.free) != before)
+        self._upload(len(self.table.free) != before or release is not None)
         self.device_offsets.copy_from_host_async(self.stream, offsets)
 
     def release(self, sequence):
+        if self.pages:
+            self.pages.extend([0] * self.sequences, [b == sequence for b in range(self.sequences)])
+            self.new_tokens = 0
+            return
         self.table.release(sequence)
         self._upload()
 
@@ -142,9 +214,35 @@ class PagedKvCache:
         finally:
             p.destroy()
 
-    def append(self, k, v, dtype=None, strides=None):
+    def rotary_append(self, q, k, v, q_out, heads, rotary, tokens, positions, slots, dtype=None, strides=None, q_strides=None):
+        """A prepared launch of `kv_cache_rotary_append_v1` into this cache (q and q_out None: keys and values alone; rotary None: no
+        rotation, and queries stay as they are); the caller launches and destroys it."""
+        _contiguous(q, q_out)
+        if q is None or q_out is None or rotary is None:
+            q, q_out, heads = None, None, 0
+        one = _pair_dtype(k, v, dtype)
+        if (hasattr(q, "dtype") and _float_dtype(q, dtype) != one) or (hasattr(q_out, "dtype") and _float_dtype(q_out, dtype) != one):
+            raise TypeError("q and its turned rows are of the type of k and v")
+        qt, qh = q_strides or (heads * self.dim, self.dim)
+        turn = rotary.args() if rotary else dict(frequencies=None, rotary_dim=0, layout=0, scale=1.0)
+        return prepare(self.ctx, "kv_cache_rotary_append_v1", q=q, q_output=q_out, heads=heads, input_dtype=one, positions=positions if rotary and rotary.rotary_dim else None,
+                       slots=slots, q_token_stride=qt, q_head_stride=qh, q_output_token_stride=heads * self.dim, q_output_head_stride=self.dim,
+                       **turn, **self._rows(k, v, tokens, strides), **self._storage())
+
+    def append(self, k, v, dtype=None, strides=None, q=None, q_out=None, heads=0, rotary=None, q_strides=None):
         """Rows of the tokens of the last `extend`, sequence after sequence: [tokens][kv_heads][dim], or with `strides`
-        ((k token, k head), (v token, v head)) in elements, as slices (address, elements)."""
+        ((k token, k head), (v token, v head)) in elements, as slices (address, elements).  With a book on the device also with rotary positions on
+        the way (`rotary`, a fe2o3_b200.rotary.Rotary): keys are turned, and queries q [tokens][heads][dim] into q_out."""
+        if rotary:
+            if not self.pages:
+                raise ValueError("rotary positions on the way into the cache need its book on the device: tokens=")
+            n = self.new_tokens
+            p = self.rotary_append(q, k, v, q_out, heads, rotary, n, (self.pages.positions.as_device_ptr(), n), (self.pages.slots.as_device_ptr(), n), dtype, strides, q_strides)
+            try:
+                p.launch(self.stream)
+            finally:
+                p.destroy()
+            return
         self._launch("kv_cache_append_v1", token_offsets=self.device_offsets, input_dtype=_pair_dtype(k, v, dtype),
                      **self._rows(k, v, self.new_tokens, strides))
 
@@ -177,30 +275,55 @@ class PagedKvCache:
             p.destroy()
 
     def free(self):
-        for b in (self.k_cache, self.v_cache, self.k_scales, self.v_scales, self.device_table, self.device_lengths, self.device_offsets):
+        for b in (self.k_cache, self.v_cache, self.k_scales, self.v_scales):
             if b is not None:
                 b.free()
+        for b in (self.pages,) if self.pages else (self.device_table, self.device_lengths, self.device_offsets):
+            b.free()
 
 
 class DecodeStep:
     """One new token of every sequence at work (of length above 0): its key and value are written, then it attends to all
     positions so far and its own.  The tensors, a row a sequence, stay where they are from step to step; the caller fills
-    q, k and v on the cache's stream.  Rows of released sequences are not read, and their output is zeros."""
+    q, k and v on the cache's stream.  Rows of released sequences are not read, and their output is zeros.
 
-    def __init__(self, cache, q, k, v, out, heads, lse=None, scale=None, window=0, dtype=None, out_dtype=None, strides=None, q_strides=None):
-        self.cache = cache
+    With the cache's book on the device a step is three launches and nothing else, and `run` may be captured in a CUDA graph (on the stream that
+    it is given); with `rotary` q and k are turned by their positions on the way (q packed, or with strides, into rows that the step keeps)."""
+
+    def __init__(self, cache, q, k, v, out, heads, lse=None, scale=None, window=0, dtype=None, out_dtype=None, strides=None, q_strides=None, rotary=None):
+        self.cache, self.turned = cache, None
+        if cache.pages:
+            one = _pair_dtype(k, v, dtype)
+            if rotary:
+                self.turned = DeviceBuffer.zeroed(cache.stream, cache.sequences * heads * cache.dim, np.uint16 if one == DTYPE_BF16 else np.float32)
+            self.append = cache.rotary_append(q, k, v, self.turned, heads, rotary, cache.sequences, cache.pages.step_positions, cache.pages.step_slots, dtype,
+                                              strides, q_strides)
+            if rotary:
+                q, q_strides, dtype = self.turned, None, one
+            self.attend = cache.attention(q, out, heads, lse, scale, window, dtype, out_dtype, q_strides)
+            return
+        if rotary:
+            raise ValueError("rotary positions in a decode step need the cache's book on the device: tokens=")
         self.attend = cache.attention(q, out, heads, lse, scale, window, dtype, out_dtype, q_strides)
         self.append = prepare(cache.ctx, "kv_cache_append_v1", input_dtype=_pair_dtype(k, v, dtype),
                               **cache._rows(k, v, cache.sequences, strides), **cache.args())
 
-    def run(self):
+    def run(self, stream=None):
         cache = self.cache
-        before = len(cache.table.free)
-        cache.table.extend((cache.table.lengths > 0).astype(np.int64))
-        cache._upload(len(cache.table.free) != before)
-        self.append.launch(cache.stream)
-        self.attend.launch(cache.stream)
+        if stream is not None and not cache.pages:
+            raise ValueError("a step whose book of pages is on the host runs on the cache's stream")
+        stream = stream or cache.stream
+        if cache.pages:
+            cache.pages.step(stream)
+        else:
+            before = len(cache.table.free)
+            cache.table.extend((cache.table.lengths > 0).astype(np.int64))
+            cache._upload(len(cache.table.free) != before)
+        self.append.launch(stream)
+        self.attend.launch(stream)
 
     def destroy(self):
         self.append.destroy()
         self.attend.destroy()
+        if self.turned is not None:
+            self.turned.free()

@@ -506,7 +506,8 @@ typedef struct fe2o3_paged_attention_v1_args {
  * next_lengths and next_free_count are what lengths and free_count become (each may be the same slice as the one it follows); page_table and
  * free_pages change in place, entries that no length reaches stay as they are.  token_offsets [batch + 1] are the running sums of the
  * counts.  The new tokens, sequence after sequence, have positions[t] in their sequence and slots[t] = page * page_size + position % page_size;
- * behind the last token, up to `tokens`, positions are 0 and slots FE2O3_SLOT_NONE.  token_offsets, positions and slots may each be empty.  A
+ * behind the last token, up to `tokens`, positions are 0 and slots FE2O3_SLOT_NONE.  Without counts, row b of positions and slots is sequence
+ * b's, as in kv_cache_append_v1 without token_offsets: position 0 and FE2O3_SLOT_NONE for one of length 0, and tokens is at least batch.  token_offsets, positions and slots may each be empty.  A
  * token whose page has a number that is none of free_pages.len pages has no slot either, and is FE2O3_KSTATUS_SLOT_RANGE.
  * All or nothing: where a length or count does not fit its row of the page table (or 31 bits), or there are more tokens than `tokens`
  * (where positions or slots are asked for) or than 32 bits hold, FE2O3_KSTATUS_LENGTH is reported, where free_pages has too few free pages

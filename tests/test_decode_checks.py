@@ -20,6 +20,10 @@ def test_page_plans():
         ok(op, **{**kw, name: None})
     ok(op, **{**kw, "next_lengths": kw["lengths"], "next_free_count": kw["free_count"]})
     ok(op, **pages(batch=0, width=0, count=0, tokens=0))
+    each = {**kw, "counts": None, "tokens": 2}   # a row for every sequence, where there are rows
+    assert err(op, **{**each, "positions": sl(9, 2), "slots": None}) == "UnsupportedShape"
+    ok(op, **{**each, "positions": None, "slots": None})
+    ok(op, **{**kw, "tokens": 2, "positions": sl(9, 2), "slots": sl(10, 2)})
     ok(op, **pages(batch=8192))
     for bad in (dict(page_size=0), dict(batch=8193), dict(table_width=1 << 31), dict(page_size=1 << 30)):
         assert err(op, **{**kw, **bad}) == "UnsupportedShape", bad
@@ -129,3 +133,36 @@ def test_rotary_append(cache):
     assert err(op, **{**kw, "v": (kw["k_cache"][0], kw["v"][1])}) == "OutputAliasesInput"
     assert err(op, **{**kw, "v_cache": kw["k_cache"]}) == "OutputAliasesInput"
     assert err(op, **{**kw, "q_output_token_stride": 100, "q_output": sl(4, 4 * 100 + 256)}) == "UnsupportedShape"
+
+
+# ---- what the host works out ------------------------------------------------------------------------------------------
+
+def test_rotary_frequencies():
+    import numpy as np
+    from fe2o3_b200.rotary import rotary_frequencies
+    f, by = rotary_frequencies(64)
+    assert f.dtype == np.float32 and by == 1.0 and np.allclose(f, 10000.0 ** (-np.arange(32) / 32), rtol=1e-7, atol=0) and f[0] == 1
+    lin, _ = rotary_frequencies(64, scaling="linear", factor=4.0)
+    assert np.allclose(lin * 4, f, rtol=1e-6, atol=0)
+    ntk, _ = rotary_frequencies(64, scaling="ntk", factor=8.0)
+    assert ntk[0] == 1 and np.isclose(ntk[-1] * 8, f[-1], rtol=1e-5) and (np.diff(ntk) < 0).all()
+    yarn, by = rotary_frequencies(128, scaling="yarn", factor=16.0, trained=4096)
+    plain, _ = rotary_frequencies(128)
+    turns = 4096 * plain.astype(np.float64) / (2 * math.pi)
+    assert np.isclose(by, 0.1 * math.log(16) + 1)
+    assert (yarn[turns > 36] == plain[turns > 36]).all() and np.allclose(yarn[turns < 0.85] * 16, plain[turns < 0.85], rtol=1e-6)
+    assert (yarn <= plain).all() and (yarn * 16 >= plain * (1 - 1e-6)).all() and (np.diff(yarn) < 0).all()
+    assert len(rotary_frequencies(0)[0]) == 0 and rotary_frequencies(2, scaling="yarn", factor=2.0, trained=100)[0].shape == (1,)
+    for bad in (dict(rotary_dim=3), dict(rotary_dim=64, factor=0.5), dict(rotary_dim=64, base=0), dict(rotary_dim=64, scaling="more"),
+                dict(rotary_dim=64, scaling="yarn", factor=2.0), dict(rotary_dim=2, scaling="ntk", factor=2.0)):
+        with pytest.raises(ValueError):
+            rotary_frequencies(**bad)
+
+
+def test_objects_refuse_before_the_device_is_touched():
+    from fe2o3_b200.kv_cache import DevicePages, PagedKvCache
+    for kw in (dict(dim=48), dict(page_size=12)):
+        with pytest.raises(ValueError):
+            PagedKvCache(None, None, **{**dict(sequences=1, positions=8, kv_heads=1, dim=64, page_size=8, format=fe.KV_E2M1), **kw})
+    with pytest.raises(ValueError):
+        DevicePages(None, None, 1, 8, 1, 8, 0)

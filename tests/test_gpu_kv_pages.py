@@ -25,7 +25,8 @@ class Book:
                     self.stack[self.top] = self.table[b, i]
                     self.top += 1
                 self.lengths[b] = 0
-        if counts is None:
+        each = counts is None   # a row for every sequence
+        if each:
             counts = (self.lengths > 0).astype(np.int64)
         positions, slots, offsets = [], [], [0]
         for b, n in enumerate(counts):
@@ -38,6 +39,9 @@ class Book:
             slots.append(self.table[b, at // self.page].astype(np.int64) * self.page + at % self.page)
             self.lengths[b] += n
             offsets.append(offsets[-1] + n)
+            if each and not n:
+                positions.append([0])
+                slots.append([FREE])
         return np.concatenate(positions + [[]]).astype(np.int64), np.concatenate(slots + [[]]).astype(np.int64), np.array(offsets)
 
 
@@ -79,7 +83,7 @@ class Device:
 
 
 @pytest.mark.parametrize("in_place", [True, False])
-@pytest.mark.parametrize("batch,page,most,tokens", [(1, 16, 40, 64), (5, 1, 9, 45), (48, 16, 3, 160), (300, 7, 30, 9001), (33, 24, 400, 14000),
+@pytest.mark.parametrize("batch,page,most,tokens", [(1, 16, 40, 64), (5, 1, 9, 45), (48, 16, 3, 160), (300, 7, 30, 9001), (33, 24, 400, 14000), (2000, 16, 3, 2001),
                                                     (1025, 16, 60, 70000), (2500, 64, 8, 20003), (1, 64, 50000, 50000)])
 def test_steps(gpu, batch, page, most, tokens, in_place):  # noqa: F811
     """Prompts, single tokens, sequences that end and others that take their slots in the same step, tokens that do not fill the map."""
