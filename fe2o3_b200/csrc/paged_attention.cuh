@@ -78,7 +78,9 @@ namespace {
 constexpr int kWeightExponent = 15;
 constexpr float kLeastWeight = 0x1p-112f, kMostWeight = 0x1.fffffep125f;   // the largest weight is held in between: powers of two and their reciprocals stay normal numbers
 constexpr float kLeastTerm = 0x1p-40f;   // of a number, the least that its lower bf16 terms are: far below its last bit, and nothing where it is 0
-constexpr float kSlack = 8.f;          // 4 bits: what a score may lie above the maximum kept (log2) before that moves: a probability is up to 2^8 then
+// 4 bits: what a score may lie above the maximum kept (log2) before that moves; a probability is up to 2^8 then, and its product with the
+// unit of the least weight still a number (where every row so far was zeros: 2^(8 + 103 + 15)).
+constexpr float kSlack = 8.f, kLeastWeight4 = 0x1p-104f;
 constexpr int kQueryExponent = 14;    // f16 queries: the largest of a row lies in [2^14, 2^15)
 
 // LONG: tiles of 64 keys on two blocks an SM, for long rows of a 4-bit cache (see paged_attention_plan).
@@ -805,12 +807,14 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         lay_query();
         float heaviest[NT][2];   // 8-bit caches: the largest weight of a head so far, as p.m is the largest score
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) heaviest[nt][0] = heaviest[nt][1] = kLeastWeight;
+        for (int nt = 0; nt < NT; ++nt) heaviest[nt][0] = heaviest[nt][1] = F4 ? kLeastWeight4 : kLeastWeight;
         float unit4[NT][2];      // 4 bits: of the weights, and the maxima with a minus, as the last tiles left them
         uint64_t minus4[NT];
+        float peak[NT][2];       // the largest score that this lane has seen: p.m may lie kSlack below it
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            unit4[nt][0] = unit4[nt][1] = __uint_as_float(0x7f000000u - __float_as_uint(above(kLeastWeight)) + (kWeightExponent << 23));
+            peak[nt][0] = peak[nt][1] = -INFINITY;
+            unit4[nt][0] = unit4[nt][1] = __uint_as_float(0x7f000000u - __float_as_uint(above(kLeastWeight4)) + (kWeightExponent << 23));
             minus4[nt] = 0;
         }
         for (uint32_t tile = max(place, kEnd) - kEnd; tile < last_tile; ++tile) {
@@ -1051,6 +1055,8 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                     // Once some tiles are done, a tile seldom moves a maximum or a unit: the lanes look at what they have themselves, and only where
                     // one of them finds more do they compare notes.  (The 8-bit order, both trees at every tile: see below.)
                     float keep[2] = {1.f, 1.f};
+                    peak[nt][0] = fmaxf(peak[nt][0], top[0]);
+                    peak[nt][1] = fmaxf(peak[nt][1], top[1]);
                     const bool higher = __any_sync(~0u, top[0] > p.m[nt][0] + kSlack || top[1] > p.m[nt][1] + kSlack);
                     if (higher) {
                         float base[2];
@@ -1101,7 +1107,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
 #pragma unroll
                             for (int d = 4; d < 32; d <<= 1) most = fmaxf(most, __shfl_xor_sync(~0u, most, d));
                             const float before = keep[e] * above(heaviest[nt][e]);
-                            heaviest[nt][e] = fminf(fmaxf(fmaxf(heaviest[nt][e] * keep[e], most), kLeastWeight), kMostWeight);
+                            heaviest[nt][e] = fminf(fmaxf(fmaxf(heaviest[nt][e] * keep[e], most), kLeastWeight4), kMostWeight);
                             const uint32_t inverse = 0x7f000000u - __float_as_uint(above(heaviest[nt][e]));
                             by[e] = before * __uint_as_float(inverse);
                             unit4[nt][e] = __uint_as_float(inverse + (kWeightExponent << 23));
@@ -1321,10 +1327,24 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
             for (int e = 0; e < 2; ++e)
 #pragma unroll
                 for (int d = 4; d < 32; d <<= 1) p.l[nt][e] += __shfl_xor_sync(~0u, p.l[nt][e], d);
+            float back[2] = {1.f, 1.f};
+            if constexpr (F4) {   // from here on probabilities are at most 1 again: sums of the largest values stay in range
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+#pragma unroll
+                    for (int d = 4; d < 32; d <<= 1) peak[nt][e] = fmaxf(peak[nt][e], __shfl_xor_sync(~0u, peak[nt][e], d));
+                    if (peak[nt][e] > p.m[nt][e]) {
+                        back[e] = ex2_approx(p.m[nt][e] - peak[nt][e]);
+                        p.l[nt][e] *= back[e];
+                        p.m[nt][e] = peak[nt][e];
+                    }
+                }
+            }
             if constexpr (F16) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const float unit = __uint_as_float(__float_as_uint(above(heaviest[nt][e & 1])) - (kWeightExponent << 23));
+                    float unit = __uint_as_float(__float_as_uint(above(heaviest[nt][e & 1])) - (kWeightExponent << 23));
+                    if constexpr (F4) unit *= back[e & 1];
 #pragma unroll
                     for (int i = 0; i < MD; ++i) p.o[i][nt][e] *= unit;
                 }

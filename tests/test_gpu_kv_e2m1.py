@@ -320,6 +320,33 @@ def test_attention_values_of_unlike_size(gpu, octaves):  # noqa: F811
             check_attention(c, qv, got, lse, attention64(c, qv, 1.0), out)
 
 
+@pytest.mark.parametrize("page,width", [(16, None), (64, 80)])
+@pytest.mark.parametrize("rise", [0.5, 3.0, 5.5, 20.0])
+def test_attention_rising_scores_over_rows_of_zeros(gpu, page, width, rise):  # noqa: F811
+    """Scores that rise tile by tile, by less or more than what moves the maximum kept, while the values are zeros; then tiny, ordinary and the largest
+    ones.  Many sequences of the same, for several tiles a warp."""
+    n, many = 1200, 500
+    for size in (0.0, 2.0 ** -90, 1.0, 1e37):
+        c = Four(gpu, [n], 1, 64, page, width=width)
+        k, v = np.zeros((n, 1, 64)), np.zeros((n, 1, 64))
+        k[:, 0, 0] = np.minimum(np.arange(n) // 64, 12) * rise
+        v[-100:] = np.random.default_rng(1).choice([-1, 1], (100, 1, 64)) * size
+        c.put(0, 0, np.arange(n), k)
+        c.put(1, 0, np.arange(n), v)
+        c.to_gpu()
+        q = c.torch.zeros(many, 3, 64, device="cuda")
+        q[:, :, 0] = c.torch.tensor([1.0, 0.3, -1.0])
+        got, lse = attend(c, q, 1.0, batch=many, page_table=c.up(c.table.repeat(many, 0)), lengths=c.up(np.full(many, n, np.uint32)))
+        o, l64, mag, big = attention64(c, q[:1].cpu().numpy(), 1.0)
+        d = (72 * 2.0 ** -23 + 2.0 ** -22) * big
+        # a probability below f32's normal numbers, 2^-126, is 0; a weight is held to 2^-25 in units of at most 2^118, the least largest one's, and
+        # counts up to 2688 times: 2^-131 a key (probabilities against the first maximum kept are at most 2^8, and their sum no less than 2^-8 ones)
+        least = n * 2.0 ** 16 * (2.0 ** -126 * size + 2.0 ** -131)
+        bound = (2 * d + 2.0 ** -19 + n * 2.0 ** -24)[..., None] * mag + n * 2.0 ** -39 * mag.max(-1, keepdims=True) + least
+        assert (np.abs(got - o) <= bound).all(), (size, float(np.nanmax(np.abs(got - o) / bound)), np.isnan(got).sum())
+        assert (np.abs(lse - l64) <= d + 2.0 ** -20 + n * 2.0 ** -24 + 2.0 ** -22 * np.abs(l64)).all()
+
+
 @pytest.mark.parametrize("spread", [2, 6, 10])
 def test_attention_blocks_of_unlike_size(gpu, spread):  # noqa: F811
     """Blocks of 16 columns whose sizes lie 2^spread apart, in keys and in values, each column to its own accuracy."""
