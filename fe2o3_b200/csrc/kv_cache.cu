@@ -187,8 +187,9 @@ __global__ void __launch_bounds__(kThreads) kv_rows_kernel(KvCache c, KvRows r) 
 }
 
 // ---- 4 bits ----
-// Rows of 32 columns a lane (at least two lanes a row): what a row costs a lane by itself is dear beside 16 bytes of codes.  (With the 16 columns
-// of the other formats, 131072 tokens of 8 heads of 128 are read in 148 us, and 16384 are written in 36.)  A lane that writes takes two
+// Rows of 32 columns a lane (at least two lanes a row): what a row costs a lane by itself is dear beside 16 bytes of codes.  131072 tokens of 8
+// heads of 128 are read into bf16 rows in 137 us (148 with the 16 columns of the other formats), of which 537 MB are written: a plain fill of as much
+// takes 142.  16384 tokens from bf16 and back to f32 51 us (59 with 16 columns), 37 of it the f32 rows' way out.  A lane that writes takes two
 // blocks of 16 columns, l and l + lanes, whose scales it finds by itself.  One that reads takes four words of eight columns, l and every lanes-th
 // further: the stores of a row's lanes lie side by side.  (f32 ones, 32 bytes a word, by two neighbours that swap halves of their words first.)
 template <bool F32, bool WRITE, bool WHOLE>

@@ -2,7 +2,7 @@
 // launches it, one source a format builds it); the formulas stand at fe2o3_paged_attention_v1_args.
 //
 // HBM-bound: the K and V rows of a (sequence, key head) are read once, for all query heads that share them (4 * group
-// flop a byte of a bf16 cache, 8 * group of an 8-bit one).
+// flop a byte of a bf16 cache, 8 * group of an 8-bit one, 14 * group of a 4-bit one).
 //   Work.  An item is a (sequence, key head, up to 8 * NT query heads); its keys fall into tiles of KT.  The tiles of all
 //   items form one line, an item's behind kEnd places that stand for what its end costs, and the line is cut into equal
 //   shares, one a warp: the lengths are known on the device only, and a launch is the same whatever they are.  A warp
@@ -26,6 +26,11 @@
 //   the largest scale: e4m3 74.6 us for 74.7, 16 heads on one i8 head 53.4 for 54.2; but a large row of no weight takes the
 //   others' bits, all of them from 2^40 on.)  f32 queries are two f16 terms, bf16 ones a single one, in units of a power of two
 //   a row.  Error against 64 bits, f32 output: 1e-7 to 5e-7, as plain f32 arithmetic has.
+//   4 bits.  Codes become f16 two at a time and are multiplied by their block's scale, 6 bits together: exact, so the rest is as for 8 bits, the
+//   row's scale included.  A lane takes neighbouring columns of its keys, 16 of V (one block) and 32 of K, and the queries lie in that order.
+//   What is left of a byte is two instructions an element pair, so what a tile costs beside its conversions counts for more: maxima and units are
+//   compared between lanes only where one finds more than kSlack (kFull) above what is kept, copies are issued by several lanes at once, and
+//   rows that may be long go by 64 keys a tile on two blocks an SM (730 instructions for 32 keys; 940 with 32 a tile, 1014 without these).
 // Measured (32 query heads of 128 on 8, on 4 for e4m3): 64 ragged sequences of up to 4096 tokens 98 to 102 us, 5.3 to 5.6 TB/s; two of 131071
 // 178 to 193 us, 5.6 to 6.0 TB/s by machine; 96 ragged ones of up to 6000, e4m3, 73 to 75 us, 4.2 TB/s; 16 heads of 64 on 512 tokens 9.6 us.  In
 // the middle of a launch bf16 and e4m3 tiles come at 7.1 TB/s.  What is left: 4 us until the first tile is there (lengths,
@@ -35,6 +40,11 @@
 // bytes a thread stored and 184 loaded).  16 query heads on an 8-bit head (NT 2, 54 us) are bound by latency: 255 registers leave two warps a
 // scheduler, each one dependent chain of some 1150 instructions a tile of 32 keys, at a third of the issue slots; the loop no longer
 // fits the first instruction cache.  Half tiles on three blocks an SM come to the same time.
+// 4 bits: two sequences of 131071 (319 MB) 96 us, 3.3 TB/s, where a sum over as many bytes takes 70; 96 ragged ones of up to 6000 on 4 heads 67 us; 16 heads
+// of 64 on 512 tokens 11.  Copies alone take 75 of the 96 us, products alone 73: what is left is what the two do not hide of each other with
+// eight warps an SM and two tiles of 64 keys each in its ring, and 12 us of beginning and end.  Three blocks of 32 keys hide less (107 us), 48 keys
+// or four blocks spill.  Neither fewer requests to the copy engine (scales by the lanes' 16-byte copies: 108) nor longer ones (boxes as
+// runs of bytes: 99) nor pages in order (the same) help.
 #pragma once
 #include "kv_cache.cuh"
 

@@ -2,9 +2,12 @@
 // pass (kv_cache_rotary_append_v1).  The formulas stand at fe2o3_rotary_v1_args and fe2o3_kv_cache_rotary_append_v1_args.
 //
 // HBM-bound: each element is read once and written once.  A block takes some tokens, all their rows or a part of them; it first
-// works out the tokens' sines and cosines, once for all heads, into shared memory.  A row is pieces of 16 bytes, two to each of 2 to 32
-// lanes: with halves as pairs the two pieces that hold them, so that a lane turns its own columns; where half of the turned columns is no
-// whole number of pieces, a lane fetches its columns' partners one by one (they are in the first cache).
+// works out the tokens' sines and cosines, once for all heads, into shared memory.  A row is pieces of 16 bytes, two to each of up to 32
+// lanes: with halves as pairs the two pieces that hold them, so that a lane turns its own columns.  Where half of the turned columns is no
+// whole number of pieces, the columns go through shared memory, where a lane takes a pair.  (Partners fetched one by one from the first
+// cache instead, and lanes by powers of two: 8191 tokens of 48 rows of 80 columns, 20 of them turned, 73 and 43 us where this takes 33.)
+// 16384 tokens, 40 rows of 128 bf16 columns: 57 us, 5.9 TB/s, 90 % of a copy's rate; 1003 tokens of 24 f32 rows of 96 4.9 us; the new tokens of 64
+// sequences 3 us, a launch.
 // Angles: position times frequency has up to 56 bits.  The product p and what rounding took from it, e, are 64-bit numbers that add up
 // to it exactly; n whole turns are taken off in two steps (2 pi as two 64-bit numbers), which leaves an angle in [-pi, pi] that is right
 // to some 2^-50.  Its sine and cosine are those of its 32-bit rounding, and the rest of it to first order.
