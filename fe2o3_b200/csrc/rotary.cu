@@ -245,26 +245,28 @@ __global__ void __launch_bounds__(kThreads, FORMAT == kPlain || FORMAT == FE2O3_
                         y[3] = fmaf(b1, t.z, a1 * t.w);
                     }
             }
-            if (kCache && what[d]) {
-                if constexpr (kCache) {
-                    const uint32_t row = first_rows[token[d]] + head[d] * c.page_size;
-                    store_row<FORMAT, kPiece>(c, x[d], raw[d], turned, what[d] - 1, row, first, inside, l, lanes, active[d] && in);
+            const bool cached = kCache && what[d];
+            if (!cached && active[d] && in) {
+                const uint32_t ts = !kCache && what[d] ? r.to_token_stride[1] : r.to_token_stride[0], hs = !kCache && what[d] ? r.to_head_stride[1] : r.to_head_stride[0];
+                uint8_t *const to = (!kCache && what[d] ? r.to[1] : r.to[0]) + ((uint64_t)(t0 + token[d]) * ts + (uint64_t)head[d] * hs) * kEb;
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const float *const q = x[d] + half * kPiece;
+                    uint32_t w[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if constexpr (F32) w[i] = __float_as_uint(q[i]);
+                        else w[i] = first[half] + 2 * i >= turned ? word_of(raw[d][half], i) : bf16_pair(q[2 * i], q[2 * i + 1]);
+                    }
+                    put<F32, WHOLE>(to + first[half] * kEb, make_uint4(w[0], w[1], w[2], w[3]));
                 }
-                continue;
             }
-            if (!active[d] || !in) continue;
-            const uint32_t ts = !kCache && what[d] ? r.to_token_stride[1] : r.to_token_stride[0], hs = !kCache && what[d] ? r.to_head_stride[1] : r.to_head_stride[0];
-            uint8_t *const to = (!kCache && what[d] ? r.to[1] : r.to[0]) + ((uint64_t)(t0 + token[d]) * ts + (uint64_t)head[d] * hs) * kEb;
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const float *const q = x[d] + half * kPiece;
-                uint32_t w[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if constexpr (F32) w[i] = __float_as_uint(q[i]);
-                    else w[i] = first[half] + 2 * i >= turned ? word_of(raw[d][half], i) : bf16_pair(q[2 * i], q[2 * i + 1]);
+            if constexpr (kCache) {
+                // (a row's largest magnitudes go round the whole warp, whose other rows may be queries: all lanes go along, or none)
+                if (FORMAT == FE2O3_KV_BF16 ? cached : __any_sync(~0u, cached)) {
+                    const uint32_t row = first_rows[token[d]] + head[d] * c.page_size;
+                    store_row<FORMAT, kPiece>(c, x[d], raw[d], turned, what[d] == 2, row, first, inside, l, lanes, cached && active[d] && in);
                 }
-                put<F32, WHOLE>(to + first[half] * kEb, make_uint4(w[0], w[1], w[2], w[3]));
             }
         }
     }

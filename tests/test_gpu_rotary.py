@@ -267,6 +267,33 @@ def test_rotated_rows_in_the_cache(gpu, form, dtype, layout, heads, kv_heads, di
 
 
 @pytest.mark.parametrize("form", FORMATS)
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("dim,rotary", [(32, 32), (64, 20), (128, 64), (256, 256)])
+def test_queries_and_keys_in_one_warp(gpu, form, dtype, dim, rotary):  # noqa: F811
+    """Any number of queries beside any number of keys: rows that are only turned and rows that are quantised meet in a warp, and some tokens are left out."""
+    torch = gpu[1]
+    rng = np.random.default_rng(dim)
+    for heads, kv_heads, T in ((1, 1, 3), (2, 1, 77), (3, 2, 40), (5, 1, 601), (7, 3, 50), (9, 5, 33), (1, 9, 64), (0, 1, 5)):
+        c = cache_of(gpu, form, [T], kv_heads, dim, 8, seed=heads).to_gpu()
+        pos = np.arange(T)
+        slots = (c.table[0, pos // 8].astype(np.int64) * 8 + pos % 8).astype(np.uint32)
+        drop = rng.random(T) < 0.2
+        slots[drop] = 0xffffffff
+        (q, _), (k, _), (v, vv) = (rows_in(torch, rng.normal(size=(T, h, dim)), dtype) for h in (heads, kv_heads, kv_heads))
+        qo, freq = torch.full_like(q, 7.0), frequencies(rotary)
+        launch(gpu, "kv_cache_rotary_append_v1", q=q if heads else None, k=k, v=v, positions=up32(torch, pos), slots=up32(torch, slots),
+               frequencies=torch.from_numpy(freq).cuda(), q_output=qo if heads else None, tokens=T, heads=heads, rotary_dim=rotary, layout=0,
+               input_dtype=int(dtype == "bf16"), scale=1.0, **packed(heads, kv_heads, dim, "q", "k", "v", "q_output"), **cache_args(c))
+        keep, there = np.nonzero(~drop)[0], torch.from_numpy(~drop).cuda()
+        if heads:
+            assert torch.equal(qo[there], rotate(gpu, q, None, up32(torch, pos), freq, "half")[0][there]) and (qo[~there] == 7).all()
+        if len(keep):
+            c.put(0, 0, pos[keep], rotate(gpu, k.float(), None, up32(torch, pos), freq, "half")[0].cpu().numpy()[keep])
+            c.put(1, 0, pos[keep], vv[keep])
+        c.assert_same()
+
+
+@pytest.mark.parametrize("form", FORMATS)
 def test_many_tokens_and_strided_rows(gpu, form):  # noqa: F811
     """Fused rows [q | k | v] of a long prompt, read as they lie; starts on odd elements."""
     torch = gpu[1]
