@@ -4,10 +4,11 @@
 // HBM-bound: each element is read once and written once.  A block takes some tokens, all their rows or a part of them; it first
 // works out the tokens' sines and cosines, once for all heads, into shared memory.  A row is pieces of 16 bytes, two to each of up to 32
 // lanes: with halves as pairs the two pieces that hold them, so that a lane turns its own columns.  Where half of the turned columns is no
-// whole number of pieces, the columns go through shared memory, where a lane takes a pair.  (Partners fetched one by one from the first
-// cache instead, and lanes by powers of two: 8191 tokens of 48 rows of 80 columns, 20 of them turned, 73 and 43 us where this takes 33.)
-// 16384 tokens, 40 rows of 128 bf16 columns: 57 us, 5.9 TB/s, 90 % of a copy's rate; 1003 tokens of 24 f32 rows of 96 4.9 us; the new tokens of 64
-// sequences 3 us, a launch.
+// whole number of pieces, the columns go through shared memory, where a lane takes a pair or two neighbouring ones.  (Partners fetched one by one
+// from the first cache instead, and lanes by powers of two: 8191 tokens of 48 rows of 80 columns, 20 of them turned, 73 and 43 us where this
+// takes 34; 16384 tokens of 40 rows of 128 with 100 turned, 50 pairs, 110 us with two pairs a lane at once and 142 with one.)  The first
+// rows are fetched before the sines are worked out (64 tokens of 40 rows 2.7 us for 3.2).
+// 16384 tokens, 40 rows of 128 bf16 columns: 57 us, 5.9 TB/s, 90 % of a copy's rate, neighbours as pairs 61; 1003 tokens of 24 f32 rows of 96 4.4 us.
 // Angles: position times frequency has up to 56 bits.  The product p and what rounding took from it, e, are 64-bit numbers that add up
 // to it exactly; n whole turns are taken off in two steps (2 pi as two 64-bit numbers), which leaves an angle in [-pi, pi] that is right
 // to some 2^-50.  Its sine and cosine are those of its 32-bit rounding, and the rest of it to first order.
@@ -118,7 +119,7 @@ __device__ __forceinline__ uint32_t turn_at(uint32_t i, uint32_t groups) {
 
 // WHOLE: the rows start on 16 bytes.
 template <uint32_t FORMAT, bool F32, int MODE, bool WHOLE>
-__global__ void __launch_bounds__(kThreads, FORMAT == kPlain || FORMAT == FE2O3_KV_BF16 ? 4 : 3) rotary_kernel(KvCache c, RotaryRows r) {
+__global__ void __launch_bounds__(kThreads, MODE != kAnywhere && (FORMAT == kPlain || FORMAT == FE2O3_KV_BF16) ? 4 : 3) rotary_kernel(KvCache c, RotaryRows r) {
     constexpr int kEb = F32 ? 4 : 2, kPiece = 16 / kEb, kDeep = 2, kPairs = MODE == kNeighbours ? kPiece / 2 : kPiece;
     constexpr bool kCache = FORMAT != kPlain;
     extern __shared__ float4 table[];              // [tokens of the block][pairs]; then the rows in flight, where partners lie anywhere
@@ -126,18 +127,6 @@ __global__ void __launch_bounds__(kThreads, FORMAT == kPlain || FORMAT == FE2O3_
     float2 *const turns = reinterpret_cast<float2 *>(table);
     begin_after_previous();
     const uint32_t part = blockIdx.x % r.parts, t0 = blockIdx.x / r.parts * r.per_block, n = min(r.per_block, r.tokens - t0);
-    if (kCache && threadIdx.x < n) {
-        const uint32_t slot = r.slots[t0 + threadIdx.x], page = slot / c.page_size;
-        const bool there = page < c.pages;
-        if (!there && slot != FE2O3_SLOT_NONE) kstatus_set(c.status, FE2O3_KSTATUS_SLOT_RANGE);
-        first_rows[threadIdx.x] = there && slot != FE2O3_SLOT_NONE ? page * c.kv_heads * c.page_size + (slot - page * c.page_size) : ~0u;
-    }
-    for (uint32_t i = threadIdx.x; i < n * r.pairs; i += kThreads) {
-        const uint32_t t = i / r.pairs, pair = i - t * r.pairs;
-        turns[t * r.token_turns + turn_at<MODE, kPairs>(pair, r.groups)] = turn_of(r.positions ? r.positions[t0 + t] : t0 + t, r.frequencies[pair], r.scale, r.sign);
-    }
-    __syncthreads();
-
     const uint32_t lanes = r.lanes, of_warp = 32 / lanes, at_once = kThreads / 32 * of_warp, in_warp = (threadIdx.x & 31) / lanes, l = (threadIdx.x & 31) - in_warp * lanes;
     const uint32_t mine = (threadIdx.x >> 5) * of_warp + in_warp;   // of the rows at once
     // a lane's columns: two pieces, the partners of one another where pairs allow
@@ -147,10 +136,10 @@ __global__ void __launch_bounds__(kThreads, FORMAT == kPlain || FORMAT == FE2O3_
     const bool inside[2] = {in, in};
     float *const scratch = reinterpret_cast<float *>(turns + (uint64_t)r.per_block * r.token_turns) + mine * kDeep * r.dim;
     const uint32_t total = n * r.rows, share = (total + r.parts - 1) / r.parts, end = min(total, (part + 1) * share);
-    for (uint32_t base = part * share; base < end; base += kDeep * at_once) {
-        uint4 raw[kDeep][2];
-        uint32_t token[kDeep], head[kDeep], what[kDeep];
-        bool active[kDeep];
+    uint4 raw[kDeep][2];
+    uint32_t token[kDeep], head[kDeep], what[kDeep];
+    bool there[kDeep];
+    auto load = [&](uint32_t base) {
 #pragma unroll
         for (int d = 0; d < kDeep; ++d) {
             const uint32_t i = min(base + mine + d * at_once, end - 1);
@@ -162,9 +151,9 @@ __global__ void __launch_bounds__(kThreads, FORMAT == kPlain || FORMAT == FE2O3_
                 what[d] = 2;
                 head[d] -= r.kv_heads;
             }
-            active[d] = base + mine + d * at_once < end && (!kCache || first_rows[token[d]] != ~0u);
+            there[d] = base + mine + d * at_once < end;
             raw[d][0] = raw[d][1] = make_uint4(0, 0, 0, 0);
-            if (active[d] && in) {
+            if (there[d] && in) {
                 const uint32_t ts = what[d] == 0 ? r.token_stride[0] : what[d] == 1 ? r.token_stride[1] : r.token_stride[2];
                 const uint32_t hs = what[d] == 0 ? r.head_stride[0] : what[d] == 1 ? r.head_stride[1] : r.head_stride[2];
                 const uint8_t *const at = (what[d] == 0 ? r.from[0] : what[d] == 1 ? r.from[1] : r.from[2]) + ((uint64_t)(t0 + token[d]) * ts + (uint64_t)head[d] * hs) * kEb;
@@ -172,6 +161,24 @@ __global__ void __launch_bounds__(kThreads, FORMAT == kPlain || FORMAT == FE2O3_
                 for (int half = 0; half < 2; ++half) raw[d][half] = fetch<F32, WHOLE>(at + first[half] * kEb);
             }
         }
+    };
+    // (the first rows are on their way while the sines are worked out; those of a token that is left out as well, for nothing)
+    if (part * share < end) load(part * share);
+    if (kCache && threadIdx.x < n) {
+        const uint32_t slot = r.slots[t0 + threadIdx.x], page = slot / c.page_size;
+        const bool there = page < c.pages;
+        if (!there && slot != FE2O3_SLOT_NONE) kstatus_set(c.status, FE2O3_KSTATUS_SLOT_RANGE);
+        first_rows[threadIdx.x] = there && slot != FE2O3_SLOT_NONE ? page * c.kv_heads * c.page_size + (slot - page * c.page_size) : ~0u;
+    }
+    for (uint32_t i = threadIdx.x; i < n * r.pairs; i += kThreads) {
+        const uint32_t t = i / r.pairs, pair = i - t * r.pairs;
+        turns[t * r.token_turns + turn_at<MODE, kPairs>(pair, r.groups)] = turn_of(r.positions ? r.positions[t0 + t] : t0 + t, r.frequencies[pair], r.scale, r.sign);
+    }
+    __syncthreads();
+    for (uint32_t base = part * share; base < end;) {
+        bool active[kDeep];
+#pragma unroll
+        for (int d = 0; d < kDeep; ++d) active[d] = there[d] && (!kCache || first_rows[token[d]] != ~0u);
         __syncwarp();   // in place: every lane has its columns before one writes
         float x[kDeep][2 * kPiece];
 #pragma unroll
@@ -196,8 +203,19 @@ __global__ void __launch_bounds__(kThreads, FORMAT == kPlain || FORMAT == FE2O3_
             for (int d = 0; d < kDeep; ++d) {
                 if (what[d] == 2 || in_warp >= of_warp) continue;
                 float *const row = scratch + d * r.dim;
+                const float2 *const cs = turns + token[d] * r.token_turns;
+                if (r.pairs % 2 == 0) {   // two pairs at once
+                    for (uint32_t i = 2 * l; i < r.pairs; i += 2 * lanes) {
+                        const float4 t = *reinterpret_cast<const float4 *>(cs + i);
+                        float2 &low = *reinterpret_cast<float2 *>(row + i), &high = *reinterpret_cast<float2 *>(row + i + r.pairs);
+                        const float2 a = low, b = high;
+                        low = make_float2(fmaf(a.x, t.x, -(b.x * t.y)), fmaf(a.y, t.z, -(b.y * t.w)));
+                        high = make_float2(fmaf(b.x, t.x, a.x * t.y), fmaf(b.y, t.z, a.y * t.w));
+                    }
+                    continue;
+                }
                 for (uint32_t i = l; i < r.pairs; i += lanes) {
-                    const float2 t = turns[token[d] * r.token_turns + i];
+                    const float2 t = cs[i];
                     const float a = row[i], b = row[i + r.pairs];
                     row[i] = fmaf(a, t.x, -(b * t.y));
                     row[i + r.pairs] = fmaf(b, t.x, a * t.y);
@@ -215,7 +233,7 @@ __global__ void __launch_bounds__(kThreads, FORMAT == kPlain || FORMAT == FE2O3_
         }
 #pragma unroll
         for (int d = 0; d < kDeep; ++d) {
-            if (base + d * at_once >= end) break;
+            if (base + d * at_once >= end) continue;   // (for the whole block)
             const uint32_t turned = what[d] < 2 ? 2 * r.pairs : 0;
             const float2 *const cs = turns + token[d] * r.token_turns;
             if (MODE == kPieces && turned && pair) {
@@ -269,6 +287,8 @@ __global__ void __launch_bounds__(kThreads, FORMAT == kPlain || FORMAT == FE2O3_
                 }
             }
         }
+        base += kDeep * at_once;
+        if (base < end) load(base);
     }
 }
 
