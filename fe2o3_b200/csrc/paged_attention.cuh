@@ -42,9 +42,9 @@
 // fits the first instruction cache.  Half tiles on three blocks an SM come to the same time.
 // 4 bits: two sequences of 131071 (319 MB) 96 us, 3.3 TB/s, where a sum over as many bytes takes 70; 96 ragged ones of up to 6000 on 4 heads 67 us; 16 heads
 // of 64 on 512 tokens 11.  Copies alone take 75 of the 96 us, products alone 73: what is left is what the two do not hide of each other with
-// eight warps an SM and two tiles of 64 keys each in its ring, and 12 us of beginning and end.  Three blocks of 32 keys hide less (107 us), 48 keys
-// or four blocks spill.  Neither fewer requests to the copy engine (scales by the lanes' 16-byte copies: 108) nor longer ones (boxes as
-// runs of bytes: 99) nor pages in order (the same) help.
+// eight warps an SM and two tiles of 64 keys each in its ring, and about 12 us of beginning and end.  By events, which add 6: three blocks of 32
+// keys 113 us where these take 102; 48 keys, or four blocks, spill (117, 129); scales by the lanes' 16-byte copies, so fewer requests to the
+// copy engine, 115; pages in order the same.
 #pragma once
 #include "kv_cache.cuh"
 
