@@ -40,8 +40,8 @@
 // bytes a thread stored and 184 loaded).  16 query heads on an 8-bit head (NT 2, 54 us) are bound by latency: 255 registers leave two warps a
 // scheduler, each one dependent chain of some 1150 instructions a tile of 32 keys, at a third of the issue slots; the loop no longer
 // fits the first instruction cache.  Half tiles on three blocks an SM come to the same time.
-// 4 bits: two sequences of 131071 (319 MB) 96 us, 3.3 TB/s, where a sum over as many bytes takes 70; 96 ragged ones of up to 6000 on 4 heads 67 us; 16 heads
-// of 64 on 512 tokens 11.  Copies alone take 75 of the 96 us, products alone 73: what is left is what the two do not hide of each other with
+// 4 bits: two sequences of 131071 (319 MB) 94 to 96 us, 3.4 TB/s, where a sum over as many bytes takes 70; 96 ragged ones of up to 6000 on 4 heads 67 us; 16 heads
+// of 64 on 512 tokens 11.  Copies alone take 75 of them, products alone 73: what is left is what the two do not hide of each other with
 // eight warps an SM and two tiles of 64 keys each in its ring, and about 12 us of beginning and end.  By events, which add 6: three blocks of 32
 // keys 113 us where these take 102; 48 keys, or four blocks, spill (117, 129); scales by the lanes' 16-byte copies, so fewer requests to the
 // copy engine, 115; pages in order the same.
@@ -500,6 +500,8 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     const uint32_t scales_row = lset < 2 ? 4 : row_blocks;   // bytes
     const uint32_t scales_to = (lset < 2 ? lset * 4 * KT : 8 * KT + (lset & 1) * S::kBlocks) + lbox * a.box * scales_row;
     const CUtensorMap *const lmap = lset & 1 ? &map_v : &map_k;
+    const uint32_t scales_bytes = a.box * scales_row, rows_to = lset * (KT * S::kRow) + lbox * a.box * S::kPitch, box_bytes = a.box * (2 * S::kRow + 8 + 2 * row_blocks);
+    uint32_t lhead = 0;   // of the cursor's item
     // Zeros for a row of a stage: K and V, and their scales.
     auto no_row = [&](uint32_t slot, uint32_t r, bool k_too) {
         for (uint32_t i = lane; i < 2 * kPieces; i += 32)
@@ -513,7 +515,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
                 blocks[S::kBlocks] = 0;
             }
     };
-    auto copy_tile = [&] {
+    auto next_item = [&] {
         while (ltile == lend && lrest) {
             if (++litem == per_seq) {
                 litem = 0;
@@ -525,6 +527,10 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
             }
             enter(0);
         }
+        if constexpr (F4) lhead = litem / a.chunks;
+    };
+    auto copy_any = [&] {
+        next_item();
         if (ltile >= lend) return;
         // a lane a box, or a row
         const uint32_t key = lspan.key(ltile) + min(lbox, boxes - 1) * a.box, head = litem / a.chunks;
@@ -594,6 +600,47 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
         }
         lslot = lslot + 1 == a.stages ? 0 : lslot + 1;
         ++ltile;
+    };
+    // Long rows of 4 bits: the same in fewer steps (two sequences of 131071 104 us, by events, where these take 100; short rows take 3 % longer so).
+    auto copy_long = [&] {
+        if (ltile == lend) {
+            next_item();
+            if (ltile >= lend) return;
+        }
+        const uint32_t key = (lspan.first / KT + ltile) * KT + min(lbox, boxes - 1) * a.box;
+        const uint32_t at = a.page_shift >= 0 ? key >> a.page_shift : key / a.c.page_size, in_page = key - at * a.c.page_size;
+        uint32_t of_entries = at - entries_from;
+        if (entries_of != lseq || __any_sync(~0u, of_entries >= 32)) {
+            entries_of = lseq;
+            entries_from = __shfl_sync(~0u, at, 0);
+            entry = ~0u;
+            if (entries_from + lane < a.c.table_width) entry = a.c.page_table[(uint64_t)lseq * a.c.table_width + entries_from + lane];
+            of_entries = at - entries_from;
+        }
+        const uint32_t page = __shfl_sync(~0u, entry, of_entries);
+        const bool wanted = lbox < boxes && key < lspan.n && key + a.box > lspan.first, there = wanted && page < a.c.pages;
+        const uint32_t found = __ballot_sync(~0u, there) & 0xffu, all = (1u << boxes) - 1;
+        uint64_t *const bar = &bars[lslot];
+        if (lane == 0) mbar_arrive_expect_tx(bar, __popc(found) * box_bytes);
+        __syncwarp();
+        if (there) {
+            const uint32_t head_of_page = page * a.c.kv_heads + lhead, row = head_of_page * a.c.page_size + in_page;
+            bulk_load_1d(my_scales + lslot * S::kScales + scales_to, scales_from + (uint64_t)row * scales_row, scales_bytes, bar);
+            if (lset < 2) tma_load_3d(my_ring + lslot * S::kStage + rows_to, lmap, bar, 0, in_page, head_of_page);
+        }
+        if (found != all) {   // at an end of the sequence, or reported
+            if (wanted && !there) kstatus_set(a.c.status, FE2O3_KSTATUS_SLOT_RANGE);
+            __syncwarp();
+            for (uint32_t r = 0; r < KT; ++r)
+                if (!(found >> r / a.box & 1)) no_row(lslot, r, true);
+            fence_proxy_async_smem();   // before the next box goes there
+        }
+        lslot = lslot + 1 == a.stages ? 0 : lslot + 1;
+        ++ltile;
+    };
+    auto copy_tile = [&] {
+        if (LONG && a.box > 1) copy_long();
+        else copy_any();
     };
     uint32_t seq, item;   // at work
     // ---- the queries of an item, as 16-bit terms: a lane takes eight columns of a row at a time ----
@@ -791,6 +838,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_c
     lseq = seq;
     litem = item;
     lrest = share;
+    if constexpr (F4) lhead = litem / a.chunks;
     enter(place);
     for (uint32_t s = 0; s < a.stages; ++s) copy_tile();
 

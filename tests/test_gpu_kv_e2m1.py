@@ -401,16 +401,18 @@ def test_attention_infinities_and_nan(gpu):  # noqa: F811
     assert np.abs(got[keep] - o[keep]).max() <= 1e-4 and np.isfinite(lse[1:3, :2]).all() and np.isfinite(lse[2]).all()
 
 
-def test_attention_reports(gpu):  # noqa: F811
+@pytest.mark.parametrize("page,width", [(16, None), (64, 70)])
+def test_attention_reports(gpu, page, width):  # noqa: F811
     """A length that the table cannot hold leaves that sequence unwritten; rows of a page outside the cache count as zeros; a cache without pages."""
     fe, torch, ctx, stream = gpu
-    c = filled(gpu, [40, 30, 33], 2, 64, 16)
+    lengths = [page * 5 // 2, 30, 2 * page + 1]
+    c = filled(gpu, lengths, 2, 64, page, width=width)
     q, qv = queries(torch, 3, 4, 64, "bf16")
     want = attention64(c, qv, 0.125)[0]
     o = torch.full((3, 4, 64), 7.0, device="cuda")
     kw = dict(q=q, output=o, heads=4, q_stride=256, q_head_stride=64, scale=0.125, window=0, q_dtype=1, output_dtype=0)
     with pytest.raises(fe.Fe2o3Error):
-        c.launch("paged_attention_v1", **kw, lengths=c.up(np.array([40, c.width * 16 + 1, 33], np.uint32)))
+        c.launch("paged_attention_v1", **kw, lengths=c.up(np.array([lengths[0], c.width * page + 1, lengths[2]], np.uint32)))
     got = o.cpu().numpy()
     assert (got[1] == 7).all() and np.abs(got[[0, 2]] - want[[0, 2]]).max() <= 1e-4
     table = c.table.copy()
@@ -418,8 +420,8 @@ def test_attention_reports(gpu):  # noqa: F811
     with pytest.raises(fe.Fe2o3Error):
         c.launch("paged_attention_v1", **kw, page_table=c.up(table))
     got = o.cpu().numpy()
-    k, v = (c.get(side, 2, np.arange(33)) for side in range(2))
-    k[16:32] = v[16:32] = 0
+    k, v = (c.get(side, 2, np.arange(lengths[2])) for side in range(2))
+    k[page:2 * page] = v[page:2 * page] = 0
     for h in range(4):
         p = np.exp(k[:, h // 2] @ qv[2, h] * 0.125)
         assert np.abs(got[2, h] - p @ v[:, h // 2] / p.sum()).max() <= 1e-4
