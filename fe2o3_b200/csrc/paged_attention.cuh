@@ -30,7 +30,7 @@
 //   row's scale included.  A lane takes neighbouring columns of its keys, 16 of V (one block) and 32 of K, and the queries lie in that order.
 //   What is left of a byte is two instructions an element pair, so what a tile costs beside its conversions counts for more: maxima and units are
 //   compared between lanes only where one finds more than kSlack (kFull) above what is kept, copies are issued by several lanes at once, and
-//   rows that may be long go by 64 keys a tile on two blocks an SM (730 instructions for 32 keys; 940 with 32 a tile, 1014 without these).
+//   rows that may be long go by 64 keys a tile on two blocks an SM (690 instructions for 32 keys; 940 with 32 a tile, 1014 without these).
 // Measured (32 query heads of 128 on 8, on 4 for e4m3): 64 ragged sequences of up to 4096 tokens 98 to 102 us, 5.3 to 5.6 TB/s; two of 131071
 // 178 to 193 us, 5.6 to 6.0 TB/s by machine; 96 ragged ones of up to 6000, e4m3, 73 to 75 us, 4.2 TB/s; 16 heads of 64 on 512 tokens 9.6 us.  In
 // the middle of a launch bf16 and e4m3 tiles come at 7.1 TB/s.  What is left: 4 us until the first tile is there (lengths,
