@@ -176,17 +176,22 @@ class PagedKvCache:
         self.device_lengths.copy_from_host_async(self.stream, self.table.lengths)
 
     def extend(self, counts, release=None):
-        """Positions for new tokens of every sequence; `append` then writes them.  (release: with a book on the device, sequences that give their
-        pages back first.)"""
+        """Positions for new tokens of every sequence; `append` then writes them.  `release`: truth values, the sequences that give their pages
+        back first."""
         if self.pages:
             self.pages.extend(counts, release)
             self.new_tokens = int(np.sum(counts))
             return
-        if release is not None:
-            for b in np.nonzero(np.asarray(release))[0]:
-                self.table.release(int(b))
         before = len(self.table.free)
-        self.table.extend(counts)
+        held = self.table.entries.copy(), self.table.lengths.copy(), list(self.table.free)
+        try:
+            if release is not None:
+                for b in np.nonzero(np.asarray(release))[0]:
+                    self.table.release(int(b))
+            self.table.extend(counts)
+        except Exception:   # all or none, what is released too
+            self.table.entries[:], self.table.lengths[:], self.table.free = held
+            raise
         offsets = np.zeros(self.sequences + 1, np.uint32)
         offsets[1:] = np.cumsum(counts)
         self.new_tokens = int(offsets[-1])

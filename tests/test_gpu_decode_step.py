@@ -177,6 +177,14 @@ def test_what_does_not_fit_is_reported_and_changes_nothing(gpu):  # noqa: F811
     host.extend([1, 1])
     with pytest.raises(ValueError):
         host.append(y, y, q=y, q_out=torch.zeros_like(y), heads=1, rotary=rotary)
+    small = PagedKvCache(ctx, stream, 2, 64, 1, 32, 8, pages=3, format=fe.KV_E2M1)
+    small.extend([8, 9])
+    with pytest.raises(MemoryError):                        # the host's book: what is released comes back with the error
+        small.extend([9, 17], [0, 1])
+    assert small.table.lengths.tolist() == [8, 9] and read_lengths(small).tolist() == [8, 9] and len(small.table.free) == 0
+    small.extend([0, 16], [1, 1])
+    assert read_lengths(small).tolist() == [0, 16]
+    small.free()
     with pytest.raises(TypeError):
         cache.append(y, y, q=y.bfloat16(), q_out=torch.zeros_like(y), heads=1, rotary=rotary)
     plain = DecodeStep(host, y, y, y, torch.zeros(2, 1, 32, device="cuda"), 1)
