@@ -177,6 +177,8 @@ def test_what_does_not_fit_is_reported_and_changes_nothing(gpu):  # noqa: F811
     host.extend([1, 1])
     with pytest.raises(ValueError):
         host.append(y, y, q=y, q_out=torch.zeros_like(y), heads=1, rotary=rotary)
+    with pytest.raises(ValueError):
+        cache.append(y, y, q=y, q_out=torch.zeros_like(y), heads=1)
     small = PagedKvCache(ctx, stream, 2, 64, 1, 32, 8, pages=3, format=fe.KV_E2M1)
     small.extend([8, 9])
     with pytest.raises(MemoryError):                        # the host's book: what is released comes back with the error
