@@ -66,7 +66,7 @@ __global__ void __launch_bounds__(kMaxThreads) kv_pages_kernel(PagesArgs a) {
     __shared__ Sums warps[32];
     __shared__ Sums carry;
     __shared__ uint32_t bad;
-    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, many = blockDim.x >> 5;
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const uint32_t thread = blockIdx.x * blockDim.x + threadIdx.x, threads = gridDim.x * blockDim.x;
     if (threadIdx.x == 0) {
         carry = Sums{0, 0, 0};
