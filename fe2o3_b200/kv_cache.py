@@ -238,8 +238,8 @@ class PagedKvCache:
         """Rows of the tokens of the last `extend`, sequence after sequence: [tokens][kv_heads][dim], or with `strides`
         ((k token, k head), (v token, v head)) in elements, as slices (address, elements).  With a book on the device also with rotary positions on
         the way (`rotary`, a fe2o3_b200.rotary.Rotary): keys are turned, and queries q [tokens][heads][dim] into q_out."""
-        if q is not None and not rotary:
-            raise ValueError("queries come along to be turned: rotary=")
+        if (q is None) != (q_out is None) or (q is not None and not rotary):
+            raise ValueError("queries come along to be turned, by rotary=, from q into q_out")
         if rotary:
             if not self.pages:
                 raise ValueError("rotary positions on the way into the cache need its book on the device: tokens=")

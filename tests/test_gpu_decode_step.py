@@ -179,6 +179,9 @@ def test_what_does_not_fit_is_reported_and_changes_nothing(gpu):  # noqa: F811
         host.append(y, y, q=y, q_out=torch.zeros_like(y), heads=1, rotary=rotary)
     with pytest.raises(ValueError):
         cache.append(y, y, q=y, q_out=torch.zeros_like(y), heads=1)
+    for one in (dict(q=y), dict(q_out=torch.zeros_like(y))):
+        with pytest.raises(ValueError):
+            cache.append(y, y, heads=1, rotary=rotary, **one)
     small = PagedKvCache(ctx, stream, 2, 64, 1, 32, 8, pages=3, format=fe.KV_E2M1)
     small.extend([8, 9])
     with pytest.raises(MemoryError):                        # the host's book: what is released comes back with the error
