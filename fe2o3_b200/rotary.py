@@ -85,8 +85,10 @@ class Rotary:
                        k_output_head_stride=koh, **self.args())
 
     def apply(self, q, k, positions, heads, kv_heads, dim, tokens=None, **kw):
-        """The same, launched once on the stream.  tokens: by q's size, if it is not said."""
+        """The same, launched once on the stream.  tokens: by the size of q, where its rows are packed."""
         if tokens is None:
+            if isinstance(q, tuple) or kw.get("strides"):
+                raise ValueError("rows inside wider storage need tokens=")
             size = q.numel() if hasattr(q, "numel") else len(q)
             tokens = size // (heads * dim)
         p = self.prepare(q, k, positions, heads, kv_heads, dim, tokens, **kw)

@@ -2,6 +2,7 @@
 import math
 
 import pytest
+import torch
 
 import fe2o3_b200 as fe
 from test_kv_cache_checks import ALL, err, ok, queries, rows, sl
@@ -166,3 +167,11 @@ def test_objects_refuse_before_the_device_is_touched():
             PagedKvCache(None, None, **{**dict(sequences=1, positions=8, kv_heads=1, dim=64, page_size=8, format=fe.KV_E2M1), **kw})
     with pytest.raises(ValueError):
         DevicePages(None, None, 1, 8, 1, 8, 0)
+
+
+def test_rotary_object_wants_the_number_of_strided_rows():
+    from fe2o3_b200.rotary import Rotary
+    rotary = Rotary(None, None, 0)   # (no columns to turn: nothing on a device)
+    for q, kw in (((1 << 20, 512), {}), (torch.zeros(4, 512), dict(strides=((512, 64), (512, 64))))):
+        with pytest.raises(ValueError):
+            rotary.apply(q, None, None, 2, 0, 64, dtype=fe.DTYPE_F32, **kw)
