@@ -69,9 +69,11 @@ class Rotary:
         given; with strides ((q token, q head), (k token, k head)) in elements the rows are slices (address, elements)."""
         if k is None:
             kv_heads = 0
-        for x in (q, k, q_out, k_out):
+        for x in (q, k, q_out, k_out, positions):
             if hasattr(x, "is_contiguous") and not x.is_contiguous():
                 raise ValueError("a tensor is contiguous here; rows inside wider storage come as (address, elements) with their strides")
+        if hasattr(positions, "dtype") and not str(positions.dtype).endswith("int32"):
+            raise TypeError(f"positions are 32-bit integers, got {positions.dtype}")
         one = _dtype(q, dtype)
         for x in (k, q_out, k_out):
             if hasattr(x, "dtype") and _dtype(x, dtype) != one:

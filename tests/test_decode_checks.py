@@ -175,3 +175,13 @@ def test_rotary_object_wants_the_number_of_strided_rows():
     for q, kw in (((1 << 20, 512), {}), (torch.zeros(4, 512), dict(strides=((512, 64), (512, 64))))):
         with pytest.raises(ValueError):
             rotary.apply(q, None, None, 2, 0, 64, dtype=fe.DTYPE_F32, **kw)
+
+
+def test_rotary_object_wants_positions_of_32_bits():
+    from fe2o3_b200.rotary import Rotary
+    rotary, q = Rotary(None, None, 0), torch.zeros(4, 2, 64)
+    for positions in (torch.arange(4), torch.arange(4.0), torch.arange(4, dtype=torch.int16)):
+        with pytest.raises(TypeError, match="32-bit"):
+            rotary.apply(q, None, positions, 2, 0, 64)
+    with pytest.raises(ValueError):
+        rotary.apply(q, None, torch.arange(8, dtype=torch.int32)[::2], 2, 0, 64)
