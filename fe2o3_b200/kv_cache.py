@@ -127,6 +127,14 @@ def _contiguous(*tensors):
             raise ValueError("a tensor is contiguous here; rows inside wider storage come as (address, elements) with their strides")
 
 
+def _numbers(**arrays):
+    """Positions and slots are read as 32-bit words, one behind the other (addresses with a length say nothing of that)."""
+    _contiguous(*arrays.values())
+    for name, x in arrays.items():
+        if hasattr(x, "dtype") and not str(x.dtype).endswith("int32"):
+            raise TypeError(f"{name} are 32-bit integers, got {x.dtype}")
+
+
 def _pair_dtype(k, v, dtype):
     """DTYPE_* of k and v, which are of one type."""
     one = _float_dtype(k, dtype)
@@ -221,8 +229,9 @@ class PagedKvCache:
 
     def rotary_append(self, q, k, v, q_out, heads, rotary, tokens, positions, slots, dtype=None, strides=None, q_strides=None):
         """A prepared launch of `kv_cache_rotary_append_v1` into this cache (q and q_out None: keys and values alone; rotary None: no
-        rotation, and queries stay as they are); the caller launches and destroys it."""
+        rotation, and queries stay as they are); the caller launches and destroys it.  positions and slots: 32-bit integers, one a token."""
         _contiguous(q, q_out)
+        _numbers(positions=positions, slots=slots)
         if q is None or q_out is None or rotary is None:
             q, q_out, heads = None, None, 0
         one = _pair_dtype(k, v, dtype)

@@ -9,6 +9,7 @@ import math
 import numpy as np
 
 from . import DTYPE_BF16, DTYPE_F32, ROTARY_HALF, DeviceBuffer, prepare
+from .kv_cache import _contiguous, _numbers
 
 
 def rotary_frequencies(rotary_dim, base=10000.0, scaling=None, factor=1.0, trained=None, fast=32.0, slow=1.0):
@@ -69,11 +70,8 @@ class Rotary:
         given; with strides ((q token, q head), (k token, k head)) in elements the rows are slices (address, elements)."""
         if k is None:
             kv_heads = 0
-        for x in (q, k, q_out, k_out, positions):
-            if hasattr(x, "is_contiguous") and not x.is_contiguous():
-                raise ValueError("a tensor is contiguous here; rows inside wider storage come as (address, elements) with their strides")
-        if hasattr(positions, "dtype") and not str(positions.dtype).endswith("int32"):
-            raise TypeError(f"positions are 32-bit integers, got {positions.dtype}")
+        _contiguous(q, k, q_out, k_out)
+        _numbers(positions=positions)
         one = _dtype(q, dtype)
         for x in (k, q_out, k_out):
             if hasattr(x, "dtype") and _dtype(x, dtype) != one:

@@ -185,3 +185,19 @@ def test_rotary_object_wants_positions_of_32_bits():
             rotary.apply(q, None, positions, 2, 0, 64)
     with pytest.raises(ValueError):
         rotary.apply(q, None, torch.arange(8, dtype=torch.int32)[::2], 2, 0, 64)
+
+
+@pytest.mark.parametrize("name", ["positions", "slots"])
+def test_rotated_rows_want_numbers_of_32_bits(name):
+    """64-bit numbers read as 32-bit words would be a slot, 0, a slot, 0: the first page's first row, again and again."""
+    from fe2o3_b200.kv_cache import PagedKvCache
+    from fe2o3_b200.rotary import Rotary
+    cache = PagedKvCache.__new__(PagedKvCache)             # (nothing of it is on a GPU before the arguments are looked at)
+    rotary, k = Rotary(None, None, 0), torch.zeros(4, 2, 32)
+    cache.kv_heads, cache.dim = 2, 32
+    good = dict(positions=torch.arange(4, dtype=torch.int32), slots=torch.arange(4, dtype=torch.int32))
+    for bad in (torch.arange(4), torch.arange(4.0), torch.arange(4, dtype=torch.int16)):
+        with pytest.raises(TypeError, match=name + " are 32-bit"):
+            cache.rotary_append(None, k, k, None, 0, rotary, 4, **{**good, name: bad})
+    with pytest.raises(ValueError, match="contiguous"):
+        cache.rotary_append(None, k, k, None, 0, rotary, 4, **{**good, name: torch.arange(8, dtype=torch.int32)[::2]})
