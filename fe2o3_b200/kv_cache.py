@@ -65,6 +65,14 @@ class PageTable:
         self.lengths[sequence] = 0
 
 
+def _mask(release, sequences):
+    """Which sequences give their pages back: a truth value each."""
+    release = np.zeros(sequences, bool) if release is None else np.asarray(release).astype(bool)
+    if release.shape != (sequences,):
+        raise ValueError(f"release has a truth value for each of the {sequences} sequences")
+    return release
+
+
 class DevicePages:
     """The same book on the device (`kv_pages_v1`): pages go out and come back in the same order.  What does not fit is found there too: it is reported
     (`ctx.take_kernel_status`), and nothing changes.  `tokens`: the most new tokens of an `extend`."""
@@ -89,8 +97,8 @@ class DevicePages:
     def extend(self, counts, release=None):
         """Places for `counts[b]` new tokens of every sequence b, after those of `release` (truth values) have given their pages back."""
         n = len(self.lengths)
-        counts, release = np.asarray(counts), np.zeros(n, np.uint32) if release is None else np.asarray(release).astype(bool).astype(np.uint32)
-        if counts.shape != (n,) or release.shape != (n,) or (counts < 0).any() or int(counts.astype(np.int64).sum()) > self.tokens:
+        counts, release = np.asarray(counts), _mask(release, n).astype(np.uint32)
+        if counts.shape != (n,) or (counts < 0).any() or int(counts.astype(np.int64).sum()) > self.tokens:
             raise ValueError(f"counts has one number, at least 0, for each of the {n} sequences, and no more than {self.tokens} in all")
         # (arrays in ordinary memory: the copies have read them when the calls return)
         self.counts.copy_from_host_async(self.stream, counts.astype(np.uint32))
@@ -190,12 +198,11 @@ class PagedKvCache:
             self.pages.extend(counts, release)
             self.new_tokens = int(np.sum(counts))
             return
-        before = len(self.table.free)
+        before, gone = len(self.table.free), np.nonzero(_mask(release, self.sequences))[0]
         held = self.table.entries.copy(), self.table.lengths.copy(), list(self.table.free)
         try:
-            if release is not None:
-                for b in np.nonzero(np.asarray(release))[0]:
-                    self.table.release(int(b))
+            for b in gone:
+                self.table.release(int(b))
             self.table.extend(counts)
         except Exception:   # all or none, what is released too
             self.table.entries[:], self.table.lengths[:], self.table.free = held

@@ -201,3 +201,50 @@ def test_rotated_rows_want_numbers_of_32_bits(name):
             cache.rotary_append(None, k, k, None, 0, rotary, 4, **{**good, name: bad})
     with pytest.raises(ValueError, match="contiguous"):
         cache.rotary_append(None, k, k, None, 0, rotary, 4, **{**good, name: torch.arange(8, dtype=torch.int32)[::2]})
+
+
+class Copies:
+    """A device array of which only what is copied into it counts."""
+
+    def __init__(self):
+        self.held = None
+
+    def copy_from_host_async(self, stream, array):
+        self.held = array.copy()
+
+
+def host_book(sequences=3, positions=64, page_size=8, pages=20):
+    """A cache with the host's book of pages, nothing of it on a GPU."""
+    from fe2o3_b200.kv_cache import PagedKvCache, PageTable
+    cache = PagedKvCache.__new__(PagedKvCache)
+    cache.pages, cache.stream, cache.sequences, cache.table = None, None, sequences, PageTable(sequences, positions, pages, page_size)
+    cache.device_table, cache.device_lengths, cache.device_offsets = Copies(), Copies(), Copies()
+    return cache
+
+
+def device_book(sequences=3, tokens=50):
+    """The same with the device's book, whose launches do nothing."""
+    from fe2o3_b200.kv_cache import DevicePages, PagedKvCache
+    cache, pages = PagedKvCache.__new__(PagedKvCache), DevicePages.__new__(DevicePages)
+    pages.stream, pages.tokens, pages.lengths, pages.counts, pages.released = None, tokens, [0] * sequences, Copies(), Copies()
+    pages._extend = type("Launch", (), {"launch": lambda self, stream: None})()
+    cache.pages, cache.sequences, cache.stream = pages, sequences, None
+    return cache
+
+
+@pytest.mark.parametrize("book", [host_book, device_book])
+def test_released_sequences_are_a_truth_value_each(book):
+    """A list of sequence numbers is not taken for one: [2] would be sequence 0."""
+    cache = book()
+    cache.extend([5, 6, 7])
+    for bad in ([2], [1, 0], [1, 0, 0, 0], [[1, 0, 0]], 1, []):
+        with pytest.raises(ValueError, match="truth value"):
+            cache.extend([0, 0, 0], bad)
+    if cache.pages:
+        assert cache.pages.counts.held.tolist() == [5, 6, 7] and cache.pages.released.held.tolist() == [0, 0, 0]
+        cache.extend([0, 1, 0], [True, False, True])
+        assert cache.pages.released.held.tolist() == [1, 0, 1]
+    else:
+        assert cache.table.lengths.tolist() == [5, 6, 7] and len(cache.table.free) == 17
+        cache.extend([0, 1, 0], [True, False, True])
+        assert cache.table.lengths.tolist() == [0, 7, 0] and cache.device_lengths.held.tolist() == [0, 7, 0] and len(cache.table.free) == 19
