@@ -198,14 +198,15 @@ class PagedKvCache:
             self.pages.extend(counts, release)
             self.new_tokens = int(np.sum(counts))
             return
-        before, gone = len(self.table.free), np.nonzero(_mask(release, self.sequences))[0]
-        held = self.table.entries.copy(), self.table.lengths.copy(), list(self.table.free)
+        book, before, gone = self.table, len(self.table.free), np.nonzero(_mask(release, self.sequences))[0]
+        held = book.entries[gone], book.lengths[gone]   # (copies)
+        for b in gone:
+            book.release(int(b))
         try:
-            for b in gone:
-                self.table.release(int(b))
-            self.table.extend(counts)
-        except Exception:   # all or none, what is released too
-            self.table.entries[:], self.table.lengths[:], self.table.free = held
+            book.extend(counts)
+        except Exception:   # all or none, what is released too: its pages lie behind those that were free
+            book.entries[gone], book.lengths[gone] = held
+            del book.free[before:]
             raise
         offsets = np.zeros(self.sequences + 1, np.uint32)
         offsets[1:] = np.cumsum(counts)

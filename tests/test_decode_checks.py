@@ -248,3 +248,58 @@ def test_released_sequences_are_a_truth_value_each(book):
         assert cache.table.lengths.tolist() == [5, 6, 7] and len(cache.table.free) == 17
         cache.extend([0, 1, 0], [True, False, True])
         assert cache.table.lengths.tolist() == [0, 7, 0] and cache.device_lengths.held.tolist() == [0, 7, 0] and len(cache.table.free) == 19
+
+
+def test_extending_the_hosts_book_costs_its_new_pages_alone():
+    """The table, the lengths and the list of free pages are not copied for an undoing that `PageTable.extend` does not need."""
+    import numpy as np
+    cache = host_book()
+    copies = []
+
+    class Watched(np.ndarray):
+        def copy(self, *args, **kw):
+            copies.append(self.shape)
+            return super().copy(*args, **kw)
+
+        def __getitem__(self, at):
+            out = super().__getitem__(at)
+            if isinstance(out, np.ndarray) and out.size and not np.shares_memory(out, self):
+                copies.append(out.shape)
+            return out
+
+    class Pages(list):
+        def __iter__(self):
+            copies.append(len(self))
+            return super().__iter__()
+
+    book = cache.table
+    book.entries, book.free = book.entries.view(Watched), Pages(book.free)
+    cache.device_table.copy_from_host_async = lambda stream, array: None
+    cache.extend([5, 6, 7])
+    assert copies == [] and book.lengths.tolist() == [5, 6, 7]
+    with pytest.raises(ValueError):
+        cache.extend([0, 100, 0])
+    assert copies == []
+    with pytest.raises(ValueError):
+        cache.extend([0, 100, 0], [1, 0, 0])
+    assert copies == [(1, 8)] and book.lengths.tolist() == [5, 6, 7]   # the row of the released sequence
+
+
+def test_a_release_that_fails_with_its_extend_is_undone():
+    import numpy as np
+    rng = np.random.default_rng(1)
+    cache = host_book(sequences=6, pages=20)
+    book, failed = cache.table, 0
+    for _ in range(300):
+        before = book.entries.copy(), book.lengths.copy(), list(book.free)
+        counts, gone = rng.integers(0, 30, 6), rng.random(6) < 0.4
+        try:
+            cache.extend(counts, gone)
+        except (ValueError, MemoryError):
+            failed += 1
+            assert (book.entries == before[0]).all() and (book.lengths == before[1]).all() and book.free == before[2]
+        else:
+            assert (book.lengths == np.where(gone, 0, before[1]) + counts).all()
+            used = book.entries[book.entries != book.FREE].tolist()
+            assert sorted(used + list(book.free)) == list(range(20))
+    assert 20 < failed < 280
