@@ -215,8 +215,11 @@ class PagedKvCache:
         self.device_offsets.copy_from_host_async(self.stream, offsets)
 
     def release(self, sequence):
+        """Gives a finished sequence's pages back; its slot starts again at no positions."""
         if self.pages:
-            self.pages.extend([0] * self.sequences, [b == sequence for b in range(self.sequences)])
+            gone = np.zeros(self.sequences, bool)
+            gone[sequence] = True
+            self.pages.extend([0] * self.sequences, gone)
             self.new_tokens = 0
             return
         self.table.release(sequence)

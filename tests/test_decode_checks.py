@@ -303,3 +303,19 @@ def test_a_release_that_fails_with_its_extend_is_undone():
             used = book.entries[book.entries != book.FREE].tolist()
             assert sorted(used + list(book.free)) == list(range(20))
     assert 20 < failed < 280
+
+
+@pytest.mark.parametrize("book", [host_book, device_book])
+def test_a_released_sequence_is_one_of_the_book(book):
+    """A number past the end is an error with either book, one below zero counts from the end."""
+    cache = book()
+    cache.extend([5, 6, 7])
+    lengths = lambda: (cache.pages.released.held == 0).tolist() if cache.pages else (cache.table.lengths > 0).tolist()  # noqa: E731
+    for bad in (3, -4, 100):
+        with pytest.raises(IndexError):
+            cache.release(bad)
+    assert lengths() == [True, True, True]
+    cache.release(-1)
+    assert lengths() == [True, True, False]
+    cache.release(0)
+    assert lengths()[0] is False
