@@ -23,6 +23,8 @@ ordinary memory may hold the host until the stream has come to it, once it is la
 preparing an attention (`attention`, `DecodeStep`) for the legacy stream, destroying one for the whole device, `attend`, which
 does both, and `read` for the cache's stream.
 """
+import operator
+
 import numpy as np
 
 from . import DTYPE_BF16, DTYPE_F32, KV_BF16, KV_E2M1, KV_E4M3, KV_I8, DeviceBuffer, prepare
@@ -218,7 +220,7 @@ class PagedKvCache:
         """Gives a finished sequence's pages back; its slot starts again at no positions."""
         if self.pages:
             gone = np.zeros(self.sequences, bool)
-            gone[sequence] = True
+            gone[operator.index(sequence)] = True   # (one, no slice or mask of them)
             self.pages.extend([0] * self.sequences, gone)
             self.new_tokens = 0
             return

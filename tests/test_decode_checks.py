@@ -319,3 +319,16 @@ def test_a_released_sequence_is_one_of_the_book(book):
     assert lengths() == [True, True, False]
     cache.release(0)
     assert lengths()[0] is False
+
+
+@pytest.mark.parametrize("book", [host_book, device_book])
+def test_a_released_sequence_is_a_number(book):
+    cache = book()
+    cache.extend([5, 6, 7])
+    for bad in (None, slice(0, 2), [0, 1], "0"):
+        with pytest.raises((TypeError, IndexError)):
+            cache.release(bad)
+    if cache.pages:
+        assert cache.pages.released.held.tolist() == [0, 0, 0]
+    else:
+        assert cache.table.lengths.tolist() == [5, 6, 7]
