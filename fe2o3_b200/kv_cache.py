@@ -30,6 +30,14 @@ import numpy as np
 from . import DTYPE_BF16, DTYPE_F32, KV_BF16, KV_E2M1, KV_E4M3, KV_I8, DeviceBuffer, prepare
 
 
+def _new_tokens(counts, sequences):
+    """New tokens of every sequence, as 64-bit integers."""
+    counts = np.asarray(counts)
+    if counts.shape != (sequences,) or not (counts >= 0).all() or (counts > 0x7fffffff).any() or (counts.dtype.kind not in "biu" and (counts % 1 != 0).any()):
+        raise ValueError(f"counts has a whole number, from 0 on and below 2^31, for each of the {sequences} sequences")
+    return counts.astype(np.int64)
+
+
 class PageTable:
     """Pages of every sequence, in order, and how many positions each has."""
 
@@ -45,9 +53,7 @@ class PageTable:
 
     def extend(self, counts):
         """Positions for `counts[b]` new tokens of every sequence b; all of them or, with an error, none."""
-        counts = np.asarray(counts)
-        if counts.shape != self.lengths.shape or (counts < 0).any():
-            raise ValueError(f"counts has one number, at least 0, for each of the {len(self.lengths)} sequences")
+        counts = _new_tokens(counts, len(self.lengths))
         after = self.lengths.astype(np.int64) + counts
         held, need = -(-self.lengths.astype(np.int64) // self.page_size), -(-after // self.page_size)
         if (need > self.entries.shape[1]).any():
@@ -99,9 +105,9 @@ class DevicePages:
     def extend(self, counts, release=None):
         """Places for `counts[b]` new tokens of every sequence b, after those of `release` (truth values) have given their pages back."""
         n = len(self.lengths)
-        counts, release = np.asarray(counts), _mask(release, n).astype(np.uint32)
-        if counts.shape != (n,) or (counts < 0).any() or int(counts.astype(np.int64).sum()) > self.tokens:
-            raise ValueError(f"counts has one number, at least 0, for each of the {n} sequences, and no more than {self.tokens} in all")
+        counts, release = _new_tokens(counts, n), _mask(release, n).astype(np.uint32)
+        if int(counts.sum()) > self.tokens:
+            raise ValueError(f"no more than {self.tokens} new tokens at once, got {int(counts.sum())}")
         # (arrays in ordinary memory: the copies have read them when the calls return)
         self.counts.copy_from_host_async(self.stream, counts.astype(np.uint32))
         self.released.copy_from_host_async(self.stream, release)

@@ -332,3 +332,16 @@ def test_a_released_sequence_is_a_number(book):
         assert cache.pages.released.held.tolist() == [0, 0, 0]
     else:
         assert cache.table.lengths.tolist() == [5, 6, 7]
+
+
+@pytest.mark.parametrize("book", [host_book, device_book])
+def test_new_tokens_are_whole_numbers(book):
+    """Also such whose sum leaves 64 bits, and would be 0 there."""
+    cache = book(4)
+    for bad in ([1.5, 0.5, 0, 0], [1 << 62] * 4, [1 << 31, 0, 0, 0], [1 << 70, 0, 0, 0], [float("nan"), 0, 0, 0], [float("inf"), 0, 0, 0], [-1, 1, 0, 0], [1, 1, 1]):
+        with pytest.raises(ValueError):
+            cache.extend(bad)
+    held = lambda: cache.pages.counts.held if cache.pages else cache.device_lengths.held  # noqa: E731
+    assert held() is None
+    cache.extend([3.0, True, 0, 2])
+    assert held().tolist() == [3, 1, 0, 2] and cache.new_tokens == 6
