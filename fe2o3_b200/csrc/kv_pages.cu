@@ -210,8 +210,10 @@ int32_t launch_kv_pages(fe2o3_ctx *ctx, cudaStream_t s, const void *args, fe2o3_
     if (geo) *geo = fe2o3_geometry{{grid, 1, 1}, {threads, 1, 1}, shared, 1};
     if (plan_only) {
         FE2O3_CUDA(cudaSetDevice(ctx->device));
-        FE2O3_CUDA(cudaFuncSetAttribute(reinterpret_cast<const void *>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, kMostSequences * sizeof(Place)));
-        FE2O3_CUDA(cudaFuncSetAttribute(reinterpret_cast<const void *>(kernel), cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+        for (const auto each : {kv_pages_kernel<1>, kv_pages_kernel<8>}) {   // (both: a patched batch or number of tokens may take the other)
+            FE2O3_CUDA(cudaFuncSetAttribute(reinterpret_cast<const void *>(each), cudaFuncAttributeMaxDynamicSharedMemorySize, kMostSequences * sizeof(Place)));
+            FE2O3_CUDA(cudaFuncSetAttribute(reinterpret_cast<const void *>(each), cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+        }
         return FE2O3_OK;
     }
     int32_t shift = -1;

@@ -245,3 +245,41 @@ def test_steps_replay_from_a_graph_and_run_on_another_stream(gpu):  # noqa: F811
     d.check(book.step(None))
     p.destroy()
     assert ctx.take_kernel_status(stream) == 0
+
+
+PATCHED = """
+import struct, sys
+sys.path[:0] = [{root!r}, {tests!r}]
+import numpy as np, torch
+import fe2o3_b200 as fe
+from test_gpu_kv_pages import Book, Device
+ctx = fe.GpuContext(0)
+gpu = (fe, torch, ctx, ctx.default_stream())
+book = Book({batch}, 300, 16, {batch} * 300)
+d = Device(gpu, book, 5000)
+counts = np.arange({batch}) % 4 * (5000 // {batch} // 8) + 1
+p = fe.prepare(ctx, "kv_pages_v1", counts=d.up(counts.astype(np.uint32)), **d.args(positions=d.positions[:{first}], slots=d.slots[:{first}], tokens={first}))
+p.patch_kernarg(188, struct.pack("<I", 5000))
+p.launch_and_wait(gpu[3], 20000)
+d.check(book.step(counts))
+p.destroy()
+print("patched plan is right")
+"""
+
+
+@pytest.mark.parametrize("batch,first", [(4, 64), (1000, 1000)])
+def test_a_plan_patched_to_many_tokens(gpu, batch, first):  # noqa: F811
+    """In a process of its own: what a prepare leaves behind for later launches stays with the process."""
+    import os
+    import subprocess
+    import sys
+    tests = os.path.dirname(os.path.abspath(__file__))
+    done = subprocess.run([sys.executable, "-c", PATCHED.format(root=os.path.dirname(tests), tests=tests, batch=batch, first=first)], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and "patched plan is right" in done.stdout, done.stderr[-2000:]
+
+
+@pytest.mark.parametrize("in_place", [True, False])
+@pytest.mark.parametrize("batch,most,tokens", [(3200, 9, 20003), (8191, 5, 30000), (8192, 1, 8192), (8192, 40, 100001)])
+def test_the_largest_batches(gpu, batch, most, tokens, in_place):  # noqa: F811
+    """More sequences than 48 KiB of shared memory hold, up to the most that are admitted."""
+    test_steps(gpu, batch, 16, most, tokens, in_place)
