@@ -86,7 +86,7 @@ PagedAttentionArgs = _struct("PagedAttentionArgs",
 KvPagesArgs = _struct("KvPagesArgs",
                       ["counts", "release", "lengths", "free_count", "page_table", "free_pages", "next_lengths", "next_free_count",
                        "token_offsets", "positions", "slots"],
-                      [("batch", u32), ("table_width", u32), ("page_size", u32), ("tokens", u32)])
+                      [("batch", u32), ("table_width", u32), ("page_size", u32), ("tokens", u32), ("attended", Slice)])
 RotaryArgs = _struct("RotaryArgs", ["q", "k", "positions", "frequencies", "q_output", "k_output"],
                      [("tokens", u32), ("heads", u32), ("kv_heads", u32), ("dim", u32), ("rotary_dim", u32), ("layout", u32), ("dtype", u32),
                       ("backward", u32), ("q_token_stride", u32), ("q_head_stride", u32), ("k_token_stride", u32), ("k_head_stride", u32),
@@ -157,7 +157,7 @@ OPS = {
     "kv_cache_append_v1": (KvCacheAppendArgs, 192, False),
     "kv_cache_read_v1": (KvCacheReadArgs, 192, False),
     "paged_attention_v1": (PagedAttentionArgs, 200, False),
-    "kv_pages_v1": (KvPagesArgs, 192, False),
+    "kv_pages_v1": (KvPagesArgs, 208, False),
     "rotary_v1": (RotaryArgs, 168, False),
     "kv_cache_rotary_append_v1": (KvCacheRotaryAppendArgs, 248, False),
     "masked_reduce_u32": (MaskedReduceArgs, 48, False),

@@ -750,6 +750,7 @@ int regions_for(uint32_t op, const void *args, Region *r, int32_t *status) {
             if (a->token_offsets.ptr || a->token_offsets.len) r[n++] = RGN("TokenOffsets", a->token_offsets, (uint64_t)a->batch + 1, 4, true);
             if (a->positions.ptr || a->positions.len) r[n++] = RGN("Positions", a->positions, a->tokens, 4, true);
             if (a->slots.ptr || a->slots.len) r[n++] = RGN("Slots", a->slots, a->tokens, 4, true);
+            if (a->attended.ptr || a->attended.len) r[n++] = RGN("Attended", a->attended, a->batch, 4, true);
             return n;
         }
         case OP_ROTARY: {

@@ -18,7 +18,7 @@ constexpr uint32_t kMostSequences = 8192, kMaxThreads = 1024, kBlocks = 16;
 
 struct PagesArgs {
     const uint32_t *counts, *release, *lengths, *free_count;
-    uint32_t *table, *free_pages, *next_lengths, *next_free_count, *offsets, *positions, *slots, *status;
+    uint32_t *table, *free_pages, *next_lengths, *next_free_count, *offsets, *positions, *slots, *attended, *status;
     uint32_t batch, width, page_size, tokens, pages;
     int32_t shift;   // log2 of page_size, or negative
 };
@@ -130,8 +130,10 @@ __global__ void __launch_bounds__(kMaxThreads) kv_pages_kernel(PagesArgs a) {
     if (thread == 0) *a.next_free_count = fits ? (uint32_t)(top - total.fresh) : count;
     for (uint32_t b = thread; b < a.batch; b += threads) {
         const uint32_t end = b + 1 < a.batch ? places[b + 1].first_token : (uint32_t)total.tokens;
-        if (fits) a.next_lengths[b] = places[b].length + (end - places[b].first_token);
+        const uint32_t length = places[b].length + (end - places[b].first_token);
+        if (fits) a.next_lengths[b] = length;
         else if (a.next_lengths != a.lengths) a.next_lengths[b] = a.lengths[b];
+        if (a.attended) a.attended[b] = fits ? length : 0;
         if (a.offsets) a.offsets[b] = fits ? places[b].first_token : 0;
     }
     if (fits)
@@ -220,7 +222,7 @@ int32_t launch_kv_pages(fe2o3_ctx *ctx, cudaStream_t s, const void *args, fe2o3_
     if ((a->page_size & (a->page_size - 1)) == 0) shift = __builtin_ctz(a->page_size);
     auto at = [](const fe2o3_slice &x) { return reinterpret_cast<uint32_t *>(x.ptr); };
     const PagesArgs p{at(a->counts), at(a->release), at(a->lengths), at(a->free_count), at(a->page_table), at(a->free_pages), at(a->next_lengths),
-                      at(a->next_free_count), at(a->token_offsets), at(a->positions), at(a->slots), ctx->status_word, a->batch, a->table_width,
+                      at(a->next_free_count), at(a->token_offsets), at(a->positions), at(a->slots), at(a->attended), ctx->status_word, a->batch, a->table_width,
                       a->page_size, a->tokens, (uint32_t)a->free_pages.len, shift};
     const cudaError_t e = fe2o3_launch_early(kernel, grid, threads, shared, s, grid, p);
     fe2o3_count_launch(1);

@@ -94,13 +94,14 @@ class DevicePages:
         self.free_count = DeviceBuffer.from_host(stream, np.array([pages], np.uint32))
         zeros = lambda n: DeviceBuffer.zeroed(stream, n, np.uint32)  # noqa: E731
         self.lengths, self.counts, self.released, self.offsets = zeros(sequences), zeros(sequences), zeros(sequences), zeros(sequences + 1)
+        self.attended = zeros(sequences)   # lengths after a step, or zeros where it did not fit
         # of an extend's new tokens; and of a step's, a row for every sequence
         self.positions, self.slots, self.step_positions, self.step_slots = zeros(tokens), zeros(tokens), zeros(sequences), zeros(sequences)
         same = dict(lengths=self.lengths, next_lengths=self.lengths, free_count=self.free_count, next_free_count=self.free_count, page_table=self.table,
                     free_pages=self.free_pages, batch=sequences, table_width=self.width, page_size=page_size)
         self._extend = prepare(ctx, "kv_pages_v1", counts=self.counts, release=self.released, token_offsets=self.offsets, positions=self.positions,
                                slots=self.slots, tokens=tokens, **same)
-        self._step = prepare(ctx, "kv_pages_v1", positions=self.step_positions, slots=self.step_slots, tokens=sequences, **same)
+        self._step = prepare(ctx, "kv_pages_v1", positions=self.step_positions, slots=self.step_slots, tokens=sequences, attended=self.attended, **same)
 
     def extend(self, counts, release=None):
         """Places for `counts[b]` new tokens of every sequence b, after those of `release` (truth values) have given their pages back."""
@@ -121,7 +122,7 @@ class DevicePages:
         self._extend.destroy()
         self._step.destroy()
         for b in (self.table, self.free_pages, self.free_count, self.lengths, self.counts, self.released, self.offsets, self.positions, self.slots,
-                  self.step_positions, self.step_slots):
+                  self.step_positions, self.step_slots, self.attended):
             b.free()
 
 
@@ -292,13 +293,14 @@ class PagedKvCache:
         self.stream.synchronize()   # before the offsets go
         at.free()
 
-    def attention(self, q, out, heads, lse=None, scale=None, window=0, q_dtype=None, out_dtype=None, q_strides=None):
-        """A prepared launch of `paged_attention_v1` over this cache; the caller launches and destroys it."""
+    def attention(self, q, out, heads, lse=None, scale=None, window=0, q_dtype=None, out_dtype=None, q_strides=None, lengths=None):
+        """A prepared launch of `paged_attention_v1` over this cache, to the positions so far or to the first `lengths` of them; the caller launches and
+        destroys it."""
         _contiguous(q, out, lse)
         qs, qh = q_strides or (heads * self.dim, self.dim)
         return prepare(self.ctx, "paged_attention_v1", q=q, output=out, lse=lse, heads=heads, q_stride=qs, q_head_stride=qh,
                        scale=self.dim ** -0.5 if scale is None else scale, window=window, q_dtype=_float_dtype(q, q_dtype),
-                       output_dtype=_float_dtype(out, out_dtype), **self.args())
+                       output_dtype=_float_dtype(out, out_dtype), **{**self.args(), **({} if lengths is None else dict(lengths=lengths))})
 
     def attend(self, q, out, heads, **kw):
         """One new token a sequence, q and out [sequences][heads][dim].  Returns when the device is idle, since the launch's workspace
@@ -320,7 +322,10 @@ class PagedKvCache:
 class DecodeStep:
     """One new token of every sequence at work (of length above 0): its key and value are written, then it attends to all
     positions so far and its own.  The tensors, a row a sequence, stay where they are from step to step; the caller fills
-    q, k and v on the cache's stream.  Rows of released sequences are not read, and their output is zeros.
+    q, k and v on the cache's stream.  Rows of released sequences count for nothing (with the device's book they may be read), and their output is zeros.
+
+    A step that does not fit changes neither book nor cache.  With the host's book `run` raises.  With the device's it cannot know: the step is reported
+    (`ctx.take_kernel_status`, which a program asks from time to time), and its output is zeros for every sequence, its log-sum-exp -inf.
 
     With the cache's book on the device a step is three launches and nothing else, and `run` may be captured in a CUDA graph (on the stream that
     it is given); with `rotary` q and k are turned by their positions on the way (q packed, or with strides, into rows that the step keeps)."""
@@ -335,7 +340,7 @@ class DecodeStep:
                                               strides, q_strides)
             if rotary:
                 q, q_strides, dtype = self.turned, None, one
-            self.attend = cache.attention(q, out, heads, lse, scale, window, dtype, out_dtype, q_strides)
+            self.attend = cache.attention(q, out, heads, lse, scale, window, dtype, out_dtype, q_strides, lengths=cache.pages.attended)
             return
         if rotary:
             raise ValueError("rotary positions in a decode step need the cache's book on the device: tokens=")

@@ -512,12 +512,14 @@ typedef struct fe2o3_paged_attention_v1_args {
  * All or nothing: where a length or count does not fit its row of the page table (or 31 bits), or there are more tokens than `tokens`
  * (where positions or slots are asked for) or than 32 bits hold, FE2O3_KSTATUS_LENGTH is reported, where free_pages has too few free pages
  * (or no room for the released ones) FE2O3_KSTATUS_PAGES; page_table and free_pages then stay as they are, next_lengths and next_free_count are
- * lengths and free_count, token_offsets 0, positions 0 and slots FE2O3_SLOT_NONE.  A page belongs to one sequence here: a table whose
+ * lengths and free_count, token_offsets 0, positions 0 and slots FE2O3_SLOT_NONE.  attended [batch] (may be empty) is next_lengths, and where the
+ * step does not fit zeros: attention that goes by it attends to nothing then, instead of passing off the positions so far for the step's.  A page belongs to one sequence here: a table whose
  * rows share pages is not to be released from.  batch is at most 8192, batch * table_width and the rows of all pages below 2^32. */
 #define FE2O3_SLOT_NONE 0xffffffffu
 typedef struct fe2o3_kv_pages_v1_args {
     fe2o3_slice counts, release, lengths, free_count, page_table, free_pages, next_lengths, next_free_count, token_offsets, positions, slots;
     uint32_t batch, table_width, page_size, tokens;
+    fe2o3_slice attended;
 } fe2o3_kv_pages_v1_args;
 
 /* Rotary positions: the first rotary_dim columns of every row of q and k, in pairs, are turned by an angle of the row's position,

@@ -345,3 +345,14 @@ def test_new_tokens_are_whole_numbers(book):
     assert held() is None
     cache.extend([3.0, True, 0, 2])
     assert held().tolist() == [3, 1, 0, 2] and cache.new_tokens == 6
+
+
+def test_lengths_to_attend_to():
+    """What a plan leaves for the attention of its step: optional, one a sequence, apart from everything else."""
+    op, kw = "kv_pages_v1", pages()
+    ok(op, **{**kw, "attended": sl(11, 3)})
+    for n in (2, 4):
+        assert err(op, **{**kw, "attended": sl(11, n)}) == "Length"
+    assert err(op, **{**kw, "attended": sl(11, 3, 2)}) == "Alignment"
+    for name in ("lengths", "next_lengths", "slots", "page_table"):
+        assert err(op, **{**kw, "attended": (kw[name][0], 3)}) == "OutputAliasesInput", name

@@ -229,3 +229,64 @@ def test_example_runs(gpu, more):  # noqa: F811
     import paged_decode
     off = paged_decode.main(["--sequences", "16", "--prompt", "37", "--steps", "20", "--heads", "4", "--dim", "64"] + more)
     assert off <= 2.0 ** -8   # (bf16 outputs)
+
+
+@pytest.mark.parametrize("form", ["bf16", "e2m1"])
+@pytest.mark.parametrize("turned", [False, True])
+@pytest.mark.parametrize("captured", [False, True])
+def test_a_step_that_does_not_fit_gives_nothing(gpu, form, turned, captured):  # noqa: F811
+    """Not the step before it once more, for no sequence, and the next step that fits is right again."""
+    fe, torch, ctx, stream = gpu
+    from fe2o3_b200.kv_cache import DecodeStep, PagedKvCache
+    from fe2o3_b200.rotary import Rotary
+    ctx.take_kernel_status(stream)
+    B, H, KH, D = 3, 4, 2, 64
+    cache = PagedKvCache(ctx, stream, B, 64, KH, D, 8, pages=6, format=code(fe, form), tokens=40)
+    rotary = Rotary(ctx, stream, D) if turned else None
+    g = torch.Generator(device="cuda")
+    g.manual_seed(7)
+    new = lambda n, h: torch.randn(n, h, D, generator=g, device="cuda")  # noqa: E731
+    cache.extend([14, 9, 0])
+    cache.append(new(23, KH), new(23, KH))
+    q, k, v = new(B, H), new(B, KH), new(B, KH)
+    out, lse = (torch.full(s, 7.0, device="cuda") for s in ((B, H, D), (B, H)))
+    step = DecodeStep(cache, q, k, v, out, H, lse=lse, rotary=rotary)
+    run = step.run
+    if captured:
+        side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side), torch.cuda.graph(graph, stream=side):
+            step.run(ctx.wrap_stream(side.cuda_stream))
+        run = graph.replay
+
+    def stepped():
+        for t, h in ((q, H), (k, KH), (v, KH)):
+            t.copy_(new(B, h))
+        torch.cuda.synchronize()
+        run()
+        torch.cuda.synchronize()
+        return out.cpu().numpy(), lse.cpu().numpy()
+
+    def right(o, l):
+        held = Held(torch, cache)
+        at = torch.as_tensor(step.turned, device="cuda").view(torch.float32).view(B, H, D) if turned else q
+        check_attention(held, at.cpu().numpy(), o, l, attention64(held, at.cpu().numpy(), f32(D ** -0.5)), "f32")
+
+    for _ in range(2):                                      # to 16 positions and 11
+        right(*stepped())
+    assert ctx.take_kernel_status(stream) == 0 and read_lengths(cache).tolist() == [16, 11, 0]
+    cache.extend([0, 0, 16])                                # the last two pages
+    cache.append(new(16, KH), new(16, KH))
+    before = cache.k_cache.to_host_vec(stream)
+    for _ in range(2):                                      # the first and the third want a page, the second does not
+        o, l = stepped()
+        assert (o == 0).all() and (l == -np.inf).all()
+        assert ctx.take_kernel_status(stream) == 7 and read_lengths(cache).tolist() == [16, 11, 16]
+        assert (cache.k_cache.to_host_vec(stream) == before).all()
+    cache.release(2)
+    right(*stepped())
+    assert ctx.take_kernel_status(stream) == 0 and read_lengths(cache).tolist() == [17, 12, 0]
+    step.destroy()
+    cache.free()
+    if rotary:
+        rotary.free()

@@ -283,3 +283,27 @@ def test_a_plan_patched_to_many_tokens(gpu, batch, first):  # noqa: F811
 def test_the_largest_batches(gpu, batch, most, tokens, in_place):  # noqa: F811
     """More sequences than 48 KiB of shared memory hold, up to the most that are admitted."""
     test_steps(gpu, batch, 16, most, tokens, in_place)
+
+
+@pytest.mark.parametrize("batch,tokens", [(5, 60), (700, 9000)])
+def test_lengths_to_attend_to(gpu, batch, tokens):  # noqa: F811
+    """The next lengths, with counts and without; zeros, and nothing else new, where a step does not fit."""
+    fe, torch = gpu[:2]
+    rng = np.random.default_rng(batch)
+    for in_place in (True, False):
+        book = Book(batch, 6, 8, 6 * batch)
+        d = Device(gpu, book, tokens, in_place)
+        attended = torch.full((batch,), 77, dtype=torch.int32, device="cuda")
+        for counts, release in ((rng.integers(0, 12, batch), None), (None, None), (rng.integers(0, 9, batch), rng.random(batch) < 0.4), (np.full(batch, 49), None),
+                                (None, rng.random(batch) < 0.4)):
+            if counts is not None and counts.max() > 48:
+                with pytest.raises(fe.Fe2o3Error):
+                    d.step(counts, release, attended=attended)
+                assert (attended == 0).all() and (d.held()["next_lengths"] == book.lengths).all()
+                continue
+            d.step(counts, release, attended=attended)
+            d.check(book.step(counts, release))
+            assert (attended.cpu().numpy() == book.lengths).all()
+            if not in_place:
+                d.lengths.copy_(d.next_lengths)
+                d.count.copy_(d.next_count)
