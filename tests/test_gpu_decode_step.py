@@ -290,3 +290,55 @@ def test_a_step_that_does_not_fit_gives_nothing(gpu, form, turned, captured):  #
     cache.free()
     if rotary:
         rotary.free()
+
+
+def near_by_blocks(got, want):
+    """4-bit rows block by block.  m: the row's largest magnitude, s = m / 2688; t = 448 m_g / m of a block, b its e4m3 scale.  Codes lie at most 2 apart, so an
+    element is off by b s at most where 6 b s reaches the block's largest, which b >= t gives, and by 6 s (t - b) more where it does not.  From t = 2^-6 on b
+    is within 2^-4 of t: (1 + 2^-4) / 6 m_g either way.  Below, b is off by 2^-10 at most: m_g / 6 + 2^-10 s, or 6 * 2^-10 s for what is cut off (all of a block
+    whose scale becomes 0).  2^-20 for the f32 quotients and products of the definition, and of the row's largest for the rotation's."""
+    blocks = lambda x: np.abs(x).reshape(*x.shape[:-1], -1, 16)  # noqa: E731
+    m, of_block = np.abs(want).max(-1)[..., None, None], blocks(want).max(-1, keepdims=True)
+    t = 448 * of_block / np.maximum(m, 1e-300)
+    bound = np.where(t >= 2.0 ** -6, 1.0625 / 6 * of_block, np.maximum(of_block / 6 + 2.0 ** -10 * m / 2688, 2.0 ** -10 * m / 448))
+    assert (blocks(got - want) <= bound * (1 + 2.0 ** -20) + 2.0 ** -20 * m).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("dim,rotary_dim", [(64, 64), (128, 20), (96, 0)])
+def test_four_bit_rows_block_by_block(gpu, dtype, dim, rotary_dim):  # noqa: F811
+    """Blocks far below the row's largest, down to such as are lost, through a prompt and a step; a block of another size than its own is noticed."""
+    fe, torch, ctx, stream = gpu
+    from fe2o3_b200.kv_cache import DecodeStep, PagedKvCache
+    from fe2o3_b200.rotary import Rotary
+    B, H, KH, T = 2, 2, 2, 70
+    rng = np.random.default_rng(dim)
+    cache, rotary = PagedKvCache(ctx, stream, B, T + 1, KH, dim, 16, format=fe.KV_E2M1, tokens=B * T), Rotary(ctx, stream, rotary_dim)
+    freq = rotary.frequencies.to_host_vec(stream) if rotary_dim else np.zeros(0, f32)
+
+    def rows(n):
+        of_block = 2.0 ** -rng.integers(0, 20, (n, KH, dim // 16))
+        of_block[..., 0] = 1
+        return rows_in(torch, rng.normal(size=(n, KH, dim)) * of_block.repeat(16, -1), dtype)
+    (k, kv), (v, vv), (k1, k1v), (v1, v1v) = rows(B * T), rows(B * T), rows(B), rows(B)
+    cache.extend([T, T])
+    cache.append(k, v, rotary=rotary)
+    step = DecodeStep(cache, torch.zeros(B, H, dim, dtype=k.dtype, device="cuda"), k1, v1, torch.zeros(B, H, dim, device="cuda"), H, rotary=rotary)
+    step.run()
+    held, at = Held(torch, cache), np.arange(T + 1)
+    for b in range(B):
+        part = slice(b * T, (b + 1) * T)
+        want_k = turned64(np.concatenate([kv[part], k1v[b:b + 1]]), at, freq, "half")
+        want_v = np.concatenate([vv[part], v1v[b:b + 1]]).astype(np.float64)
+        near_by_blocks(held.rows[b][0], want_k)
+        near_by_blocks(held.rows[b][1], want_v)
+        # the smallest block of a row that is not lost, twice as large
+        wrong, size = held.rows[b][1].copy(), np.abs(want_v).reshape(T + 1, KH, -1, 16).max(-1)
+        worst = np.unravel_index(np.argmin(np.where(size * 448 >= 2.0 ** -6 * size.max(-1, keepdims=True), size / size.max(-1, keepdims=True), np.inf)), size.shape)
+        wrong.reshape(T + 1, KH, -1, 16)[worst] *= 2
+        with pytest.raises(AssertionError):
+            near_by_blocks(wrong, want_v)
+    assert ctx.take_kernel_status(stream) == 0
+    step.destroy()
+    cache.free()
+    rotary.free()
