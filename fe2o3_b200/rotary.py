@@ -8,8 +8,8 @@ import math
 
 import numpy as np
 
-from . import DTYPE_BF16, DTYPE_F32, ROTARY_HALF, DeviceBuffer, prepare
-from .kv_cache import _contiguous, _numbers
+from . import ROTARY_HALF, DeviceBuffer, prepare
+from .kv_cache import _contiguous, _float_dtype, _numbers
 
 
 def rotary_frequencies(rotary_dim, base=10000.0, scaling=None, factor=1.0, trained=None, fast=32.0, slow=1.0):
@@ -19,7 +19,9 @@ def rotary_frequencies(rotary_dim, base=10000.0, scaling=None, factor=1.0, train
       "linear"  positions are squeezed: every frequency by factor;
       "ntk"     the base grows so that the slowest pair turns factor times slower and the fastest as before;
       "yarn"    pairs that turn more than `fast` times in the trained context stay, those that turn less than `slow` times are squeezed by
-                factor, those between in proportion to their number; sine and cosine times 0.1 ln(factor) + 1."""
+                factor, those between in proportion to their number; sine and cosine times 0.1 ln(factor) + 1 (Peng, Quesnelle, Fan and Shippole, YaRN:
+                Efficient Context Window Extension of Large Language Models, 2023, whose bounds of the ramp and smallest width of it are kept, since
+                models were trained with them)."""
     if rotary_dim < 0 or rotary_dim % 2 or base <= 0 or factor < 1:
         raise ValueError("rotary_dim is even, base above 0 and factor at least 1")
     pairs = np.arange(0, rotary_dim, 2, dtype=np.float64)
@@ -42,17 +44,6 @@ def rotary_frequencies(rotary_dim, base=10000.0, scaling=None, factor=1.0, train
     raise ValueError(f"scaling is None, linear, ntk or yarn, not {scaling!r}")
 
 
-def _dtype(x, dtype):
-    if dtype is not None:
-        return dtype
-    name = str(getattr(x, "dtype", ""))
-    if name.endswith("bfloat16") or name == "uint16":
-        return DTYPE_BF16
-    if name.endswith("float32"):
-        return DTYPE_F32
-    raise TypeError(f"rows are f32 or bf16 (bits as uint16), got {name or type(x)}: say dtype=")
-
-
 class Rotary:
     """Frequencies on the device, and launches of `rotary_v1` with them."""
 
@@ -72,9 +63,9 @@ class Rotary:
             kv_heads = 0
         _contiguous(q, k, q_out, k_out)
         _numbers(positions=positions)
-        one = _dtype(q, dtype)
+        one = _float_dtype(q, dtype)
         for x in (k, q_out, k_out):
-            if hasattr(x, "dtype") and _dtype(x, dtype) != one:
+            if hasattr(x, "dtype") and _float_dtype(x, dtype) != one:
                 raise TypeError(f"q, k and their outputs are of one type, got {q.dtype} and {x.dtype}")
         packed = ((heads * dim, dim), (kv_heads * dim, dim))
         (qt, qh), (kt, kh) = strides or packed
