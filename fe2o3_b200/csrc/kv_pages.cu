@@ -6,10 +6,11 @@
 // replaced in place and the released pages lie on the stack.  Then pages and tokens are dealt out evenly, whatever sequence
 // they are of: a thread finds the sequence of its first token by bisection in shared memory and goes on from there.  The page
 // of a position comes from the table's row or straight from the stack, so tables and slots are written at the same time.
-// A step of 48 sequences 3.6 us, where an empty launch takes 3; 131072 tokens of 512 sequences, 61 of which leave their pages, 10.3 us
-// (eight blocks, four tokens a thread and a warp to every released sequence: 37; eight tokens a thread 19; sixteen blocks 10.3).  What is left is a chain of trips
-// to memory, lengths, table, stack, and 1100 instructions a warp on sixteen SMs; more blocks would need a meeting in memory that
-// stays between launches, which two captured graphs would share.
+// A step of 48 sequences 3.3 us, where an empty launch takes 3; 131072 tokens of 512 sequences, 61 of which leave their pages, 10.7 us
+// (eight blocks, four tokens a thread and a warp to every released sequence: 37; eight tokens a thread 19; sixteen blocks 10.7).  What is left is a chain of trips
+// to memory, lengths, table, stack, and 1100 instructions a warp on sixteen SMs.  More blocks in one launch would need a meeting in memory
+// that stays between launches, which two captured graphs would share; positions and slots could be a second launch's, over all SMs, from what the first has
+// written.
 #include "common.cuh"
 
 namespace {

@@ -103,9 +103,10 @@ int32_t paged_attention_plan(fe2o3_ctx *ctx, const fe2o3_paged_attention_v1_args
     const uint32_t group = a->heads / a->kv_heads;
     // 16 query heads at once for a group of more than 8 (three terms of f32 queries of such long rows would not fit a block)
     const uint32_t nt = group <= 8 || (a->dim > 128 && a->format == FE2O3_KV_BF16 && a->q_dtype == FE2O3_DTYPE_F32) ? 1 : 2;
-    // Tiles of 64 keys for 4-bit rows that may be long: 32 query heads on 4 of 128, pages of 64, 96 ragged sequences of up to 6000 82 us with 32 keys
-    // and 77 with 64, two of 131071 (on 8) 113 and 102, rows of 64 columns 62 and 58; but 256 sequences of up to 500 41 and 49, and pages of 16
-    // (four boxes a tile) 91 and 98, of 32 82 and 92.
+    // Tiles of 64 keys for 4-bit rows that may be long.  32 query heads on 4 of 128, pages of 64, ragged sequences of up to 500, 2000, 4000, 6000 and 8192
+    // tokens: 96 of them 24, 37, 54, 76 and 92 us with 32 keys and 26, 39, 53, 72 and 88 with 64; 256 of them 37, 73, 115, 161 and 217, and 44, 76,
+    // 113, 152 and 197.  (Lengths are known on the device only, so the rule goes by the table's room: short sequences in a wide table pay for it.)  By events,
+    // which add 6: two of 131071 (on 8) 113 and 102, rows of 64 columns 62 and 58; but pages of 16 (four boxes a tile) 91 and 98, of 32 82 and 92.
     const uint64_t positions = (uint64_t)a->table_width * a->page_size, seen = a->window && a->window < positions ? a->window : positions;
     const bool long_rows = a->format == FE2O3_KV_E2M1 && nt == 1 && a->dim <= 128 && a->page_size % 64 == 0 && seen >= 4096;
     const PagedBuild b = a->format == FE2O3_KV_BF16 ? paged_build_bf16(a->dim, nt) : a->format == FE2O3_KV_E4M3 ? paged_build_e4m3(a->dim, nt)

@@ -40,7 +40,7 @@
 // bytes a thread stored and 184 loaded).  16 query heads on an 8-bit head (NT 2, 54 us) are bound by latency: 255 registers leave two warps a
 // scheduler, each one dependent chain of some 1150 instructions a tile of 32 keys, at a third of the issue slots; the loop no longer
 // fits the first instruction cache.  Half tiles on three blocks an SM come to the same time.
-// 4 bits: two sequences of 131071 (319 MB) 94 to 96 us, 3.4 TB/s, where a sum over as many bytes takes 70; 96 ragged ones of up to 6000 on 4 heads 67 us; 16 heads
+// 4 bits: two sequences of 131071 (319 MB) 94 to 96 us, 3.4 TB/s, where a sum over as many bytes takes 70; 96 ragged ones of up to 6000 on 4 heads 70 us; 16 heads
 // of 64 on 512 tokens 11.  Copies alone take 75 of them, products alone 73: what is left is what the two do not hide of each other with
 // eight warps an SM and two tiles of 64 keys each in its ring, and about 12 us of beginning and end.  By events, which add 6: three blocks of 32
 // keys 113 us where these take 102; 48 keys, or four blocks, spill (117, 129); scales by the lanes' 16-byte copies, so fewer requests to the

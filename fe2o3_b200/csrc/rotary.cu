@@ -7,8 +7,9 @@
 // whole number of pieces, the columns go through shared memory, where a lane takes a pair or two neighbouring ones.  (Partners fetched one by one
 // from the first cache instead, and lanes by powers of two: 8191 tokens of 48 rows of 80 columns, 20 of them turned, 73 and 43 us where this
 // takes 34; 16384 tokens of 40 rows of 128 with 100 turned, 50 pairs, 110 us with two pairs a lane at once and 142 with one.)  The first
-// rows are fetched before the sines are worked out (64 tokens of 40 rows 2.7 us for 3.2).
-// 16384 tokens, 40 rows of 128 bf16 columns: 57 us, 5.9 TB/s, 90 % of a copy's rate, neighbours as pairs 61; 1003 tokens of 24 f32 rows of 96 4.4 us.
+// rows are fetched before the sines are worked out (64 tokens of 40 rows 2.7 us for 3.2).  Into a cache, 16384 tokens of 48 rows of 128: bf16 70 us (6.1 TB/s),
+// e4m3, i8 and e2m1 78 (4.7 and 4.6 TB/s: the quantising chain of a row); 64 tokens 2.7 and 3.1.
+// 16384 tokens, 40 rows of 128 bf16 columns: 58 us, 5.8 TB/s, 88 % of a copy's rate, neighbours as pairs 61; 1003 tokens of 24 f32 rows of 96 4.4 us.
 // Angles: position times frequency has up to 56 bits.  The product p and what rounding took from it, e, are 64-bit numbers that add up
 // to it exactly; n whole turns are taken off in two steps (2 pi as two 64-bit numbers), which leaves an angle in [-pi, pi] that is right
 // to some 2^-50.  Its sine and cosine are those of its 32-bit rounding, and the rest of it to first order.
