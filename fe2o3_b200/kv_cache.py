@@ -297,6 +297,7 @@ class PagedKvCache:
         """A prepared launch of `paged_attention_v1` over this cache, to the positions so far or to the first `lengths` of them; the caller launches and
         destroys it."""
         _contiguous(q, out, lse)
+        _numbers(lengths=lengths)
         qs, qh = q_strides or (heads * self.dim, self.dim)
         return prepare(self.ctx, "paged_attention_v1", q=q, output=out, lse=lse, heads=heads, q_stride=qs, q_head_stride=qh,
                        scale=self.dim ** -0.5 if scale is None else scale, window=window, q_dtype=_float_dtype(q, q_dtype),

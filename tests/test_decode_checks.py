@@ -356,3 +356,14 @@ def test_lengths_to_attend_to():
     assert err(op, **{**kw, "attended": sl(11, 3, 2)}) == "Alignment"
     for name in ("lengths", "next_lengths", "slots", "page_table"):
         assert err(op, **{**kw, "attended": (kw[name][0], 3)}) == "OutputAliasesInput", name
+
+
+def test_lengths_of_an_attention_are_32_bits():
+    from fe2o3_b200.kv_cache import PagedKvCache
+    cache, q = PagedKvCache.__new__(PagedKvCache), torch.zeros(3, 2, 32)
+    cache.dim = 32
+    for bad in (torch.arange(3), torch.arange(3.0)):
+        with pytest.raises(TypeError, match="lengths are 32-bit"):
+            cache.attention(q, q, 2, lengths=bad)
+    with pytest.raises(ValueError, match="contiguous"):
+        cache.attention(q, q, 2, lengths=torch.arange(6, dtype=torch.int32)[::2])
