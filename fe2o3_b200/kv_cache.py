@@ -15,7 +15,7 @@ step is two launches and the copy of the lengths, or three launches with a book 
 
     cache = PagedKvCache(ctx, stream, 8, 4096, 8, 128, format=KV_E2M1, tokens=8 * prompt_length)   # with a book on the device
     cache.extend([prompt_length] * 8)
-    cache.append(k, v, q=q, q_out=turned, rotary=rotary)   # rotary positions on the way
+    cache.append(k, v, q=q, q_out=turned, heads=32, rotary=rotary)   # rotary positions on the way
     step = DecodeStep(cache, q1, k1, v1, out, heads=32, rotary=rotary)
 
 `append`, `extend`, `release` and the steps are enqueued on the cache's stream and do not wait for its launches (but a copy from
