@@ -4,6 +4,7 @@
 // generated host adapters (crates/fe2o3-host/src/generated_*.rs) and the
 // executable lifecycle adapter (crates/fe2o3-host/src/hsa_executable_lifecycle.rs).
 #include <math.h>
+#include <stddef.h>
 #include <stdarg.h>
 #include <stdio.h>
 #include <string.h>
@@ -1968,6 +1969,12 @@ int32_t fe2o3_resolve_kernel(fe2o3_executable *exe, const char *symbol, uint32_t
 int32_t fe2o3_launch_and_wait(fe2o3_executable *exe, uint32_t kernel_id, const fe2o3_geometry *geometry, const void *kernarg,
                               uint64_t kernarg_bytes, fe2o3_stream *stream, uint32_t timeout_ms, uint32_t *kernel_status) {
     if (!exe || !kernarg || !stream || kernel_id >= OP_COUNT) return FE2O3_ERR_INVALID_ARGUMENT;
+    fe2o3_kv_pages_v1_args pages{};
+    if (kernel_id == OP_KV_PAGES && kernarg_bytes == offsetof(fe2o3_kv_pages_v1_args, attended)) {   // a block from before it had its last slice
+        memcpy(&pages, kernarg, kernarg_bytes);
+        kernarg = &pages;
+        kernarg_bytes = sizeof pages;
+    }
     if (kernarg_bytes != kOps[kernel_id].kernarg_bytes) {
         fe2o3_set_error("Length{role=kernarg, expected=%llu, actual=%llu}",
                         (unsigned long long)kOps[kernel_id].kernarg_bytes, (unsigned long long)kernarg_bytes);

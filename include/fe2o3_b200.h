@@ -513,7 +513,8 @@ typedef struct fe2o3_paged_attention_v1_args {
  * (where positions or slots are asked for) or than 32 bits hold, FE2O3_KSTATUS_LENGTH is reported, where free_pages has too few free pages
  * (or no room for the released ones) FE2O3_KSTATUS_PAGES; page_table and free_pages then stay as they are, next_lengths and next_free_count are
  * lengths and free_count, token_offsets 0, positions 0 and slots FE2O3_SLOT_NONE.  attended [batch] (may be empty) is next_lengths, and where the
- * step does not fit zeros: attention that goes by it attends to nothing then, instead of passing off the positions so far for the step's.  A page belongs to one sequence here: a table whose
+ * step does not fit zeros: attention that goes by it attends to nothing then, instead of passing off the positions so far for the step's (fe2o3_launch_and_wait
+ * also takes a block that ends before it, 192 bytes, as one where it is empty).  A page belongs to one sequence here: a table whose
  * rows share pages is not to be released from.  batch is at most 8192, batch * table_width and the rows of all pages below 2^32. */
 #define FE2O3_SLOT_NONE 0xffffffffu
 typedef struct fe2o3_kv_pages_v1_args {

@@ -307,3 +307,32 @@ def test_lengths_to_attend_to(gpu, batch, tokens):  # noqa: F811
             if not in_place:
                 d.lengths.copy_(d.next_lengths)
                 d.count.copy_(d.next_count)
+
+
+def test_packed_blocks_of_both_sizes(gpu):  # noqa: F811
+    """The runtime adapter takes a block without its last slice, the lengths to attend to, as one where that is empty; no other size."""
+    import ctypes as C
+    import hashlib
+    fe, torch, ctx, stream = gpu
+    from fe2o3_b200._lib import LIB_PATH, lib
+    with open(LIB_PATH, "rb") as f:
+        image = f.read()
+    exe, kid, nbytes, status = C.c_void_p(), C.c_uint32(), C.c_uint64(), C.c_uint32()
+    digest = (C.c_uint8 * 32).from_buffer_copy(hashlib.sha256(image).digest())
+    fe.check(lib.fe2o3_load_executable(ctx._h, image, C.c_uint64(len(image)), digest, C.byref(exe)))
+    fe.check(lib.fe2o3_resolve_kernel(exe, b"kv_pages_v1", C.byref(kid), C.byref(nbytes)))
+    assert nbytes.value == 208
+    book = Book(7, 10, 8, 70)
+    d = Device(gpu, book, 60)
+    attended = torch.full((7,), 77, dtype=torch.int32, device="cuda")
+    for size, counts in ((192, [5, 0, 9, 1, 8, 16, 3]), (208, [1, 2, 3, 4, 5, 6, 7]), (192, [0, 1, 0, 1, 0, 1, 0])):
+        n = d.up(np.array(counts, np.uint32))
+        args = fe.make_args("kv_pages_v1", counts=n, **d.args(**(dict(attended=attended) if size == 208 else {})))
+        block = (C.c_uint8 * size).from_buffer_copy(bytes(args)[:size])
+        for wrong in (191, 200):
+            assert lib.fe2o3_launch_and_wait(exe, kid, None, block, C.c_uint64(wrong), stream._h, C.c_uint32(5000), C.byref(status)) == -5
+        fe.check(lib.fe2o3_launch_and_wait(exe, kid, None, block, C.c_uint64(size), stream._h, C.c_uint32(5000), C.byref(status)))
+        d.check(book.step(counts))
+        if size == 208:
+            assert (attended.cpu().numpy() == book.lengths).all()
+    fe.check(lib.fe2o3_unload_executable(exe))
